@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../include/vs_hip.h"
+#include "vs_host.h"
 #include "vs_internal.h"
 
 namespace {
@@ -46,18 +47,7 @@ int hip_err(hipError_t e, const char *what) {
         if (e_ != hipSuccess) return hip_err(e_, what); \
     } while (0)
 
-// Restores the caller's current device on scope exit.
-struct DeviceGuard {
-    int prev = -1;
-    hipError_t err = hipSuccess;
-    explicit DeviceGuard(int dev) {
-        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-        err = hipSetDevice(dev);
-    }
-    ~DeviceGuard() {
-        if (prev >= 0) (void)hipSetDevice(prev);
-    }
-};
+using vs::DeviceGuard;
 
 // Test support (option "fail_alloc"): when > 0, the device or pinned host
 // allocation that brings it to 0 fails as out of memory, so tests reach the
@@ -186,6 +176,23 @@ constexpr size_t kCtlBytes = 256;  // control words at the head of an index's pi
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 }  // namespace
+
+// What the other sources' entry points share (vs_host.h).
+namespace vs {
+
+int report(int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof g_err, fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+int report_hip(hipError_t e, const char *what) { return hip_err(e, what); }
+
+hipError_t device_alloc(void **p, size_t bytes) { return dev_malloc(p, bytes); }
+
+}  // namespace vs
 
 // Per-handle planner options (vs_index_set_option).  The defaults are the
 // tuned plan; the others force a path or a shape so that tests can reach

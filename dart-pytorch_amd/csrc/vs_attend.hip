@@ -1,0 +1,891 @@
+// vs_attend.hip -- attention of one new token over the paged key-value cache,
+// and the cache's rows in and out: kernels and entry points.
+#include <cmath>
+
+#include "vs_kv.h"
+
+namespace vs {
+namespace {
+
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kWaves = 4;         // per workgroup
+constexpr int kMinBlocks = 4;     // blocks per work item, at least: one per wave
+constexpr int kJoinDims = 128;    // dimensions joined over the waves at once (LDS)
+
+struct AttendArgs {
+    char *pool;
+    int64_t page_bytes, layer_off, kv_off, head_off;  // bytes; kv_off from keys to values
+    const int32_t *table, *lens;
+    int64_t width;
+    int nseq, npages, page_shift;
+    const char *q, *k, *v;
+    char *out;
+    int64_t q_seq, q_head, k_seq, k_head, v_seq, v_head, o_seq, o_head;  // elements
+    float *lse;
+    int heads, kv_heads, group, gtiles;  // group: query heads per key-value head; gtiles: 16 at a time
+    float scale2;                        // scale * log2(e)
+    int window, sinks;
+    int q_vec, k_vec;                    // rows readable in 16-byte pieces
+    int target_items;
+    float *part_o;   // [item][heads][dim]
+    float2 *part_ml; // [item][heads] running maximum and sum
+    int2 *first;     // [nseq] first item, items
+};
+
+// The blocks that a sequence of n positions attends to: nsb from its start,
+// then wb0 .. nb - 1.
+struct Span {
+    int nsb, wb0, total;
+};
+
+__device__ __forceinline__ Span span_of(int n, int window, int sinks) {
+    Span s;
+    const int nb = n / kKvBlock + (n % kKvBlock != 0);
+    s.nsb = s.wb0 = 0;
+    if (window > 0 && n > window) {
+        s.wb0 = (n - window) / kKvBlock;
+        const int k = min(sinks, n);
+        s.nsb = min(k / kKvBlock + (k % kKvBlock != 0), s.wb0);
+    }
+    s.total = s.nsb + nb - s.wb0;
+    return s;
+}
+
+__device__ __forceinline__ int length_of(const AttendArgs &a, int b) {
+    const int64_t most = a.width << a.page_shift;
+    const int n = max(a.lens[b], 0);
+    return n < most ? n : (int)most;
+}
+
+// Work item `item`: blocks [split * per, ...) of sequence b.  Every wave
+// works the whole division out by itself from the lengths: all blocks of the
+// call over the number of items that fills the card, so that ragged batches
+// are split where their long sequences are.
+struct Item {
+    int b, split, nsplit, per;
+};
+
+__device__ __forceinline__ bool find_item(const AttendArgs &a, int item, int lane, Item &it) {
+    uint64_t total = 0;
+    for (int b0 = 0; b0 < a.nseq; b0 += 64) {
+        const int b = b0 + lane;
+        if (b < a.nseq) total += (uint64_t)max(span_of(length_of(a, b), a.window, a.sinks).total, 1);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) total += __shfl_xor((unsigned long long)total, d);
+    int per;
+    if (total >> 32)
+        per = (int)((total + a.target_items - 1) / (uint64_t)a.target_items);
+    else
+        per = (int)(((uint32_t)total + (uint32_t)a.target_items - 1) / (uint32_t)a.target_items);
+    per = max(per, kMinBlocks);
+    int base = 0;
+    for (int b0 = 0; b0 < a.nseq; b0 += 64) {
+        const int b = b0 + lane;
+        int cnt = 0;
+        if (b < a.nseq) {
+            const int t = span_of(length_of(a, b), a.window, a.sinks).total;
+            cnt = max(t / per + (t % per != 0), 1);
+        }
+        int incl = cnt;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d);
+            if (lane >= d) incl += o;
+        }
+        const uint64_t past = __ballot(base + incl > item);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            it.b = b0 + l;
+            it.nsplit = __shfl(cnt, l);
+            it.split = item - base - (__shfl(incl, l) - it.nsplit);
+            it.per = per;
+            return true;
+        }
+        base += __shfl(incl, 63);
+    }
+    return false;
+}
+
+// 16 bytes of a row from element x on, whatever the row's alignment.
+template <int ST>
+__device__ __forceinline__ u32x4_t load_piece(const char *row, int x, bool vec) {
+    constexpr int E = ST ? 8 : 4;
+    if (vec) return *(const u32x4_t *)(row + (int64_t)x * (16 / E));
+    u32x4_t w;
+    if constexpr (ST) {
+        const uint16_t *p = (const uint16_t *)row + x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    } else {
+        const uint32_t *p = (const uint32_t *)row + x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = p[i];
+    }
+    return w;
+}
+
+// One pass over a work item's keys and values with the running maximum and
+// sum of the softmax.  A wave takes every fourth unit of the item: 32
+// positions of bf16, 16 of fp32.  Lane (r, g) = (lane & 15, lane >> 4).
+//   S^T = K Q^T    A operand: key rows (position r, 16 bytes of dimensions g);
+//                  B operand: the query heads of the group, column r
+//   O^T = V^T P^T  A operand: dimension r, the positions of lane group g;
+//                  B operand: P^T, which is S^T's accumulator as it stands:
+//                  lane (r, g) holds query r at positions 16 h + 4 g + i, and
+//                  the values lie in the cache in that order
+// so nothing passes through LDS but the join of the four waves, every load is
+// 1 KB of consecutive bytes per wave, and a column's maximum, sum and
+// rescaling belong to one lane.  Unused columns (fewer than 16 query heads
+// per key-value head) cost matrix time that the loads leave idle anyway.
+// bf16: P is multiplied as the sum of two bf16 values (its first 8 bits and
+// the rest rounded to 8), so it is good to 2^-17 and the output is as exact
+// as its last rounding.
+template <int ST, int D>
+__global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a) {
+    constexpr int E = ST ? 8 : 4;
+    constexpr int ES = 16 / E;             // element size
+    constexpr int H = ST ? 2 : 1;          // 16-position halves per unit
+    constexpr int NC = (D / E + 3) / 4;    // 16-byte pieces per lane of a key row
+    constexpr int ND = D / 16;
+    constexpr int DW = D < kJoinDims ? D : kJoinDims;
+    constexpr int LD = DW + 4;
+    extern __shared__ __align__(16) float lds_o[];  // [wave][query][LD]
+    __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int per_item = a.kv_heads * a.gtiles;
+    const int item = blockIdx.x / per_item, hh = blockIdx.x % per_item;
+    const int gt = hh / a.kv_heads, kvh = hh % a.kv_heads;
+    const int gc = min(a.group - gt * 16, 16);  // query heads of this workgroup
+    Item it;
+    if (!find_item(a, item, lane, it)) return;
+    it.b = __builtin_amdgcn_readfirstlane(it.b);
+    it.split = __builtin_amdgcn_readfirstlane(it.split);
+    it.nsplit = __builtin_amdgcn_readfirstlane(it.nsplit);
+    const int per = __builtin_amdgcn_readfirstlane(it.per);
+    const int n = __builtin_amdgcn_readfirstlane(length_of(a, it.b));
+    const Span sp = span_of(n, a.window, a.sinks);
+    const int head0 = kvh * a.group + gt * 16;
+
+    // the queries, as the B operand
+    u32x4_t qf[NC];
+    {
+        const char *row = a.q + ((int64_t)it.b * a.q_seq + (int64_t)(head0 + r) * a.q_head) * ES;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            qf[c] = u32x4_t{0, 0, 0, 0};
+            if (r < gc && c * 4 + g < D / E) qf[c] = load_piece<ST>(row, (c * 4 + g) * E, a.q_vec);
+        }
+    }
+
+    float m = -__builtin_huge_valf(), l = 0.f;
+    f32x4_t o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    const int32_t *trow = a.table + (int64_t)it.b * a.width;
+    const int64_t head_base = a.layer_off + (int64_t)kvh * a.head_off;
+    const int bpp1 = (1 << (a.page_shift - 5)) - 1;
+    const int j0 = it.split * per, j1 = min(j0 + per, sp.total);
+    const int u1 = ST ? j1 : 2 * j1;
+    for (int u = (ST ? j0 : 2 * j0) + wave; u < u1; u += kWaves) {
+        const int j = ST ? u : u >> 1, half = ST ? 0 : u & 1;
+        const int blk = j < sp.nsb ? j : j - sp.nsb + sp.wb0;
+        const int pos0 = blk * kKvBlock + half * 16;
+        const int page = trow[pos0 >> a.page_shift];
+        if ((unsigned)page >= (unsigned)a.npages) continue;
+        char *kb = a.pool + ((int64_t)page * a.page_bytes + head_base +
+                             ((blk & bpp1) * kKvBlock + half * 16) * (D * ES));
+        char *vb = kb + a.kv_off;
+        u32x4_t kf[H * NC], vf[ND];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                // (a piece past the row's end is read again and zeroed)
+                const int piece = D % (4 * E) ? min(c * 4 + g, D / E - 1) : c * 4 + g;
+                u32x4_t w = *(const u32x4_t *)(kb + ((h * (D / E) + piece) * 16 + r) * 16);
+                if (D % (4 * E) && c * 4 + g >= D / E) w = u32x4_t{0, 0, 0, 0};
+                kf[h * NC + c] = w;
+            }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            vf[d] = *(const u32x4_t *)(vb + ((d * 16 + r) * 4 + g) * 16);
+
+        const int tn = n - 1 - pos0;  // the new token's place in this unit
+        if (a.k && tn < 16 * H && tn >= 0) {
+            // its keys and values take their places in the registers and, from
+            // one workgroup per key-value head, in the page
+            const char *krow = a.k + ((int64_t)it.b * a.k_seq + (int64_t)kvh * a.k_head) * ES;
+            const char *vrow = a.v + ((int64_t)it.b * a.v_seq + (int64_t)kvh * a.v_head) * ES;
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+                    if (tn == 16 * h + r && c * 4 + g < D / E) {
+                        const u32x4_t w = load_piece<ST>(krow, (c * 4 + g) * E, a.k_vec);
+                        kf[h * NC + c] = w;
+                        if (gt == 0)
+                            *(u32x4_t *)(kb + ((h * (D / E) + c * 4 + g) * 16 + r) * 16) = w;
+                    }
+            if (((tn & 15) >> 2) == g) {
+                const int e = (tn >> 4) * 4 + (tn & 3);  // its element of the lane's 16 bytes
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    char *to = vb + ((d * 16 + r) * 4 + g) * 16 + e * ES;
+                    if constexpr (ST) {
+                        const uint16_t x = ((const uint16_t *)vrow)[d * 16 + r];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            if (w == e >> 1)
+                                vf[d][w] = e & 1 ? (vf[d][w] & 0xFFFFu) | (uint32_t)x << 16
+                                                 : (vf[d][w] & 0xFFFF0000u) | x;
+                        if (gt == 0) *(uint16_t *)to = x;
+                    } else {
+                        const uint32_t x = ((const uint32_t *)vrow)[d * 16 + r];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            if (w == e) vf[d][w] = x;
+                        if (gt == 0) *(uint32_t *)to = x;
+                    }
+                }
+            }
+        }
+
+        f32x4_t s[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            s[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if constexpr (ST) {
+                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8_t, kf[h * NC + c]),
+                        __builtin_bit_cast(bf16x8_t, qf[c]), s[h], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            float_of(kf[h * NC + c][e]),
+                            float_of(qf[c][e]), s[h], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[h][i] *= a.scale2;
+        }
+
+        const int lo = n - a.window;  // with a window: positions below are invisible but for the sinks
+        if (pos0 + 16 * H > n || (a.window > 0 && pos0 < lo && pos0 + 16 * H > a.sinks)) {
+            // a masked position's score is -inf and its values are 0: what
+            // lies there may be anything, and 0 times a NaN is one
+            uint32_t hide = 0;
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int p = pos0 + 16 * h + 4 * g + i;
+                    if (p >= n || (a.window > 0 && p < lo && p >= a.sinks)) {
+                        s[h][i] = -__builtin_huge_valf();
+                        hide |= 1u << (4 * h + i);
+                    }
+                }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t keep = ~0u;
+                if constexpr (ST) {
+                    if (hide >> (2 * w) & 1) keep &= 0xFFFF0000u;
+                    if (hide >> (2 * w + 1) & 1) keep &= 0x0000FFFFu;
+                } else {
+                    if (hide >> w & 1) keep = 0;
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d) vf[d][w] &= keep;
+            }
+        }
+
+        float top = s[0][0];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__ballot(top > m)) {
+            const float mn = fmaxf(m, top);
+            const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] *= f;
+        }
+        const float ms = m == -__builtin_huge_valf() ? 0.f : m;
+        f32x4_t p[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[h][i] = __builtin_amdgcn_exp2f(s[h][i] - ms);
+                l += p[h][i];
+            }
+        if constexpr (ST) {
+            bf16x8_t hi, lo8;
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float t = float_of(bits_of(p[h][i]) & 0xFFFF0000u);
+                    hi[4 * h + i] = (__bf16)t;
+                    // (never 0 beside a weight: an infinite value times 0 would be a NaN)
+                    lo8[4 * h + i] = (__bf16)fmaxf(p[h][i] - t, p[h][i] * 0x1p-60f);
+                }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const bf16x8_t w = __builtin_bit_cast(bf16x8_t, vf[d]);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, hi, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, lo8, o[d], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        float_of(vf[d][i]), p[0][i], o[d], 0, 0, 0);
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) {
+        lds_m[wave][r] = m;
+        lds_l[wave][r] = l;
+    }
+
+    // the four waves' sums, kJoinDims dimensions at a time
+    const bool last = it.nsplit == 1;
+#pragma unroll
+    for (int d0 = 0; d0 < ND; d0 += DW / 16) {
+        if (d0) __syncthreads();
+        if (r < gc)
+#pragma unroll
+            for (int d = 0; d < DW / 16; ++d)
+                if (d0 + d < ND)
+                    *(f32x4_t *)(lds_o + (wave * gc + r) * LD + d * 16 + g * 4) = o[d0 + d];
+        __syncthreads();
+        const int dims = min(DW, D - d0 * 16);
+        for (int x = threadIdx.x; x < gc * (DW / 4); x += 64 * kWaves) {
+            const int row = x / (DW / 4), c4 = x % (DW / 4);
+            if (c4 * 4 >= dims) continue;
+            float top = lds_m[0][row];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][row]);
+            const float ms = top == -__builtin_huge_valf() ? 0.f : top;
+            float sum = 0.f;
+            f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(lds_m[w][row] - ms);
+                sum += f * lds_l[w][row];
+                const f32x4_t t = *(const f32x4_t *)(lds_o + (w * gc + row) * LD + c4 * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] += f * t[i];
+            }
+            const int head = head0 + row, dim = d0 * 16 + c4 * 4;
+            if (last) {
+                char *to = a.out + ((int64_t)it.b * a.o_seq + (int64_t)head * a.o_head + dim) * ES;
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (ST)
+                        ((__bf16 *)to)[i] = (__bf16)(acc[i] * inv);
+                    else
+                        ((float *)to)[i] = acc[i] * inv;
+                }
+                if (a.lse && dim == 0)
+                    a.lse[(int64_t)it.b * a.heads + head] =
+                        sum == 0.f ? -__builtin_huge_valf()
+                                   : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+            } else {
+                const int64_t slot = (int64_t)item * a.heads + head;
+                *(f32x4_t *)(a.part_o + slot * D + dim) = acc;
+                if (dim == 0) a.part_ml[slot] = make_float2(top, sum);
+            }
+        }
+    }
+    if (!last && hh == 0 && it.split == 0 && threadIdx.x == 0)
+        a.first[it.b] = make_int2(item, it.nsplit);
+    if (last && hh == 0 && threadIdx.x == 0) a.first[it.b] = make_int2(item, 1);
+}
+
+// Joins the items of a sequence, in their order: one wave per query head.
+template <int ST, int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+    constexpr int NR = (D + 63) / 64;
+    constexpr int ES = ST ? 2 : 4;
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (at >= (int64_t)a.nseq * a.heads) return;
+    const int b = (int)(at / a.heads), head = (int)(at % a.heads);
+    const int2 f = a.first[b];
+    if (f.y <= 1) return;
+    float top = -__builtin_huge_valf();
+    for (int s = lane; s < f.y; s += 64)
+        top = fmaxf(top, a.part_ml[(int64_t)(f.x + s) * a.heads + head].x);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float ms = top == -__builtin_huge_valf() ? 0.f : top;
+    float sum = 0.f, acc[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) acc[i] = 0.f;
+    for (int s0 = 0; s0 < f.y; s0 += 64) {
+        float w = 0.f;
+        if (s0 + lane < f.y) {
+            const float2 ml = a.part_ml[(int64_t)(f.x + s0 + lane) * a.heads + head];
+            w = __builtin_amdgcn_exp2f(ml.x - ms);
+            sum += w * ml.y;
+        }
+        const int cnt = min(64, f.y - s0);
+        const float *po = a.part_o + ((int64_t)(f.x + s0) * a.heads + head) * D + lane;
+        for (int s = 0; s < cnt; s += 8) {
+            float t[8][NR];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    t[e][i] = 0.f;
+                    if (s + e < cnt && lane + 64 * i < D)
+                        t[e][i] = po[(int64_t)(s + e) * a.heads * D + 64 * i];
+                }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float ws = __shfl(w, s + e);  // (0 past the last item)
+#pragma unroll
+                for (int i = 0; i < NR; ++i) acc[i] += ws * t[e][i];
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    char *to = a.out + ((int64_t)b * a.o_seq + (int64_t)head * a.o_head) * ES;
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+        if (lane + 64 * i < D) {
+            if constexpr (ST)
+                ((__bf16 *)to)[lane + 64 * i] = (__bf16)(acc[i] * inv);
+            else
+                ((float *)to)[lane + 64 * i] = acc[i] * inv;
+        }
+    if (a.lse && lane == 0)
+        a.lse[at] = sum == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// The place of position t of a block, dimension x, in elements.
+template <int ST>
+__host__ __device__ inline int key_place(int t, int x, int dim) {
+    constexpr int E = ST ? 8 : 4;
+    return ((t / 16 * (dim / E) + x / E) * 16 + t % 16) * E + x % E;
+}
+template <int ST>
+__host__ __device__ inline int value_place(int t, int x, int dim) {
+    const int h = t / 16, g = t % 16 / 4, i = t % 4;
+    return ST ? ((x * 4 + g) * 2 + h) * 4 + i : ((h * dim + x) * 4 + g) * 4 + i;
+}
+
+struct RowsArgs {
+    char *pool;
+    int64_t page_bytes, layer_off, kv_off, head_off;
+    const int32_t *table, *lens, *starts;
+    int64_t width, nrows;
+    int nseq, npages, page_shift, heads, dim;
+    const char *k, *v;
+    int64_t k_row, k_head, v_row, v_head;
+    char *k_out, *v_out;
+    int b, first;
+};
+
+// Where position pos of sequence b lies; null if nowhere.
+__device__ __forceinline__ char *block_of(const RowsArgs &a, int b, int64_t pos, int es) {
+    if (pos < 0 || pos >> a.page_shift >= a.width) return nullptr;
+    const int page = a.table[(int64_t)b * a.width + (pos >> a.page_shift)];
+    if ((unsigned)page >= (unsigned)a.npages) return nullptr;
+    const int64_t blk = (pos & ((1 << a.page_shift) - 1)) / kKvBlock;
+    return a.pool + (int64_t)page * a.page_bytes + a.layer_off + blk * kKvBlock * a.dim * es;
+}
+
+// One workgroup per row: read once, written once; a few scattered bytes per
+// element, which the caches gather as the next rows follow.
+template <int ST>
+__global__ __launch_bounds__(256) void append_kernel(RowsArgs a) {
+    using T = typename std::conditional<ST, uint16_t, uint32_t>::type;
+    for (int64_t row = blockIdx.x; row < a.nrows; row += gridDim.x) {
+        int b = (int)row;
+        int64_t pos;
+        if (a.starts) {
+            // the last sequence whose rows start at or before this one
+            int lo = 0, hi = a.nseq;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (a.starts[mid] <= row)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            b = lo;
+            if (row < a.starts[b] || row >= a.starts[b + 1]) continue;
+            pos = (int64_t)a.lens[b] - (a.starts[b + 1] - row);
+        } else {
+            pos = (int64_t)a.lens[b] - 1;
+        }
+        char *at = block_of(a, b, pos, sizeof(T));
+        if (!at) continue;
+        for (int x = threadIdx.x; x < a.heads * a.dim; x += 256) {
+            const int h = x / a.dim, d = x % a.dim;
+            T *k = (T *)(at + h * a.head_off), *v = (T *)(at + a.kv_off + h * a.head_off);
+            k[key_place<ST>(pos % kKvBlock, d, a.dim)] =
+                ((const T *)a.k)[row * a.k_row + h * a.k_head + d];
+            v[value_place<ST>(pos % kKvBlock, d, a.dim)] =
+                ((const T *)a.v)[row * a.v_row + h * a.v_head + d];
+        }
+    }
+}
+
+template <int ST>
+__global__ __launch_bounds__(256) void read_kernel(RowsArgs a) {
+    using T = typename std::conditional<ST, uint16_t, uint32_t>::type;
+    for (int64_t row = blockIdx.x; row < a.nrows; row += gridDim.x) {
+        const int64_t pos = a.first + row;
+        const char *at = block_of(a, a.b, pos, sizeof(T));
+        for (int x = threadIdx.x; x < a.heads * a.dim; x += 256) {
+            const int h = x / a.dim, d = x % a.dim;
+            T k = 0, v = 0;
+            if (at) {
+                k = ((const T *)(at + h * a.head_off))[key_place<ST>(pos % kKvBlock, d, a.dim)];
+                v = ((const T *)(at + a.kv_off +
+                                 h * a.head_off))[value_place<ST>(pos % kKvBlock, d, a.dim)];
+            }
+            ((T *)a.k_out)[row * a.heads * a.dim + x] = k;
+            ((T *)a.v_out)[row * a.heads * a.dim + x] = v;
+        }
+    }
+}
+
+template <int ST, int D>
+hipError_t launch_attend(const AttendArgs &a, int64_t items, bool join, hipStream_t st) {
+    constexpr int DW = D < kJoinDims ? D : kJoinDims;
+    const size_t lds = (size_t)kWaves * std::min(a.group, 16) * (DW + 4) * sizeof(float);
+    hipLaunchKernelGGL((attend_kernel<ST, D>), dim3((uint32_t)(items * a.kv_heads * a.gtiles)),
+                       dim3(64 * kWaves), lds, st, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !join) return e;
+    const int64_t rows = (int64_t)a.nseq * a.heads;
+    hipLaunchKernelGGL((attend_join_kernel<ST, D>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0,
+                       st, a);
+    return hipGetLastError();
+}
+
+template <int ST>
+hipError_t launch_attend_dim(const AttendArgs &a, int64_t items, bool join, int dim,
+                             hipStream_t st) {
+    switch (dim) {
+#define VS_DIM(D) \
+    case D:       \
+        return launch_attend<ST, D>(a, items, join, st);
+        VS_DIM(16) VS_DIM(32) VS_DIM(48) VS_DIM(64) VS_DIM(80) VS_DIM(96) VS_DIM(112) VS_DIM(128)
+        VS_DIM(144) VS_DIM(160) VS_DIM(176) VS_DIM(192) VS_DIM(208) VS_DIM(224) VS_DIM(240)
+        VS_DIM(256)
+#undef VS_DIM
+    }
+    return hipErrorInvalidValue;
+}
+
+void fill_geometry(const vs_kv *kv, int64_t layer, AttendArgs &a) {
+    const int64_t e = kv_elem(kv->dtype);
+    a.pool = kv->mem;
+    a.page_bytes = kv->page_bytes;
+    a.head_off = kv->page_size * kv->head_dim * e;
+    a.kv_off = kv->kv_heads * a.head_off;
+    a.layer_off = layer * 2 * a.kv_off;
+}
+
+// |stride| elements of rows and heads stay inside 2^62 bytes
+bool stride_ok(int64_t s) { return s >= -((int64_t)1 << 40) && s <= ((int64_t)1 << 40); }
+
+bool pieces_ok(const void *p, int64_t s0, int64_t s1, int64_t e) {
+    return (((uintptr_t)p | (uintptr_t)(s0 * e) | (uintptr_t)(s1 * e)) & 15) == 0;
+}
+
+}  // namespace
+}  // namespace vs
+
+using vs::report;
+using vs::report_hip;
+
+extern "C" {
+
+int vs_kv_create(int device, int64_t npages, int64_t page_size, int64_t layers, int64_t kv_heads,
+                 int64_t head_dim, int dtype, void *memory, vs_kv **out) {
+    if (!out) return report(VS_ERR_INVALID, "null output handle");
+    *out = nullptr;
+    if (npages <= 0 || layers <= 0 || kv_heads <= 0)
+        return report(VS_ERR_INVALID, "npages, layers and kv_heads must be > 0");
+    if (dtype != VS_DTYPE_F32 && dtype != VS_DTYPE_BF16)
+        return report(VS_ERR_INVALID, "unknown dtype code %d", dtype);
+    if (page_size < 32 || page_size > 1024 || (page_size & (page_size - 1)))
+        return report(VS_ERR_INVALID, "page_size must be a power of two from 32 to 1024 (got %lld)",
+                      (long long)page_size);
+    if (head_dim <= 0 || head_dim % 16 || head_dim > 256)
+        return report(VS_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 up to 256 (got %lld)",
+                      (long long)head_dim);
+    if (npages > INT32_MAX || kv_heads > 4096 || layers > (1 << 20))
+        return report(VS_ERR_UNSUPPORTED, "more than 2^31 - 1 pages, 4096 heads or 2^20 layers");
+    if ((uintptr_t)memory % 16) return report(VS_ERR_INVALID, "memory is not 16-byte aligned");
+    const int64_t pb = layers * 2 * kv_heads * page_size * head_dim * vs::kv_elem(dtype);
+    if (pb > ((int64_t)1 << 46) / npages)
+        return report(VS_ERR_OOM, "%lld pages of %lld bytes", (long long)npages, (long long)pb);
+    int rc = vs::check_device(device);
+    if (rc) return rc;
+    vs::DeviceGuard g(device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    vs_kv *kv = new (std::nothrow) vs_kv();
+    if (!kv) return report(VS_ERR_OOM, "host allocation");
+    kv->device = device;
+    kv->npages = npages;
+    kv->page_size = page_size;
+    kv->layers = layers;
+    kv->kv_heads = kv_heads;
+    kv->head_dim = head_dim;
+    kv->dtype = dtype;
+    kv->page_bytes = pb;
+    kv->mem = (char *)memory;
+    int cus = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) == hipSuccess &&
+        cus > 0)
+        kv->num_cu = cus;
+    void *p = nullptr;
+    hipError_t e = vs::device_alloc(&p, vs::kStatusWords * sizeof(int32_t));
+    kv->status = (int32_t *)p;
+    if (e == hipSuccess) {
+        const int32_t zero[vs::kStatusWords] = {0};
+        e = hipMemcpy(p, zero, sizeof zero, hipMemcpyHostToDevice);
+    }
+    if (e == hipSuccess && !memory) {
+        e = vs::device_alloc(&p, (size_t)(npages * pb));
+        if (e == hipSuccess) {
+            kv->mem = (char *)p;
+            kv->owns_mem = true;
+        }
+    }
+    if (e != hipSuccess) {
+        if (kv->status) (void)hipFree(kv->status);
+        delete kv;
+        return report_hip(e, "cache memory");
+    }
+    *out = kv;
+    return VS_OK;
+}
+
+void vs_kv_destroy(vs_kv *kv) {
+    if (!kv) return;
+    vs::DeviceGuard g(kv->device);
+    (void)hipDeviceSynchronize();
+    kv->scratch.release();
+    if (kv->status) (void)hipFree(kv->status);
+    if (kv->owns_mem) (void)hipFree(kv->mem);
+    delete kv;
+}
+
+int64_t vs_kv_page_bytes(const vs_kv *kv) { return kv ? kv->page_bytes : 0; }
+void *vs_kv_memory(const vs_kv *kv) { return kv ? kv->mem : nullptr; }
+
+int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, const void *q,
+                 int64_t q_seq, int64_t q_head, const void *k, int64_t k_seq, int64_t k_head,
+                 const void *v, int64_t v_seq, int64_t v_head, void *out, int64_t out_seq,
+                 int64_t out_head, float *lse, float scale, int64_t window, int64_t sinks,
+                 void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, s);
+    if (rc) return rc;
+    if (layer < 0 || layer >= kv->layers)
+        return report(VS_ERR_INVALID, "layer %lld out of range [0, %lld)", (long long)layer,
+                      (long long)kv->layers);
+    if (heads <= 0 || heads % kv->kv_heads)
+        return report(VS_ERR_INVALID, "heads (%lld) must be a multiple of kv_heads (%lld)",
+                      (long long)heads, (long long)kv->kv_heads);
+    if (heads > (1 << 16)) return report(VS_ERR_UNSUPPORTED, "more than 65,536 heads");
+    if (!q || !out) return report(VS_ERR_INVALID, "null q or out");
+    if (!k != !v) return report(VS_ERR_INVALID, "k and v are given together or not at all");
+    if (window < 0 || sinks < 0) return report(VS_ERR_INVALID, "negative window or sinks");
+    if (!std::isfinite(scale)) return report(VS_ERR_INVALID, "scale is not finite");
+    const int64_t e = vs::kv_elem(kv->dtype);
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % e || (uintptr_t)lse % 4)
+        return report(VS_ERR_INVALID, "a buffer is not aligned to its elements");
+    for (int64_t x : {q_seq, q_head, k_seq, k_head, v_seq, v_head, out_seq, out_head})
+        if (!vs::stride_ok(x)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
+    if (s->nseq == 0) return VS_OK;
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipStream_t st = (hipStream_t)stream;
+
+    vs::AttendArgs a = {};
+    vs::fill_geometry(kv, layer, a);
+    a.table = s->table;
+    a.lens = s->lens;
+    a.width = s->width;
+    a.nseq = (int)s->nseq;
+    a.npages = (int)kv->npages;
+    a.page_shift = __builtin_ctzll((uint64_t)kv->page_size);
+    a.q = (const char *)q;
+    a.k = (const char *)k;
+    a.v = (const char *)v;
+    a.out = (char *)out;
+    a.q_seq = q_seq;
+    a.q_head = q_head;
+    a.k_seq = k_seq;
+    a.k_head = k_head;
+    a.v_seq = v_seq;
+    a.v_head = v_head;
+    a.o_seq = out_seq;
+    a.o_head = out_head;
+    a.lse = lse;
+    a.heads = (int)heads;
+    a.kv_heads = (int)kv->kv_heads;
+    a.group = (int)(heads / kv->kv_heads);
+    a.gtiles = (a.group + 15) / 16;
+    a.scale2 = scale * vs::kLog2e;
+    a.window = (int)std::min<int64_t>(window, INT32_MAX);
+    a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX);
+    a.q_vec = vs::pieces_ok(q, q_seq, q_head, e);
+    a.k_vec = vs::pieces_ok(k, k_seq, k_head, e);
+
+    // Work items: as many as fill the card, and one more per sequence at most
+    // for the division's remainders.
+    const int64_t per_item = (int64_t)a.kv_heads * a.gtiles;
+    const int64_t target = std::max<int64_t>(1, (4 * kv->num_cu + per_item - 1) / per_item);
+    // the most blocks that a sequence of this table can have
+    int64_t most = s->width * (kv->page_size / vs::kKvBlock);
+    if (window > 0)
+        most = std::min(most, (window + vs::kKvBlock - 1) / vs::kKvBlock + 1 +
+                                  (sinks + vs::kKvBlock - 1) / vs::kKvBlock);
+    const int64_t splits = std::max<int64_t>(1, (most + vs::kMinBlocks - 1) / vs::kMinBlocks);
+    a.target_items = (int)target;
+    const int64_t items = std::min(target + s->nseq, splits * s->nseq);
+    const bool join = splits > 1;
+    if (items * per_item > INT32_MAX)
+        return report(VS_ERR_UNSUPPORTED, "%lld sequences of %lld heads", (long long)s->nseq,
+                      (long long)heads);
+    void *ws = nullptr;
+    const int64_t slots = join ? items * heads : 0;
+    const size_t o_bytes = (size_t)slots * kv->head_dim * sizeof(float);
+    const size_t ml_bytes = (size_t)slots * sizeof(float2);
+    rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)s->nseq * sizeof(int2), &ws);
+    if (rc) return rc;
+    a.part_o = (float *)ws;
+    a.part_ml = (float2 *)((char *)ws + o_bytes);
+    a.first = (int2 *)((char *)ws + o_bytes + ml_bytes);
+    hipError_t err = kv->dtype == VS_DTYPE_BF16
+                         ? vs::launch_attend_dim<1>(a, items, join, (int)kv->head_dim, st)
+                         : vs::launch_attend_dim<0>(a, items, join, (int)kv->head_dim, st);
+    if (err != hipSuccess) return report_hip(err, "attend");
+    return VS_OK;
+}
+
+static int fill_rows(const vs_kv *kv, const vs_kv_seqs *s, int64_t layer, vs::RowsArgs &a) {
+    if (layer < 0 || layer >= kv->layers)
+        return report(VS_ERR_INVALID, "layer %lld out of range [0, %lld)", (long long)layer,
+                      (long long)kv->layers);
+    vs::AttendArgs geo = {};
+    vs::fill_geometry(kv, layer, geo);
+    a.pool = geo.pool;
+    a.page_bytes = geo.page_bytes;
+    a.layer_off = geo.layer_off;
+    a.kv_off = geo.kv_off;
+    a.head_off = geo.head_off;
+    a.table = s->table;
+    a.lens = s->lens;
+    a.width = s->width;
+    a.nseq = (int)s->nseq;
+    a.npages = (int)kv->npages;
+    a.page_shift = __builtin_ctzll((uint64_t)kv->page_size);
+    a.heads = (int)kv->kv_heads;
+    a.dim = (int)kv->head_dim;
+    return VS_OK;
+}
+
+int vs_kv_append(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, const void *k, int64_t k_row,
+                 int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
+                 const int32_t *starts, int64_t nrows, void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, s);
+    if (rc) return rc;
+    vs::RowsArgs a = {};
+    rc = fill_rows(kv, s, layer, a);
+    if (rc) return rc;
+    if (nrows < 0 || (!starts && nrows != s->nseq))
+        return report(VS_ERR_INVALID, "nrows %lld: without starts, one row per sequence",
+                      (long long)nrows);
+    for (int64_t x : {k_row, k_head, v_row, v_head})
+        if (!vs::stride_ok(x)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
+    if (nrows == 0 || s->nseq == 0) return VS_OK;
+    if (!k || !v) return report(VS_ERR_INVALID, "null k or v");
+    if (((uintptr_t)k | (uintptr_t)v) % vs::kv_elem(kv->dtype) || (uintptr_t)starts % 4)
+        return report(VS_ERR_INVALID, "a buffer is not aligned to its elements");
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    a.starts = starts;
+    a.nrows = nrows;
+    a.k = (const char *)k;
+    a.v = (const char *)v;
+    a.k_row = k_row;
+    a.k_head = k_head;
+    a.v_row = v_row;
+    a.v_head = v_head;
+    const dim3 grid((uint32_t)std::min<int64_t>(nrows, 65536));
+    if (kv->dtype == VS_DTYPE_BF16)
+        hipLaunchKernelGGL(vs::append_kernel<1>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL(vs::append_kernel<0>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipError_t e = hipGetLastError();
+    return e == hipSuccess ? VS_OK : report_hip(e, "append");
+}
+
+int vs_kv_read(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t b, int64_t first, int64_t n,
+               void *k_out, void *v_out, void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, s);
+    if (rc) return rc;
+    vs::RowsArgs a = {};
+    rc = fill_rows(kv, s, layer, a);
+    if (rc) return rc;
+    if (b < 0 || b >= s->nseq)
+        return report(VS_ERR_INVALID, "sequence %lld out of range [0, %lld)", (long long)b,
+                      (long long)s->nseq);
+    if (first < 0 || n < 0 || first > INT32_MAX - n)
+        return report(VS_ERR_INVALID, "positions [%lld, %lld)", (long long)first,
+                      (long long)(first + n));
+    if (n == 0) return VS_OK;
+    if (!k_out || !v_out) return report(VS_ERR_INVALID, "null k_out or v_out");
+    if (((uintptr_t)k_out | (uintptr_t)v_out) % vs::kv_elem(kv->dtype))
+        return report(VS_ERR_INVALID, "a buffer is not aligned to its elements");
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    a.nrows = n;
+    a.b = (int)b;
+    a.first = (int)first;
+    a.k_out = (char *)k_out;
+    a.v_out = (char *)v_out;
+    const dim3 grid((uint32_t)std::min<int64_t>(n, 65536));
+    if (kv->dtype == VS_DTYPE_BF16)
+        hipLaunchKernelGGL(vs::read_kernel<1>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL(vs::read_kernel<0>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipError_t e = hipGetLastError();
+    return e == hipSuccess ? VS_OK : report_hip(e, "read");
+}
+
+}  // extern "C"

@@ -1,0 +1,90 @@
+// vs_host.h -- host helpers shared by the sources that hold entry points.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "../../include/vs_hip.h"
+
+namespace vs {
+
+// Sets the calling thread's error text and returns `code`.
+int report(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+// The same for a failed runtime call.
+int report_hip(hipError_t e, const char *what);
+// hipMalloc that takes idle row copies of indexes back when the device is full.
+hipError_t device_alloc(void **p, size_t bytes);
+
+// Restores the caller's current device on scope exit.
+struct DeviceGuard {
+    int prev = -1, dev;
+    hipError_t err = hipSuccess;
+    explicit DeviceGuard(int device) : dev(device) {
+        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+        if (prev != dev) err = hipSetDevice(dev);
+    }
+    ~DeviceGuard() {
+        if (prev >= 0 && prev != dev) (void)hipSetDevice(prev);
+    }
+};
+
+// Scratch memory of a handle, one buffer per stream, so that calls on
+// different streams never share one.  A buffer that is outgrown is kept until
+// the handle ends: a recorded graph may still use it.
+struct StreamScratch {
+    struct Buf {
+        hipStream_t st;
+        void *p;
+        size_t bytes;
+    };
+    std::vector<Buf> bufs;
+
+    int get(hipStream_t st, size_t need, void **out) {
+        for (auto it = bufs.rbegin(); it != bufs.rend(); ++it)
+            if (it->st == st) {
+                if (it->bytes < need) break;
+                *out = it->p;
+                return VS_OK;
+            }
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(st, &cap) != hipSuccess) {
+            (void)hipGetLastError();
+            cap = hipStreamCaptureStatusNone;
+        }
+        if (cap != hipStreamCaptureStatusNone)
+            return report(VS_ERR_UNSUPPORTED,
+                          "scratch memory has to grow: run this call once before recording it");
+        size_t bytes = 1 << 16;
+        while (bytes < need) bytes *= 2;
+        void *p = nullptr;
+        hipError_t e = device_alloc(&p, bytes);
+        if (e != hipSuccess) return report_hip(e, "scratch memory");
+        try {
+            bufs.push_back({st, p, bytes});
+        } catch (const std::bad_alloc &) {
+            (void)hipFree(p);
+            return report(VS_ERR_OOM, "host allocation");
+        }
+        *out = p;
+        return VS_OK;
+    }
+    void release() {
+        for (auto &b : bufs) (void)hipFree(b.p);
+        bufs.clear();
+    }
+};
+
+// The device exists; VS_OK or the error.
+inline int check_device(int device) {
+    int count = 0;
+    if (hipGetDeviceCount(&count) != hipSuccess || count <= 0)
+        return report(VS_ERR_NO_DEVICE, "no HIP device visible");
+    if (device < 0 || device >= count)
+        return report(VS_ERR_INVALID, "device %d out of range [0, %d)", device, count);
+    return VS_OK;
+}
+
+}  // namespace vs

@@ -38,6 +38,11 @@ __host__ __device__ inline float bf16_to_f32(uint16_t h) {
 
 namespace vs {
 
+// Bits of a value taken by value: __builtin_bit_cast of an element of an
+// ext_vector (x[i]) reads element 0 whatever i is.
+__host__ __device__ inline float float_of(uint32_t u) { return __builtin_bit_cast(float, u); }
+__host__ __device__ inline uint32_t bits_of(float f) { return __builtin_bit_cast(uint32_t, f); }
+
 // ---------------------------------------------------------------------------
 // Kernel-side argument blocks
 // ---------------------------------------------------------------------------

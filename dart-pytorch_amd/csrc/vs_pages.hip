@@ -1,0 +1,560 @@
+// vs_pages.hip -- the pages of the key-value cache: extending (with copies on
+// write), forking, freeing, evicting, compacting and copying.  The tables,
+// lengths and reference counts live on the device, so a decoding loop never
+// waits for the host to manage them.
+#include "vs_kv.h"
+
+namespace vs {
+namespace {
+
+constexpr int kPlan = 1024;         // threads of the one-workgroup plans
+constexpr int kMostFresh = 1 << 20;  // pages that one extend gives a sequence
+constexpr int kPieceBytes = 16384;  // of a page, per workgroup pass of the copy
+
+// Exclusive prefix sum of x over the workgroup's kPlan threads; *total its sum.
+__device__ __forceinline__ int block_scan(int x, int *total, int *lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = incl;
+    __syncthreads();
+    if (wave == 0) {
+        int w = lane < kPlan / 64 ? lds[lane] : 0;
+#pragma unroll
+        for (int d = 1; d < kPlan / 64; d <<= 1) {
+            const int o = __shfl_up(w, d);
+            if (lane >= d) w += o;
+        }
+        if (lane < kPlan / 64) lds[lane] = w;
+    }
+    __syncthreads();
+    *total = lds[kPlan / 64 - 1];
+    return incl - x + (wave ? lds[wave - 1] : 0);
+}
+
+struct ExtendArgs {
+    int32_t *table, *lens, *refs;
+    int64_t width;
+    int nseq, npages, page_shift, count;
+    const int32_t *count_dev;
+    int32_t *status;
+    int32_t *holders, *lowest;  // [npages], used where a shared last page is
+    int32_t *offset;            // [nseq] place of a sequence's first new page | copies (bit 31)
+    int32_t *fresh;             // [npages] free pages, lowest first
+    int32_t *copies;            // [0] how many, then pairs (from, to)
+};
+
+// Divides the free pages among the sequences, as one workgroup: the work is a
+// few thousand numbers, and its steps need each other's results.
+__global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
+    __shared__ int lds[kPlan / 64];
+    __shared__ int bad, huge;
+    const int P = 1 << a.page_shift;
+    const int64_t most = a.width << a.page_shift;
+    if (threadIdx.x == 0) {
+        bad = huge = 0;
+        a.copies[0] = 0;
+    }
+    // the last page of a sequence, where it is partly filled and others hold it too
+    auto count_of = [&](int b) { return max(a.count_dev ? a.count_dev[b] : a.count, 0); };
+    auto shared_page = [&](int b, int n) {
+        if (!(n & (P - 1)) || n > most || !count_of(b)) return -1;
+        const int p = a.table[(int64_t)b * a.width + ((n - 1) >> a.page_shift)];
+        return (unsigned)p < (unsigned)a.npages && a.refs[p] > 1 ? p : -1;
+    };
+    for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
+        const int p = shared_page(b, max(a.lens[b], 0));
+        if (p >= 0) {
+            a.holders[p] = 0;
+            a.lowest[p] = INT32_MAX;
+        }
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
+        const int p = shared_page(b, max(a.lens[b], 0));
+        if (p >= 0) {
+            atomicAdd(&a.holders[p], 1);
+            atomicMin(&a.lowest[p], b);
+        }
+    }
+    __syncthreads();
+    int64_t need = 0;  // (equal in all threads)
+    for (int b0 = 0; b0 < a.nseq; b0 += kPlan) {
+        const int b = b0 + threadIdx.x;
+        int want = 0, copy = 0;
+        if (b < a.nseq) {
+            const int n = max(a.lens[b], 0), c = count_of(b);
+            if (c && (int64_t)n + c > most) {
+                bad = 1;
+            } else if (c) {
+                const int p = shared_page(b, n);
+                copy = p >= 0 && !(a.lowest[p] == b && a.holders[p] == a.refs[p]);
+                want = copy + (int)(((int64_t)n + c + P - 1) >> a.page_shift) -
+                       (int)(((int64_t)n + P - 1) >> a.page_shift);
+                if (want > min(a.npages, kMostFresh)) huge = 1;  // refused: no sum below passes 32 bits
+                want = min(want, kMostFresh);
+            }
+        }
+        int total;
+        const int at = block_scan(want, &total, lds);
+        if (b < a.nseq)
+            a.offset[b] = (int)min(need + at, (int64_t)INT32_MAX) | (copy ? (int)0x80000000 : 0);
+        need += total;
+    }
+    __syncthreads();
+    if (bad) {
+        if (threadIdx.x == 0) atomicOr(&a.status[0], kStatusWidth);
+        return;
+    }
+    if (need == 0) {  // everyone has room
+        for (int b = threadIdx.x; b < a.nseq; b += kPlan) a.lens[b] = max(a.lens[b], 0) + count_of(b);
+        return;
+    }
+    // the lowest `need` free pages
+    int64_t found = 0;
+    for (int64_t p0 = 0; p0 < a.npages && found < need; p0 += 4 * kPlan) {
+        int free[4], cnt = 0;
+        const int64_t p = p0 + 4 * threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            free[i] = p + i < a.npages && a.refs[p + i] == 0;
+            cnt += free[i];
+        }
+        int total, at = block_scan(cnt, &total, lds);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (free[i]) {
+                if (found + at < need) a.fresh[found + at] = (int)(p + i);
+                ++at;
+            }
+        found += total;
+    }
+    if (found < need || huge) {
+        if (threadIdx.x == 0) {
+            atomicOr(&a.status[0], kStatusPages);
+            atomicMax(&a.status[1], (int)min(max(need - found, (int64_t)1), (int64_t)INT32_MAX));
+        }
+        return;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
+        const int n = max(a.lens[b], 0), c = count_of(b);
+        if (!c) continue;
+        int at = a.offset[b] & 0x7FFFFFFF;
+        int32_t *row = a.table + (int64_t)b * a.width;
+        if (a.offset[b] < 0) {
+            int32_t *entry = &row[(n - 1) >> a.page_shift];
+            const int from = *entry, to = a.fresh[at++];
+            const int i = atomicAdd(&a.copies[0], 1);  // (their order does not matter)
+            a.copies[1 + 2 * i] = from;
+            a.copies[2 + 2 * i] = to;
+            atomicSub(&a.refs[from], 1);
+            a.refs[to] = 1;
+            *entry = to;
+        }
+        const int64_t end = ((int64_t)n + c + P - 1) >> a.page_shift;
+        for (int64_t e = ((int64_t)n + P - 1) >> a.page_shift; e < end; ++e) {
+            const int to = a.fresh[at++];
+            a.refs[to] = 1;
+            row[e] = to;
+        }
+        a.lens[b] = n + c;
+    }
+}
+
+// Copies pages: HBM-bound, so only the 16-byte loads in flight matter.  The
+// grid walks (page, piece) pairs; `n_dev` is read on the device because the
+// host does not know how many pages a plan moves.
+__global__ __launch_bounds__(256) void copy_pages_kernel(char *pool, int64_t page_bytes, int npages,
+                                                         const int32_t *n_dev, int64_t n_host,
+                                                         const int32_t *from, const int32_t *to,
+                                                         int stride) {
+    const int64_t n = n_dev ? *n_dev : n_host;
+    const int64_t pieces = (page_bytes + kPieceBytes - 1) / kPieceBytes;
+    for (int64_t w = blockIdx.x; w < n * pieces; w += gridDim.x) {
+        const int64_t i = w / pieces, x0 = w % pieces * kPieceBytes;
+        const int f = from[i * stride], t = to[i * stride];
+        if ((unsigned)f >= (unsigned)npages || (unsigned)t >= (unsigned)npages) continue;
+        const char *src = pool + f * page_bytes + x0;
+        char *dst = pool + t * page_bytes + x0;
+        const int bytes = (int)min((int64_t)kPieceBytes, page_bytes - x0);
+        u32x4_t v[kPieceBytes / 4096];
+#pragma unroll
+        for (int k = 0; k < kPieceBytes / 4096; ++k) {
+            const int x = k * 4096 + threadIdx.x * 16;
+            if (x < bytes) v[k] = *(const u32x4_t *)(src + x);
+        }
+#pragma unroll
+        for (int k = 0; k < kPieceBytes / 4096; ++k) {
+            const int x = k * 4096 + threadIdx.x * 16;
+            if (x < bytes) *(u32x4_t *)(dst + x) = v[k];
+        }
+    }
+}
+
+struct ForkArgs {
+    const int32_t *table, *lens, *parents;
+    int32_t *table2, *lens2, *refs;
+    int64_t width;
+    int nin, nout, npages;
+    int32_t *status;
+};
+
+__global__ __launch_bounds__(256) void copy_words_kernel(const int32_t *in, int32_t *out, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+        out[i] = in[i];
+}
+
+// One workgroup per sequence of either side.  References are whole numbers,
+// so the order of the atomics changes nothing.
+__global__ __launch_bounds__(256) void fork_kernel(ForkArgs a) {
+    __shared__ int part[4];
+    for (int w = blockIdx.x; w < a.nin + a.nout; w += gridDim.x) {
+        if (w < a.nout) {
+            int parent = a.parents[w];
+            const bool ok = (unsigned)parent < (unsigned)a.nin;
+            if (!ok && parent != -1 && threadIdx.x == 0) atomicOr(&a.status[0], kStatusParent);
+            for (int64_t x = threadIdx.x; x < a.width; x += 256)
+                a.table2[w * a.width + x] = ok ? a.table[parent * a.width + x] : -1;
+            if (threadIdx.x == 0) a.lens2[w] = ok ? a.lens[parent] : 0;
+        } else {
+            const int b = w - a.nout;
+            int c = 0;
+            for (int i = threadIdx.x; i < a.nout; i += 256) c += a.parents[i] == b;
+#pragma unroll
+            for (int d = 32; d; d >>= 1) c += __shfl_xor(c, d);
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = c;
+            __syncthreads();
+            c = part[0] + part[1] + part[2] + part[3] - 1;
+            if (c)
+                for (int64_t x = threadIdx.x; x < a.width; x += 256) {
+                    const int p = a.table[b * a.width + x];
+                    if ((unsigned)p < (unsigned)a.npages) atomicAdd(&a.refs[p], c);
+                }
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void free_kernel(int32_t *table, int32_t *lens, int32_t *refs,
+                                                   int64_t width, int nseq, int npages,
+                                                   const int32_t *ids, int64_t n) {
+    for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
+        const int b = ids ? ids[w] : (int)w;
+        if ((unsigned)b >= (unsigned)nseq) continue;
+        for (int64_t x = threadIdx.x; x < width; x += 256) {
+            // (whoever takes the entry gives its reference back: once)
+            const int p = atomicExch(&table[b * width + x], -1);
+            if ((unsigned)p < (unsigned)npages) atomicSub(&refs[p], 1);
+        }
+        if (threadIdx.x == 0) lens[b] = 0;
+    }
+}
+
+__global__ __launch_bounds__(256) void evict_kernel(int32_t *table, const int32_t *lens,
+                                                    int32_t *refs, int64_t width, int nseq,
+                                                    int npages, int page_shift, int64_t window,
+                                                    int64_t sinks) {
+    for (int b = blockIdx.x; b < nseq; b += gridDim.x) {
+        // pages [lo, hi) hold no visible position, now or later
+        const int64_t size = (int64_t)1 << page_shift;
+        const int64_t lo = (min(sinks, (int64_t)1 << 31) + size - 1) >> page_shift;
+        const int64_t hi = min((lens[b] - window) >> page_shift, width);
+        for (int64_t x = lo + threadIdx.x; x < hi; x += 256) {
+            const int p = table[b * width + x];
+            if ((unsigned)p < (unsigned)npages) {
+                atomicSub(&refs[p], 1);
+                table[b * width + x] = -1;
+            }
+        }
+    }
+}
+
+struct CompactArgs {
+    const int32_t *refs;
+    int32_t *refs2;
+    int npages;
+    int32_t *map;      // [npages] where a page goes
+    int32_t *from, *to;
+    int32_t *moves;    // how many
+};
+
+// Live pages past the front and free pages in it, paired in order.
+__global__ __launch_bounds__(kPlan) void compact_plan_kernel(CompactArgs a) {
+    __shared__ int lds[kPlan / 64];
+    const int64_t step = 4 * kPlan;
+    int64_t live = 0;
+    for (int64_t p0 = 0; p0 < a.npages; p0 += step) {
+        int cnt = 0;
+        const int64_t p = p0 + 4 * threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cnt += p + i < a.npages && a.refs[p + i] != 0;
+        int total;
+        block_scan(cnt, &total, lds);
+        live += total;
+    }
+    int nto = 0, nfrom = 0;
+    for (int64_t p0 = 0; p0 < a.npages; p0 += step) {
+        int ref[4], cnt = 0;
+        const int64_t p = p0 + 4 * threadIdx.x;
+        // free pages of the front count 1, live pages past it 2^16: both are at most 4096 here
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ref[i] = p + i < a.npages ? a.refs[p + i] : 0;
+            if (p + i >= a.npages) continue;
+            if (p + i < live)
+                cnt += ref[i] == 0;
+            else
+                cnt += (ref[i] != 0) << 16;
+        }
+        int total;
+        const int at = block_scan(cnt, &total, lds);
+        int t = nto + (at & 0xFFFF), f = nfrom + (at >> 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (p + i >= a.npages) continue;
+            a.map[p + i] = (int)(p + i);
+            if (p + i < live) {
+                a.refs2[p + i] = ref[i];
+                if (ref[i] == 0) a.to[t++] = (int)(p + i);
+            } else {
+                if (ref[i] != 0) a.from[f++] = (int)(p + i);
+            }
+        }
+        nto += total & 0xFFFF;
+        nfrom += total >> 16;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nto; i += kPlan) {
+        const int f = a.from[i], t = a.to[i];
+        a.map[f] = t;
+        a.refs2[t] = a.refs[f];
+    }
+    __syncthreads();
+    for (int64_t p = live + threadIdx.x; p < a.npages; p += kPlan) a.refs2[p] = 0;
+    if (threadIdx.x == 0) *a.moves = nto;
+}
+
+__global__ __launch_bounds__(256) void compact_table_kernel(const int32_t *table, const int32_t *lens,
+                                                            int32_t *table2, int32_t *lens2,
+                                                            const int32_t *map, int npages,
+                                                            int64_t entries, int nseq) {
+    const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (int64_t x = first; x < entries; x += step) {
+        const int p = table[x];
+        table2[x] = (unsigned)p < (unsigned)npages ? map[p] : p;
+    }
+    for (int64_t b = first; b < nseq; b += step) lens2[b] = lens[b];
+}
+
+hipError_t launch_copy(const vs_kv *kv, const int32_t *n_dev, int64_t n_max, const int32_t *from,
+                       const int32_t *to, int stride, hipStream_t st) {
+    const int64_t pieces = (kv->page_bytes + kPieceBytes - 1) / kPieceBytes;
+    const int64_t wgs = std::min<int64_t>((int64_t)kv->num_cu * 8, n_max * pieces);
+    if (wgs <= 0) return hipSuccess;
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((uint32_t)wgs), dim3(256), 0, st, kv->mem,
+                       kv->page_bytes, (int)kv->npages, n_dev, n_max, from, to, stride);
+    return hipGetLastError();
+}
+
+uint32_t grid_of(int64_t n, int64_t most) { return (uint32_t)std::max<int64_t>(1, std::min(n, most)); }
+
+}  // namespace
+}  // namespace vs
+
+using vs::report;
+using vs::report_hip;
+
+#define VS_LAUNCHED(what)                                   \
+    do {                                                    \
+        hipError_t e_ = hipGetLastError();                  \
+        if (e_ != hipSuccess) return report_hip(e_, what);  \
+    } while (0)
+
+extern "C" {
+
+int vs_kv_extend(vs_kv *kv, const vs_kv_seqs *s, int64_t count, const int32_t *count_dev,
+                 void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, s);
+    if (rc) return rc;
+    if (!count_dev && (count < 0 || count > INT32_MAX))
+        return report(VS_ERR_INVALID, "count %lld", (long long)count);
+    if ((uintptr_t)count_dev % 4) return report(VS_ERR_INVALID, "counts are not aligned");
+    if (s->nseq == 0 || (!count_dev && count == 0)) return VS_OK;
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t np = kv->npages, ns = s->nseq;
+    void *ws = nullptr;
+    rc = kv->scratch.get(st, (size_t)(3 * np + 3 * ns + 1) * sizeof(int32_t), &ws);
+    if (rc) return rc;
+    vs::ExtendArgs a = {};
+    a.table = s->table;
+    a.lens = s->lens;
+    a.refs = s->refs;
+    a.width = s->width;
+    a.nseq = (int)ns;
+    a.npages = (int)np;
+    a.page_shift = __builtin_ctzll((uint64_t)kv->page_size);
+    a.count = (int)count;
+    a.count_dev = count_dev;
+    a.status = kv->status;
+    a.holders = (int32_t *)ws;
+    a.lowest = a.holders + np;
+    a.fresh = a.lowest + np;
+    a.offset = a.fresh + np;
+    a.copies = a.offset + ns;
+    hipLaunchKernelGGL(vs::extend_plan_kernel, dim3(1), dim3(vs::kPlan), 0, st, a);
+    VS_LAUNCHED("extend");
+    hipError_t e = vs::launch_copy(kv, a.copies, ns, a.copies + 1, a.copies + 2, 2, st);
+    return e == hipSuccess ? VS_OK : report_hip(e, "page copies");
+}
+
+int vs_kv_fork(vs_kv *kv, const vs_kv_seqs *in, const int32_t *parents, const vs_kv_seqs *out,
+               void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, in);
+    if (!rc) rc = vs::check_seqs(kv, out);
+    if (rc) return rc;
+    if (in->width != out->width)
+        return report(VS_ERR_INVALID, "tables of %lld and %lld columns", (long long)in->width,
+                      (long long)out->width);
+    if (in->lens == out->lens || (in->table == out->table && in->width))
+        return report(VS_ERR_INVALID, "fork needs another table and other lens to write to");
+    if ((out->nseq && !parents) || (uintptr_t)parents % 4)
+        return report(VS_ERR_INVALID, "null or unaligned parents");
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipStream_t st = (hipStream_t)stream;
+    if (in->refs != out->refs) {
+        hipLaunchKernelGGL(vs::copy_words_kernel, dim3(vs::grid_of((kv->npages + 255) / 256, 2048)),
+                           dim3(256), 0, st, in->refs, out->refs, kv->npages);
+        VS_LAUNCHED("fork");
+    }
+    if (in->nseq + out->nseq == 0) return VS_OK;
+    vs::ForkArgs a = {};
+    a.table = in->table;
+    a.lens = in->lens;
+    a.parents = parents;
+    a.table2 = out->table;
+    a.lens2 = out->lens;
+    a.refs = out->refs;
+    a.width = in->width;
+    a.nin = (int)in->nseq;
+    a.nout = (int)out->nseq;
+    a.npages = (int)kv->npages;
+    a.status = kv->status;
+    hipLaunchKernelGGL(vs::fork_kernel, dim3(vs::grid_of(in->nseq + out->nseq, 65536)), dim3(256), 0,
+                       st, a);
+    VS_LAUNCHED("fork");
+    return VS_OK;
+}
+
+int vs_kv_free(vs_kv *kv, const vs_kv_seqs *s, const int32_t *ids, int64_t n, void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, s);
+    if (rc) return rc;
+    if (ids && n < 0) return report(VS_ERR_INVALID, "n %lld", (long long)n);
+    if ((uintptr_t)ids % 4) return report(VS_ERR_INVALID, "ids are not aligned");
+    if (!ids) n = s->nseq;
+    if (n == 0 || s->nseq == 0) return VS_OK;
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipLaunchKernelGGL(vs::free_kernel, dim3(vs::grid_of(n, 65536)), dim3(256), 0,
+                       (hipStream_t)stream, s->table, s->lens, s->refs, s->width, (int)s->nseq,
+                       (int)kv->npages, ids, n);
+    VS_LAUNCHED("free");
+    return VS_OK;
+}
+
+int vs_kv_evict(vs_kv *kv, const vs_kv_seqs *s, int64_t window, int64_t sinks, void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, s);
+    if (rc) return rc;
+    if (window <= 0 || sinks < 0)
+        return report(VS_ERR_INVALID, "evict needs a window > 0 and sinks >= 0");
+    if (s->nseq == 0 || window > INT32_MAX) return VS_OK;
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipLaunchKernelGGL(vs::evict_kernel, dim3(vs::grid_of(s->nseq, 65536)), dim3(256), 0,
+                       (hipStream_t)stream, s->table, s->lens, s->refs, s->width, (int)s->nseq,
+                       (int)kv->npages, __builtin_ctzll((uint64_t)kv->page_size), window, sinks);
+    VS_LAUNCHED("evict");
+    return VS_OK;
+}
+
+int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out, void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, in);
+    if (!rc) rc = vs::check_seqs(kv, out);
+    if (rc) return rc;
+    if (in->width != out->width || in->nseq != out->nseq)
+        return report(VS_ERR_INVALID, "compact: in and out differ in shape");
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t np = kv->npages;
+    void *ws = nullptr;
+    rc = kv->scratch.get(st, (size_t)(3 * np + 1) * sizeof(int32_t), &ws);
+    if (rc) return rc;
+    vs::CompactArgs a = {};
+    a.refs = in->refs;
+    a.refs2 = out->refs;
+    a.npages = (int)np;
+    a.map = (int32_t *)ws;
+    a.from = a.map + np;
+    a.to = a.from + np;
+    a.moves = a.to + np;
+    hipLaunchKernelGGL(vs::compact_plan_kernel, dim3(1), dim3(vs::kPlan), 0, st, a);
+    VS_LAUNCHED("compact");
+    const int64_t entries = in->nseq * in->width;
+    if (in->nseq) {
+        hipLaunchKernelGGL(vs::compact_table_kernel,
+                           dim3(vs::grid_of((std::max(entries, in->nseq) + 255) / 256, 2048)),
+                           dim3(256), 0, st, in->table, in->lens, out->table, out->lens, a.map,
+                           (int)np, entries, (int)in->nseq);
+        VS_LAUNCHED("compact");
+    }
+    hipError_t e = vs::launch_copy(kv, a.moves, np / 2 + 1, a.from, a.to, 1, st);
+    return e == hipSuccess ? VS_OK : report_hip(e, "page copies");
+}
+
+int vs_kv_copy(vs_kv *kv, const int32_t *from, const int32_t *to, int64_t n, void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    if (n < 0) return report(VS_ERR_INVALID, "n %lld", (long long)n);
+    if (n == 0) return VS_OK;
+    if (!from || !to || ((uintptr_t)from | (uintptr_t)to) % 4)
+        return report(VS_ERR_INVALID, "null or unaligned page lists");
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipError_t e = vs::launch_copy(kv, nullptr, n, from, to, 1, (hipStream_t)stream);
+    return e == hipSuccess ? VS_OK : report_hip(e, "page copies");
+}
+
+int vs_kv_check(vs_kv *kv, void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipStream_t st = (hipStream_t)stream;
+    int32_t got[vs::kStatusWords] = {0};
+    hipError_t e = hipStreamSynchronize(st);
+    if (e == hipSuccess) e = hipMemcpy(got, kv->status, sizeof got, hipMemcpyDeviceToHost);
+    const int32_t zero[vs::kStatusWords] = {0};
+    if (e == hipSuccess && got[0])
+        e = hipMemcpy(kv->status, zero, sizeof zero, hipMemcpyHostToDevice);
+    if (e != hipSuccess) return report_hip(e, "check");
+    if (got[0] & vs::kStatusPages)
+        return report(VS_ERR_OOM, "the cache was %d pages short", (int)got[1]);
+    if (got[0] & vs::kStatusWidth)
+        return report(VS_ERR_INVALID, "a sequence outgrew its %s", "table row");
+    if (got[0] & vs::kStatusParent) return report(VS_ERR_INVALID, "a parent is out of range");
+    return VS_OK;
+}
+
+}  // extern "C"

@@ -42,6 +42,10 @@ EXPORTED = [
     "vs_device_count",
     "vs_device_name", "vs_gen_normal", "vs_prof_enable", "vs_prof_get", "vs_prof_reset",
     "vs_index_sync", "vs_index_set_option",
+    "vs_kv_create", "vs_kv_destroy", "vs_kv_page_bytes", "vs_kv_memory", "vs_kv_attend",
+    "vs_kv_append", "vs_kv_read", "vs_kv_extend", "vs_kv_fork", "vs_kv_free", "vs_kv_evict",
+    "vs_kv_compact", "vs_kv_copy", "vs_kv_check",
+    "vs_beam_create", "vs_beam_destroy", "vs_beam_select", "vs_beam_reorder",
 ]
 
 
@@ -141,6 +145,25 @@ def load() -> ctypes.CDLL:
         "vs_prof_reset": ([p], i32),
         "vs_index_sync": ([p], i32),
         "vs_index_set_option": ([p, ctypes.c_char_p, i64], i32),
+        "vs_kv_create": ([i32, i64, i64, i64, i64, i64, i32, p, pp], i32),
+        "vs_kv_destroy": ([p], None),
+        "vs_kv_page_bytes": ([p], i64),
+        "vs_kv_memory": ([p], p),
+        "vs_kv_attend": ([p, p, i64, i64] + [p, i64, i64] * 4
+                         + [p, ctypes.c_float, i64, i64, p], i32),
+        "vs_kv_append": ([p, p, i64, p, i64, i64, p, i64, i64, p, i64, p], i32),
+        "vs_kv_read": ([p, p, i64, i64, i64, i64, p, p, p], i32),
+        "vs_kv_extend": ([p, p, i64, p, p], i32),
+        "vs_kv_fork": ([p, p, p, p, p], i32),
+        "vs_kv_free": ([p, p, p, i64, p], i32),
+        "vs_kv_evict": ([p, p, i64, i64, p], i32),
+        "vs_kv_compact": ([p, p, p, p], i32),
+        "vs_kv_copy": ([p, p, p, i64, p], i32),
+        "vs_kv_check": ([p, p], i32),
+        "vs_beam_create": ([i32, pp], i32),
+        "vs_beam_destroy": ([p], None),
+        "vs_beam_select": ([p, p, i32, i64, i64, i64, i64, p, p, i64, i64, p, p, p, p, p], i32),
+        "vs_beam_reorder": ([p, p, i64, p, i64, i64, p, i64, i64, p, p], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

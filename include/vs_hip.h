@@ -209,6 +209,155 @@ VS_API int vs_kmeans_step(vs_index *points, const float *centroids_in, int64_t K
                           int64_t min_points, const double *jitter_u, int64_t njitter,
                           int32_t *assign, float *centroids_out, int32_t *counts, double *obj);
 
+/* ---- decoding: a paged key-value cache and beam search ----
+ *
+ * No counterpart in the reference's vector store: what a model needs on the
+ * GPU to answer with the passages that a search found, one token at a time.
+ *
+ * These calls differ from the index's in one way: they work on device
+ * buffers only, run on the caller's stream (`stream` is a hipStream_t, 0 the
+ * default stream) and return without waiting for it.  Arguments that the
+ * host can see are checked before anything is launched; what only the device
+ * sees (table entries, lengths, parents) is checked by the kernels and told
+ * by vs_kv_check.  Scratch memory is kept per handle and stream and grows at
+ * a first call of a size: a call that is recorded into a graph and would
+ * have to allocate is refused (VS_ERR_UNSUPPORTED; run it once before).
+ *
+ * The cache is npages pages of page_size positions; a page holds the keys and
+ * values of consecutive positions of one sequence, of every layer and
+ * key-value head, in blocks of 32 positions that lie as the attention's
+ * matrix instructions take them.  With E = 16 / element size, position
+ * t = 16 h + 4 g + i of a block (h < 2, g < 4, i < 4) and dimension x:
+ *   memory  [page][layer][0: keys, 1: values][head][page_size / 32][32 * head_dim]
+ *   keys    [h][x / E][4 g + i][x % E]
+ *   values  BF16: [x][g][h][i]     F32: [h][x][g][i] */
+typedef struct vs_kv vs_kv;
+
+/* Sequences on a cache: device buffers of the caller.  Position p of sequence
+ * b lies in page table[b * width + p / page_size]; an entry outside
+ * [0, npages) (use -1) is no page, its positions are never visible.  refs[p]
+ * counts the table entries (and the caller's own holds) on page p; a page
+ * with refs 0 is free. */
+typedef struct vs_kv_seqs {
+    int32_t *table; /* nseq x width */
+    int32_t *lens;  /* nseq: positions in use */
+    int32_t *refs;  /* npages */
+    int64_t nseq;
+    int64_t width;
+} vs_kv_seqs;
+
+/* page_size: a power of two from 32 to 1024; head_dim: a multiple of 16 up to
+ * 256; dtype VS_DTYPE_F32 or VS_DTYPE_BF16.  `memory`: device memory of
+ * npages * vs_kv_page_bytes bytes, 16-byte aligned, that stays the caller's;
+ * null: the library allocates it (its contents are undefined). */
+VS_API int vs_kv_create(int device, int64_t npages, int64_t page_size, int64_t layers,
+                        int64_t kv_heads, int64_t head_dim, int dtype, void *memory, vs_kv **out);
+/* Waits for the device's work. */
+VS_API void vs_kv_destroy(vs_kv *kv);
+VS_API int64_t vs_kv_page_bytes(const vs_kv *kv);
+VS_API void *vs_kv_memory(const vs_kv *kv);
+
+/* Attention of one new token of every sequence, at its last position n - 1
+ * (n = lens[b]), for `heads` query heads (a multiple of kv_heads; head h reads
+ * key-value head h / (heads / kv_heads)):
+ *   visible  p < n on a page, and window == 0 or p >= n - window or p < sinks
+ *   s_p      scale * q . K_p
+ *   out      sum over visible p of softmax(s)_p V_p
+ *   lse      log of the sum of exp(s_p), natural; may be null
+ * Nothing visible: out 0, lse -inf.  q and out have the cache's type, rows of
+ * head_dim values at [b * *_seq + h * *_head] elements; lse is [nseq][heads]
+ * fp32.  With k and v (both or neither; [nseq][kv_heads] rows like q) the new
+ * token's keys and values are stored at position n - 1 in the same pass, so
+ * that page must be this sequence's alone (vs_kv_extend sees to it).
+ * Products of bf16 values, sums and the softmax are held in fp32. */
+VS_API int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t heads,
+                        const void *q, int64_t q_seq, int64_t q_head, const void *k, int64_t k_seq,
+                        int64_t k_head, const void *v, int64_t v_seq, int64_t v_head, void *out,
+                        int64_t out_seq, int64_t out_head, float *lse, float scale, int64_t window,
+                        int64_t sinks, void *stream);
+/* Stores keys and values of a layer: rows [starts[b], starts[b + 1]) of k and
+ * v go to the last starts[b + 1] - starts[b] positions of sequence b (starts:
+ * nseq + 1 ascending device values, starts[0] >= 0; null: one row each, row b
+ * of sequence b).  nrows: how many rows k and v have. */
+VS_API int vs_kv_append(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, const void *k,
+                        int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
+                        const int32_t *starts, int64_t nrows, void *stream);
+/* The reverse: positions [first, first + n) of sequence b as rows
+ * [n][kv_heads][head_dim] of k_out and v_out; 0 where no page is. */
+VS_API int vs_kv_read(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t b, int64_t first,
+                      int64_t n, void *k_out, void *v_out, void *stream);
+
+/* Gives every sequence `count` more positions (or count_dev[b], if not null;
+ * negative counts are 0): lens grow, and the pages for them are taken, the
+ * lowest free ones in the order of the sequences.  A partly filled last page
+ * that others hold too is copied to a page of the sequence's own first (all
+ * layers); where everyone who holds it is being extended here, the lowest of
+ * them keeps it.  If pages or table columns do not suffice nothing changes,
+ * and vs_kv_check says so. */
+VS_API int vs_kv_extend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t count, const int32_t *count_dev,
+                        void *stream);
+/* out's sequence i becomes a copy of in's sequence parents[i] (nseq of out
+ * entries; -1: an empty sequence) that shares its pages: the table and length
+ * are copied and refs follow; sequences of `in` that are no one's parent lose
+ * their references, which frees pages that no one else holds.  in and out
+ * have different table and lens buffers and equal width; refs may be one
+ * buffer.  A parent outside [-1, nseq of in) counts as -1 and is reported. */
+VS_API int vs_kv_fork(vs_kv *kv, const vs_kv_seqs *in, const int32_t *parents,
+                      const vs_kv_seqs *out, void *stream);
+/* Drops the n listed sequences (device ids; null: all): their references are
+ * given back, entries become -1, lengths 0.  Ids outside [0, nseq) are
+ * ignored, repeated ones count once. */
+VS_API int vs_kv_free(vs_kv *kv, const vs_kv_seqs *seqs, const int32_t *ids, int64_t n,
+                      void *stream);
+/* Gives back the pages that no later vs_kv_attend with this window and these
+ * sinks can see: whole pages of positions in [sinks, n - window). */
+VS_API int vs_kv_evict(vs_kv *kv, const vs_kv_seqs *seqs, int64_t window, int64_t sinks,
+                       void *stream);
+/* Moves the pages in use to the front: with L pages in use, the j-th of those
+ * at or past L moves to the j-th free page below L; tables and refs follow.
+ * Afterwards pages L and up are free.  out may be in. */
+VS_API int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out, void *stream);
+/* Copies whole pages, to[i] = from[i] (n device ids each): pages outside
+ * [0, npages) are skipped; no page may be both read and written, or written
+ * twice. */
+VS_API int vs_kv_copy(vs_kv *kv, const int32_t *from, const int32_t *to, int64_t n, void *stream);
+/* Waits for the stream and tells what earlier calls met on the device since
+ * the last check: VS_ERR_OOM (an extend found too few free pages),
+ * VS_ERR_INVALID (too few table columns; a parent out of range). */
+VS_API int vs_kv_check(vs_kv *kv, void *stream);
+
+/* Beam search over device buffers.  A handle owns scratch memory only. */
+typedef struct vs_beam vs_beam;
+VS_API int vs_beam_create(int device, vs_beam **out);
+/* Waits for the device's work. */
+VS_API void vs_beam_destroy(vs_beam *bs);
+/* One step of each of nreq requests with nbeam beams: row r * nbeam + w of
+ * `logits` (vocab values of `dtype`, rows row_stride apart) is beam w of
+ * request r, scores[r * nbeam + w] its sum of log-probabilities.
+ *   total(w, t) = scores[w] + logits[w][t] - log sum exp logits[w]
+ * and the k best (w, t) of each request are returned, best first: by total,
+ * then the lower beam, the larger logit, the lower token.  A beam whose
+ * `finished` byte is not 0 only continues with token eos at its own score
+ * (finished may be null; an eos outside [0, vocab): no such token).  A logit
+ * of -inf is never chosen, nor is anything of a beam whose score is -inf or
+ * NaN or whose logits hold a NaN or +inf.  Outputs [nreq][k]: scores_out
+ * (the 64-bit total rounded to fp32), tokens, parents (the row
+ * r * nbeam + w) and, if finished_out is not null, whether the token is eos.
+ * Missing candidates: -inf, -1, -1, 0.  k <= 64, nbeam <= 128. */
+VS_API int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_stride,
+                          int64_t nreq, int64_t nbeam, int64_t vocab, const float *scores,
+                          const uint8_t *finished, int64_t eos, int64_t k, float *scores_out,
+                          int32_t *tokens_out, int32_t *parents_out, uint8_t *finished_out,
+                          void *stream);
+/* States follow their beams: row i of `out` (nrows rows out_stride bytes
+ * apart) is the first `bytes` bytes of row parents[i] of `in` (nrows_in rows
+ * in_stride bytes apart), zeros where parents[i] is outside [0, nrows_in);
+ * with tail, tail[i] (4 bytes) is stored behind them.  in and out do not
+ * overlap; with tail, out, out_stride and bytes are multiples of 4. */
+VS_API int vs_beam_reorder(vs_beam *bs, const int32_t *parents, int64_t nrows, const void *in,
+                           int64_t nrows_in, int64_t in_stride, void *out, int64_t out_stride,
+                           int64_t bytes, const int32_t *tail, void *stream);
+
 /* ---- errors ---- */
 VS_API const char *vs_last_error(void);
 
