@@ -142,8 +142,8 @@ __device__ __forceinline__ u32x4_t load_piece(const char *row, int x, bool vec) 
 // bf16: P is multiplied as the sum of two bf16 values (its first 8 bits and
 // the rest rounded to 8), so it is good to 2^-17 and the output is as exact
 // as its last rounding.
-template <int ST, int D>
-__global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a) {
+template <int ST, int D, int WG = (D <= 96 ? 3 : D <= 208 ? 2 : 1)>
+__global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
     constexpr int E = ST ? 8 : 4;
     constexpr int ES = 16 / E;             // element size
     constexpr int H = ST ? 2 : 1;          // 16-position halves per unit
@@ -192,32 +192,59 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a) {
     const int bpp1 = (1 << (a.page_shift - 5)) - 1;
     const int j0 = it.split * per, j1 = min(j0 + per, sp.total);
     const int u1 = ST ? j1 : 2 * j1;
-    for (int u = (ST ? j0 : 2 * j0) + wave; u < u1; u += kWaves) {
-        const int j = ST ? u : u >> 1, half = ST ? 0 : u & 1;
-        const int blk = j < sp.nsb ? j : j - sp.nsb + sp.wb0;
-        const int pos0 = blk * kKvBlock + half * 16;
-        const int page = trow[pos0 >> a.page_shift];
-        if ((unsigned)page >= (unsigned)a.npages) continue;
-        char *kb = a.pool + ((int64_t)page * a.page_bytes + head_base +
-                             ((blk & bpp1) * kKvBlock + half * 16) * (D * ES));
-        char *vb = kb + a.kv_off;
-        u32x4_t kf[H * NC], vf[ND];
+    // first position of unit u
+    auto unit_pos = [&](int u) {
+        const int j = ST ? u : u >> 1;
+        return (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock + (ST ? 0 : (u & 1) * 16);
+    };
+    // its keys; a position without a page reads page 0 and is hidden below
+    auto unit_base = [&](int page, int pos0) {
+        return a.pool + ((int64_t)((unsigned)page < (unsigned)a.npages ? page : 0) * a.page_bytes +
+                         head_base + ((pos0 >> 5 & bpp1) * kKvBlock + (pos0 & 16)) * (D * ES));
+    };
+    u32x4_t kf[H * NC], vf[ND];
+    auto load_keys = [&](const char *kb) {
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 // (a piece past the row's end is read again and zeroed)
                 const int piece = D % (4 * E) ? min(c * 4 + g, D / E - 1) : c * 4 + g;
-                u32x4_t w = *(const u32x4_t *)(kb + ((h * (D / E) + piece) * 16 + r) * 16);
-                if (D % (4 * E) && c * 4 + g >= D / E) w = u32x4_t{0, 0, 0, 0};
-                kf[h * NC + c] = w;
+                kf[h * NC + c] = *(const u32x4_t *)(kb + ((h * (D / E) + piece) * 16 + r) * 16);
             }
+    };
+    auto load_values = [&](const char *kb) {
 #pragma unroll
         for (int d = 0; d < ND; ++d)
-            vf[d] = *(const u32x4_t *)(vb + ((d * 16 + r) * 4 + g) * 16);
+            vf[d] = *(const u32x4_t *)(kb + a.kv_off + ((d * 16 + r) * 4 + g) * 16);
+    };
+    int u = (ST ? j0 : 2 * j0) + wave;
+    int pos0 = 0, page = 0;
+    char *kb = a.pool;
+    if (u < u1) {
+        pos0 = unit_pos(u);
+        page = trow[pos0 >> a.page_shift];
+        kb = unit_base(page, pos0);
+        load_keys(kb);
+        load_values(kb);
+    }
+    while (u < u1) {
+        const int un = u + kWaves;
+        int pos_n = 0, page_n = 0;
+        if (un < u1) {
+            pos_n = unit_pos(un);
+            page_n = trow[pos_n >> a.page_shift];
+        }
+        char *vb = kb + a.kv_off;
+        const bool here = (unsigned)page < (unsigned)a.npages;
+        if constexpr (D % (4 * E) != 0) {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                if ((NC - 1) * 4 + g >= D / E) kf[h * NC + NC - 1] = u32x4_t{0, 0, 0, 0};
+        }
 
         const int tn = n - 1 - pos0;  // the new token's place in this unit
-        if (a.k && tn < 16 * H && tn >= 0) {
+        if (a.k && here && tn < 16 * H && tn >= 0) {
             // its keys and values take their places in the registers and, from
             // one workgroup per key-value head, in the page
             const char *krow = a.k + ((int64_t)it.b * a.k_seq + (int64_t)kvh * a.k_head) * ES;
@@ -277,9 +304,17 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[h][i] *= a.scale2;
         }
+        // the next unit's keys take the place of these, its values that of
+        // these further down: loads are in flight all the time
+        char *kb_n = kb;
+        if (un < u1) {
+            kb_n = unit_base(page_n, pos_n);
+            load_keys(kb_n);
+        }
 
         const int lo = n - a.window;  // with a window: positions below are invisible but for the sinks
-        if (pos0 + 16 * H > n || (a.window > 0 && pos0 < lo && pos0 + 16 * H > a.sinks)) {
+        if (!here || pos0 + 16 * H > n ||
+            (a.window > 0 && pos0 < lo && pos0 + 16 * H > a.sinks)) {
             // a masked position's score is -inf and its values are 0: what
             // lies there may be anything, and 0 times a NaN is one
             uint32_t hide = 0;
@@ -288,7 +323,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int p = pos0 + 16 * h + 4 * g + i;
-                    if (p >= n || (a.window > 0 && p < lo && p >= a.sinks)) {
+                    if (!here || p >= n || (a.window > 0 && p < lo && p >= a.sinks)) {
                         s[h][i] = -__builtin_huge_valf();
                         hide |= 1u << (4 * h + i);
                     }
@@ -358,6 +393,11 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a) {
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
                         float_of(vf[d][i]), p[0][i], o[d], 0, 0, 0);
         }
+        if (un < u1) load_values(kb_n);
+        u = un;
+        pos0 = pos_n;
+        page = page_n;
+        kb = kb_n;
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -663,10 +703,7 @@ int vs_kv_create(int device, int64_t npages, int64_t page_size, int64_t layers, 
     kv->dtype = dtype;
     kv->page_bytes = pb;
     kv->mem = (char *)memory;
-    int cus = 0;
-    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) == hipSuccess &&
-        cus > 0)
-        kv->num_cu = cus;
+    kv->num_cu = vs::cu_count(device);
     void *p = nullptr;
     hipError_t e = vs::device_alloc(&p, vs::kStatusWords * sizeof(int32_t));
     kv->status = (int32_t *)p;

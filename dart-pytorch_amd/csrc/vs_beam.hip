@@ -1,10 +1,11 @@
 // vs_beam.hip -- beam search: the choice of the next beams over beams and
 // vocabulary, and the reordering of their states.
 #include "vs_host.h"
-#include "vs_internal.h"
+#include "vs_device.h"
 
 struct vs_beam {
     int device = 0;
+    int num_cu = 256;
     vs::StreamScratch scratch;
 };
 
@@ -12,9 +13,12 @@ namespace vs {
 namespace {
 
 constexpr int kMaxK = 64, kMaxBeams = 128;
-constexpr int kPiece = 2048;   // logits per wave: 32 per lane, held in registers
-constexpr int kCap = 256;      // candidates per piece kept in LDS
+constexpr int kPer = 16;            // logits per lane and step (an f32x16_t)
+constexpr int kStep = 64 * kPer;    // logits per wave and step
+constexpr int kMostSteps = 64;      // per piece
+constexpr int kCap = 256;           // candidates per piece kept in LDS
 constexpr int kMergeCap = 1024;
+constexpr int kMergeThreads = 512;
 constexpr float kLog2e = 1.44269504088896340736f;
 #define VS_NINF (-__builtin_huge_valf())
 
@@ -22,7 +26,7 @@ struct BeamArgs {
     const char *logits;
     int64_t row_stride;  // elements
     int64_t vocab;
-    int nreq, nbeam, k, npieces;
+    int nreq, nbeam, k, npieces, steps;  // pieces per row, steps per piece
     const float *scores;
     const uint8_t *finished;
     int64_t eos;
@@ -34,166 +38,250 @@ struct BeamArgs {
     int32_t *top_t;      // their tokens; -inf and -1 where there are fewer
 };
 
-// larger float, larger code; neither infinity nor -0 needs a case of its own
+// Larger float, larger code; both zeros have one code.
 __device__ __forceinline__ uint32_t code_of(float x) {
-    const uint32_t u = bits_of(x);
+    const uint32_t u = bits_of(x + 0.f);  // (-0 + 0 is 0)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t c) {
     return float_of(c & 0x80000000u ? c & 0x7FFFFFFFu : ~c);
 }
 
-// One pass over the logits: a wave loads its piece of a row once and leaves
-// the piece's maximum and exponential sum (for the row's log sum exp) and its
-// k largest logits.  A threshold that k logits are at or above is the k-th
-// largest of the lanes' maxima, found by bisection on ballots; what lies at or
-// above it, a few more than k, is ranked through LDS.  Only where more than
-// kCap logits tie at the threshold are the k best picked one by one.
+// kStep consecutive logits of a row in a wave's registers.  Which lane holds
+// which token goes by the token alone, wherever the row starts: equal rows have
+// equal sums to the bit, and their beams tie.
 template <int ST>
-__global__ __launch_bounds__(256) void beam_piece_kernel(BeamArgs a) {
-    constexpr int E = ST ? 8 : 4, NL = 32 / E, ES = 16 / E;
-    __shared__ float cand_v[4][kCap];
-    __shared__ int cand_t[4][kCap];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t slot = (int64_t)blockIdx.x * 4 + wave;
-    if (slot >= (int64_t)a.nreq * a.nbeam * a.npieces) return;
-    const int64_t row = slot / a.npieces;
-    const int piece = (int)(slot % a.npieces);
-    // a beam without continuations of its own: its logits do not matter
-    const float score = a.scores[row];
-    if (!(score > VS_NINF) || (a.finished && a.finished[row])) return;
-    const char *base = a.logits + row * a.row_stride * ES;
-    const int first = piece * kPiece;
+struct Step {
+    static constexpr int E = ST ? 8 : 4, NL = kPer / E, ES = 16 / E;
+    u32x4_t w[NL];
 
-    // (which lane holds which token goes by the token alone, wherever the row
-    // starts: equal rows have equal sums to the bit, and their beams tie)
-
-    float x[32];
-    if (first + kPiece <= a.vocab) {
+    // (unaligned 16-byte loads: rows start anywhere)
+    __device__ __forceinline__ void load(const char *row, int first, int vocab, int lane) {
+        if (first + kStep <= vocab) {
 #pragma unroll
-        for (int l = 0; l < NL; ++l) {
-            u32x4_t w;
-            __builtin_memcpy(&w, base + (int64_t)(first + (l * 64 + lane) * E) * ES, 16);
+            for (int l = 0; l < NL; ++l)
+                __builtin_memcpy(&w[l], row + (int64_t)(first + (l * 64 + lane) * E) * ES, 16);
+        } else {
+            // the row's last, partial step: one load per token, all in flight
+#pragma unroll
+            for (int l = 0; l < NL; ++l)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = first + (l * 64 + lane) * E + i * (E / 4);
+                    if constexpr (ST) {
+                        const uint16_t *p = (const uint16_t *)row;
+                        const uint32_t lo = p[min(t, vocab - 1)], hi = p[min(t + 1, vocab - 1)];
+                        w[l][i] = (t < vocab ? lo : 0xFF80u) | (t + 1 < vocab ? hi : 0xFF80u) << 16;
+                    } else {
+                        const uint32_t v = ((const uint32_t *)row)[min(t, vocab - 1)];
+                        w[l][i] = t < vocab ? v : 0xFF800000u;
+                    }
+                }
+        }
+    }
+    __device__ __forceinline__ f32x16_t values() const {
+        f32x16_t x;
+#pragma unroll
+        for (int l = 0; l < NL; ++l)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (ST) {
-                    x[l * E + 2 * i] = float_of(w[i] << 16);
-                    x[l * E + 2 * i + 1] = float_of(w[i] & 0xFFFF0000u);
+                    x[l * E + 2 * i] = float_of(w[l][i] << 16);
+                    x[l * E + 2 * i + 1] = float_of(w[l][i] & 0xFFFF0000u);
                 } else {
-                    x[l * E + i] = float_of(w[i]);
+                    x[l * E + i] = float_of(w[l][i]);
+                }
+            }
+        return x;
+    }
+    static __device__ __forceinline__ int token(int first, int i, int lane) {
+        return first + ((i / E) * 64 + lane) * E + i % E;
+    }
+};
+
+// Wave-wide reductions in the vector registers (data-parallel primitives: a
+// shuffle through LDS takes several times as long).  What a step does not
+// reach keeps `same`, which changes nothing.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp(uint32_t same, uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)same, (int)x, CTRL, ROWS, 0xf, false);
+}
+constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+constexpr int kBcast15 = 0x142, kBcast31 = 0x143;
+
+// The largest x of the wave, in every lane (NaNs are passed over).
+__device__ __forceinline__ float wave_max(float x) {
+    x = fmaxf(x, float_of(dpp<kSwap1>(bits_of(x), bits_of(x))));
+    x = fmaxf(x, float_of(dpp<kSwap2>(bits_of(x), bits_of(x))));
+    x = fmaxf(x, float_of(dpp<kHalfMirror>(bits_of(x), bits_of(x))));
+    x = fmaxf(x, float_of(dpp<kMirror>(bits_of(x), bits_of(x))));
+    const float a = float_of(__builtin_amdgcn_readlane(bits_of(x), 0));
+    const float b = float_of(__builtin_amdgcn_readlane(bits_of(x), 16));
+    const float c = float_of(__builtin_amdgcn_readlane(bits_of(x), 32));
+    const float d = float_of(__builtin_amdgcn_readlane(bits_of(x), 48));
+    return fmaxf(fmaxf(a, b), fmaxf(c, d));
+}
+
+// Inclusive prefix sum over the lanes.
+__device__ __forceinline__ int prefix_sum(int x) {
+    x += (int)dpp<0x111>(0, x);            // one lane up within rows of 16, then 2, 4, 8
+    x += (int)dpp<0x112>(0, x);
+    x += (int)dpp<0x114>(0, x);
+    x += (int)dpp<0x118>(0, x);
+    x += (int)dpp<kBcast15, 0xa>(0, x);    // rows 1 and 3 take the sum of the one before
+    x += (int)dpp<kBcast31, 0xc>(0, x);    // the upper half that of the lower
+    return x;
+}
+
+// Larger logit first, then the lower token, as one 64-bit number.
+__device__ __forceinline__ uint64_t key_of(float v, int token) {
+    return (uint64_t)code_of(v) << 32 | ~(uint32_t)token;
+}
+
+// The wave's list of n keys (at most kCap) cut to its k best, in order.
+__device__ __forceinline__ void cut_list(uint64_t *cand, int n, int k, int lane) {
+    uint64_t me[kCap / 64];
+    int rank[kCap / 64];
+    lds_wave_sync();
+#pragma unroll
+    for (int c = 0; c < kCap / 64; ++c) {
+        me[c] = c * 64 + lane < n ? cand[c * 64 + lane] : 0;
+        rank[c] = c * 64 + lane < n ? 0 : k;
+    }
+    for (int j = 0; j < n; ++j) {
+        const uint64_t o = cand[j];
+#pragma unroll
+        for (int c = 0; c < kCap / 64; ++c) rank[c] += o > me[c];
+    }
+    lds_wave_sync();
+#pragma unroll
+    for (int c = 0; c < kCap / 64; ++c)
+        if (rank[c] < k) cand[rank[c]] = me[c];
+    lds_wave_sync();
+}
+
+// One pass over the logits.  A wave takes a piece of a row (every fourth step
+// of a stretch that the workgroup's waves read together), kStep logits at a
+// time with the next step in flight, and leaves the piece's maximum and
+// exponential sum (for the row's log sum exp) and its k largest logits.
+// The list in LDS takes what is at or above a threshold that k logits seen so
+// far reach: the k-th largest of the lanes' running maxima, found by bisection
+// on ballots.  Most steps of a long piece have nothing at or above it and cost
+// a maximum and an exponential per logit.
+template <int ST>
+__global__ __launch_bounds__(256) void beam_piece_kernel(BeamArgs a) {
+    __shared__ uint64_t lists[4][kCap];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint64_t *cand = lists[wave];
+    const uint32_t slot = blockIdx.x * 4 + wave;
+    if (slot >= (uint32_t)(a.nreq * a.nbeam) * (uint32_t)a.npieces) return;
+    const uint32_t row = slot / (uint32_t)a.npieces;
+    // a beam without continuations of its own: its logits do not matter
+    if (!(a.scores[row] > VS_NINF) || (a.finished && a.finished[row])) return;
+    const char *base = a.logits + row * a.row_stride * Step<ST>::ES;
+    const int vocab = (int)a.vocab;
+    // four waves share a stretch of the row and take its steps in turn
+    const int share = (int)(slot % (uint32_t)a.npieces) >> 2;
+    const int begin = (share * 4 * a.steps + wave) * kStep;
+    const int end = min((share + 1) * 4 * a.steps * kStep, vocab);
+    constexpr int kNext = 4 * kStep;
+
+    float run = VS_NINF;    // the lane's maximum so far
+    float top = VS_NINF;    // the wave's
+    float sum = 0.f;        // of exp(x - top), the lane's share
+    float thr = -__FLT_MAX__;  // (so -inf is no candidate)
+    int n = 0;
+    Step<ST> step;
+    if (begin < end) step.load(base, begin, vocab, lane);
+    for (int first = begin; first < end; first += kNext) {
+        const f32x16_t x = step.values();
+        if (first + kNext < end) step.load(base, first + kNext, vocab, lane);
+        float most = x[0];
+#pragma unroll
+        for (int i = 1; i < kPer; ++i) most = fmaxf(most, x[i]);
+        if (__ballot(most >= thr)) {
+            run = fmaxf(run, most);
+            const float w = wave_max(most);
+            if (w > top) {
+                sum *= __builtin_amdgcn_exp2f((top - w) * kLog2e);  // (0 at first: top is -inf)
+                top = w;
+            }
+            // the k-th largest of the lanes' maxima: no lower than the last
+            // one, whose leading bits that the largest has too are its
+            const uint32_t code = code_of(run), low = code_of(thr);
+            const uint32_t apart = low ^ max(low, code_of(top));
+            uint32_t bit = apart ? 0x80000000u >> __builtin_clz(apart) : 0;
+            uint32_t t = low & ~(2 * bit - (bit != 0));
+            for (; bit; bit >>= 1) {
+                const int cnt = __popcll(__ballot(code >= (t | bit)));
+                if (cnt >= a.k) {
+                    t |= bit;
+                    if (cnt == a.k) break;
+                }
+            }
+            if (t > code_of(thr)) thr = value_of(t);
+            uint32_t mask = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) mask |= x[i] >= thr ? 1u << i : 0u;
+            const int mine = __popc(mask);
+            int at = prefix_sum(mine);
+            const int more = __builtin_amdgcn_readlane(at, 63);
+            if (n + more <= kCap) {
+                at += n - mine;
+                for (; mask; mask &= mask - 1) {
+                    const int i = __ffs(mask) - 1;
+                    cand[at++] = key_of(x[i], Step<ST>::token(first, i, lane));
+                }
+                n += more;
+            } else {
+                // more than the list holds, ties mostly: a register at a time,
+                // cut to the k best in between.  What ties with the k-th of
+                // these in a later step has a higher token and is out.
+                for (int i = 0; i < kPer; ++i) {
+                    const float v = x[i];
+                    const uint64_t in = __ballot(v >= thr);
+                    if (!in) continue;
+                    if (n > kCap - 64) {
+                        cut_list(cand, n, a.k, lane);
+                        n = a.k;
+                    }
+                    if (v >= thr)
+                        cand[n + __popcll(in & (((uint64_t)1 << lane) - 1))] =
+                            key_of(v, Step<ST>::token(first, i, lane));
+                    n += __popcll(in);
+                }
+                lds_wave_sync();
+                if (n >= a.k) {
+                    cut_list(cand, n, a.k, lane);
+                    n = a.k;
+                    thr = value_of((uint32_t)(cand[a.k - 1] >> 32) + 1);
                 }
             }
         }
-    } else {
-        // the row's last, partial piece: one load per token, all in flight
+        const float ref = top == VS_NINF ? 0.f : top;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int64_t t = first + ((i / E) * 64 + lane) * E + i % E;
-            const int64_t at = min(t, a.vocab - 1);
-            float v;
-            if constexpr (ST)
-                v = bf16_to_f32(((const uint16_t *)base)[at]);
-            else
-                v = ((const float *)base)[at];
-            x[i] = t < a.vocab ? v : VS_NINF;
-        }
+        for (int i = 0; i < kPer; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * kLog2e);
     }
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < 32; ++i) top = fmaxf(top, x[i]);
-    top = top > VS_NINF ? top : VS_NINF;  // (all NaN)
-    float wtop = top;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) wtop = fmaxf(wtop, __shfl_xor(wtop, d));
-    const float ref = wtop == VS_NINF ? 0.f : wtop;
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * kLog2e);
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    if (lane == 0) a.stat[slot] = make_float2(wtop, sum);
-
-    const uint32_t code = code_of(top);
-    uint32_t thr = 0;
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-        const int cnt = __popcll(__ballot(code >= (thr | bit)));
-        if (cnt >= a.k) {
-            thr |= bit;
-            if (cnt == a.k) break;
+    if (lane == 0) a.stat[slot] = make_float2(top, sum);
+    float *ov = a.top_v + (int64_t)slot * a.k;
+    int32_t *ot = a.top_t + (int64_t)slot * a.k;
+    lds_wave_sync();
+    for (int c = lane; c < n; c += 64) {
+        const uint64_t me = cand[c];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += cand[j] > me;
+        if (rank < a.k) {
+            ov[rank] = value_of((uint32_t)(me >> 32));
+            ot[rank] = (int)~(uint32_t)me;
         }
     }
-    const float tv = value_of(thr);
-    // (the bisection ends below -inf's code only if that lane's maximum is
-    // smaller still, which none is)
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const bool in = x[i] > VS_NINF && !(x[i] < tv);
-        const uint64_t mask = __ballot(in);
-        if (mask) {
-            const int at = n + __popcll(mask & (((uint64_t)1 << lane) - 1));
-            if (in && at < kCap) {
-                cand_v[wave][at] = x[i];
-                cand_t[wave][at] = first + ((i / E) * 64 + lane) * E + i % E;
-            }
-            n += __popcll(mask);
-        }
-    }
-    float *ov = a.top_v + slot * a.k;
-    int32_t *ot = a.top_t + slot * a.k;
-    if (n <= kCap) {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-        for (int c = lane; c < n; c += 64) {
-            const float v = cand_v[wave][c];
-            const int t = cand_t[wave][c];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) {
-                const float vj = cand_v[wave][j];
-                rank += vj > v || (vj == v && cand_t[wave][j] < t);
-            }
-            if (rank < a.k) {
-                ov[rank] = v;
-                ot[rank] = t;
-            }
-        }
-        for (int c = n + lane; c < a.k; c += 64) {
-            ov[c] = VS_NINF;
-            ot[c] = -1;
-        }
-        return;
-    }
-    float lv = __builtin_huge_valf();
-    int lt = -1;  // the last one picked
-    for (int s = 0; s < a.k; ++s) {
-        float bv = VS_NINF;
-        int bt = INT32_MAX;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int t = first + ((i / E) * 64 + lane) * E + i % E;
-            const bool after = x[i] < lv || (x[i] == lv && t > lt);
-            if (after && x[i] > VS_NINF && (x[i] > bv || (x[i] == bv && t < bt))) {
-                bv = x[i];
-                bt = t;
-            }
-        }
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            const float v = __shfl_xor(bv, d);
-            const int t = __shfl_xor(bt, d);
-            if (v > bv || (v == bv && t < bt)) {
-                bv = v;
-                bt = t;
-            }
-        }
-        if (lane == 0) {
-            ov[s] = bv;
-            ot[s] = bt == INT32_MAX ? -1 : bt;
-        }
-        lv = bv;
-        lt = bt;
+    for (int c = n + lane; c < a.k; c += 64) {
+        ov[c] = VS_NINF;
+        ot[c] = -1;
     }
 }
 
@@ -211,104 +299,134 @@ __device__ __forceinline__ bool better(const Cand &a, const Cand &b) {
 }
 
 // One workgroup per request: the rows' log sum exp from the pieces, then the
-// k best of the pieces' candidates, in 64 bits.  The pieces' lists are sorted,
-// so the threshold (the k-th largest of the threads' best heads) needs their
-// first entries only and each list is walked no further than it.
-__global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
+// k best of the pieces' candidates, in 64 bits.  What bounds it is the chain
+// of loads that wait for each other, so there are two: the pieces' statistics
+// with their lists' first entries, and then, at once, all entries of the lists
+// whose first is at or above a threshold that k first entries reach (k lists,
+// ties aside).
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
     // total = (logit - largest) + (score - log of the sum of exponentials): in
     // this order no size of the logits costs the total its digits
     __shared__ double offset[kMaxBeams];  // score - log sum; NaN: no candidates
     __shared__ float largest[kMaxBeams];
-    __shared__ double best[256];
+    __shared__ double own[kMaxBeams];     // a finished beam's score; NaN: not finished, or no eos
+    __shared__ float best[kMergeThreads];
     __shared__ Cand list[kMergeCap];
-    __shared__ int nlist;
-    __shared__ double thr;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ int picked[kMergeCap];     // lists to read whole
+    __shared__ int place[kMergeCap];
+    __shared__ int nlist, npicked;
+    __shared__ float thr;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = blockIdx.x;
     const int64_t row0 = (int64_t)r * a.nbeam;
     const double none = -__builtin_huge_val();
-    for (int w = wave; w < a.nbeam; w += 4) {
+    const int lists = a.nbeam * a.npieces;
+    // a thread's first entries, in flight while the statistics are summed
+    constexpr int kHeads = 2;
+    float head[kHeads];
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+        const int i = threadIdx.x + j * kMergeThreads;
+        head[j] = i < lists ? a.top_v[(row0 * a.npieces + i) * a.k] : VS_NINF;
+    }
+    if (threadIdx.x == 0) nlist = npicked = 0;
+    for (int w = wave; w < a.nbeam; w += kMergeThreads / 64) {
+        // (loaded whether the beam is alive or not: what is not needed is not used)
         const int64_t row = row0 + w;
         const float score = a.scores[row];
-        const bool live = score > VS_NINF && !(a.finished && a.finished[row]);
+        const float2 *st = a.stat + row * a.npieces;
+        const float2 x = lane < a.npieces ? st[lane] : make_float2(VS_NINF, 0.f);
+        const bool ended = a.finished && a.finished[row];
+        const bool alive = score > VS_NINF;
         double off = __builtin_nan("");
-        if (live) {
-            const float2 *st = a.stat + row * a.npieces;
-            float top = VS_NINF;
-            for (int p = lane; p < a.npieces; p += 64) top = fmaxf(top, st[p].x);
+        if (alive && !ended) {
+            float top = x.x;
+            for (int p = 64 + lane; p < a.npieces; p += 64) top = fmaxf(top, st[p].x);
 #pragma unroll
             for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
             const float ref = top == VS_NINF ? 0.f : top;
-            double sum = 0.0;
-            for (int p = lane; p < a.npieces; p += 64)
-                sum += (double)st[p].y * (double)__builtin_amdgcn_exp2f((st[p].x - ref) * kLog2e);
+            double sum = (double)(x.y * __builtin_amdgcn_exp2f((x.x - ref) * kLog2e));
+            for (int p = 64 + lane; p < a.npieces; p += 64)
+                sum += (double)(st[p].y * __builtin_amdgcn_exp2f((st[p].x - ref) * kLog2e));
 #pragma unroll
             for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
             // (a NaN or +inf among the logits makes the sum a NaN; nothing but -inf makes it 0)
             if (sum > 0.0) off = (double)score - log(sum);
             if (lane == 0) largest[w] = top;
         }
-        if (lane == 0) offset[w] = off;
+        if (lane == 0) {
+            offset[w] = off;
+            own[w] = alive && ended && a.eos >= 0 && a.eos < a.vocab ? (double)score
+                                                                     : __builtin_nan("");
+        }
     }
-    if (threadIdx.x == 0) nlist = 0;
     __syncthreads();
 
-    // candidate `c` of list (w, p), or nothing
-    auto fetch = [&](int w, int p, int c, Cand &out) {
-        const double off = offset[w];
-        if (off != off) return false;
-        const int64_t at = ((row0 + w) * a.npieces + p) * a.k + c;
-        out.v = a.top_v[at];
-        if (!(out.v > VS_NINF)) return false;
-        out.token = a.top_t[at];
-        out.beam = w;
-        out.total = off + ((double)out.v - (double)largest[w]);
-        return true;
+    // the total of logit v of list i; NaN where there is none
+    auto total_of = [&](int i, float v) {
+        const int w = i / a.npieces;
+        return v > VS_NINF ? offset[w] + ((double)v - (double)largest[w]) : __builtin_nan("");
     };
-    auto ended = [&](int w, Cand &out) {
-        const int64_t row = row0 + w;
-        const float score = a.scores[row];
-        if (!(score > VS_NINF) || !a.finished || !a.finished[row]) return false;
-        if (a.eos < 0 || a.eos >= a.vocab) return false;
-        out.total = (double)score;
-        out.v = 0.f;
-        out.beam = w;
-        out.token = (int)a.eos;
-        return true;
-    };
-    const int lists = a.nbeam * a.npieces;
     double mine = none;
-    for (int i = threadIdx.x; i < lists; i += 256) {
-        Cand c;
-        if (fetch(i / a.npieces, i % a.npieces, 0, c)) mine = max(mine, c.total);
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+        const int i = threadIdx.x + j * kMergeThreads;
+        if (i < lists) mine = fmax(mine, total_of(i, head[j]));  // (fmax passes NaNs over)
     }
-    for (int w = threadIdx.x; w < a.nbeam; w += 256) {
-        Cand c;
-        if (ended(w, c)) mine = max(mine, c.total);
-    }
-    best[threadIdx.x] = mine;
+    for (int i = threadIdx.x + kHeads * kMergeThreads; i < lists; i += kMergeThreads)
+        mine = fmax(mine, total_of(i, a.top_v[(row0 * a.npieces + i) * a.k]));
+    if ((int)threadIdx.x < a.nbeam) mine = fmax(mine, own[threadIdx.x]);
+    // The threshold is compared in 32 bits: rounding keeps the order, so what
+    // is among the k best is at or above it there too.
+    best[threadIdx.x] = (float)mine;
     __syncthreads();
-    int rank = 0;
-    for (int i = 0; i < 256; ++i) {
-        const double o = best[i];
-        rank += o > mine || (o == mine && i < (int)threadIdx.x);
-    }
-    if (rank == a.k - 1) thr = mine;
-    __syncthreads();
-    const double t = thr;
-    for (int i = threadIdx.x; i < lists; i += 256)
-        for (int j = 0; j < a.k; ++j) {
-            Cand c;
-            if (!fetch(i / a.npieces, i % a.npieces, j, c) || c.total < t) break;
-            const int at = atomicAdd(&nlist, 1);
-            if (at >= kMergeCap) break;
-            list[at] = c;
+    if (wave == 0) {
+        float m = best[lane];
+#pragma unroll
+        for (int j = 1; j < kMergeThreads / 64; ++j) m = fmaxf(m, best[lane + 64 * j]);
+        const uint32_t code = code_of(m);
+        uint32_t t = 0;
+        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+            const int cnt = __popcll(__ballot(code >= (t | bit)));
+            if (cnt >= a.k) {
+                t |= bit;
+                if (cnt == a.k) break;
+            }
         }
-    for (int w = threadIdx.x; w < a.nbeam; w += 256) {
-        Cand c;
-        if (ended(w, c) && !(c.total < t)) {
-            const int at = atomicAdd(&nlist, 1);
-            if (at < kMergeCap) list[at] = c;
+        // (a code below -inf's: all lanes count, and so does everything)
+        if (lane == 0) thr = t < code_of(VS_NINF) ? VS_NINF : value_of(t);
+    }
+    __syncthreads();
+    const float t = thr;
+    auto pick = [&](int i, double total) {
+        if (!((float)total >= t)) return;
+        const int at = atomicAdd(&npicked, 1);
+        if (at < kMergeCap) picked[at] = i;
+    };
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+        const int i = threadIdx.x + j * kMergeThreads;
+        if (i < lists) pick(i, total_of(i, head[j]));
+    }
+    for (int i = threadIdx.x + kHeads * kMergeThreads; i < lists; i += kMergeThreads)
+        pick(i, total_of(i, a.top_v[(row0 * a.npieces + i) * a.k]));
+    auto add = [&](const Cand &c) {
+        const int at = atomicAdd(&nlist, 1);
+        if (at < kMergeCap) list[at] = c;
+    };
+    if ((int)threadIdx.x < a.nbeam && (float)own[threadIdx.x] >= t)
+        add({own[threadIdx.x], 0.f, (int)threadIdx.x, (int)a.eos});
+    __syncthreads();
+    const int lots = npicked;
+    if (lots <= kMergeCap) {
+        for (int x = threadIdx.x; x < lots * a.k; x += kMergeThreads) {
+            const int i = picked[x / a.k];
+            const int64_t at = (row0 * a.npieces + i) * a.k + x % a.k;
+            const float v = a.top_v[at];
+            const int token = a.top_t[at];
+            const double total = total_of(i, v);
+            if ((float)total >= t) add({total, v, i / a.npieces, token});
         }
     }
     __syncthreads();
@@ -326,45 +444,40 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
         a.parents_out[o0 + s] = -1;
         if (a.finished_out) a.finished_out[o0 + s] = 0;
     };
-    if (n <= kMergeCap) {
-        for (int c = threadIdx.x; c < n; c += 256) {
-            const Cand me = list[c];
-            int rk = 0;
-            for (int j = 0; j < n; ++j) rk += better(list[j], me);
-            if (rk < a.k) put(rk, me);
-        }
-        for (int s = n + threadIdx.x; s < a.k; s += 256) put_none(s);
+    if (lots <= kMergeCap && n <= kMergeCap) {
+        // a candidate's place is how many are better: all pairs at once
+        for (int c = threadIdx.x; c < n; c += kMergeThreads) place[c] = 0;
+        __syncthreads();
+        for (int x = threadIdx.x; x < n * n; x += kMergeThreads)
+            if (better(list[x % n], list[x / n])) atomicAdd(&place[x / n], 1);
+        __syncthreads();
+        for (int c = threadIdx.x; c < n; c += kMergeThreads)
+            if (place[c] < a.k) put(place[c], list[c]);
+        for (int s = n + threadIdx.x; s < a.k; s += kMergeThreads) put_none(s);
         return;
     }
-    // more ties than the list holds: one by one
-    Cand last;
-    last.total = __builtin_huge_val();
-    last.beam = -1;
-    last.v = 0.f;
-    last.token = -1;
+    // more ties than there is room for: the k best one by one, from the lists
+    Cand last = {__builtin_huge_val(), 0.f, -1, -1};
     for (int s = 0; s < a.k; ++s) {
-        Cand b;
-        b.total = none;
-        b.beam = INT32_MAX;
-        b.v = 0.f;
-        b.token = INT32_MAX;
-        for (int i = threadIdx.x; i < lists; i += 256)
+        Cand b = {none, 0.f, INT32_MAX, INT32_MAX};
+        for (int i = threadIdx.x; i < lists; i += kMergeThreads)
             for (int j = 0; j < a.k; ++j) {
-                Cand c;
-                if (!fetch(i / a.npieces, i % a.npieces, j, c) || c.total < t) break;
+                const int64_t at = (row0 * a.npieces + i) * a.k + j;
+                const Cand c = {total_of(i, a.top_v[at]), a.top_v[at], i / a.npieces, a.top_t[at]};
+                if (!((float)c.total >= t)) break;
                 if (better(last, c)) {
                     if (better(c, b)) b = c;
                     break;  // (the rest of this list is no better)
                 }
             }
-        for (int w = threadIdx.x; w < a.nbeam; w += 256) {
-            Cand c;
-            if (ended(w, c) && better(last, c) && better(c, b)) b = c;
+        if ((int)threadIdx.x < a.nbeam && (float)own[threadIdx.x] >= t) {
+            const Cand c = {own[threadIdx.x], 0.f, (int)threadIdx.x, (int)a.eos};
+            if (better(last, c) && better(c, b)) b = c;
         }
         __syncthreads();
         list[threadIdx.x] = b;
         __syncthreads();
-        for (int d = 128; d; d >>= 1) {
+        for (int d = kMergeThreads / 2; d; d >>= 1) {
             if ((int)threadIdx.x < d && better(list[threadIdx.x + d], list[threadIdx.x]))
                 list[threadIdx.x] = list[threadIdx.x + d];
             __syncthreads();
@@ -438,6 +551,7 @@ int vs_beam_create(int device, vs_beam **out) {
     vs_beam *b = new (std::nothrow) vs_beam();
     if (!b) return report(VS_ERR_OOM, "host allocation");
     b->device = device;
+    b->num_cu = vs::cu_count(device);
     *out = b;
     return VS_OK;
 }
@@ -485,7 +599,14 @@ int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_strid
     a.nreq = (int)nreq;
     a.nbeam = (int)nbeam;
     a.k = (int)k;
-    a.npieces = (int)((vocab + vs::kPiece - 1) / vs::kPiece);
+    // Pieces short enough for 64 waves to a CU, three times what it holds at
+    // once: where beams have ended their waves leave at once, and the others
+    // spread.  (64 x 8 x 128,000 fp32: 32 waves to a CU 61, 64 58, 128 58 us.)
+    const int64_t row_steps = (vocab + 4 * vs::kStep - 1) / (4 * vs::kStep) * 4;
+    const int64_t waves = (int64_t)bs->num_cu * 64;
+    a.steps = (int)std::min<int64_t>(vs::kMostSteps,
+                                     std::max<int64_t>(1, (nreq * nbeam * row_steps + waves - 1) / waves));
+    a.npieces = (int)((row_steps / 4 + a.steps - 1) / a.steps * 4);
     a.scores = scores;
     a.finished = finished;
     a.eos = eos;
@@ -494,7 +615,7 @@ int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_strid
     a.parents_out = parents_out;
     a.finished_out = finished_out;
     const int64_t slots = nreq * nbeam * a.npieces;
-    if ((slots + 3) / 4 > INT32_MAX) return report(VS_ERR_UNSUPPORTED, "too many logits");
+    if (slots > INT32_MAX) return report(VS_ERR_UNSUPPORTED, "too many logits");
     void *ws = nullptr;
     int rc = bs->scratch.get(st, (size_t)slots * (sizeof(float2) + (size_t)k * 8), &ws);
     if (rc) return rc;
@@ -508,7 +629,7 @@ int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_strid
         hipLaunchKernelGGL(vs::beam_piece_kernel<0>, grid, dim3(256), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return report_hip(e, "beam select");
-    hipLaunchKernelGGL(vs::beam_merge_kernel, dim3((uint32_t)nreq), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(vs::beam_merge_kernel, dim3((uint32_t)nreq), dim3(vs::kMergeThreads), 0, st, a);
     e = hipGetLastError();
     return e == hipSuccess ? VS_OK : report_hip(e, "beam select");
 }

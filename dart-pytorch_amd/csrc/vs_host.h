@@ -87,4 +87,12 @@ inline int check_device(int device) {
     return VS_OK;
 }
 
+inline int cu_count(int device) {
+    int n = 0;
+    return hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) == hipSuccess &&
+                   n > 0
+               ? n
+               : 256;
+}
+
 }  // namespace vs

@@ -95,27 +95,44 @@ class DeviceArray:
         return out
 
 
+# A decoding step of a small model is a few microseconds on the GPU, so the
+# checks below take the straight way where all is well.
+
+
 def _rows(t, what, shape, code):
-    """Pointer and leading strides of a buffer of `shape` whose last dimension is contiguous."""
-    if _SEEN.get(t.dtype) != code and _code(t.dtype) != code:
-        raise ValueError(f"{what}: element type {t.dtype}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    """Pointer and strides of a buffer of `shape` whose last dimension is contiguous."""
     st = t.stride()
-    if st[-1] != 1 and shape[-1] > 1:
-        raise ValueError(f"{what}: the last dimension is not contiguous")
+    if t.shape != shape or _SEEN.get(t.dtype) != code or st[-1] != 1:
+        if _code(t.dtype) != code:
+            raise ValueError(f"{what}: element type {t.dtype}")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+        if st[-1] != 1 and shape[-1] > 1:
+            raise ValueError(f"{what}: the last dimension is not contiguous")
     return t.data_ptr(), st
 
 
 def _flat(t, what, shape, code) -> int:
     """Pointer of a contiguous buffer of `shape`."""
-    p, st = _rows(t, what, shape, code)
+    if t.shape != shape or _SEEN.get(t.dtype) != code:
+        if _code(t.dtype) != code:
+            raise ValueError(f"{what}: element type {t.dtype}")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
     n = 1
-    for size, s in zip(reversed(shape), reversed(st)):
-        if size > 1 and s != n:
+    for size, s in zip(shape[::-1], t.stride()[::-1]):
+        if s != n and size > 1:
             raise ValueError(f"{what}: not contiguous")
         n *= size
-    return p
+    return t.data_ptr()
+
+
+def _list(t, what, n, code) -> int:
+    """Pointer of a contiguous buffer of n elements, whatever its shape."""
+    shape = t.shape
+    if (shape[0] if len(shape) == 1 else math.prod(shape)) != n:
+        raise ValueError(f"{what}: shape {tuple(shape)}, expected {n} elements")
+    return _flat(t, what, tuple(shape), code)
 
 
 class _SeqsC(ctypes.Structure):
@@ -133,7 +150,7 @@ class KVSequences:
             raise ValueError(f"table: shape {tuple(table.shape)}")
         n, width = (int(s) for s in table.shape)
         self.table, self.lens, self.refs = table, lens, refs
-        self.n, self.width = n, width
+        self.n, self.width, self.npages = n, width, int(refs.shape[0])
         self.c = _SeqsC(_flat(table, "table", (n, width), _I32), _flat(lens, "lens", (n,), _I32),
                         _flat(refs, "refs", (int(refs.shape[0]),), _I32), n, width)
         self._ref = ctypes.byref(self.c)
@@ -190,8 +207,8 @@ class PagedKVCache:
         return KVSequences(table, lens, refs)
 
     def _seqs(self, s: KVSequences):
-        if int(s.refs.shape[0]) != self.npages:
-            raise ValueError(f"refs of {int(s.refs.shape[0])} pages on a cache of {self.npages}")
+        if s.npages != self.npages:
+            raise ValueError(f"refs of {s.npages} pages on a cache of {self.npages}")
         return s._ref
 
     def attend(self, seqs: KVSequences, q, out, *, k=None, v=None, lse=None, layer: int = 0, scale=None,
@@ -252,10 +269,7 @@ class PagedKVCache:
     def fork(self, seqs: KVSequences, parents, out: KVSequences, *, stream: int = 0) -> None:
         """out[i] = a copy of seqs[parents[i]] that shares its pages; what is
         no one's parent gives its pages back (vs_kv_fork)."""
-        shape = tuple(parents.shape)
-        if math.prod(shape) != out.n:
-            raise ValueError(f"parents: shape {shape} for {out.n} sequences")
-        rc = self._lib.vs_kv_fork(self._h, self._seqs(seqs), _flat(parents, "parents", shape, _I32),
+        rc = self._lib.vs_kv_fork(self._h, self._seqs(seqs), _list(parents, "parents", out.n, _I32),
                                   self._seqs(out), stream)
         if rc:
             N.check(rc)
@@ -316,15 +330,16 @@ class BeamSearch:
         logits [requests * beams, vocab] f32 or bf16; scores [requests, beams]
         f32; finished [requests, beams] u8.  Outputs [requests, k]: scores f32,
         tokens and parents (rows of logits) i32, finished u8."""
-        requests, beams = (int(s) for s in scores.shape)
-        k, (rows, vocab) = int(scores_out.shape[1]), (int(s) for s in logits.shape)
+        requests, beams = shape = tuple(scores.shape)
+        rows, vocab = logits.shape
+        k = scores_out.shape[1]
         code = _SEEN.get(logits.dtype)
         if code is None:
             code = _code(logits.dtype)
         if code < 0:
             raise ValueError(f"logits: element type {logits.dtype}")
         lp, ls = _rows(logits, "logits", (requests * beams, vocab), code)
-        shape, out = (requests, beams), (requests, k)
+        out = (requests, k)
         rc = self._lib.vs_beam_select(
             self._h, lp, code, ls[0] if rows > 1 else vocab, requests, beams, vocab,
             _flat(scores, "scores", shape, N.VS_DTYPE_F32),
@@ -340,25 +355,20 @@ class BeamSearch:
         such row (vs_beam_reorder).  With tail (i32, one per row) an int32
         state's last column is not copied: tail goes there."""
         code = _code(out.dtype)
-        rows, cols = (int(s) for s in out.shape)
-        if len(state.shape) != 2 or int(state.shape[1]) != cols:
-            raise ValueError(f"state: shape {tuple(state.shape)}, out: {(rows, cols)}")
-        ip, is_ = _rows(state, "state", (int(state.shape[0]), cols), code)
+        rows, cols = out.shape
+        nin = state.shape[0]
+        ip, is_ = _rows(state, "state", (nin, cols), code)
         op, os_ = _rows(out, "out", (rows, cols), code)
         size = _SIZES[code]
         tp, keep = None, cols
         if tail is not None:
             if code != _I32 or cols < 1:
                 raise ValueError("tail needs an i32 state of at least one column")
-            tp, keep = _flat(tail, "tail", tuple(int(s) for s in tail.shape), _I32), cols - 1
-            if math.prod(tail.shape) != rows:
-                raise ValueError(f"tail: shape {tuple(tail.shape)} for {rows} rows")
-        pp = _flat(parents, "parents", tuple(int(s) for s in parents.shape), _I32)
-        if math.prod(parents.shape) != rows:
-            raise ValueError(f"parents: shape {tuple(parents.shape)} for {rows} rows")
+            tp, keep = _list(tail, "tail", rows, _I32), cols - 1
+        pp = _list(parents, "parents", rows, _I32)
         wide = cols * size
         rc = self._lib.vs_beam_reorder(
-            self._h, pp, rows, ip, int(state.shape[0]), is_[0] * size if state.shape[0] > 1 else wide, op,
+            self._h, pp, rows, ip, nin, is_[0] * size if nin > 1 else wide, op,
             os_[0] * size if rows > 1 else wide, keep * size, tp, stream)
         if rc:
             N.check(rc)
