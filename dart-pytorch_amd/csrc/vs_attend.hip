@@ -2,16 +2,19 @@
 // and the cache's rows in and out: kernels and entry points.
 #include <cmath>
 
+#include "vs_device.h"
 #include "vs_kv.h"
+#include "vs_wave.h"
 
 namespace vs {
 namespace {
 
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kWaves = 4;         // per workgroup
-constexpr int kMinBlocks = 4;     // blocks per work item, at least: one per wave
-constexpr int kJoinDims = 128;    // dimensions joined over the waves at once (LDS)
+constexpr int kWaves = 4;      // per workgroup
+constexpr int kMinBlocks = 4;  // blocks per work item, at least: one per wave
+constexpr int kGoodBlocks = 8; // and before a CU takes a second workgroup
+constexpr int kJoinDims = 128; // dimensions joined over the waves at once (LDS)
 
 struct AttendArgs {
     char *pool;
@@ -27,10 +30,10 @@ struct AttendArgs {
     float scale2;                        // scale * log2(e)
     int window, sinks;
     int q_vec, k_vec;                    // rows readable in 16-byte pieces
-    int target_items;
+    int most_items, few_items;           // six workgroups to a CU, and one
     float *part_o;   // [item][heads][dim]
     float2 *part_ml; // [item][heads] running maximum and sum
-    int2 *first;     // [nseq] first item, items
+    int2 *first;     // [nseq] first whole item; whole ones * 2 + whether there is a rest
 };
 
 // The blocks that a sequence of n positions attends to: nsb from its start,
@@ -58,54 +61,81 @@ __device__ __forceinline__ int length_of(const AttendArgs &a, int b) {
     return n < most ? n : (int)most;
 }
 
-// Work item `item`: blocks [split * per, ...) of sequence b.  Every wave
-// works the whole division out by itself from the lengths: all blocks of the
-// call over the number of items that fills the card, so that ragged batches
-// are split where their long sequences are.
+// Work item `item`: blocks [split * per, ...) of sequence b.  Every wave works
+// the division out by itself from the lengths.  `per` is all blocks of the
+// call over the workgroups that the card holds at once, so that long sequences
+// of a ragged batch are split and short ones are not.  First come all whole
+// pieces of `per` blocks, then what is left of the sequences: the smaller ones
+// fill the places that come free.  There are no gaps in the numbers: a
+// workgroup that finds no work does not give its place to the next (one
+// sequence of 100,000 positions 82 against 72 us).
 struct Item {
-    int b, split, nsplit, per;
+    int b, split, per;
+    int first, whole, rest;  // the sequence's pieces: items first .. first + whole - 1, and a rest
 };
 
 __device__ __forceinline__ bool find_item(const AttendArgs &a, int item, int lane, Item &it) {
-    uint64_t total = 0;
-    for (int b0 = 0; b0 < a.nseq; b0 += 64) {
-        const int b = b0 + lane;
-        if (b < a.nseq) total += (uint64_t)max(span_of(length_of(a, b), a.window, a.sinks).total, 1);
+    auto blocks_of = [&](int b) {
+        return b < a.nseq ? span_of(length_of(a, b), a.window, a.sinks).total : -1;
+    };
+    const int t0 = blocks_of(lane);  // (all there is to read for up to 64 sequences)
+    uint64_t mine = max(t0, 0);
+    int widest = max(t0, 0);
+    for (int b = lane + 64; b < a.nseq; b += 64) {
+        const int t = blocks_of(b);
+        mine += (uint64_t)t;
+        widest = max(widest, t);
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) total += __shfl_xor((unsigned long long)total, d);
-    int per;
-    if (total >> 32)
-        per = (int)((total + a.target_items - 1) / (uint64_t)a.target_items);
-    else
-        per = (int)(((uint32_t)total + (uint32_t)a.target_items - 1) / (uint32_t)a.target_items);
-    per = max(per, kMinBlocks);
-    int base = 0;
+    // (2^20 sequences of 2^26 blocks at most)
+    const uint64_t total = ((uint64_t)wave_sum((uint32_t)(mine >> 20)) << 20) +
+                           wave_sum((uint32_t)mine & 0xFFFFF);
+    auto over = [&](int items) {
+        return total >> 31 ? (int)((total + items - 1) / (uint64_t)items)
+                           : (int)(((uint32_t)total + items - 1) / (uint32_t)items);
+    };
+    // Lengths far apart: pieces a third as long, which spread better (64
+    // sequences of 65 to 8,190 positions 98 against 107 us, 256 of 100 to 4,000
+    // 128 against 139); about equal ones: as few joins as can be (64 of 4,096
+    // 191 against 196 us).
+    const int longest = (int)wave_max((float)widest);
+    const int items = (uint64_t)longest * a.nseq > 2 * total ? a.most_items : a.most_items / 3;
+    const int per = max(max(over(max(items, 1)), min(over(a.few_items), kGoodBlocks)), kMinBlocks);
+    it.per = per;
+    int wholes = 0;
+    for (int b0 = 0; b0 < a.nseq; b0 += 64)
+        wholes += (int)wave_sum((uint32_t)max(b0 ? blocks_of(b0 + lane) : t0, 0) / (uint32_t)per);
+    // the sequence whose whole pieces, or whose rest, the item's number falls into
+    const bool rest_item = item >= wholes;
+    int base = 0, rank = wholes;
     for (int b0 = 0; b0 < a.nseq; b0 += 64) {
-        const int b = b0 + lane;
-        int cnt = 0;
-        if (b < a.nseq) {
-            const int t = span_of(length_of(a, b), a.window, a.sinks).total;
-            cnt = max(t / per + (t % per != 0), 1);
-        }
-        int incl = cnt;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(incl, d);
-            if (lane >= d) incl += o;
-        }
-        const uint64_t past = __ballot(base + incl > item);
+        const int t = b0 ? blocks_of(b0 + lane) : t0;
+        const int whole = (int)((uint32_t)max(t, 0) / (uint32_t)per);
+        // (a sequence without blocks has its empty answer to write)
+        const int rest = t >= 0 && (t == 0 || t != whole * per);
+        const int wsum = base + prefix_sum(whole), rsum = rank + prefix_sum(rest);
+        const uint64_t past = __ballot(rest_item ? rsum > item : wsum > item);
         if (past) {
             const int l = __builtin_ctzll(past);
             it.b = b0 + l;
-            it.nsplit = __shfl(cnt, l);
-            it.split = item - base - (__shfl(incl, l) - it.nsplit);
-            it.per = per;
+            it.whole = __builtin_amdgcn_readlane(whole, l);
+            it.rest = __builtin_amdgcn_readlane(rest, l);
+            it.first = __builtin_amdgcn_readlane(wsum, l) - it.whole;
+            it.split = rest_item ? it.whole : item - it.first;
             return true;
         }
-        base += __shfl(incl, 63);
+        base = __builtin_amdgcn_readlane(wsum, 63);
+        rank = __builtin_amdgcn_readlane(rsum, 63);
     }
     return false;
+}
+
+// The larger of the four lanes that share a column (lanes apart by 16).
+__device__ __forceinline__ float column_max(float x) {
+    typedef unsigned u32pair __attribute__((ext_vector_type(2)));
+    u32pair p = __builtin_amdgcn_permlane16_swap(bits_of(x), bits_of(x), false, false);
+    x = fmaxf(float_of(p.x), float_of(p.y));
+    p = __builtin_amdgcn_permlane32_swap(bits_of(x), bits_of(x), false, false);
+    return fmaxf(float_of(p.x), float_of(p.y));
 }
 
 // 16 bytes of a row from element x on, whatever the row's alignment.
@@ -142,17 +172,24 @@ __device__ __forceinline__ u32x4_t load_piece(const char *row, int x, bool vec) 
 // bf16: P is multiplied as the sum of two bf16 values (its first 8 bits and
 // the rest rounded to 8), so it is good to 2^-17 and the output is as exact
 // as its last rounding.
-template <int ST, int D, int WG = (D <= 96 ? 3 : D <= 208 ? 2 : 1)>
+//
+// In the loop a unit's keys are replaced by the next one's as soon as they are
+// multiplied, and so are its values: loads are in flight all the time.
+template <int ST, int D, int WG = (D <= 96 ? 3 : D <= (ST ? 192 : 160) ? 2 : 1)>
 __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
     constexpr int E = ST ? 8 : 4;
     constexpr int ES = 16 / E;             // element size
     constexpr int H = ST ? 2 : 1;          // 16-position halves per unit
+    constexpr int UB = ST ? 1 : 2;         // units per block
     constexpr int NC = (D / E + 3) / 4;    // 16-byte pieces per lane of a key row
     constexpr int ND = D / 16;
     constexpr int DW = D < kJoinDims ? D : kJoinDims;
     constexpr int LD = DW + 4;
+    constexpr float kNone = -__builtin_huge_valf();
     extern __shared__ __align__(16) float lds_o[];  // [wave][query][LD]
     __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
+    __shared__ u32x4_t lds_k[D / E];  // the new token
+    __shared__ uint32_t lds_v[D];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -163,10 +200,6 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
     const int gc = min(a.group - gt * 16, 16);  // query heads of this workgroup
     Item it;
     if (!find_item(a, item, lane, it)) return;
-    it.b = __builtin_amdgcn_readfirstlane(it.b);
-    it.split = __builtin_amdgcn_readfirstlane(it.split);
-    it.nsplit = __builtin_amdgcn_readfirstlane(it.nsplit);
-    const int per = __builtin_amdgcn_readfirstlane(it.per);
     const int n = __builtin_amdgcn_readfirstlane(length_of(a, it.b));
     const Span sp = span_of(n, a.window, a.sinks);
     const int head0 = kvh * a.group + gt * 16;
@@ -182,25 +215,28 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
         }
     }
 
-    float m = -__builtin_huge_valf(), l = 0.f;
+    float m = kNone, l = 0.f;
     f32x4_t o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     const int32_t *trow = a.table + (int64_t)it.b * a.width;
-    const int64_t head_base = a.layer_off + (int64_t)kvh * a.head_off;
+    char *const head_base = a.pool + a.layer_off + (int64_t)kvh * a.head_off;
     const int bpp1 = (1 << (a.page_shift - 5)) - 1;
-    const int j0 = it.split * per, j1 = min(j0 + per, sp.total);
-    const int u1 = ST ? j1 : 2 * j1;
-    // first position of unit u
+    const int j0 = it.split * it.per, j1 = min(j0 + it.per, sp.total);
+    // first position of unit u, counted along the span
     auto unit_pos = [&](int u) {
-        const int j = ST ? u : u >> 1;
-        return (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock + (ST ? 0 : (u & 1) * 16);
+        const int j = u / UB;
+        return (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock + u % UB * 16;
     };
-    // its keys; a position without a page reads page 0 and is hidden below
-    auto unit_base = [&](int page, int pos0) {
-        return a.pool + ((int64_t)((unsigned)page < (unsigned)a.npages ? page : 0) * a.page_bytes +
-                         head_base + ((pos0 >> 5 & bpp1) * kKvBlock + (pos0 & 16)) * (D * ES));
+    auto unit_keys = [&](int page, int pos) {
+        return head_base + (int64_t)page * a.page_bytes +
+               (((pos >> 5) & bpp1) * kKvBlock + (pos & 16)) * (D * ES);
+    };
+    // blocks with a mask in them
+    const bool cut = a.window > 0 && n > a.window;
+    auto edge = [&](int j) {
+        return j == sp.total - 1 || (cut && (j == sp.nsb || j == sp.nsb - 1));
     };
     u32x4_t kf[H * NC], vf[ND];
     auto load_keys = [&](const char *kb) {
@@ -218,74 +254,13 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
         for (int d = 0; d < ND; ++d)
             vf[d] = *(const u32x4_t *)(kb + a.kv_off + ((d * 16 + r) * 4 + g) * 16);
     };
-    int u = (ST ? j0 : 2 * j0) + wave;
-    int pos0 = 0, page = 0;
-    char *kb = a.pool;
-    if (u < u1) {
-        pos0 = unit_pos(u);
-        page = trow[pos0 >> a.page_shift];
-        kb = unit_base(page, pos0);
-        load_keys(kb);
-        load_values(kb);
-    }
-    while (u < u1) {
-        const int un = u + kWaves;
-        int pos_n = 0, page_n = 0;
-        if (un < u1) {
-            pos_n = unit_pos(un);
-            page_n = trow[pos_n >> a.page_shift];
-        }
-        char *vb = kb + a.kv_off;
-        const bool here = (unsigned)page < (unsigned)a.npages;
-        if constexpr (D % (4 * E) != 0) {
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-                if ((NC - 1) * 4 + g >= D / E) kf[h * NC + NC - 1] = u32x4_t{0, 0, 0, 0};
-        }
-
-        const int tn = n - 1 - pos0;  // the new token's place in this unit
-        if (a.k && here && tn < 16 * H && tn >= 0) {
-            // its keys and values take their places in the registers and, from
-            // one workgroup per key-value head, in the page
-            const char *krow = a.k + ((int64_t)it.b * a.k_seq + (int64_t)kvh * a.k_head) * ES;
-            const char *vrow = a.v + ((int64_t)it.b * a.v_seq + (int64_t)kvh * a.v_head) * ES;
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int c = 0; c < NC; ++c)
-                    if (tn == 16 * h + r && c * 4 + g < D / E) {
-                        const u32x4_t w = load_piece<ST>(krow, (c * 4 + g) * E, a.k_vec);
-                        kf[h * NC + c] = w;
-                        if (gt == 0)
-                            *(u32x4_t *)(kb + ((h * (D / E) + c * 4 + g) * 16 + r) * 16) = w;
-                    }
-            if (((tn & 15) >> 2) == g) {
-                const int e = (tn >> 4) * 4 + (tn & 3);  // its element of the lane's 16 bytes
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    char *to = vb + ((d * 16 + r) * 4 + g) * 16 + e * ES;
-                    if constexpr (ST) {
-                        const uint16_t x = ((const uint16_t *)vrow)[d * 16 + r];
-#pragma unroll
-                        for (int w = 0; w < 4; ++w)
-                            if (w == e >> 1)
-                                vf[d][w] = e & 1 ? (vf[d][w] & 0xFFFFu) | (uint32_t)x << 16
-                                                 : (vf[d][w] & 0xFFFF0000u) | x;
-                        if (gt == 0) *(uint16_t *)to = x;
-                    } else {
-                        const uint32_t x = ((const uint32_t *)vrow)[d * 16 + r];
-#pragma unroll
-                        for (int w = 0; w < 4; ++w)
-                            if (w == e) vf[d][w] = x;
-                        if (gt == 0) *(uint32_t *)to = x;
-                    }
-                }
-            }
-        }
-
-        f32x4_t s[H];
+    f32x4_t s[H];
+    auto scores = [&]() {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
+            if constexpr (D % (4 * E) != 0) {
+                if ((NC - 1) * 4 + g >= D / E) kf[h * NC + NC - 1] = u32x4_t{0, 0, 0, 0};
+            }
             s[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -297,58 +272,20 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                            float_of(kf[h * NC + c][e]),
-                            float_of(qf[c][e]), s[h], 0, 0, 0);
+                            float_of(kf[h * NC + c][e]), float_of(qf[c][e]), s[h], 0, 0, 0);
                 }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[h][i] *= a.scale2;
         }
-        // the next unit's keys take the place of these, its values that of
-        // these further down: loads are in flight all the time
-        char *kb_n = kb;
-        if (un < u1) {
-            kb_n = unit_base(page_n, pos_n);
-            load_keys(kb_n);
-        }
-
-        const int lo = n - a.window;  // with a window: positions below are invisible but for the sinks
-        if (!here || pos0 + 16 * H > n ||
-            (a.window > 0 && pos0 < lo && pos0 + 16 * H > a.sinks)) {
-            // a masked position's score is -inf and its values are 0: what
-            // lies there may be anything, and 0 times a NaN is one
-            uint32_t hide = 0;
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int p = pos0 + 16 * h + 4 * g + i;
-                    if (!here || p >= n || (a.window > 0 && p < lo && p >= a.sinks)) {
-                        s[h][i] = -__builtin_huge_valf();
-                        hide |= 1u << (4 * h + i);
-                    }
-                }
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t keep = ~0u;
-                if constexpr (ST) {
-                    if (hide >> (2 * w) & 1) keep &= 0xFFFF0000u;
-                    if (hide >> (2 * w + 1) & 1) keep &= 0x0000FFFFu;
-                } else {
-                    if (hide >> w & 1) keep = 0;
-                }
-#pragma unroll
-                for (int d = 0; d < ND; ++d) vf[d][w] &= keep;
-            }
-        }
-
+    };
+    auto weigh = [&]() {
         float top = s[0][0];
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = column_max(top);
         if (__ballot(top > m)) {
             const float mn = fmaxf(m, top);
             const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -359,45 +296,189 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[d][i] *= f;
         }
-        const float ms = m == -__builtin_huge_valf() ? 0.f : m;
-        f32x4_t p[H];
+        const float ms = m == kNone ? 0.f : m;
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[h][i] = __builtin_amdgcn_exp2f(s[h][i] - ms);
-                l += p[h][i];
+                s[h][i] = __builtin_amdgcn_exp2f(s[h][i] - ms);
+                l += s[h][i];
             }
+    };
+    auto add_values = [&]() {
         if constexpr (ST) {
-            bf16x8_t hi, lo8;
+            bf16x8_t hi, lo;
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float t = float_of(bits_of(p[h][i]) & 0xFFFF0000u);
+                    const float p = s[h][i], t = float_of(bits_of(p) & 0xFFFF0000u);
                     hi[4 * h + i] = (__bf16)t;
                     // (never 0 beside a weight: an infinite value times 0 would be a NaN)
-                    lo8[4 * h + i] = (__bf16)fmaxf(p[h][i] - t, p[h][i] * 0x1p-60f);
+                    lo[4 * h + i] = (__bf16)fmaxf(p - t, p * 0x1p-60f);
                 }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 const bf16x8_t w = __builtin_bit_cast(bf16x8_t, vf[d]);
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, hi, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, lo8, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, lo, o[d], 0, 0, 0);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                        float_of(vf[d][i]), p[0][i], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(float_of(vf[d][i]), s[0][i], o[d],
+                                                                0, 0, 0);
         }
-        if (un < u1) load_values(kb_n);
-        u = un;
-        pos0 = pos_n;
-        page = page_n;
-        kb = kb_n;
+    };
+
+    // The wave's units in order: 64 at a time, lane i looks the page of the i-th
+    // up, and those that have one are a bit mask.
+    const int u0 = j0 * UB + wave, count = max((j1 * UB - u0 + kWaves - 1) / kWaves, 0);
+    int chunk = -64, pages = -1;
+    uint64_t ready = 0;
+    int u_n = 0;  // the unit found, and its keys
+    const char *kb_n = a.pool;
+    auto next_unit = [&]() {
+        while (!ready) {
+            chunk += 64;
+            if (chunk >= count) return false;
+            pages = -1;
+            if (chunk + lane < count)
+                pages = trow[unit_pos(u0 + (chunk + lane) * kWaves) >> a.page_shift];
+            ready = __ballot((unsigned)pages < (unsigned)a.npages);
+        }
+        const int i = __builtin_ctzll(ready);
+        ready &= ready - 1;
+        u_n = u0 + (chunk + i) * kWaves;
+        kb_n = unit_keys(__builtin_amdgcn_readlane(pages, i), unit_pos(u_n));
+        return true;
+    };
+
+    // The new token, at position n - 1: read before all else and laid down in
+    // LDS, so that no load of it is waited for at the end.
+    int u_new = -1, t_new = 0;  // the unit that holds it, if it is the wave's, and its place there
+    u32x4_t k_new = {0, 0, 0, 0};
+    uint32_t v_new[(D + 63) / 64];
+    int new_page = -1;
+    if (a.k && sp.total > 0) {
+        t_new = (n - 1) % (16 * H);
+        const int u = (sp.total - 1) * UB + (n - 1) % kKvBlock / (16 * H);
+        if (u >= u0 && u < j1 * UB && (u - u0) % kWaves == 0) {
+            new_page = trow[(n - 1) >> a.page_shift];
+            if ((unsigned)new_page < (unsigned)a.npages) u_new = u;
+        }
+    }
+    if (u_new >= 0) {
+        const char *krow = a.k + ((int64_t)it.b * a.k_seq + (int64_t)kvh * a.k_head) * ES;
+        const char *vrow = a.v + ((int64_t)it.b * a.v_seq + (int64_t)kvh * a.v_head) * ES;
+        if (lane < D / E) k_new = load_piece<ST>(krow, lane * E, a.k_vec);
+#pragma unroll
+        for (int i = 0; i < (D + 63) / 64; ++i) {
+            const int x = min(lane + 64 * i, D - 1);
+            v_new[i] = ST ? ((const uint16_t *)vrow)[x] : ((const uint32_t *)vrow)[x];
+        }
+    }
+    bool more = next_unit();
+    const bool any = more;
+    if (any) {
+        load_keys(kb_n);
+        load_values(kb_n);
+    }
+    if (u_new >= 0) {
+        if (lane < D / E) lds_k[lane] = k_new;
+#pragma unroll
+        for (int i = 0; i < (D + 63) / 64; ++i)
+            if (lane + 64 * i < D) lds_v[lane + 64 * i] = v_new[i];
+        lds_wave_sync();
+    }
+    if (any) {
+        int u;
+        do {
+            u = u_n;
+            more = next_unit();
+            // (loads under a condition would be waited for as if those behind
+            // them had not been issued: the last unit reads some page again)
+            const char *kb = more ? kb_n : head_base;
+            if (u == u_new) {
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+                        if (t_new == 16 * h + r && c * 4 + g < D / E)
+                            kf[h * NC + c] = lds_k[c * 4 + g];
+                // stored with its neighbours, in whole cache lines
+                if (gt == 0) {
+                    char *to = unit_keys(new_page, unit_pos(u));
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int c = 0; c < NC; ++c)
+                            if (t_new / 16 == h && c * 4 + g < D / E)
+                                *(u32x4_t *)(to + ((h * (D / E) + c * 4 + g) * 16 + r) * 16) =
+                                    kf[h * NC + c];
+                }
+            }
+            scores();
+            load_keys(kb);
+            if (u == u_new) {
+                const bool mine = (t_new & 15) >> 2 == g;
+                const int at = (t_new >> 4) * 4 + (t_new & 3);  // its element of the lane's 16 bytes
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const uint32_t x = lds_v[d * 16 + r];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        if constexpr (ST) {
+                            if (mine && w == at >> 1)
+                                vf[d][w] = at & 1 ? (vf[d][w] & 0xFFFFu) | x << 16
+                                                  : (vf[d][w] & 0xFFFF0000u) | x;
+                        } else {
+                            if (mine && w == at) vf[d][w] = x;
+                        }
+                    }
+                }
+                if (gt == 0) {
+                    char *to = unit_keys(new_page, unit_pos(u)) + a.kv_off;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        *(u32x4_t *)(to + ((d * 16 + r) * 4 + g) * 16) = vf[d];
+                }
+            }
+            if (edge(u / UB)) {
+                // a masked position's score is -inf and its values are 0: what
+                // lies there may be anything, and 0 times a NaN is one
+                const int pos0 = unit_pos(u);
+                const int low = a.window > 0 ? n - a.window : 0;  // below, only sinks are visible
+                uint32_t hide = 0;
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int p = pos0 + 16 * h + 4 * g + i;
+                        if (p >= n || (p < low && p >= a.sinks)) {
+                            s[h][i] = kNone;
+                            hide |= 1u << (4 * h + i);
+                        }
+                    }
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t keep = ~0u;
+                    if constexpr (ST) {
+                        if (hide >> (2 * w) & 1) keep &= 0xFFFF0000u;
+                        if (hide >> (2 * w + 1) & 1) keep &= 0x0000FFFFu;
+                    } else {
+                        if (hide >> w & 1) keep = 0;
+                    }
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) vf[d][w] &= keep;
+                }
+            }
+            weigh();
+            add_values();
+            load_values(kb);
+        } while (more);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -407,7 +488,7 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
     }
 
     // the four waves' sums, kJoinDims dimensions at a time
-    const bool last = it.nsplit == 1;
+    const bool last = it.whole + it.rest <= 1;
 #pragma unroll
     for (int d0 = 0; d0 < ND; d0 += DW / 16) {
         if (d0) __syncthreads();
@@ -424,7 +505,7 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
             float top = lds_m[0][row];
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][row]);
-            const float ms = top == -__builtin_huge_valf() ? 0.f : top;
+            const float ms = top == kNone ? 0.f : top;
             float sum = 0.f;
             f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -448,81 +529,94 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
                 }
                 if (a.lse && dim == 0)
                     a.lse[(int64_t)it.b * a.heads + head] =
-                        sum == 0.f ? -__builtin_huge_valf()
-                                   : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+                        sum == 0.f ? kNone : (top + __builtin_amdgcn_logf(sum)) * kLn2;
             } else {
-                const int64_t slot = (int64_t)item * a.heads + head;
+                const int64_t slot =
+                    (int64_t)(it.split < it.whole ? item : a.most_items + it.b) * a.heads + head;
                 *(f32x4_t *)(a.part_o + slot * D + dim) = acc;
                 if (dim == 0) a.part_ml[slot] = make_float2(top, sum);
             }
         }
     }
-    if (!last && hh == 0 && it.split == 0 && threadIdx.x == 0)
-        a.first[it.b] = make_int2(item, it.nsplit);
-    if (last && hh == 0 && threadIdx.x == 0) a.first[it.b] = make_int2(item, 1);
+    if (a.first && hh == 0 && it.split == 0 && threadIdx.x == 0)
+        a.first[it.b] = make_int2(it.first, it.whole * 2 + it.rest);
 }
 
-// Joins the items of a sequence, in their order: one wave per query head.
+// Joins the items of a sequence, in their order: one workgroup per query head,
+// its waves taking every fourth item.  (The workgroup that is done last could
+// do it and save the launch; but the fences that this needs between the L2
+// caches, one per workgroup, took longer: 16 sequences of 4,096 positions 76
+// against 58 us.)
 template <int ST, int D>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * kWaves) void attend_join_kernel(AttendArgs a) {
     constexpr int NR = (D + 63) / 64;
     constexpr int ES = ST ? 2 : 4;
+    constexpr float kNone = -__builtin_huge_valf();
+    __shared__ float lds_a[kWaves][NR * 64];
     const int lane = threadIdx.x & 63;
-    const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (at >= (int64_t)a.nseq * a.heads) return;
-    const int b = (int)(at / a.heads), head = (int)(at % a.heads);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
     const int2 f = a.first[b];
-    if (f.y <= 1) return;
-    float top = -__builtin_huge_valf();
-    for (int s = lane; s < f.y; s += 64)
-        top = fmaxf(top, a.part_ml[(int64_t)(f.x + s) * a.heads + head].x);
+    const int whole = f.y >> 1, cnt = whole + (f.y & 1);
+    if (cnt <= 1) return;
+    auto slot_of = [&](int s) {
+        return (int64_t)(s < whole ? f.x + s : a.most_items + b) * a.heads + head;
+    };
+    // eight of the wave's partial sums at a time, the first ones in flight while
+    // the maximum and the sum over all items are found (by every wave)
+    float t[8][NR], w[8], acc[NR];
+    auto load = [&](int s0) {
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float ms = top == -__builtin_huge_valf() ? 0.f : top;
-    float sum = 0.f, acc[NR];
+        for (int e = 0; e < 8; ++e) {
+            const int64_t slot = slot_of(min(s0 + e * kWaves, cnt - 1));
+            w[e] = a.part_ml[slot].x;
 #pragma unroll
-    for (int i = 0; i < NR; ++i) acc[i] = 0.f;
-    for (int s0 = 0; s0 < f.y; s0 += 64) {
-        float w = 0.f;
-        if (s0 + lane < f.y) {
-            const float2 ml = a.part_ml[(int64_t)(f.x + s0 + lane) * a.heads + head];
-            w = __builtin_amdgcn_exp2f(ml.x - ms);
-            sum += w * ml.y;
+            for (int i = 0; i < NR; ++i)
+                t[e][i] = a.part_o[slot * D + min(lane + 64 * i, D - 1)];
         }
-        const int cnt = min(64, f.y - s0);
-        const float *po = a.part_o + ((int64_t)(f.x + s0) * a.heads + head) * D + lane;
-        for (int s = 0; s < cnt; s += 8) {
-            float t[8][NR];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    t[e][i] = 0.f;
-                    if (s + e < cnt && lane + 64 * i < D)
-                        t[e][i] = po[(int64_t)(s + e) * a.heads * D + 64 * i];
-                }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float ws = __shfl(w, s + e);  // (0 past the last item)
-#pragma unroll
-                for (int i = 0; i < NR; ++i) acc[i] += ws * t[e][i];
-            }
-        }
+    };
+    load(wave);
+    float top = kNone, sum = 0.f;
+    for (int s = lane; s < cnt; s += 64) {
+        const float2 ml = a.part_ml[slot_of(s)];
+        const float mn = fmaxf(top, ml.x);
+        const float ms = mn == kNone ? 0.f : mn;
+        sum = sum * __builtin_amdgcn_exp2f(top - ms) + ml.y * __builtin_amdgcn_exp2f(ml.x - ms);
+        top = mn;
     }
+    const float m = wave_max(top), ms = m == kNone ? 0.f : m;
+    sum *= __builtin_amdgcn_exp2f(top - ms);
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    char *to = a.out + ((int64_t)b * a.o_seq + (int64_t)head * a.o_head) * ES;
 #pragma unroll
-    for (int i = 0; i < NR; ++i)
-        if (lane + 64 * i < D) {
-            if constexpr (ST)
-                ((__bf16 *)to)[lane + 64 * i] = (__bf16)(acc[i] * inv);
-            else
-                ((float *)to)[lane + 64 * i] = acc[i] * inv;
-        }
-    if (a.lse && lane == 0)
-        a.lse[at] = sum == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    for (int i = 0; i < NR; ++i) acc[i] = 0.f;
+    for (int s0 = wave; s0 < cnt; s0 += 8 * kWaves) {
+        if (s0 != wave) load(s0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (s0 + e * kWaves < cnt) {
+                const float x = __builtin_amdgcn_exp2f(w[e] - ms);
+#pragma unroll
+                for (int i = 0; i < NR; ++i) acc[i] += x * t[e][i];
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) lds_a[wave][lane + 64 * i] = acc[i];
+    __syncthreads();
+    const int dim = threadIdx.x;
+    if (dim < D) {
+        float x = lds_a[0][dim];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) x += lds_a[w][dim];
+        x *= sum == 0.f ? 0.f : 1.f / sum;
+        char *to = a.out + ((int64_t)b * a.o_seq + (int64_t)head * a.o_head) * ES;
+        if constexpr (ST)
+            ((__bf16 *)to)[dim] = (__bf16)x;
+        else
+            ((float *)to)[dim] = x;
+    }
+    if (a.lse && threadIdx.x == 0)
+        a.lse[blockIdx.x] = sum == 0.f ? kNone : (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // The place of position t of a block, dimension x, in elements.
@@ -623,9 +717,8 @@ hipError_t launch_attend(const AttendArgs &a, int64_t items, bool join, hipStrea
                        dim3(64 * kWaves), lds, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !join) return e;
-    const int64_t rows = (int64_t)a.nseq * a.heads;
-    hipLaunchKernelGGL((attend_join_kernel<ST, D>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0,
-                       st, a);
+    hipLaunchKernelGGL((attend_join_kernel<ST, D>), dim3((uint32_t)a.nseq * (uint32_t)a.heads),
+                       dim3(64 * kWaves), 0, st, a);
     return hipGetLastError();
 }
 
@@ -800,31 +893,35 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
     a.q_vec = vs::pieces_ok(q, q_seq, q_head, e);
     a.k_vec = vs::pieces_ok(k, k_seq, k_head, e);
 
-    // Work items: as many as fill the card, and one more per sequence at most
-    // for the division's remainders.
+    // Work items: whole ones of so many blocks that two or six workgroups come
+    // to a CU, and one per sequence for what is left of it.
     const int64_t per_item = (int64_t)a.kv_heads * a.gtiles;
-    const int64_t target = std::max<int64_t>(1, (4 * kv->num_cu + per_item - 1) / per_item);
+    auto items_of = [&](int64_t wgs) {
+        return std::max<int64_t>(1, (wgs + per_item - 1) / per_item);
+    };
+    a.most_items = (int)items_of(6 * kv->num_cu);
+    a.few_items = (int)items_of(kv->num_cu);
     // the most blocks that a sequence of this table can have
     int64_t most = s->width * (kv->page_size / vs::kKvBlock);
     if (window > 0)
         most = std::min(most, (window + vs::kKvBlock - 1) / vs::kKvBlock + 1 +
                                   (sinks + vs::kKvBlock - 1) / vs::kKvBlock);
-    const int64_t splits = std::max<int64_t>(1, (most + vs::kMinBlocks - 1) / vs::kMinBlocks);
-    a.target_items = (int)target;
-    const int64_t items = std::min(target + s->nseq, splits * s->nseq);
-    const bool join = splits > 1;
-    if (items * per_item > INT32_MAX)
+    const bool join = most > vs::kMinBlocks;
+    const int64_t items = a.most_items + s->nseq;
+    if (items * per_item > INT32_MAX || s->nseq * heads > INT32_MAX)
         return report(VS_ERR_UNSUPPORTED, "%lld sequences of %lld heads", (long long)s->nseq,
                       (long long)heads);
-    void *ws = nullptr;
-    const int64_t slots = join ? items * heads : 0;
-    const size_t o_bytes = (size_t)slots * kv->head_dim * sizeof(float);
-    const size_t ml_bytes = (size_t)slots * sizeof(float2);
-    rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)s->nseq * sizeof(int2), &ws);
-    if (rc) return rc;
-    a.part_o = (float *)ws;
-    a.part_ml = (float2 *)((char *)ws + o_bytes);
-    a.first = (int2 *)((char *)ws + o_bytes + ml_bytes);
+    if (join) {
+        const size_t slots = (size_t)(items * heads);
+        const size_t o_bytes = slots * kv->head_dim * sizeof(float);
+        const size_t ml_bytes = slots * sizeof(float2);
+        void *ws = nullptr;
+        rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)s->nseq * sizeof(int2), &ws);
+        if (rc) return rc;
+        a.part_o = (float *)ws;
+        a.part_ml = (float2 *)((char *)ws + o_bytes);
+        a.first = (int2 *)((char *)ws + o_bytes + ml_bytes);
+    }
     hipError_t err = kv->dtype == VS_DTYPE_BF16
                          ? vs::launch_attend_dim<1>(a, items, join, (int)kv->head_dim, st)
                          : vs::launch_attend_dim<0>(a, items, join, (int)kv->head_dim, st);

@@ -2,6 +2,7 @@
 // vocabulary, and the reordering of their states.
 #include "vs_host.h"
 #include "vs_device.h"
+#include "vs_wave.h"
 
 struct vs_beam {
     int device = 0;
@@ -98,40 +99,6 @@ struct Step {
         return first + ((i / E) * 64 + lane) * E + i % E;
     }
 };
-
-// Wave-wide reductions in the vector registers (data-parallel primitives: a
-// shuffle through LDS takes several times as long).  What a step does not
-// reach keeps `same`, which changes nothing.
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ uint32_t dpp(uint32_t same, uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_update_dpp((int)same, (int)x, CTRL, ROWS, 0xf, false);
-}
-constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
-constexpr int kBcast15 = 0x142, kBcast31 = 0x143;
-
-// The largest x of the wave, in every lane (NaNs are passed over).
-__device__ __forceinline__ float wave_max(float x) {
-    x = fmaxf(x, float_of(dpp<kSwap1>(bits_of(x), bits_of(x))));
-    x = fmaxf(x, float_of(dpp<kSwap2>(bits_of(x), bits_of(x))));
-    x = fmaxf(x, float_of(dpp<kHalfMirror>(bits_of(x), bits_of(x))));
-    x = fmaxf(x, float_of(dpp<kMirror>(bits_of(x), bits_of(x))));
-    const float a = float_of(__builtin_amdgcn_readlane(bits_of(x), 0));
-    const float b = float_of(__builtin_amdgcn_readlane(bits_of(x), 16));
-    const float c = float_of(__builtin_amdgcn_readlane(bits_of(x), 32));
-    const float d = float_of(__builtin_amdgcn_readlane(bits_of(x), 48));
-    return fmaxf(fmaxf(a, b), fmaxf(c, d));
-}
-
-// Inclusive prefix sum over the lanes.
-__device__ __forceinline__ int prefix_sum(int x) {
-    x += (int)dpp<0x111>(0, x);            // one lane up within rows of 16, then 2, 4, 8
-    x += (int)dpp<0x112>(0, x);
-    x += (int)dpp<0x114>(0, x);
-    x += (int)dpp<0x118>(0, x);
-    x += (int)dpp<kBcast15, 0xa>(0, x);    // rows 1 and 3 take the sum of the one before
-    x += (int)dpp<kBcast31, 0xc>(0, x);    // the upper half that of the lower
-    return x;
-}
 
 // Larger logit first, then the lower token, as one 64-bit number.
 __device__ __forceinline__ uint64_t key_of(float v, int token) {
