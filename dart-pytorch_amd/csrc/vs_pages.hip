@@ -3,38 +3,29 @@
 // lengths and reference counts live on the device, so a decoding loop never
 // waits for the host to manage them.
 #include "vs_kv.h"
+#include "vs_wave.h"
 
 namespace vs {
 namespace {
 
 constexpr int kPlan = 1024;         // threads of the one-workgroup plans
 constexpr int kMostFresh = 1 << 20;  // pages that one extend gives a sequence
-constexpr int kPieceBytes = 16384;  // of a page, per workgroup pass of the copy
+constexpr int kSmallPages = 16384;    // of a cache whose compaction is planned in registers
+constexpr int kForkSeqs = 1024;      // sequences and words of a fork that one workgroup does
+constexpr int kForkWords = 1 << 12;
+constexpr int kPieceBytes = 8192;   // of a page, per workgroup pass of the copy
 
 // Exclusive prefix sum of x over the workgroup's kPlan threads; *total its sum.
 __device__ __forceinline__ int block_scan(int x, int *total, int *lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int incl = x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(incl, d);
-        if (lane >= d) incl += o;
-    }
+    const int incl = prefix_sum(x);
     __syncthreads();
     if (lane == 63) lds[wave] = incl;
     __syncthreads();
-    if (wave == 0) {
-        int w = lane < kPlan / 64 ? lds[lane] : 0;
-#pragma unroll
-        for (int d = 1; d < kPlan / 64; d <<= 1) {
-            const int o = __shfl_up(w, d);
-            if (lane >= d) w += o;
-        }
-        if (lane < kPlan / 64) lds[lane] = w;
-    }
-    __syncthreads();
-    *total = lds[kPlan / 64 - 1];
-    return incl - x + (wave ? lds[wave - 1] : 0);
+    // every wave sums the waves' totals for itself
+    const int w = prefix_sum(lane < kPlan / 64 ? lds[lane] : 0);
+    *total = __builtin_amdgcn_readlane(w, 63);
+    return incl - x + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
 }
 
 struct ExtendArgs {
@@ -50,60 +41,114 @@ struct ExtendArgs {
 };
 
 // Divides the free pages among the sequences, as one workgroup: the work is a
-// few thousand numbers, and its steps need each other's results.
+// few thousand numbers, and its steps need each other's results.  What bounds
+// it is the chain of loads (length, table entry, count), so a thread keeps what
+// it reads of its first sequence, the first pages' counts are read beside it,
+// and up to kPlan sequences meet on their shared pages in LDS (SMALL).
+template <bool SMALL>
 __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
+    constexpr int kHash = 2 * kPlan;
     __shared__ int lds[kPlan / 64];
     __shared__ int bad, huge;
+    __shared__ int h_page[SMALL ? kHash : 1], h_holders[SMALL ? kHash : 1], h_lowest[SMALL ? kHash : 1];
+    __shared__ int fresh[4 * kPlan];  // the first free pages that are needed
     const int P = 1 << a.page_shift;
     const int64_t most = a.width << a.page_shift;
+    int refs0[4];  // of the first 4 kPlan pages
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t p = 4 * threadIdx.x + i;
+        refs0[i] = p < a.npages ? a.refs[p] : 1;
+    }
+    struct Seq {
+        int n, count, page, refs;  // page: a partly filled last page that others hold too, or -1
+    };
+    auto read = [&](int b) {
+        Seq s = {0, 0, -1, 0};
+        if (b >= a.nseq) return s;
+        s.n = max(a.lens[b], 0);
+        s.count = max(a.count_dev ? a.count_dev[b] : a.count, 0);
+        if ((s.n & (P - 1)) && s.n <= most && s.count) {
+            const int p = a.table[(int64_t)b * a.width + ((s.n - 1) >> a.page_shift)];
+            if ((unsigned)p < (unsigned)a.npages) {
+                s.refs = a.refs[p];
+                if (s.refs > 1) s.page = p;
+            }
+        }
+        return s;
+    };
     if (threadIdx.x == 0) {
         bad = huge = 0;
         a.copies[0] = 0;
     }
-    // the last page of a sequence, where it is partly filled and others hold it too
-    auto count_of = [&](int b) { return max(a.count_dev ? a.count_dev[b] : a.count, 0); };
-    auto shared_page = [&](int b, int n) {
-        if (!(n & (P - 1)) || n > most || !count_of(b)) return -1;
-        const int p = a.table[(int64_t)b * a.width + ((n - 1) >> a.page_shift)];
-        return (unsigned)p < (unsigned)a.npages && a.refs[p] > 1 ? p : -1;
-    };
-    for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
-        const int p = shared_page(b, max(a.lens[b], 0));
-        if (p >= 0) {
-            a.holders[p] = 0;
-            a.lowest[p] = INT32_MAX;
+    if constexpr (SMALL) {
+        for (int i = threadIdx.x; i < kHash; i += kPlan) {
+            h_page[i] = -1;
+            h_holders[i] = 0;
+            h_lowest[i] = INT32_MAX;
         }
     }
+    const Seq first = read(threadIdx.x);
+    int place = 0;  // of its page in the hash table
     __syncthreads();
-    for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
-        const int p = shared_page(b, max(a.lens[b], 0));
-        if (p >= 0) {
-            atomicAdd(&a.holders[p], 1);
-            atomicMin(&a.lowest[p], b);
+    if constexpr (SMALL) {
+        if (first.page >= 0) {
+            place = (int)((uint32_t)first.page * 2654435761u >> 21) & (kHash - 1);
+            for (;;) {  // (at most kPlan pages in 2 kPlan places: one is free)
+                const int was = atomicCAS(&h_page[place], -1, first.page);
+                if (was == -1 || was == first.page) break;
+                place = (place + 1) & (kHash - 1);
+            }
+            atomicAdd(&h_holders[place], 1);
+            atomicMin(&h_lowest[place], (int)threadIdx.x);
+        }
+    } else {
+        for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
+            const int p = read(b).page;
+            if (p >= 0) {
+                a.holders[p] = 0;
+                a.lowest[p] = INT32_MAX;
+            }
+        }
+        __syncthreads();
+        for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
+            const int p = read(b).page;
+            if (p >= 0) {
+                atomicAdd(&a.holders[p], 1);
+                atomicMin(&a.lowest[p], b);
+            }
         }
     }
     __syncthreads();
     int64_t need = 0;  // (equal in all threads)
+    int at0 = 0;       // the thread's first sequence's first new page; its copy
+    bool copy0 = false;
     for (int b0 = 0; b0 < a.nseq; b0 += kPlan) {
         const int b = b0 + threadIdx.x;
-        int want = 0, copy = 0;
-        if (b < a.nseq) {
-            const int n = max(a.lens[b], 0), c = count_of(b);
-            if (c && (int64_t)n + c > most) {
-                bad = 1;
-            } else if (c) {
-                const int p = shared_page(b, n);
-                copy = p >= 0 && !(a.lowest[p] == b && a.holders[p] == a.refs[p]);
-                want = copy + (int)(((int64_t)n + c + P - 1) >> a.page_shift) -
-                       (int)(((int64_t)n + P - 1) >> a.page_shift);
-                if (want > min(a.npages, kMostFresh)) huge = 1;  // refused: no sum below passes 32 bits
-                want = min(want, kMostFresh);
+        const Seq s = b0 ? read(b) : first;
+        int want = 0;
+        bool copy = false;
+        if (s.count && (int64_t)s.n + s.count > most) {
+            bad = 1;
+        } else if (s.count) {
+            if (s.page >= 0) {
+                if constexpr (SMALL)
+                    copy = !(h_lowest[place] == b && h_holders[place] == s.refs);
+                else
+                    copy = !(a.lowest[s.page] == b && a.holders[s.page] == s.refs);
             }
+            want = copy + (int)(((int64_t)s.n + s.count + P - 1) >> a.page_shift) -
+                   (int)(((int64_t)s.n + P - 1) >> a.page_shift);
+            if (want > min(a.npages, kMostFresh)) huge = 1;  // refused: no sum below passes 32 bits
+            want = min(want, kMostFresh);
         }
         int total;
-        const int at = block_scan(want, &total, lds);
-        if (b < a.nseq)
-            a.offset[b] = (int)min(need + at, (int64_t)INT32_MAX) | (copy ? (int)0x80000000 : 0);
+        const int at = (int)min(need + block_scan(want, &total, lds), (int64_t)INT32_MAX);
+        if (b0 == 0) {
+            at0 = at;
+            copy0 = copy;
+        }
+        if (!SMALL && b < a.nseq) a.offset[b] = at | (copy ? (int)0x80000000 : 0);
         need += total;
     }
     __syncthreads();
@@ -111,26 +156,26 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
         if (threadIdx.x == 0) atomicOr(&a.status[0], kStatusWidth);
         return;
     }
-    if (need == 0) {  // everyone has room
-        for (int b = threadIdx.x; b < a.nseq; b += kPlan) a.lens[b] = max(a.lens[b], 0) + count_of(b);
-        return;
-    }
-    // the lowest `need` free pages
+    // the lowest `need` free pages, the first in LDS
     int64_t found = 0;
     for (int64_t p0 = 0; p0 < a.npages && found < need; p0 += 4 * kPlan) {
         int free[4], cnt = 0;
         const int64_t p = p0 + 4 * threadIdx.x;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            free[i] = p + i < a.npages && a.refs[p + i] == 0;
+            free[i] = p0 ? p + i < a.npages && a.refs[p + i] == 0 : refs0[i] == 0;
             cnt += free[i];
         }
         int total, at = block_scan(cnt, &total, lds);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (free[i]) {
-                if (found + at < need) a.fresh[found + at] = (int)(p + i);
-                ++at;
+                const int64_t x = found + at++;
+                if (x >= need) continue;
+                if (x < 4 * kPlan)
+                    fresh[x] = (int)(p + i);
+                else
+                    a.fresh[x] = (int)(p + i);
             }
         found += total;
     }
@@ -142,14 +187,17 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
         return;
     }
     __syncthreads();
+    auto take = [&](int x) { return x < 4 * kPlan ? fresh[x] : a.fresh[x]; };
     for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
-        const int n = max(a.lens[b], 0), c = count_of(b);
+        const bool mine = b == (int)threadIdx.x;
+        const int n = mine ? first.n : max(a.lens[b], 0);
+        const int c = mine ? first.count : max(a.count_dev ? a.count_dev[b] : a.count, 0);
         if (!c) continue;
-        int at = a.offset[b] & 0x7FFFFFFF;
+        int at = mine ? at0 : a.offset[b] & 0x7FFFFFFF;
         int32_t *row = a.table + (int64_t)b * a.width;
-        if (a.offset[b] < 0) {
+        if (mine ? copy0 : a.offset[b] < 0) {
             int32_t *entry = &row[(n - 1) >> a.page_shift];
-            const int from = *entry, to = a.fresh[at++];
+            const int from = mine ? first.page : *entry, to = take(at++);
             const int i = atomicAdd(&a.copies[0], 1);  // (their order does not matter)
             a.copies[1 + 2 * i] = from;
             a.copies[2 + 2 * i] = to;
@@ -159,7 +207,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
         }
         const int64_t end = ((int64_t)n + c + P - 1) >> a.page_shift;
         for (int64_t e = ((int64_t)n + P - 1) >> a.page_shift; e < end; ++e) {
-            const int to = a.fresh[at++];
+            const int to = take(at++);
             a.refs[to] = 1;
             row[e] = to;
         }
@@ -167,13 +215,30 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
     }
 }
 
-// Copies pages: HBM-bound, so only the 16-byte loads in flight matter.  The
-// grid walks (page, piece) pairs; `n_dev` is read on the device because the
-// host does not know how many pages a plan moves.
+// Copies pages: HBM-bound.  Nothing is read twice, so loads and stores pass the
+// caches by, and many small pieces spread best (1.03 GB of pages: 417 us with
+// cached accesses, 401 without, 390 in 8 KB pieces by 32 workgroups to a CU:
+// 5.3 TB/s read and written).  The grid walks (page, piece) pairs; `n_dev` is
+// read on the device because the host does not know how many pages a plan moves.
+// Compaction's tables (`tables`) are rewritten on the way.
+struct Tables {
+    const int32_t *table, *lens, *map;
+    int32_t *table2, *lens2;
+    int64_t entries;
+    int nseq;
+};
+
 __global__ __launch_bounds__(256) void copy_pages_kernel(char *pool, int64_t page_bytes, int npages,
                                                          const int32_t *n_dev, int64_t n_host,
                                                          const int32_t *from, const int32_t *to,
-                                                         int stride) {
+                                                         int stride, Tables tables) {
+    const int64_t every = (int64_t)gridDim.x * 256;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < tables.entries; x += every) {
+        const int p = tables.table[x];
+        tables.table2[x] = (unsigned)p < (unsigned)npages ? tables.map[p] : p;
+    }
+    for (int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x; b < tables.nseq; b += every)
+        tables.lens2[b] = tables.lens[b];
     const int64_t n = n_dev ? *n_dev : n_host;
     const int64_t pieces = (page_bytes + kPieceBytes - 1) / kPieceBytes;
     for (int64_t w = blockIdx.x; w < n * pieces; w += gridDim.x) {
@@ -187,12 +252,12 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(char *pool, int64_t pag
 #pragma unroll
         for (int k = 0; k < kPieceBytes / 4096; ++k) {
             const int x = k * 4096 + threadIdx.x * 16;
-            if (x < bytes) v[k] = *(const u32x4_t *)(src + x);
+            if (x < bytes) v[k] = __builtin_nontemporal_load((const u32x4_t *)(src + x));
         }
 #pragma unroll
         for (int k = 0; k < kPieceBytes / 4096; ++k) {
             const int x = k * 4096 + threadIdx.x * 16;
-            if (x < bytes) *(u32x4_t *)(dst + x) = v[k];
+            if (x < bytes) __builtin_nontemporal_store(v[k], (u32x4_t *)(dst + x));
         }
     }
 }
@@ -238,6 +303,42 @@ __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a) {
                     if ((unsigned)p < (unsigned)a.npages) atomicAdd(&a.refs[p], c);
                 }
         }
+    }
+}
+
+// The same as one workgroup, where that takes less than a second launch: the
+// counts are copied, then changed.  (4 sequences of 14 entries, 96 pages: 2.2
+// against 4.0 us; 256 of 36, 3,500 pages: 13.7 against 8.8, hence kForkWords.)
+__global__ __launch_bounds__(kPlan) void fork_small_kernel(ForkArgs a, const int32_t *refs_in) {
+    __shared__ int children[kForkSeqs], parent_of[kForkSeqs];
+    for (int i = threadIdx.x; i < a.nin; i += kPlan) children[i] = 0;
+    if (refs_in != a.refs) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < a.npages; i += kPlan) a.refs[i] = refs_in[i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.nout; i += kPlan) {
+        int parent = a.parents[i];
+        if ((unsigned)parent < (unsigned)a.nin) {
+            atomicAdd(&children[parent], 1);
+        } else {
+            if (parent != -1) atomicOr(&a.status[0], kStatusParent);
+            parent = -1;
+        }
+        parent_of[i] = parent;
+        a.lens2[i] = parent >= 0 ? a.lens[parent] : 0;
+    }
+    __syncthreads();
+    const uint32_t width = (uint32_t)a.width, entries = (uint32_t)a.nin * width;
+#pragma unroll 4
+    for (uint32_t x = threadIdx.x; x < (uint32_t)a.nout * width; x += kPlan) {
+        const int parent = parent_of[x / width];
+        a.table2[x] = parent >= 0 ? a.table[(uint32_t)parent * width + x % width] : -1;
+    }
+#pragma unroll 4
+    for (uint32_t x = threadIdx.x; x < entries; x += kPlan) {
+        const int c = children[x / width] - 1, p = a.table[x];
+        if (c && (unsigned)p < (unsigned)a.npages) atomicAdd(&a.refs[p], c);
     }
 }
 
@@ -340,25 +441,74 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(CompactArgs a) {
     if (threadIdx.x == 0) *a.moves = nto;
 }
 
-__global__ __launch_bounds__(256) void compact_table_kernel(const int32_t *table, const int32_t *lens,
-                                                            int32_t *table2, int32_t *lens2,
-                                                            const int32_t *map, int npages,
-                                                            int64_t entries, int nseq) {
-    const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    for (int64_t x = first; x < entries; x += step) {
-        const int p = table[x];
-        table2[x] = (unsigned)p < (unsigned)npages ? map[p] : p;
+// The same for up to kSmallPages pages: the counts are read once, into
+// registers, and the pairs meet in LDS.
+__global__ __launch_bounds__(kPlan) void compact_plan_small_kernel(CompactArgs a) {
+    constexpr int N = kSmallPages / (4 * kPlan);  // rounds of four consecutive pages per thread
+    __shared__ int lds[kPlan / 64];
+    __shared__ uint16_t to[kSmallPages / 2];
+    const int chunks = (a.npages + 4 * kPlan - 1) / (4 * kPlan);
+    int ref[N][4], cnt = 0;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = (c * kPlan + threadIdx.x) * 4 + i;
+            ref[c][i] = p < a.npages ? a.refs[p] : 0;
+            cnt += ref[c][i] != 0;
+        }
+    int live, total, done = 0, at[N];
+    block_scan(cnt, &live, lds);
+    // free pages of the front count 1, live pages past it 2^16
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        if (c >= chunks) break;
+        cnt = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = (c * kPlan + threadIdx.x) * 4 + i;
+            if (p < a.npages) cnt += p < live ? ref[c][i] == 0 : (ref[c][i] != 0) << 16;
+        }
+        at[c] = done + block_scan(cnt, &total, lds);
+        done += total;
+        int t = at[c] & 0xFFFF;  // the thread's place in the list of free pages
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = (c * kPlan + threadIdx.x) * 4 + i;
+            if (p >= a.npages) continue;
+            if (p < live && ref[c][i] == 0) to[t++] = (uint16_t)p;
+            a.refs2[p] = p < live ? ref[c][i] : 0;
+            a.map[p] = p;
+        }
     }
-    for (int64_t b = first; b < nseq; b += step) lens2[b] = lens[b];
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        if (c >= chunks) break;
+        int f = at[c] >> 16;  // and in that of pages to move
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = (c * kPlan + threadIdx.x) * 4 + i;
+            if (p >= a.npages || p < live || ref[c][i] == 0) continue;
+            const int dst = to[f];
+            a.map[p] = dst;
+            a.refs2[dst] = ref[c][i];
+            a.from[f] = p;
+            a.to[f] = dst;
+            ++f;
+        }
+    }
+    if (threadIdx.x == 0) *a.moves = done & 0xFFFF;
 }
 
 hipError_t launch_copy(const vs_kv *kv, const int32_t *n_dev, int64_t n_max, const int32_t *from,
-                       const int32_t *to, int stride, hipStream_t st) {
+                       const int32_t *to, int stride, hipStream_t st, const Tables &tables = {}) {
     const int64_t pieces = (kv->page_bytes + kPieceBytes - 1) / kPieceBytes;
-    const int64_t wgs = std::min<int64_t>((int64_t)kv->num_cu * 8, n_max * pieces);
+    const int64_t wgs = std::min<int64_t>((int64_t)kv->num_cu * 32,
+                                          std::max(n_max * pieces, (tables.entries + 255) / 256));
     if (wgs <= 0) return hipSuccess;
     hipLaunchKernelGGL(copy_pages_kernel, dim3((uint32_t)wgs), dim3(256), 0, st, kv->mem,
-                       kv->page_bytes, (int)kv->npages, n_dev, n_max, from, to, stride);
+                       kv->page_bytes, (int)kv->npages, n_dev, n_max, from, to, stride, tables);
     return hipGetLastError();
 }
 
@@ -410,7 +560,10 @@ int vs_kv_extend(vs_kv *kv, const vs_kv_seqs *s, int64_t count, const int32_t *c
     a.fresh = a.lowest + np;
     a.offset = a.fresh + np;
     a.copies = a.offset + ns;
-    hipLaunchKernelGGL(vs::extend_plan_kernel, dim3(1), dim3(vs::kPlan), 0, st, a);
+    if (ns <= vs::kPlan)
+        hipLaunchKernelGGL(vs::extend_plan_kernel<true>, dim3(1), dim3(vs::kPlan), 0, st, a);
+    else
+        hipLaunchKernelGGL(vs::extend_plan_kernel<false>, dim3(1), dim3(vs::kPlan), 0, st, a);
     VS_LAUNCHED("extend");
     hipError_t e = vs::launch_copy(kv, a.copies, ns, a.copies + 1, a.copies + 2, 2, st);
     return e == hipSuccess ? VS_OK : report_hip(e, "page copies");
@@ -432,12 +585,6 @@ int vs_kv_fork(vs_kv *kv, const vs_kv_seqs *in, const int32_t *parents, const vs
     vs::DeviceGuard g(kv->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
-    if (in->refs != out->refs) {
-        hipLaunchKernelGGL(vs::copy_words_kernel, dim3(vs::grid_of((kv->npages + 255) / 256, 2048)),
-                           dim3(256), 0, st, in->refs, out->refs, kv->npages);
-        VS_LAUNCHED("fork");
-    }
-    if (in->nseq + out->nseq == 0) return VS_OK;
     vs::ForkArgs a = {};
     a.table = in->table;
     a.lens = in->lens;
@@ -450,8 +597,19 @@ int vs_kv_fork(vs_kv *kv, const vs_kv_seqs *in, const int32_t *parents, const vs
     a.nout = (int)out->nseq;
     a.npages = (int)kv->npages;
     a.status = kv->status;
-    hipLaunchKernelGGL(vs::fork_kernel, dim3(vs::grid_of(in->nseq + out->nseq, 65536)), dim3(256), 0,
-                       st, a);
+    const int64_t both = in->nseq + out->nseq;
+    if (std::max(in->nseq, out->nseq) <= vs::kForkSeqs && kv->npages + both * (in->width + 1) < vs::kForkWords) {
+        hipLaunchKernelGGL(vs::fork_small_kernel, dim3(1), dim3(vs::kPlan), 0, st, a, in->refs);
+        VS_LAUNCHED("fork");
+        return VS_OK;
+    }
+    if (in->refs != out->refs) {
+        hipLaunchKernelGGL(vs::copy_words_kernel, dim3(vs::grid_of((kv->npages + 255) / 256, 2048)),
+                           dim3(256), 0, st, in->refs, out->refs, kv->npages);
+        VS_LAUNCHED("fork");
+    }
+    if (both == 0) return VS_OK;
+    hipLaunchKernelGGL(vs::fork_kernel, dim3(vs::grid_of(both, 65536)), dim3(256), 0, st, a);
     VS_LAUNCHED("fork");
     return VS_OK;
 }
@@ -511,17 +669,15 @@ int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out, void *
     a.from = a.map + np;
     a.to = a.from + np;
     a.moves = a.to + np;
-    hipLaunchKernelGGL(vs::compact_plan_kernel, dim3(1), dim3(vs::kPlan), 0, st, a);
+    if (np <= vs::kSmallPages)
+        hipLaunchKernelGGL(vs::compact_plan_small_kernel, dim3(1), dim3(vs::kPlan), 0, st, a);
+    else
+        hipLaunchKernelGGL(vs::compact_plan_kernel, dim3(1), dim3(vs::kPlan), 0, st, a);
     VS_LAUNCHED("compact");
-    const int64_t entries = in->nseq * in->width;
-    if (in->nseq) {
-        hipLaunchKernelGGL(vs::compact_table_kernel,
-                           dim3(vs::grid_of((std::max(entries, in->nseq) + 255) / 256, 2048)),
-                           dim3(256), 0, st, in->table, in->lens, out->table, out->lens, a.map,
-                           (int)np, entries, (int)in->nseq);
-        VS_LAUNCHED("compact");
-    }
-    hipError_t e = vs::launch_copy(kv, a.moves, np / 2 + 1, a.from, a.to, 1, st);
+    const vs::Tables tables = {in->table,  in->lens,  a.map,
+                               out->table, out->lens, in->nseq * in->width,
+                               (int)in->nseq};
+    hipError_t e = vs::launch_copy(kv, a.moves, np / 2 + 1, a.from, a.to, 1, st, tables);
     return e == hipSuccess ? VS_OK : report_hip(e, "page copies");
 }
 

@@ -141,7 +141,8 @@ def test_fork_in_one_set_of_counts(vs):
     p.agrees(out)
 
 
-@pytest.mark.parametrize("npages,live", [(10, 4), (4096, 1000), (4097, 4000), (9000, 3), (5, 5), (70, 0)])
+@pytest.mark.parametrize("npages,live", [(10, 4), (4096, 1000), (4097, 4000), (9000, 3), (5, 5), (70, 0), (16384, 8192),
+                                         (16385, 8000), (20_001, 15_000)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_compact(vs, npages, live, in_place):
     rng = np.random.default_rng(npages)
@@ -190,10 +191,11 @@ def test_copy_pages(vs, layers, kv, dim):
     p.agrees()
 
 
-def test_many_sequences_and_pages(vs):
-    """Past one workgroup's threads, with most last pages shared."""
+@pytest.mark.parametrize("n", [1500, 1024, 700])
+def test_many_sequences_and_pages(vs, n):
+    """Up to and past one workgroup's threads, with most last pages shared."""
     rng = np.random.default_rng(5)
-    n, npages = 1500, 9000
+    npages = 9000
     ids = rng.permutation(npages)
     lens = rng.integers(0, 90, n)
     table = np.full((n, 4), -1, np.int32)
