@@ -14,7 +14,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kWaves = 4;      // per workgroup
 constexpr int kMinBlocks = 4;  // blocks per work item, at least: one per wave
 constexpr int kGoodBlocks = 8; // and before a CU takes a second workgroup
-constexpr int kJoinDims = 128; // dimensions joined over the waves at once (LDS)
+// dimensions joined over the waves at once, by what LDS holds
+constexpr int join_dims(int waves) { return waves == 8 ? 64 : 128; }
+constexpr int kWideDim = 128;  // heads up to this size have an eight-wave kernel
 
 struct AttendArgs {
     char *pool;
@@ -29,6 +31,7 @@ struct AttendArgs {
     int heads, kv_heads, group, gtiles;  // group: query heads per key-value head; gtiles: 16 at a time
     float scale2;                        // scale * log2(e)
     int window, sinks;
+    int unsplit;                         // one item per sequence
     int q_vec, k_vec;                    // rows readable in 16-byte pieces
     int most_items, few_items;           // six workgroups to a CU, and one
     float *part_o;   // [item][heads][dim]
@@ -175,19 +178,22 @@ __device__ __forceinline__ u32x4_t load_piece(const char *row, int x, bool vec) 
 //
 // In the loop a unit's keys are replaced by the next one's as soon as they are
 // multiplied, and so are its values: loads are in flight all the time.
-template <int ST, int D, int WG = (D <= 96 ? 3 : D <= (ST ? 192 : 160) ? 2 : 1)>
-__global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
+// NW waves: four, or eight where short sequences are not split and a workgroup
+// has a whole one (a.unsplit).
+template <int ST, int D, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 160) ? 2 : 1)
+    void attend_kernel(AttendArgs a) {
     constexpr int E = ST ? 8 : 4;
     constexpr int ES = 16 / E;             // element size
     constexpr int H = ST ? 2 : 1;          // 16-position halves per unit
     constexpr int UB = ST ? 1 : 2;         // units per block
     constexpr int NC = (D / E + 3) / 4;    // 16-byte pieces per lane of a key row
     constexpr int ND = D / 16;
-    constexpr int DW = D < kJoinDims ? D : kJoinDims;
+    constexpr int DW = D < join_dims(NW) ? D : join_dims(NW);
     constexpr int LD = DW + 4;
     constexpr float kNone = -__builtin_huge_valf();
     extern __shared__ __align__(16) float lds_o[];  // [wave][query][LD]
-    __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
+    __shared__ float lds_m[NW][16], lds_l[NW][16];
     __shared__ u32x4_t lds_k[D / E];  // the new token
     __shared__ uint32_t lds_v[D];
 
@@ -198,8 +204,14 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
     const int item = blockIdx.x / per_item, hh = blockIdx.x % per_item;
     const int gt = hh / a.kv_heads, kvh = hh % a.kv_heads;
     const int gc = min(a.group - gt * 16, 16);  // query heads of this workgroup
-    Item it;
-    if (!find_item(a, item, lane, it)) return;
+    Item it = {};
+    if (a.unsplit) {
+        it.b = item;
+        it.per = INT32_MAX / kKvBlock;
+        it.rest = 1;
+    } else if (!find_item(a, item, lane, it)) {
+        return;
+    }
     const int n = __builtin_amdgcn_readfirstlane(length_of(a, it.b));
     const Span sp = span_of(n, a.window, a.sinks);
     const int head0 = kvh * a.group + gt * 16;
@@ -335,7 +347,7 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
 
     // The wave's units in order: 64 at a time, lane i looks the page of the i-th
     // up, and those that have one are a bit mask.
-    const int u0 = j0 * UB + wave, count = max((j1 * UB - u0 + kWaves - 1) / kWaves, 0);
+    const int u0 = j0 * UB + wave, count = max((j1 * UB - u0 + NW - 1) / NW, 0);
     int chunk = -64, pages = -1;
     uint64_t ready = 0;
     int u_n = 0;  // the unit found, and its keys
@@ -346,12 +358,12 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
             if (chunk >= count) return false;
             pages = -1;
             if (chunk + lane < count)
-                pages = trow[unit_pos(u0 + (chunk + lane) * kWaves) >> a.page_shift];
+                pages = trow[unit_pos(u0 + (chunk + lane) * NW) >> a.page_shift];
             ready = __ballot((unsigned)pages < (unsigned)a.npages);
         }
         const int i = __builtin_ctzll(ready);
         ready &= ready - 1;
-        u_n = u0 + (chunk + i) * kWaves;
+        u_n = u0 + (chunk + i) * NW;
         kb_n = unit_keys(__builtin_amdgcn_readlane(pages, i), unit_pos(u_n));
         return true;
     };
@@ -365,7 +377,7 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
     if (a.k && sp.total > 0) {
         t_new = (n - 1) % (16 * H);
         const int u = (sp.total - 1) * UB + (n - 1) % kKvBlock / (16 * H);
-        if (u >= u0 && u < j1 * UB && (u - u0) % kWaves == 0) {
+        if (u >= u0 && u < j1 * UB && (u - u0) % NW == 0) {
             new_page = trow[(n - 1) >> a.page_shift];
             if ((unsigned)new_page < (unsigned)a.npages) u_new = u;
         }
@@ -487,7 +499,7 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
         lds_l[wave][r] = l;
     }
 
-    // the four waves' sums, kJoinDims dimensions at a time
+    // the waves' sums, DW dimensions at a time
     const bool last = it.whole + it.rest <= 1;
 #pragma unroll
     for (int d0 = 0; d0 < ND; d0 += DW / 16) {
@@ -499,17 +511,17 @@ __global__ __launch_bounds__(64 * kWaves, WG) void attend_kernel(AttendArgs a) {
                     *(f32x4_t *)(lds_o + (wave * gc + r) * LD + d * 16 + g * 4) = o[d0 + d];
         __syncthreads();
         const int dims = min(DW, D - d0 * 16);
-        for (int x = threadIdx.x; x < gc * (DW / 4); x += 64 * kWaves) {
+        for (int x = threadIdx.x; x < gc * (DW / 4); x += 64 * NW) {
             const int row = x / (DW / 4), c4 = x % (DW / 4);
             if (c4 * 4 >= dims) continue;
             float top = lds_m[0][row];
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][row]);
+            for (int w = 1; w < NW; ++w) top = fmaxf(top, lds_m[w][row]);
             const float ms = top == kNone ? 0.f : top;
             float sum = 0.f;
             f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float f = __builtin_amdgcn_exp2f(lds_m[w][row] - ms);
                 sum += f * lds_l[w][row];
                 const f32x4_t t = *(const f32x4_t *)(lds_o + (w * gc + row) * LD + c4 * 4);
@@ -709,13 +721,21 @@ __global__ __launch_bounds__(256) void read_kernel(RowsArgs a) {
     }
 }
 
+template <int ST, int D, int NW>
+hipError_t launch_items(const AttendArgs &a, int64_t items, hipStream_t st) {
+    constexpr int DW = D < join_dims(NW) ? D : join_dims(NW);
+    const size_t lds = (size_t)NW * std::min(a.group, 16) * (DW + 4) * sizeof(float);
+    hipLaunchKernelGGL((attend_kernel<ST, D, NW>), dim3((uint32_t)(items * a.kv_heads * a.gtiles)),
+                       dim3(64 * NW), lds, st, a);
+    return hipGetLastError();
+}
+
 template <int ST, int D>
-hipError_t launch_attend(const AttendArgs &a, int64_t items, bool join, hipStream_t st) {
-    constexpr int DW = D < kJoinDims ? D : kJoinDims;
-    const size_t lds = (size_t)kWaves * std::min(a.group, 16) * (DW + 4) * sizeof(float);
-    hipLaunchKernelGGL((attend_kernel<ST, D>), dim3((uint32_t)(items * a.kv_heads * a.gtiles)),
-                       dim3(64 * kWaves), lds, st, a);
-    hipError_t e = hipGetLastError();
+hipError_t launch_attend(const AttendArgs &a, int64_t items, int waves, bool join, hipStream_t st) {
+    if constexpr (D <= kWideDim) {
+        if (waves == 8) return launch_items<ST, D, 8>(a, items, st);
+    }
+    hipError_t e = launch_items<ST, D, kWaves>(a, items, st);
     if (e != hipSuccess || !join) return e;
     hipLaunchKernelGGL((attend_join_kernel<ST, D>), dim3((uint32_t)a.nseq * (uint32_t)a.heads),
                        dim3(64 * kWaves), 0, st, a);
@@ -723,12 +743,12 @@ hipError_t launch_attend(const AttendArgs &a, int64_t items, bool join, hipStrea
 }
 
 template <int ST>
-hipError_t launch_attend_dim(const AttendArgs &a, int64_t items, bool join, int dim,
+hipError_t launch_attend_dim(const AttendArgs &a, int64_t items, int waves, bool join, int dim,
                              hipStream_t st) {
     switch (dim) {
 #define VS_DIM(D) \
     case D:       \
-        return launch_attend<ST, D>(a, items, join, st);
+        return launch_attend<ST, D>(a, items, waves, join, st);
         VS_DIM(16) VS_DIM(32) VS_DIM(48) VS_DIM(64) VS_DIM(80) VS_DIM(96) VS_DIM(112) VS_DIM(128)
         VS_DIM(144) VS_DIM(160) VS_DIM(176) VS_DIM(192) VS_DIM(208) VS_DIM(224) VS_DIM(240)
         VS_DIM(256)
@@ -848,7 +868,6 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
         return report(VS_ERR_INVALID, "heads (%lld) must be a multiple of kv_heads (%lld)",
                       (long long)heads, (long long)kv->kv_heads);
     if (heads > (1 << 16)) return report(VS_ERR_UNSUPPORTED, "more than 65,536 heads");
-    if (!q || !out) return report(VS_ERR_INVALID, "null q or out");
     if (!k != !v) return report(VS_ERR_INVALID, "k and v are given together or not at all");
     if (window < 0 || sinks < 0) return report(VS_ERR_INVALID, "negative window or sinks");
     if (!std::isfinite(scale)) return report(VS_ERR_INVALID, "scale is not finite");
@@ -858,6 +877,7 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
     for (int64_t x : {q_seq, q_head, k_seq, k_head, v_seq, v_head, out_seq, out_head})
         if (!vs::stride_ok(x)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
     if (s->nseq == 0) return VS_OK;
+    if (!q || !out) return report(VS_ERR_INVALID, "null q or out");
     vs::DeviceGuard g(kv->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
@@ -906,8 +926,19 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
     if (window > 0)
         most = std::min(most, (window + vs::kKvBlock - 1) / vs::kKvBlock + 1 +
                                   (sinks + vs::kKvBlock - 1) / vs::kKvBlock);
-    const bool join = most > vs::kMinBlocks;
-    const int64_t items = a.most_items + s->nseq;
+    // Short sequences are not split: a workgroup of eight waves, or four where
+    // there are workgroups enough, goes through one faster than a second launch
+    // joins its parts.  How short, by how many workgroups that leaves (8
+    // key-value heads of 128, not split against split: 1 sequence of 500
+    // positions 8.8 and 9.5 us, of 1,000 11.4 and 9.6; 16 of 1,000 15 and 19; 64
+    // of 1,000 55 and 58, 256 of them 214 and 222; lengths far apart want parts
+    // earlier: fp32, 16 sequences of 17 to 1,023 16 and 14).
+    const int64_t units = most * (e == 2 ? 1 : 2), wgs = s->nseq * per_item;
+    const int waves = wgs >= 2 * kv->num_cu || kv->head_dim > vs::kWideDim ? vs::kWaves : 8;
+    const int each = wgs < kv->num_cu / 2 ? 2 : wgs < 2 * kv->num_cu ? 4 : 8;
+    a.unsplit = most <= vs::kMinBlocks || units <= each * waves;
+    const bool join = !a.unsplit;
+    const int64_t items = a.unsplit ? s->nseq : a.most_items + s->nseq;
     if (items * per_item > INT32_MAX || s->nseq * heads > INT32_MAX)
         return report(VS_ERR_UNSUPPORTED, "%lld sequences of %lld heads", (long long)s->nseq,
                       (long long)heads);
@@ -923,8 +954,10 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
         a.first = (int2 *)((char *)ws + o_bytes + ml_bytes);
     }
     hipError_t err = kv->dtype == VS_DTYPE_BF16
-                         ? vs::launch_attend_dim<1>(a, items, join, (int)kv->head_dim, st)
-                         : vs::launch_attend_dim<0>(a, items, join, (int)kv->head_dim, st);
+                         ? vs::launch_attend_dim<1>(a, items, join ? vs::kWaves : waves, join,
+                                                    (int)kv->head_dim, st)
+                         : vs::launch_attend_dim<0>(a, items, join ? vs::kWaves : waves, join,
+                                                    (int)kv->head_dim, st);
     if (err != hipSuccess) return report_hip(err, "attend");
     return VS_OK;
 }

@@ -36,7 +36,7 @@ inline int check_seqs(const vs_kv *kv, const vs_kv_seqs *s) {
     if (s->nseq > (1 << 20)) return report(VS_ERR_UNSUPPORTED, "more than 2^20 sequences");
     if (s->width > INT32_MAX / kv->page_size)
         return report(VS_ERR_UNSUPPORTED, "table columns past 2^31 positions");
-    if (!s->lens || !s->refs || (!s->table && s->width > 0))
+    if (!s->refs || (s->nseq > 0 && (!s->lens || (!s->table && s->width > 0))))
         return report(VS_ERR_INVALID, "null table, lens or refs");
     return VS_OK;
 }

@@ -152,6 +152,17 @@ def test_split_over_the_length(vs, dtype, kv, heads, n):
     c.compare(c.run())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("width", [1, 4, 5, 15, 16, 17, 31, 32, 33, 63, 64, 65, 66])
+@pytest.mark.parametrize("dim,n", [(64, 1), (64, 40), (144, 2)])
+def test_short_tables_are_not_split(vs, dtype, width, dim, n):
+    """Around the table widths where a sequence is one work item, of four waves or eight, with every length."""
+    lens = [(7 * i * i + 3) % (32 * width + 1) for i in range(n - 1)] + [32 * width]
+    c = Case(vs, lens, 24, 8, dim, 32, dtype, width=width)
+    c.compare(c.run())
+    c.compare(c.run(window=300, sinks=33), 300, 33)
+
+
 def test_many_ragged_sequences(vs):
     """More sequences than lanes; empty ones among them."""
     lens = [(i * 37) % 150 if i % 7 else 0 for i in range(333)] + [2000]
@@ -364,12 +375,12 @@ def test_streams_have_scratch_of_their_own(vs):
 def test_recorded_into_a_graph(vs):
     """A decoding step recorded once and replayed with other contents and eager calls between; a call that would
     have to allocate while it is recorded is refused."""
-    c = Case(vs, [90, 31, 64], 4, 2, 64, 32, "bf16", width=8)
+    c = Case(vs, [90, 31, 64], 4, 2, 64, 32, "bf16", width=300)  # room for sequences that have to be split
     refs = np.bincount(c.table[c.table >= 0], minlength=c.cache.npages).astype(np.int32)
     c.sequences(refs)
     A = vs.DeviceArray
     q, out, st = A.of(c.qb, "bf16"), A.of(np.zeros((3, 4, 64)), "bf16"), Stream()
-    other = c.cache.new_sequences(3, 8)
+    other = c.cache.new_sequences(3, 300)
     parents = A.of([2, 1, 0], "i32")
 
     def step():
@@ -378,10 +389,12 @@ def test_recorded_into_a_graph(vs):
         c.cache.extend(other, 1, stream=st.ptr)
 
     st.begin()
-    with pytest.raises(NotImplementedError, match="scratch"):
-        c.cache.attend(c.seqs, q, out, stream=st.ptr)
-    c.cache.fork(c.seqs, parents, other, stream=st.ptr)
-    st.end()
+    try:
+        with pytest.raises(NotImplementedError, match="scratch"):
+            c.cache.attend(c.seqs, q, out, stream=st.ptr)
+        c.cache.fork(c.seqs, parents, other, stream=st.ptr)
+    finally:
+        st.end()
     step()  # scratch of this size exists now
     st.sync()
     st.begin()
