@@ -105,6 +105,9 @@ const int _storageF32 = 0, _storageAuto = 2;
 
 /// Resolution like cuda_engine.dart:428-455: env override, then
 /// <cwd>/native/lib, then next to the executable, then the loader path.
+/// Where libvs_hip.so is: what every class over it opens.
+String vsLibraryPath() => _findVsLib();
+
 String _findVsLib() {
   final env = Platform.environment['DART_PYTORCH_VS_LIB'];
   if (env != null && env.isNotEmpty) return env;
