@@ -101,8 +101,15 @@ __device__ __forceinline__ bool find_item(const AttendArgs &a, int item, int lan
     // 128 against 139); about equal ones: as few joins as can be (64 of 4,096
     // 191 against 196 us).
     const int longest = (int)wave_max((float)widest);
-    const int items = (uint64_t)longest * a.nseq > 2 * total ? a.most_items : a.most_items / 3;
-    const int per = max(max(over(max(items, 1)), min(over(a.few_items), kGoodBlocks)), kMinBlocks);
+    const bool ragged = (uint64_t)longest * a.nseq > 2 * total;
+    const int items = max(ragged ? a.most_items : a.most_items / 3, 1);
+    int per = max(max(over(items), min(over(a.few_items), kGoodBlocks)), kMinBlocks);
+    // (and equal ones: a small rest of every sequence would be a workgroup more each)
+    if (!ragged && longest > per) {
+        int pieces = (longest + per - 1) / per;
+        if ((uint64_t)pieces * a.nseq > (uint64_t)items) pieces = longest / per;
+        per = (longest + pieces - 1) / pieces;
+    }
     it.per = per;
     int wholes = 0;
     for (int b0 = 0; b0 < a.nseq; b0 += 64)
