@@ -412,14 +412,46 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
         if (a.finished_out) a.finished_out[o0 + s] = 0;
     };
     if (lots <= kMergeCap && n <= kMergeCap) {
+        // Many more than k (few lists, or many of them finished, make the first
+        // entries a weak threshold): the k-th largest of them all, as above.
+        float t2 = t;
+        if (n > 4 * a.k) {
+            if (wave == 0) {
+                uint32_t code[kMergeCap / 64];
+#pragma unroll
+                for (int j = 0; j < kMergeCap / 64; ++j)
+                    code[j] = lane + 64 * j < n ? code_of((float)list[lane + 64 * j].total) : 0;
+                uint32_t c = 0;
+                for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+                    int cnt = 0;
+#pragma unroll
+                    for (int j = 0; j < kMergeCap / 64; ++j)
+                        if (64 * j < n) cnt += __popcll(__ballot(code[j] >= (c | bit)));
+                    if (cnt >= a.k) {
+                        c |= bit;
+                        if (cnt == a.k) break;
+                    }
+                }
+                if (lane == 0) thr = value_of(c);
+            }
+            __syncthreads();
+            t2 = thr;
+        }
         // a candidate's place is how many are better: all pairs at once
+        if (threadIdx.x == 0) npicked = 0;
         for (int c = threadIdx.x; c < n; c += kMergeThreads) place[c] = 0;
         __syncthreads();
-        for (int x = threadIdx.x; x < n * n; x += kMergeThreads)
-            if (better(list[x % n], list[x / n])) atomicAdd(&place[x / n], 1);
-        __syncthreads();
         for (int c = threadIdx.x; c < n; c += kMergeThreads)
-            if (place[c] < a.k) put(place[c], list[c]);
+            if ((float)list[c].total >= t2) picked[atomicAdd(&npicked, 1)] = c;
+        __syncthreads();
+        const int m = npicked;
+        for (int x = threadIdx.x; x < m * m; x += kMergeThreads) {
+            const int me = picked[x / m];
+            if (better(list[picked[x % m]], list[me])) atomicAdd(&place[me], 1);
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < m; c += kMergeThreads)
+            if (place[picked[c]] < a.k) put(place[picked[c]], list[picked[c]]);
         for (int s = n + threadIdx.x; s < a.k; s += kMergeThreads) put_none(s);
         return;
     }

@@ -413,3 +413,17 @@ def test_recorded_into_a_graph(vs):
         assert np.array_equal(table, m.table) and np.array_equal(lens, m.lens)
         assert np.array_equal(other.refs.numpy(), m.refs)
     c.cache.check()
+
+
+def test_failed_allocations(vs):
+    """Scratch that cannot be had: the call fails as out of memory, and the next one works; so does a cache."""
+    c = Case(vs, [5000, 70], 4, 1, 64, 32, "bf16")
+    index = vs.GpuIndexFlat.ip(8)
+    for f in (c.run, lambda: c.cache.extend(c.seqs, 1), lambda: vs.PagedKVCache(4, 32, 1, 32)):
+        index.set_option("fail_alloc", 1)
+        with pytest.raises(vs.VsError, match="memory"):
+            f()
+    index.set_option("fail_alloc", 0)
+    c.compare(c.run())
+    vs.PagedKVCache(4, 32, 1, 32).close()
+    index.close()
