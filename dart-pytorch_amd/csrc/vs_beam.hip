@@ -20,6 +20,7 @@ constexpr int kMostSteps = 64;      // per piece
 constexpr int kCap = 256;           // candidates per piece kept in LDS
 constexpr int kMergeCap = 1024;
 constexpr int kMergeThreads = 512;
+constexpr int kWide = 16;           // entries per thread that a merge holds in registers
 constexpr float kLog2e = 1.44269504088896340736f;
 #define VS_NINF (-__builtin_huge_valf())
 
@@ -282,6 +283,7 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
     __shared__ int picked[kMergeCap];     // lists to read whole
     __shared__ int place[kMergeCap];
     __shared__ int nlist, npicked;
+    __shared__ int counts[2][kMergeThreads / 64];
     __shared__ float thr;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -378,26 +380,68 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
     }
     for (int i = threadIdx.x + kHeads * kMergeThreads; i < lists; i += kMergeThreads)
         pick(i, total_of(i, a.top_v[(row0 * a.npieces + i) * a.k]));
-    auto add = [&](const Cand &c) {
-        const int at = atomicAdd(&nlist, 1);
-        if (at < kMergeCap) list[at] = c;
-    };
-    if ((int)threadIdx.x < a.nbeam && (float)own[threadIdx.x] >= t)
-        add({own[threadIdx.x], 0.f, (int)threadIdx.x, (int)a.eos});
     __syncthreads();
     const int lots = npicked;
-    if (lots <= kMergeCap) {
-        for (int x = threadIdx.x; x < lots * a.k; x += kMergeThreads) {
-            const int i = picked[x / a.k];
-            const int64_t at = (row0 * a.npieces + i) * a.k + x % a.k;
-            const float v = a.top_v[at];
-            const int token = a.top_t[at];
-            const double total = total_of(i, v);
-            if ((float)total >= t) add({total, v, i / a.npieces, token});
+    // what is at or above `low`: of the picked lists, and of the finished beams
+    auto gather = [&](float low) {
+        auto add = [&](const Cand &c) {
+            const int at = atomicAdd(&nlist, 1);
+            if (at < kMergeCap) list[at] = c;
+        };
+        if ((int)threadIdx.x < a.nbeam && (float)own[threadIdx.x] >= low)
+            add({own[threadIdx.x], 0.f, (int)threadIdx.x, (int)a.eos});
+        if (lots <= kMergeCap) {
+            for (int x = threadIdx.x; x < lots * a.k; x += kMergeThreads) {
+                const int i = picked[x / a.k];
+                const int64_t at = (row0 * a.npieces + i) * a.k + x % a.k;
+                const float v = a.top_v[at];
+                const int token = a.top_t[at];
+                const double total = total_of(i, v);
+                if ((float)total >= low) add({total, v, i / a.npieces, token});
+            }
         }
+        __syncthreads();
+        return nlist;
+    };
+    int n = gather(t);
+    if (n > kMergeCap && lots <= kMergeCap && lots * a.k <= kWide * kMergeThreads) {
+        // More than there is room for (the beams' scores lie far apart, and one
+        // beam's lists outdo the others' first entries): the k-th largest of the
+        // lists' entries, held in registers, by counting over the workgroup.
+        uint32_t code[kWide];
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) {
+            const int x = threadIdx.x + j * kMergeThreads;
+            code[j] = 0;
+            if (x < lots * a.k) {
+                const int i = picked[x / a.k];
+                const double total =
+                    total_of(i, a.top_v[(row0 * a.npieces + i) * a.k + x % a.k]);
+                if (total == total) code[j] = code_of((float)total);
+            }
+        }
+        uint32_t c = 0;
+        int flip = 0;
+        for (uint32_t bit = 0x80000000u; bit; bit >>= 1, flip ^= 1) {
+            int cnt = 0;
+#pragma unroll
+            for (int j = 0; j < kWide; ++j)
+                if (j * kMergeThreads < lots * a.k)
+                    cnt += __popcll(__ballot(code[j] >= (c | bit)));
+            if (lane == 0) counts[flip][wave] = cnt;
+            __syncthreads();
+            cnt = 0;
+#pragma unroll
+            for (int w = 0; w < kMergeThreads / 64; ++w) cnt += counts[flip][w];
+            if (cnt >= a.k) {
+                c |= bit;
+                if (cnt == a.k) break;
+            }
+        }
+        if (threadIdx.x == 0) nlist = 0;
+        __syncthreads();
+        n = gather(fmaxf(t, c < code_of(VS_NINF) ? VS_NINF : value_of(c)));
     }
-    __syncthreads();
-    const int n = nlist;
     const int64_t o0 = (int64_t)r * a.k;
     auto put = [&](int s, const Cand &c) {
         a.scores_out[o0 + s] = (float)c.total;

@@ -76,6 +76,17 @@ def test_beams_and_k(vs, W, k):
     check(got, val, sc, k)
 
 
+@pytest.mark.parametrize("W,k,V", [(16, 32, 30_000), (64, 64, 9000), (40, 20, 50_000)])
+@pytest.mark.parametrize("spread", [0.01, 3.0, 28.0])
+def test_scores_near_and_far_apart(vs, W, k, V, spread):
+    """One beam's pieces outdo every other beam's best: more candidates than the merge has room for."""
+    rng = np.random.default_rng(W)
+    x, sc = 2.5 * rng.standard_normal((2 * W, V)), -spread * rng.random((2, W)).astype(np.float32)
+    fin = (rng.random((2, W)) < 0.3).astype(np.uint8)
+    got, val = select(vs, x, sc, k, "bf16", finished=fin, eos=2)
+    check(got, val, sc, k, fin, 2)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_exact_ties(vs, dtype):
     """Few distinct logits, so that most of the choice is among equals: in one beam by token, between beams of
