@@ -100,6 +100,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs &a, int item, int lan
     // sequences of 65 to 8,190 positions 98 against 107 us, 256 of 100 to 4,000
     // 128 against 139); about equal ones: as few joins as can be (64 of 4,096
     // 191 against 196 us).
+    // (past 2^24 blocks a float is off by two of them at most, less than a piece)
     const int longest = (int)wave_max((float)widest);
     const bool ragged = (uint64_t)longest * a.nseq > 2 * total;
     const int items = max(ragged ? a.most_items : a.most_items / 3, 1);
@@ -182,6 +183,12 @@ __device__ __forceinline__ u32x4_t load_piece(const char *row, int x, bool vec) 
 // bf16: P is multiplied as the sum of two bf16 values (its first 8 bits and
 // the rest rounded to 8), so it is good to 2^-17 and the output is as exact
 // as its last rounding.
+//
+// Bound by HBM: each byte of the cache is read once per 16 query heads.  8
+// key-value heads of 128 in bf16: 2 sequences of 120,000 to 131,000 positions
+// 176 us (1.03 GB, 5.9 TB/s of the 6.3 that a plain read reaches), 64 of 65 to
+// 8,190 93 us (470 MB, 5.0 TB/s: the spread of the pieces' ends).  One of 1,000
+// is bound by latency, 7 us.
 //
 // In the loop a unit's keys are replaced by the next one's as soon as they are
 // multiplied, and so are its values: loads are in flight all the time.
@@ -562,7 +569,8 @@ __global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 
 }
 
 // Joins the items of a sequence, in their order: one workgroup per query head,
-// its waves taking every fourth item.  (The workgroup that is done last could
+// its waves taking every fourth item.  Bound by two loads that follow each
+// other and the launch: 2.5 to 5 us.  (The workgroup that is done last could
 // do it and save the launch; but the fences that this needs between the L2
 // caches, one per workgroup, took longer: 16 sequences of 4,096 positions 76
 // against 58 us.)

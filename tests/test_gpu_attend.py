@@ -326,6 +326,29 @@ def test_cache_past_four_gib(vs):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_as_many_positions_as_a_length_counts(vs, dtype):
+    """Positions near 2^31, in a table that names one page over and over: weights and values of one, whose sums
+    are whole numbers and exact but for the join of some 600 items in 32 bits, log sum exp is log n."""
+    page, dim = 1024, 16
+    cache = vs.PagedKVCache(1, page, 1, dim, dtype=dtype)
+    A = vs.DeviceArray
+    one = D.stored(np.ones((page, 1, dim)), dtype)[0]
+    first = vs.KVSequences(A.of([[0]], "i32"), A.of([page], "i32"), A.of([1], "i32"))
+    cache.append(first, A.of(one, dtype), A.of(one, dtype), starts=A.of([0, page], "i32"))
+    q = A.of(D.stored(np.zeros((1, 2, dim)), dtype)[0], dtype)
+    for n in (2 ** 29 + 33, 2 ** 31 - 1024 - 33):
+        seqs = vs.KVSequences(A.of(np.zeros((1, -(-n // page)), np.int32), "i32"), A.of([n], "i32"), A.of([1], "i32"))
+        out, lse = A((1, 2, dim), dtype), A((1, 2), "f32")
+        cache.attend(seqs, q, out, lse=lse)
+        cache.check()
+        o = D.from_bf16(out.numpy()) if dtype == "bf16" else out.numpy()
+        tol = 2 * 600 * 2.0 ** -23
+        D.assert_rounded(o, np.ones(o.shape), tol, dtype)
+        assert np.abs(lse.numpy() - np.log(n)).max() <= tol + 2.0 ** -21 * (np.log(n) + 20)
+    cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_append_and_read(vs, dtype):
     """Rows of several sequences to their last positions, and back; positions without a page are dropped and read 0."""
     c = Case(vs, [70, 0, 33, 128, 5], 2, 2, 48, 32, dtype, layers=2, layer=1)
