@@ -14,9 +14,9 @@ namespace vs {
 namespace {
 
 constexpr int kMaxK = 64, kMaxBeams = 128;
-constexpr int kPer = 16;            // logits per lane and step (an f32x16_t)
-constexpr int kStep = 64 * kPer;    // logits per wave and step
 constexpr int kMostSteps = 64;      // per piece
+constexpr int kLongStep = 32;       // logits per lane and step, in large calls
+constexpr int kShortStep = 16;      // and small ones
 constexpr int kCap = 256;           // candidates per piece kept in LDS
 constexpr int kMergeCap = 1024;
 constexpr int kMergeThreads = 512;
@@ -49,24 +49,35 @@ __device__ __forceinline__ float value_of(uint32_t c) {
     return float_of(c & 0x80000000u ? c & 0x7FFFFFFFu : ~c);
 }
 
-// kStep consecutive logits of a row in a wave's registers.  Which lane holds
+// The larger of three, passing quiet NaNs over (fmaxf would first quiet each of
+// its operands, an instruction more per logit; a signalling NaN may get
+// through, and the row's sum is a NaN then in any case).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// 64 PER consecutive logits of a row in a wave's registers.  Which lane holds
 // which token goes by the token alone, wherever the row starts: equal rows have
 // equal sums to the bit, and their beams tie.
-template <int ST>
+template <int ST, int PER>
 struct Step {
-    static constexpr int E = ST ? 8 : 4, NL = kPer / E, ES = 16 / E;
+    static constexpr int E = ST ? 8 : 4, NL = PER / E, ES = 16 / E;
     u32x4_t w[NL];
 
     // (unaligned 16-byte loads: rows start anywhere)
     __device__ __forceinline__ void load(const char *row, int first, int vocab, int lane) {
-        if (first + kStep <= vocab) {
+        const int left = vocab - first;
 #pragma unroll
-            for (int l = 0; l < NL; ++l)
+        for (int l = 0; l < NL; ++l) {
+            if ((l + 1) * 64 * E <= left) {
                 __builtin_memcpy(&w[l], row + (int64_t)(first + (l * 64 + lane) * E) * ES, 16);
-        } else {
-            // the row's last, partial step: one load per token, all in flight
-#pragma unroll
-            for (int l = 0; l < NL; ++l)
+            } else if (l * 64 * E >= left) {
+                w[l] = ST ? u32x4_t{0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u}
+                          : u32x4_t{0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u};
+            } else {
+                // where the row ends: one load per token, all in flight
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int t = first + (l * 64 + lane) * E + i * (E / 4);
@@ -79,27 +90,34 @@ struct Step {
                         w[l][i] = t < vocab ? v : 0xFF800000u;
                     }
                 }
+            }
         }
     }
-    __device__ __forceinline__ f32x16_t values() const {
-        f32x16_t x;
-#pragma unroll
-        for (int l = 0; l < NL; ++l)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (ST) {
-                    x[l * E + 2 * i] = float_of(w[l][i] << 16);
-                    x[l * E + 2 * i + 1] = float_of(w[l][i] & 0xFFFF0000u);
-                } else {
-                    x[l * E + i] = float_of(w[l][i]);
-                }
-            }
-        return x;
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (ST) {
+            const uint32_t x = w[i / E][i % E / 2];
+            return float_of(i % 2 ? x & 0xFFFF0000u : x << 16);
+        } else {
+            return float_of(w[i / E][i % E]);
+        }
     }
     static __device__ __forceinline__ int token(int first, int i, int lane) {
         return first + ((i / E) * 64 + lane) * E + i % E;
     }
+    // the logit of token(first, i, lane), from memory
+    static __device__ __forceinline__ float reload(const char *row, int first, int i, int vocab,
+                                                   int lane) {
+        const int t = token(first, i, lane);
+        if (t >= vocab) return VS_NINF;
+        return ST ? float_of((uint32_t)((const uint16_t *)row)[t] << 16) : ((const float *)row)[t];
+    }
 };
+
+// How many of the lanes in `in` come before this one.
+__device__ __forceinline__ int below(uint64_t in) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32),
+                                          __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+}
 
 // Larger logit first, then the lower token, as one 64-bit number.
 __device__ __forceinline__ uint64_t key_of(float v, int token) {
@@ -129,18 +147,20 @@ __device__ __forceinline__ void cut_list(uint64_t *cand, int n, int k, int lane)
 }
 
 // One pass over the logits.  A wave takes a piece of a row (every fourth step
-// of a stretch that the workgroup's waves read together), kStep logits at a
-// time with the next step in flight, and leaves the piece's maximum and
-// exponential sum (for the row's log sum exp) and its k largest logits.
+// of a stretch that the workgroup's waves read together), 64 PER logits at a
+// time, and leaves the piece's maximum and exponential sum (for the row's log
+// sum exp) and its k largest logits.
 // The list in LDS takes what is at or above a threshold that k logits seen so
 // far reach: the k-th largest of the lanes' running maxima, found by bisection
-// on ballots.  Most steps of a long piece have nothing at or above it and cost
-// a maximum and an exponential per logit.
+// on ballots.  In most steps of a piece as short as a call's are something is,
+// so large calls take steps of twice the length: half the searches.
 // Large batches in fp32 are bound by HBM: 64 x 8 x 128,000, k = 8, some beams
-// ended, 46 us (232 MB read: 5.0 TB/s).  1 x 4 x 50,001 takes 4.9 us, latency.
-// bf16 has half the bytes for the same arithmetic and is bound by that: BFFIG.
-template <int ST>
-__global__ __launch_bounds__(256) void beam_piece_kernel(BeamArgs a) {
+// ended, 46 us (232 MB read: 5.0 TB/s).  bf16 has half the bytes for the same
+// work and is bound by that, 32 us.  1 x 4 x 50,001 takes 4.9 us, latency.
+template <int ST, int PER>
+__global__ __launch_bounds__(256, PER == kLongStep ? 6 : 1) void beam_piece_kernel(BeamArgs a) {
+    using S = Step<ST, PER>;
+    constexpr int kStep = 64 * PER;
     __shared__ uint64_t lists[4][kCap];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -150,7 +170,7 @@ __global__ __launch_bounds__(256) void beam_piece_kernel(BeamArgs a) {
     const uint32_t row = slot / (uint32_t)a.npieces;
     // a beam without continuations of its own: its logits do not matter
     if (!(a.scores[row] > VS_NINF) || (a.finished && a.finished[row])) return;
-    const char *base = a.logits + row * a.row_stride * Step<ST>::ES;
+    const char *base = a.logits + row * a.row_stride * S::ES;
     const int vocab = (int)a.vocab;
     // four waves share a stretch of the row and take its steps in turn
     const int share = (int)(slot % (uint32_t)a.npieces) >> 2;
@@ -163,14 +183,17 @@ __global__ __launch_bounds__(256) void beam_piece_kernel(BeamArgs a) {
     float sum = 0.f;        // of exp(x - top), the lane's share
     float thr = -__FLT_MAX__;  // (so -inf is no candidate)
     int n = 0;
-    Step<ST> step;
+    S step;
     if (begin < end) step.load(base, begin, vocab, lane);
     for (int first = begin; first < end; first += kNext) {
-        const f32x16_t x = step.values();
-        if (first + kNext < end) step.load(base, first + kNext, vocab, lane);
-        float most = x[0];
+        const S x = step;
+        // (a short step's next one is in flight meanwhile; beside a long one are
+        // other waves', and registers for more of those are worth more: 28.1
+        // against 26.8 us at 97 x 5 x 49,096)
+        if (PER == kShortStep && first + kNext < end) step.load(base, first + kNext, vocab, lane);
+        float most = fmaxf(x.value(0), x.value(1));
 #pragma unroll
-        for (int i = 1; i < kPer; ++i) most = fmaxf(most, x[i]);
+        for (int i = 2; i < PER; i += 2) most = max3(most, x.value(i), x.value(i + 1));
         if (__ballot(most >= thr)) {
             run = fmaxf(run, most);
             const float w = wave_max(most);
@@ -192,34 +215,32 @@ __global__ __launch_bounds__(256) void beam_piece_kernel(BeamArgs a) {
                 }
             }
             if (t > code_of(thr)) thr = value_of(t);
-            uint32_t mask = 0;
+            const int n0 = n;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) mask |= x[i] >= thr ? 1u << i : 0u;
-            const int mine = __popc(mask);
-            int at = prefix_sum(mine);
-            const int more = __builtin_amdgcn_readlane(at, 63);
-            if (n + more <= kCap) {
-                at += n - mine;
-                for (; mask; mask &= mask - 1) {
-                    const int i = __ffs(mask) - 1;
-                    cand[at++] = key_of(x[i], Step<ST>::token(first, i, lane));
+            for (int i = 0; i < PER; ++i) {
+                const float v = x.value(i);
+                const uint64_t in = __ballot(v >= thr);
+                if (in) {
+                    const int at = n + below(in);
+                    if (v >= thr && at < kCap) cand[at] = key_of(v, S::token(first, i, lane));
+                    n += __popcll(in);
                 }
-                n += more;
-            } else {
-                // more than the list holds, ties mostly: a register at a time,
-                // cut to the k best in between.  What ties with the k-th of
-                // these in a later step has a higher token and is out.
-                for (int i = 0; i < kPer; ++i) {
-                    const float v = x[i];
+            }
+            if (n > kCap) {
+                // more than the list holds, ties mostly: again, a register at a
+                // time, cut to the k best in between.  What ties with the k-th
+                // of these in a later step has a higher token and is out.
+                n = n0;
+#pragma unroll 1
+                for (int i = 0; i < PER; ++i) {
+                    const float v = S::reload(base, first, i, vocab, lane);
                     const uint64_t in = __ballot(v >= thr);
                     if (!in) continue;
                     if (n > kCap - 64) {
                         cut_list(cand, n, a.k, lane);
-                        n = a.k;
+                        n = min(n, a.k);
                     }
-                    if (v >= thr)
-                        cand[n + __popcll(in & (((uint64_t)1 << lane) - 1))] =
-                            key_of(v, Step<ST>::token(first, i, lane));
+                    if (v >= thr) cand[n + below(in)] = key_of(v, S::token(first, i, lane));
                     n += __popcll(in);
                 }
                 lds_wave_sync();
@@ -232,7 +253,8 @@ __global__ __launch_bounds__(256) void beam_piece_kernel(BeamArgs a) {
         }
         const float ref = top == VS_NINF ? 0.f : top;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * kLog2e);
+        for (int i = 0; i < PER; ++i) sum += __builtin_amdgcn_exp2f((x.value(i) - ref) * kLog2e);
+        if (PER != kShortStep && first + kNext < end) step.load(base, first + kNext, vocab, lane);
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
@@ -651,8 +673,13 @@ int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_strid
     // Pieces short enough for 64 waves to a CU, three times what it holds at
     // once: where beams have ended their waves leave at once, and the others
     // spread.  (64 x 8 x 128,000 fp32: 32 waves to a CU 61, 64 58, 128 58 us.)
-    const int64_t row_steps = (vocab + 4 * vs::kStep - 1) / (4 * vs::kStep) * 4;
+    // Long steps where 32 waves to a CU have one (bf16, short against long: 16 x
+    // 5 x 32,000, k = 10 14.0 and 14.5 us; 30 x 4 x 40,000, k = 4 14.5 and 14.6; 97
+    // x 5 x 49,096, k = 10 28.1 and 26.8; 64 x 8 x 128,000, k = 8 43.5 and 40.1).
     const int64_t waves = (int64_t)bs->num_cu * 64;
+    const bool is_long = nreq * nbeam * vocab >= (int64_t)bs->num_cu * 32 * 64 * vs::kLongStep;
+    const int64_t stretch = 4 * 64 * (is_long ? vs::kLongStep : vs::kShortStep);
+    const int64_t row_steps = (vocab + stretch - 1) / stretch * 4;
     a.steps = (int)std::min<int64_t>(vs::kMostSteps,
                                      std::max<int64_t>(1, (nreq * nbeam * row_steps + waves - 1) / waves));
     a.npieces = (int)((row_steps / 4 + a.steps - 1) / a.steps * 4);
@@ -672,10 +699,15 @@ int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_strid
     a.top_v = (float *)(a.stat + slots);
     a.top_t = (int32_t *)(a.top_v + slots * k);
     const dim3 grid((uint32_t)((slots + 3) / 4));
-    if (dtype == VS_DTYPE_BF16)
-        hipLaunchKernelGGL(vs::beam_piece_kernel<1>, grid, dim3(256), 0, st, a);
+    const bool bf16 = dtype == VS_DTYPE_BF16;
+    if (is_long && bf16)
+        hipLaunchKernelGGL((vs::beam_piece_kernel<1, vs::kLongStep>), grid, dim3(256), 0, st, a);
+    else if (is_long)
+        hipLaunchKernelGGL((vs::beam_piece_kernel<0, vs::kLongStep>), grid, dim3(256), 0, st, a);
+    else if (bf16)
+        hipLaunchKernelGGL((vs::beam_piece_kernel<1, vs::kShortStep>), grid, dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL(vs::beam_piece_kernel<0>, grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((vs::beam_piece_kernel<0, vs::kShortStep>), grid, dim3(256), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return report_hip(e, "beam select");
     hipLaunchKernelGGL(vs::beam_merge_kernel, dim3((uint32_t)nreq), dim3(vs::kMergeThreads), 0, st, a);

@@ -88,6 +88,22 @@ def test_scores_near_and_far_apart(vs, W, k, V, spread):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("ties", [False, True])
+def test_large_calls(vs, dtype, ties):
+    """Logits enough for the pieces of large calls; with ties, a sixth of every piece is its largest value."""
+    rng = np.random.default_rng(17)
+    x = rng.standard_normal((32, 530_001)).astype(np.float32)
+    if ties:
+        x = np.minimum(x, 1)
+        x[:, ::3] = np.minimum(x[:, ::3], 0.5)
+    sc = -3 * rng.random((4, 8)).astype(np.float32)
+    fin = np.zeros((4, 8), np.uint8)
+    fin[1, 3] = fin[2, 0] = 1
+    got, val = select(vs, x, sc, 20, dtype, finished=fin, eos=530_000, pad=1, shift=1)
+    check(got, val, sc, 20, fin, 530_000)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_exact_ties(vs, dtype):
     """Few distinct logits, so that most of the choice is among equals: in one beam by token, between beams of
     equal rows and scores by beam, wherever the rows start in memory."""
