@@ -61,6 +61,11 @@ class DeviceArray:
             raise ValueError(f"negative size in {self.shape}")
         self.dtype = dtype
         self._code = _code(dtype)
+        out, s = [], 1
+        for n in reversed(self.shape):
+            out.append(s)
+            s *= n
+        self._stride = tuple(reversed(out))
         self.buf = N.DeviceBuffer(max(1, math.prod(self.shape)) * _SIZES[self._code], device)
 
     @classmethod
@@ -73,11 +78,7 @@ class DeviceArray:
         return self.buf.ptr.value
 
     def stride(self):
-        out, s = [], 1
-        for n in reversed(self.shape):
-            out.append(s)
-            s *= n
-        return tuple(reversed(out))
+        return self._stride
 
     def upload(self, a) -> "DeviceArray":
         a = np.ascontiguousarray(a, self._NUMPY[self._code])
@@ -114,23 +115,32 @@ def _rows(t, what, shape, code):
 
 def _flat(t, what, shape, code) -> int:
     """Pointer of a contiguous buffer of `shape`."""
-    if t.shape != shape or _SEEN.get(t.dtype) != code:
-        if _code(t.dtype) != code:
-            raise ValueError(f"{what}: element type {t.dtype}")
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    if (t.shape != shape or _SEEN.get(t.dtype) != code
+            or t.stride() != ((shape[1], 1) if len(shape) == 2 else (1,))):
+        _look_closely(t, what, shape, code)
+    return t.data_ptr()
+
+
+def _look_closely(t, what, shape, code) -> None:
+    if _code(t.dtype) != code:
+        raise ValueError(f"{what}: element type {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
     n = 1
     for size, s in zip(shape[::-1], t.stride()[::-1]):
         if s != n and size > 1:
             raise ValueError(f"{what}: not contiguous")
         n *= size
-    return t.data_ptr()
 
 
 def _list(t, what, n, code) -> int:
     """Pointer of a contiguous buffer of n elements, whatever its shape."""
     shape = t.shape
-    if (shape[0] if len(shape) == 1 else math.prod(shape)) != n:
+    if len(shape) == 2 and shape[0] * shape[1] == n:  # (beams' outputs, [requests, k])
+        if _SEEN.get(t.dtype) != code or t.stride() != (shape[1], 1):
+            _look_closely(t, what, tuple(shape), code)
+        return t.data_ptr()
+    if math.prod(shape) != n:
         raise ValueError(f"{what}: shape {tuple(shape)}, expected {n} elements")
     return _flat(t, what, tuple(shape), code)
 
@@ -330,18 +340,21 @@ class BeamSearch:
         logits [requests * beams, vocab] f32 or bf16; scores [requests, beams]
         f32; finished [requests, beams] u8.  Outputs [requests, k]: scores f32,
         tokens and parents (rows of logits) i32, finished u8."""
-        requests, beams = shape = tuple(scores.shape)
+        requests, beams = shape = scores.shape
         rows, vocab = logits.shape
-        k = scores_out.shape[1]
         code = _SEEN.get(logits.dtype)
         if code is None:
             code = _code(logits.dtype)
         if code < 0:
             raise ValueError(f"logits: element type {logits.dtype}")
-        lp, ls = _rows(logits, "logits", (requests * beams, vocab), code)
-        out = (requests, k)
+        ls = logits.stride()
+        if rows != requests * beams or ls[1] != 1:
+            _rows(logits, "logits", (requests * beams, vocab), code)
+        _, k = out = scores_out.shape
+        if out[0] != requests:
+            raise ValueError(f"scores_out: shape {tuple(out)}, expected {requests} rows")
         rc = self._lib.vs_beam_select(
-            self._h, lp, code, ls[0] if rows > 1 else vocab, requests, beams, vocab,
+            self._h, logits.data_ptr(), code, ls[0] if rows > 1 else vocab, requests, beams, vocab,
             _flat(scores, "scores", shape, N.VS_DTYPE_F32),
             None if finished is None else _flat(finished, "finished", shape, _U8), eos, k,
             _flat(scores_out, "scores_out", out, N.VS_DTYPE_F32), _flat(tokens_out, "tokens_out", out, _I32),
@@ -354,11 +367,15 @@ class BeamSearch:
         """Row i of `out` = row parents[i] of `state`, zeros where there is no
         such row (vs_beam_reorder).  With tail (i32, one per row) an int32
         state's last column is not copied: tail goes there."""
-        code = _code(out.dtype)
+        code = _SEEN.get(out.dtype)
+        if code is None:
+            code = _code(out.dtype)
         rows, cols = out.shape
-        nin = state.shape[0]
-        ip, is_ = _rows(state, "state", (nin, cols), code)
-        op, os_ = _rows(out, "out", (rows, cols), code)
+        nin, wide = state.shape
+        is_, os_ = state.stride(), out.stride()
+        if wide != cols or _SEEN.get(state.dtype) != code or is_[1] != 1 or os_[1] != 1:
+            _rows(state, "state", (nin, cols), code)
+            _rows(out, "out", (rows, cols), code)
         size = _SIZES[code]
         tp, keep = None, cols
         if tail is not None:
@@ -368,7 +385,7 @@ class BeamSearch:
         pp = _list(parents, "parents", rows, _I32)
         wide = cols * size
         rc = self._lib.vs_beam_reorder(
-            self._h, pp, rows, ip, nin, is_[0] * size if nin > 1 else wide, op,
+            self._h, pp, rows, state.data_ptr(), nin, is_[0] * size if nin > 1 else wide, out.data_ptr(),
             os_[0] * size if rows > 1 else wide, keep * size, tp, stream)
         if rc:
             N.check(rc)
