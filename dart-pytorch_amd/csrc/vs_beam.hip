@@ -20,6 +20,7 @@ constexpr int kShortStep = 16;      // and small ones
 constexpr int kCap = 256;           // candidates per piece kept in LDS
 constexpr int kMergeCap = 1024;
 constexpr int kMergeThreads = 512;
+constexpr int kManyK = 16;          // past it, thresholds come from more than one wave's lanes
 constexpr int kWide = 16;           // entries per thread that a merge holds in registers
 constexpr float kLog2e = 1.44269504088896340736f;
 #define VS_NINF (-__builtin_huge_valf())
@@ -162,6 +163,7 @@ __global__ __launch_bounds__(256, PER == kLongStep ? 6 : 1) void beam_piece_kern
     using S = Step<ST, PER>;
     constexpr int kStep = 64 * PER;
     __shared__ uint64_t lists[4][kCap];
+    __shared__ uint32_t maxima[256];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint64_t *cand = lists[wave];
@@ -183,9 +185,14 @@ __global__ __launch_bounds__(256, PER == kLongStep ? 6 : 1) void beam_piece_kern
     float sum = 0.f;        // of exp(x - top), the lane's share
     float thr = -__FLT_MAX__;  // (so -inf is no candidate)
     int n = 0;
+    // With many candidates the first threshold is found over the four waves'
+    // first steps together, which leaves each a quarter of them (k = 32, 128 x 16
+    // x 30,000 bf16 46 against 36 us, k = 24, 50 x 12 x 50,000 with the merge 46
+    // against 42.5; k = 16 the same; k = 8 and 10 a us longer for the barrier).
+    const bool together = PER == kLongStep && a.k > kManyK;
     S step;
-    if (begin < end) step.load(base, begin, vocab, lane);
-    for (int first = begin; first < end; first += kNext) {
+    step.load(base, begin, vocab, lane);  // (past the row's end: nothing but -inf)
+    for (int first = begin;;) {
         const S x = step;
         // (a short step's next one is in flight meanwhile; beside a long one are
         // other waves', and registers for more of those are worth more: 28.1
@@ -194,27 +201,54 @@ __global__ __launch_bounds__(256, PER == kLongStep ? 6 : 1) void beam_piece_kern
         float most = fmaxf(x.value(0), x.value(1));
 #pragma unroll
         for (int i = 2; i < PER; i += 2) most = max3(most, x.value(i), x.value(i + 1));
-        if (__ballot(most >= thr)) {
-            run = fmaxf(run, most);
+        if (__ballot(most > top)) {
             const float w = wave_max(most);
-            if (w > top) {
-                sum *= __builtin_amdgcn_exp2f((top - w) * kLog2e);  // (0 at first: top is -inf)
-                top = w;
+            sum *= __builtin_amdgcn_exp2f((top - w) * kLog2e);  // (0 at first: top is -inf)
+            top = w;
+        }
+        if (together && first == begin) {
+            // (all waves of the workgroup are here: they share a row)
+            maxima[threadIdx.x] = code_of(most);
+            __syncthreads();
+            uint32_t code[4], high = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                code[j] = maxima[lane + 64 * j];
+                high = max(high, code[j]);
             }
-            // the k-th largest of the lanes' maxima: no lower than the last
-            // one, whose leading bits that the largest has too are its
-            const uint32_t code = code_of(run), low = code_of(thr);
-            const uint32_t apart = low ^ max(low, code_of(top));
+            high = code_of(wave_max(value_of(high)));
+            const uint32_t low = code_of(thr), apart = low ^ max(low, high);
             uint32_t bit = apart ? 0x80000000u >> __builtin_clz(apart) : 0;
             uint32_t t = low & ~(2 * bit - (bit != 0));
             for (; bit > (ST ? 0x8000u : 0u); bit >>= 1) {  // (bf16: 16 bits tell)
-                const int cnt = __popcll(__ballot(code >= (t | bit)));
+                int cnt = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) cnt += __popcll(__ballot(code[j] >= (t | bit)));
                 if (cnt >= a.k) {
                     t |= bit;
                     if (cnt == a.k) break;
                 }
             }
-            if (t > code_of(thr)) thr = value_of(t);
+            if (t > low) thr = value_of(t);
+        }
+        if (__ballot(most >= thr)) {
+            run = fmaxf(run, most);
+            if (!together || first != begin) {
+                // the k-th largest of the lanes' maxima: no lower than the last
+                // one, whose leading bits that the largest has too are its
+                const uint32_t code = code_of(run), low = code_of(thr);
+                const uint32_t apart = low ^ max(low, code_of(top));
+                uint32_t bit = apart ? 0x80000000u >> __builtin_clz(apart) : 0;
+                uint32_t t = low & ~(2 * bit - (bit != 0));
+                for (; bit > (ST ? 0x8000u : 0u); bit >>= 1) {  // (bf16: 16 bits tell)
+                    const int cnt = __popcll(__ballot(code >= (t | bit)));
+                    if (cnt >= a.k) {
+                        t |= bit;
+                        if (cnt == a.k) break;
+                    }
+                }
+                if (t > code_of(thr)) thr = value_of(t);
+            }
             const int n0 = n;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
@@ -255,6 +289,8 @@ __global__ __launch_bounds__(256, PER == kLongStep ? 6 : 1) void beam_piece_kern
 #pragma unroll
         for (int i = 0; i < PER; ++i) sum += __builtin_amdgcn_exp2f((x.value(i) - ref) * kLog2e);
         if (PER != kShortStep && first + kNext < end) step.load(base, first + kNext, vocab, lane);
+        first += kNext;
+        if (first >= end) break;
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
@@ -377,16 +413,34 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
     best[threadIdx.x] = (float)mine;
     __syncthreads();
     if (wave == 0) {
-        float m = best[lane];
-#pragma unroll
-        for (int j = 1; j < kMergeThreads / 64; ++j) m = fmaxf(m, best[lane + 64 * j]);
-        const uint32_t code = code_of(m);
         uint32_t t = 0;
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-            const int cnt = __popcll(__ballot(code >= (t | bit)));
-            if (cnt >= a.k) {
-                t |= bit;
-                if (cnt == a.k) break;
+        if (a.k <= kManyK) {
+            float m = best[lane];
+#pragma unroll
+            for (int j = 1; j < kMergeThreads / 64; ++j) m = fmaxf(m, best[lane + 64 * j]);
+            const uint32_t code = code_of(m);
+            for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+                const int cnt = __popcll(__ballot(code >= (t | bit)));
+                if (cnt >= a.k) {
+                    t |= bit;
+                    if (cnt == a.k) break;
+                }
+            }
+        } else {
+            // (of 64 maxima the k-th largest would be a weak threshold: 20 x 64 x
+            // 50,000, k = 64, with what follows below 434 against 168 us)
+            uint32_t code[kMergeThreads / 64];
+#pragma unroll
+            for (int j = 0; j < kMergeThreads / 64; ++j) code[j] = code_of(best[lane + 64 * j]);
+            for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+                int cnt = 0;
+#pragma unroll
+                for (int j = 0; j < kMergeThreads / 64; ++j)
+                    cnt += __popcll(__ballot(code[j] >= (t | bit)));
+                if (cnt >= a.k) {
+                    t |= bit;
+                    if (cnt == a.k) break;
+                }
             }
         }
         // (a code below -inf's: all lanes count, and so does everything)
@@ -430,19 +484,21 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
         return nlist;
     };
     int n = gather(t);
-    if (n > kMergeCap && lots <= kMergeCap && lots * a.k <= kWide * kMergeThreads) {
+    if (n > kMergeCap && lots <= kMergeCap) {
         // More than there is room for (the beams' scores lie far apart, and one
         // beam's lists outdo the others' first entries): the k-th largest of the
-        // lists' entries, held in registers, by counting over the workgroup.
+        // lists' entries, or as many first ones as fit the registers, by
+        // counting over the workgroup.
         uint32_t code[kWide];
+        const int deep = min(a.k, kWide * kMergeThreads / lots), most = lots * deep;
 #pragma unroll
         for (int j = 0; j < kWide; ++j) {
             const int x = threadIdx.x + j * kMergeThreads;
             code[j] = 0;
-            if (x < lots * a.k) {
-                const int i = picked[x / a.k];
+            if (x < most) {
+                const int i = picked[x / deep];
                 const double total =
-                    total_of(i, a.top_v[(row0 * a.npieces + i) * a.k + x % a.k]);
+                    total_of(i, a.top_v[(row0 * a.npieces + i) * a.k + x % deep]);
                 if (total == total) code[j] = code_of((float)total);
             }
         }
@@ -452,7 +508,7 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
             int cnt = 0;
 #pragma unroll
             for (int j = 0; j < kWide; ++j)
-                if (j * kMergeThreads < lots * a.k)
+                if (j * kMergeThreads < most)
                     cnt += __popcll(__ballot(code[j] >= (c | bit)));
             if (lane == 0) counts[flip][wave] = cnt;
             __syncthreads();

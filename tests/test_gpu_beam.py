@@ -103,6 +103,17 @@ def test_large_calls(vs, dtype, ties):
     check(got, val, sc, 20, fin, 530_000)
 
 
+@pytest.mark.parametrize("spread", [0.01, 20.0])
+def test_large_calls_of_many_candidates(vs, spread):
+    """64 beams and candidates: thresholds over four waves together, and more lists than the merge's registers."""
+    rng = np.random.default_rng(64)
+    x = 2 * rng.standard_normal((128, 140_001)).astype(np.float32)
+    x[5, 140_000] = 90.0  # far above its piece's other logits, and alone in the last one
+    sc = -spread * rng.random((2, 64)).astype(np.float32)
+    got, val = select(vs, x, sc, 64, "bf16")
+    check(got, val, sc, 64)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_exact_ties(vs, dtype):
     """Few distinct logits, so that most of the choice is among equals: in one beam by token, between beams of
