@@ -36,6 +36,7 @@ struct AttendArgs {
     int most_items, few_items;           // six workgroups to a CU, and one
     float *part_o;   // [item][heads][dim]
     float2 *part_ml; // [item][heads] running maximum and sum
+    int32_t *status;
     int2 *first;     // [nseq] first whole item; whole ones * 2 + whether there is a rest
 };
 
@@ -393,7 +394,11 @@ __global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 
         const int u = (sp.total - 1) * UB + (n - 1) % kKvBlock / (16 * H);
         if (u >= u0 && u < j1 * UB && (u - u0) % NW == 0) {
             new_page = trow[(n - 1) >> a.page_shift];
-            if ((unsigned)new_page < (unsigned)a.npages) u_new = u;
+            if (a.lens[it.b] > n) {  // past the table: n - 1 is not the new token's place
+                if (lane == 0) atomicOr(&a.status[0], kStatusWidth);
+            } else if ((unsigned)new_page < (unsigned)a.npages) {
+                u_new = u;
+            }
         }
     }
     if (u_new >= 0) {
@@ -928,6 +933,7 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
     a.q_vec = vs::pieces_ok(q, q_seq, q_head, e);
     a.k_vec = vs::pieces_ok(k, k_seq, k_head, e);
 
+    a.status = kv->status;
     // Work items: whole ones of so many blocks that two or six workgroups come
     // to a CU, and one per sequence for what is left of it.
     const int64_t per_item = (int64_t)a.kv_heads * a.gtiles;

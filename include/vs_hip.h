@@ -221,7 +221,10 @@ VS_API int vs_kmeans_step(vs_index *points, const float *centroids_in, int64_t K
  * sees (table entries, lengths, parents) is checked by the kernels and told
  * by vs_kv_check.  Scratch memory is kept per handle and stream and grows at
  * a first call of a size: a call that is recorded into a graph and would
- * have to allocate is refused (VS_ERR_UNSUPPORTED; run it once before).
+ * have to allocate is refused (VS_ERR_UNSUPPORTED; run it once before).  A
+ * recorded call keeps the scratch of the stream it was recorded on: replays
+ * must not overlap that stream's other calls on the handle.  One thread at a
+ * time uses a handle.
  *
  * The cache is npages pages of page_size positions; a page holds the keys and
  * values of consecutive positions of one sequence, of every layer and
@@ -323,7 +326,8 @@ VS_API int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out,
 VS_API int vs_kv_copy(vs_kv *kv, const int32_t *from, const int32_t *to, int64_t n, void *stream);
 /* Waits for the stream and tells what earlier calls met on the device since
  * the last check: VS_ERR_OOM (an extend found too few free pages),
- * VS_ERR_INVALID (too few table columns; a parent out of range). */
+ * VS_ERR_INVALID (too few table columns for an extend or for an attend's new
+ * token; a parent out of range). */
 VS_API int vs_kv_check(vs_kv *kv, void *stream);
 
 /* Beam search over device buffers.  A handle owns scratch memory only. */

@@ -145,6 +145,30 @@ def test_negative_length_is_empty(vs, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_length_past_the_table(vs, dtype):
+    """A new token without a column is stored nowhere and told; the positions that have one are attended to."""
+    c = Case(vs, [64, 70], 4, 2, 32, 32, dtype, width=3)
+    true, c.lens = c.lens, np.array([97, 70], np.int32)
+    c.table[0, 2] = c.table[0, 0]  # (a page in every column: 96 positions, the first 32 of them twice)
+    c.sequences(np.zeros(c.cache.npages, np.int32))
+    A = vs.DeviceArray
+    n, before = 2, c.mem.numpy().copy()
+    kb, _ = D.stored(np.full((n, 2, 32), 3.0), dtype)
+    out, lse = A((n, 4, 32), dtype), A((n, 4), "f32")
+    c.cache.attend(c.seqs, A.of(c.qb, dtype), out, k=A.of(kb, dtype), v=A.of(kb, dtype), lse=lse)
+    with pytest.raises(ValueError, match="outgrew"):
+        c.cache.check()
+    after = c.mem.numpy()
+    changed = {int(p) for p in np.nonzero((before.view(np.uint8) != after.view(np.uint8))
+                                          .reshape(len(before), -1).any(1))[0]}
+    assert changed == {int(c.table[1, 2])}
+    k0, v0 = np.concatenate([c.k[0], c.k[0][:32]]), np.concatenate([c.v[0], c.v[0][:32]])
+    args = (c.q[0], k0, v0, np.arange(96), 32 ** -0.5)
+    got = D.from_bf16(out.numpy()) if dtype == "bf16" else out.numpy()
+    D.assert_rounded(got[0], D.attend(*args)[0], D.attend_tolerance(*args, dtype)[0], dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("kv,heads,n", [(1, 4, 40_000), (1, 16, 9_001), (2, 6, 70_000)])
 def test_split_over_the_length(vs, dtype, kv, heads, n):
     """Hundreds of work items of one sequence (more than a wave's lanes), beside a short one."""
