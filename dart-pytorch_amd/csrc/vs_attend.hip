@@ -671,6 +671,7 @@ struct RowsArgs {
     int nseq, npages, page_shift, heads, dim;
     const char *k, *v;
     int64_t k_row, k_head, v_row, v_head;
+    int k_vec, v_vec;  // rows readable in 16-byte pieces
     char *k_out, *v_out;
     int b, first;
 };
@@ -684,43 +685,97 @@ __device__ __forceinline__ char *block_of(const RowsArgs &a, int b, int64_t pos,
     return a.pool + (int64_t)page * a.page_bytes + a.layer_off + blk * kKvBlock * a.dim * es;
 }
 
-// One workgroup per row: read once, written once; a few scattered bytes per
-// element, which the caches gather as the next rows follow.
+// Rows into the cache: a copy, bound by HBM.  One workgroup per block of 32
+// positions and head, so that both sides move whole lines: keys go straight to
+// their places, lanes in the order of those; values are turned in LDS.
+// Sequence b's rows touch at most rows / 32 + 2 blocks, so its items start at
+// starts[b] / 32 + 2 b, which needs no sum over the sequences before it.
+// 8 heads of 128 in bf16: 4,096 rows 7.8 us (33.6 MB read and written, 4.3
+// TB/s; a row at a time, with scattered stores, 27.8), 16 x 1,000 rows 23.7 (131
+// MB, 5.5 TB/s; 91).
 template <int ST>
-__global__ __launch_bounds__(256) void append_kernel(RowsArgs a) {
+__global__ __launch_bounds__(256) void append_kernel(RowsArgs a, int64_t items) {
     using T = typename std::conditional<ST, uint16_t, uint32_t>::type;
-    for (int64_t row = blockIdx.x; row < a.nrows; row += gridDim.x) {
-        int b = (int)row;
-        int64_t pos;
+    constexpr int E = ST ? 8 : 4;
+    extern __shared__ __align__(16) char lds_rows[];  // the block's values [32][dim + E]
+    const int dim = a.dim, pieces = dim / E, ld = dim + E;
+    T *rows = (T *)lds_rows;
+    for (int64_t w = blockIdx.x; w < items * a.heads; w += gridDim.x) {
+        const int64_t item = w / a.heads;
+        const int h = (int)(w % a.heads);
+        int64_t b = item, blk = 0, row0 = item, count = 1;  // the sequence's rows
         if (a.starts) {
-            // the last sequence whose rows start at or before this one
-            int lo = 0, hi = a.nseq;
+            auto base = [&](int64_t x) { return ((int64_t)a.starts[x] >> 5) + 2 * x; };
+            int64_t lo = 0, hi = a.nseq;  // the last one that starts at or before the item
             while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (a.starts[mid] <= row)
+                const int64_t mid = (lo + hi) / 2;
+                if (base(mid) <= item)
                     lo = mid;
                 else
                     hi = mid;
             }
             b = lo;
-            if (row < a.starts[b] || row >= a.starts[b + 1]) continue;
-            pos = (int64_t)a.lens[b] - (a.starts[b + 1] - row);
-        } else {
-            pos = (int64_t)a.lens[b] - 1;
+            blk = item - base(b);
+            row0 = a.starts[b];
+            count = a.starts[b + 1] - row0;
         }
-        char *at = block_of(a, b, pos, sizeof(T));
+        const int64_t end = a.lens[b], first = end - count;  // positions
+        const int64_t p0 = ((first >> 5) + blk) * kKvBlock;
+        if (blk < 0 || count <= 0 || p0 < 0 || p0 >= end) continue;
+        char *const at = block_of(a, (int)b, p0, sizeof(T));
         if (!at) continue;
-        for (int x = threadIdx.x; x < a.heads * a.dim; x += 256) {
-            const int h = x / a.dim, d = x % a.dim;
-            T *k = (T *)(at + h * a.head_off), *v = (T *)(at + a.kv_off + h * a.head_off);
-            k[key_place<ST>(pos % kKvBlock, d, a.dim)] =
-                ((const T *)a.k)[row * a.k_row + h * a.k_head + d];
-            v[value_place<ST>(pos % kKvBlock, d, a.dim)] =
-                ((const T *)a.v)[row * a.v_row + h * a.v_head + d];
+        // positions t of the block that have a row
+        const int64_t from = max(row0 < 0 ? first - row0 : first, p0);
+        const int64_t to = min(min(end, first + (a.nrows - row0)), p0 + kKvBlock);
+        if (from >= to) continue;
+        const int t0 = (int)(from - p0), t1 = (int)(to - p0);
+        auto row_of = [&](int t) { return row0 + (p0 + t - first); };
+        const T *ks = (const T *)a.k + h * a.k_head, *vs = (const T *)a.v + h * a.v_head;
+        char *const kd = at + h * a.head_off, *const vd = kd + a.kv_off;
+        __syncthreads();  // (the last block's values have been read)
+        for (int x = threadIdx.x; x < kKvBlock * pieces; x += 256) {
+            const int t = x / pieces, c = x % pieces;
+            if (t >= t0 && t < t1)
+                *(u32x4_t *)(rows + t * ld + c * E) =
+                    load_piece<ST>((const char *)(vs + row_of(t) * a.v_row), c * E, a.v_vec);
+        }
+        for (int x = threadIdx.x; x < kKvBlock * pieces; x += 256) {
+            const int t = x / 16 / pieces * 16 + x % 16, c = x / 16 % pieces;
+            if (t >= t0 && t < t1)
+                *(u32x4_t *)(kd + x * 16) =
+                    load_piece<ST>((const char *)(ks + row_of(t) * a.k_row), c * E, a.k_vec);
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < kKvBlock * pieces; x += 256) {
+            // bf16: [dimension][g][half][i], fp32: [half][dimension][g][i]
+            const int g = x % 4, d = ST ? x / 4 : x / 4 % dim, half = ST ? 0 : x / 4 / dim;
+            T out[E];
+            int have = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int t = 16 * (ST ? e / 4 : half) + 4 * g + e % 4;
+                const bool in = t >= t0 && t < t1;
+                out[e] = in ? rows[t * ld + d] : (T)0;
+                have += in;
+            }
+            T *dst = (T *)(vd + x * 16);
+            if (have == E) {
+                u32x4_t v;
+                __builtin_memcpy(&v, out, 16);
+                *(u32x4_t *)dst = v;
+            } else if (have) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int t = 16 * (ST ? e / 4 : half) + 4 * g + e % 4;
+                    if (t >= t0 && t < t1) dst[e] = out[e];
+                }
+            }
         }
     }
 }
 
+// The same backwards, a workgroup per position: for looking at a cache, not for
+// a decoding loop (4,096 positions of 8 x 128 in bf16 21 us).
 template <int ST>
 __global__ __launch_bounds__(256) void read_kernel(RowsArgs a) {
     using T = typename std::conditional<ST, uint16_t, uint32_t>::type;
@@ -1033,11 +1088,16 @@ int vs_kv_append(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, const void *k, i
     a.k_head = k_head;
     a.v_row = v_row;
     a.v_head = v_head;
-    const dim3 grid((uint32_t)std::min<int64_t>(nrows, 65536));
+    const int64_t e_bytes = vs::kv_elem(kv->dtype);
+    a.k_vec = vs::pieces_ok(k, k_row, k_head, e_bytes);
+    a.v_vec = vs::pieces_ok(v, v_row, v_head, e_bytes);
+    const int64_t items = starts ? nrows / vs::kKvBlock + 2 * s->nseq + 1 : nrows;
+    const dim3 grid((uint32_t)std::min<int64_t>(items * kv->kv_heads, 1 << 20));
+    const size_t lds = (size_t)vs::kKvBlock * (kv->head_dim * e_bytes + 16);
     if (kv->dtype == VS_DTYPE_BF16)
-        hipLaunchKernelGGL(vs::append_kernel<1>, grid, dim3(256), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(vs::append_kernel<1>, grid, dim3(256), lds, (hipStream_t)stream, a, items);
     else
-        hipLaunchKernelGGL(vs::append_kernel<0>, grid, dim3(256), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(vs::append_kernel<0>, grid, dim3(256), lds, (hipStream_t)stream, a, items);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? VS_OK : report_hip(e, "append");
 }

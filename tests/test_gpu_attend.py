@@ -403,6 +403,34 @@ def test_append_and_read(vs, dtype):
     c.cache.check()
 
 
+@pytest.mark.parametrize("dtype,dim,shift", [("bf16", 128, 0), ("bf16", 80, 3), ("f32", 256, 0), ("f32", 16, 1)])
+def test_append_at_every_offset(vs, dtype, dim, shift):
+    """Rows that start and end anywhere in a block, sequences of every small count, from a strided buffer;
+    positions before 0, rows outside the buffer and everything else in the pool stay as they were."""
+    counts = [n for n in range(0, 40)] + [64, 65, 95, 97, 130]
+    lens = [n + (7 * n) % 45 for n in counts]
+    lens[5] = 3  # fewer positions than rows: the first two rows have none
+    c = Case(vs, lens, 2, 2, dim, 64, dtype, layers=2, layer=1)
+    starts = 4 + np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    rows = int(starts[-1]) - 2  # (the last two rows are not there)
+    A = vs.DeviceArray
+    wide = 5 * dim + 3
+    flat, _ = D.stored(c.rng.standard_normal(shift + rows * wide), dtype)
+    buf = A.of(flat, dtype)
+    at = flat[shift:].reshape(rows, wide)
+    k = View(buf, (rows, 2, dim), (wide, dim, 1), shift)
+    v = View(buf, (rows, 2, dim), (wide, dim, 1), shift + 3 * dim)
+    c.cache.append(c.seqs, k, v, starts=A.of(starts, "i32"), layer=1)
+    c.cache.check()
+    for b, (n, ln) in enumerate(zip(counts, lens)):
+        for j in range(n):
+            p, r = ln - n + j, int(starts[b]) + j
+            if p >= 0 and r < rows:
+                D.write_rows(c.pool[:, 1], c.table, b, p, at[r, :2 * dim].reshape(1, 2, dim),
+                             at[r, 3 * dim:5 * dim].reshape(1, 2, dim), 64, dtype)
+    assert np.array_equal(c.mem.numpy().view(np.uint16), c.pool.view(np.uint16))
+
+
 def test_streams_have_scratch_of_their_own(vs):
     """One handle, three streams at a time, split work on each."""
     c = Case(vs, [4000, 9], 4, 1, 64, 32, "bf16")
