@@ -181,9 +181,13 @@ __device__ __forceinline__ u32x4_t load_piece(const char *row, int x, bool vec) 
 // 1 KB of consecutive bytes per wave, and a column's maximum, sum and
 // rescaling belong to one lane.  Unused columns (fewer than 16 query heads
 // per key-value head) cost matrix time that the loads leave idle anyway.
-// bf16: P is multiplied as the sum of two bf16 values (its first 8 bits and
-// the rest rounded to 8), so it is good to 2^-17 and the output is as exact
-// as its last rounding.
+// bf16: P is multiplied as the sum of three bf16 values, its 24 bits eight at a
+// time, so the output is that of 32-bit weights, rounded once.  (Two of them, 16
+// bits, sent two to four answers in a thousand to the other neighbour.)  The
+// third product costs 0 to 2 % (head sizes 32 to 256, 64 sequences of 2,000:
+// 25.7 to 26.1 us at 32, 102.7 to 103.0 at 128), because each part is split off
+// after the one before is multiplied: all three at once took 12 to 30 registers
+// and a wave per SIMD more (head size 32, 64 ragged ones 19.7 against 18.1 us).
 //
 // Bound by HBM: each byte of the cache is read once per 16 query heads.  8
 // key-value heads of 128 in bf16: 2 sequences of 120,000 to 131,000 positions
@@ -334,21 +338,23 @@ __global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 
     };
     auto add_values = [&]() {
         if constexpr (ST) {
-            bf16x8_t hi, lo;
 #pragma unroll
-            for (int h = 0; h < H; ++h)
+            for (int j = 0; j < 3; ++j) {
+                bf16x8_t part;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = s[h][i], t = float_of(bits_of(p) & 0xFFFF0000u);
-                    hi[4 * h + i] = (__bf16)t;
-                    // (never 0 beside a weight: an infinite value times 0 would be a NaN)
-                    lo[4 * h + i] = (__bf16)fmaxf(p - t, p * 0x1p-60f);
-                }
+                for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const bf16x8_t w = __builtin_bit_cast(bf16x8_t, vf[d]);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, hi, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, lo, o[d], 0, 0, 0);
+                    for (int i = 0; i < 4; ++i) {
+                        const float t = float_of(bits_of(s[h][i]) & 0xFFFF0000u);
+                        // (the rest is never 0 beside a weight: an infinite value times
+                        // 0 would be a NaN)
+                        if (j < 2) s[h][i] = fmaxf(s[h][i] - t, t * 0x1p-30f);
+                        part[4 * h + i] = (__bf16)t;
+                    }
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8_t, vf[d]), part, o[d], 0, 0, 0);
             }
         } else {
 #pragma unroll
