@@ -37,6 +37,7 @@ struct AttendArgs {
     float *part_o;   // [item][heads][dim]
     float2 *part_ml; // [item][heads] running maximum and sum
     int32_t *status;
+    const uint8_t *closed;
     int2 *first;     // [nseq] first whole item; whole ones * 2 + whether there is a rest
 };
 
@@ -223,6 +224,8 @@ __global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 
     const int item = blockIdx.x / per_item, hh = blockIdx.x % per_item;
     const int gt = hh / a.kv_heads, kvh = hh % a.kv_heads;
     const int gc = min(a.group - gt * 16, 16);  // query heads of this workgroup
+    // some page may take no new token (loaded here, to be back when that counts)
+    const int marked = a.status[2];
     Item it = {};
     if (a.unsplit) {
         it.b = item;
@@ -402,7 +405,8 @@ __global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 
             new_page = trow[(n - 1) >> a.page_shift];
             if (a.lens[it.b] > n) {  // past the table: n - 1 is not the new token's place
                 if (lane == 0) atomicOr(&a.status[0], kStatusWidth);
-            } else if ((unsigned)new_page < (unsigned)a.npages) {
+            } else if ((unsigned)new_page < (unsigned)a.npages &&
+                       !(marked && a.closed[new_page])) {
                 u_new = u;
             }
         }
@@ -675,6 +679,8 @@ struct RowsArgs {
     const int32_t *table, *lens, *starts;
     int64_t width, nrows;
     int nseq, npages, page_shift, heads, dim;
+    const int32_t *status;
+    const uint8_t *closed;
     const char *k, *v;
     int64_t k_row, k_head, v_row, v_head;
     int k_vec, v_vec;  // rows readable in 16-byte pieces
@@ -706,6 +712,7 @@ __global__ __launch_bounds__(256) void append_kernel(RowsArgs a, int64_t items) 
     extern __shared__ __align__(16) char lds_rows[];  // the block's values [32][dim + E]
     const int dim = a.dim, pieces = dim / E, ld = dim + E;
     T *rows = (T *)lds_rows;
+    const bool marked = a.status[2] != 0;  // some page may take no new rows
     for (int64_t w = blockIdx.x; w < items * a.heads; w += gridDim.x) {
         const int64_t item = w / a.heads;
         const int h = (int)(w % a.heads);
@@ -730,6 +737,10 @@ __global__ __launch_bounds__(256) void append_kernel(RowsArgs a, int64_t items) 
         if (blk < 0 || count <= 0 || p0 < 0 || p0 >= end) continue;
         char *const at = block_of(a, (int)b, p0, sizeof(T));
         if (!at) continue;
+        if (end <= a.width << a.page_shift) {
+            const int last = a.table[b * a.width + ((end - 1) >> a.page_shift)];
+            if ((unsigned)last < (unsigned)a.npages && marked && a.closed[last]) continue;
+        }
         // positions t of the block that have a row
         const int64_t from = max(row0 < 0 ? first - row0 : first, p0);
         const int64_t to = min(min(end, first + (a.nrows - row0)), p0 + kKvBlock);
@@ -899,12 +910,12 @@ int vs_kv_create(int device, int64_t npages, int64_t page_size, int64_t layers, 
     kv->mem = (char *)memory;
     kv->num_cu = vs::cu_count(device);
     void *p = nullptr;
-    hipError_t e = vs::device_alloc(&p, vs::kStatusWords * sizeof(int32_t));
+    const size_t marks = vs::kStatusWords * sizeof(int32_t) + (size_t)npages;
+    hipError_t e = vs::device_alloc(&p, marks);
     kv->status = (int32_t *)p;
-    if (e == hipSuccess) {
-        const int32_t zero[vs::kStatusWords] = {0};
-        e = hipMemcpy(p, zero, sizeof zero, hipMemcpyHostToDevice);
-    }
+    kv->closed = (uint8_t *)(kv->status + vs::kStatusWords);
+    if (e == hipSuccess) e = hipMemset(p, 0, marks);
+    if (e == hipSuccess) e = hipStreamSynchronize(nullptr);  // (before any stream's call)
     if (e == hipSuccess && !memory) {
         e = vs::device_alloc(&p, (size_t)(npages * pb));
         if (e == hipSuccess) {
@@ -995,6 +1006,7 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
     a.k_vec = vs::pieces_ok(k, k_seq, k_head, e);
 
     a.status = kv->status;
+    a.closed = kv->closed;
     // Work items: whole ones of so many blocks that two or six workgroups come
     // to a CU, and one per sequence for what is left of it.
     const int64_t per_item = (int64_t)a.kv_heads * a.gtiles;
@@ -1060,6 +1072,8 @@ static int fill_rows(const vs_kv *kv, const vs_kv_seqs *s, int64_t layer, vs::Ro
     a.width = s->width;
     a.nseq = (int)s->nseq;
     a.npages = (int)kv->npages;
+    a.status = kv->status;
+    a.closed = kv->closed;
     a.page_shift = __builtin_ctzll((uint64_t)kv->page_size);
     a.heads = (int)kv->kv_heads;
     a.dim = (int)kv->head_dim;

@@ -14,12 +14,24 @@ struct vs_kv {
     bool owns_mem = false;
     int num_cu = 256;
     int32_t *status = nullptr;  // kStatusWords device words
+    uint8_t *closed = nullptr;  // [npages], behind them: pages that take no new token
     vs::StreamScratch scratch;
 };
 
 namespace vs {
 
-// What kernels tell vs_kv_check: [0] bits below, [1] pages an extend was short of.
+// What kernels tell vs_kv_check: [0] bits below, [1] pages an extend was short
+// of, [2] whether a page may be closed.
+//
+// An extend that does not fit is known on the device only, with the calls that
+// store what it should have made room for behind it: they would store at the
+// last positions that there are, over tokens that are in use, and in pages whose
+// copies were part of the refused plan several at once.  So it closes the last
+// page of each of its sequences, and those calls leave a sequence alone whose
+// last page is closed.  The page is what is marked, not the sequence: that
+// follows forks and compactions, and concerns no one else's sequences.  An
+// extend that fits opens the pages that it gives or leaves to a sequence,
+// vs_kv_check opens all.
 constexpr int kStatusWords = 4;
 constexpr int kStatusPages = 1, kStatusWidth = 2, kStatusParent = 4;
 

@@ -34,6 +34,7 @@ struct ExtendArgs {
     int nseq, npages, page_shift, count;
     const int32_t *count_dev;
     int32_t *status;
+    uint8_t *closed;
     int32_t *holders, *lowest;  // [npages], used where a shared last page is
     int32_t *offset;            // [nseq] place of a sequence's first new page | copies (bit 31)
     int32_t *fresh;             // [npages] free pages, lowest first
@@ -78,6 +79,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
         }
         return s;
     };
+    const bool marked = a.status[2] != 0;  // some page may be closed
     if (threadIdx.x == 0) {
         bad = huge = 0;
         a.copies[0] = 0;
@@ -153,8 +155,19 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
         need += total;
     }
     __syncthreads();
+    // what is stored behind a refused extend has no place: see kStatusWords
+    auto close_pages = [&]() {
+        for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
+            const int n = max(a.lens[b], 0);
+            if (n == 0 || n > most || (a.count_dev ? a.count_dev[b] : a.count) <= 0) continue;
+            const int p = a.table[(int64_t)b * a.width + ((n - 1) >> a.page_shift)];
+            if ((unsigned)p < (unsigned)a.npages) a.closed[p] = 1;
+        }
+        if (threadIdx.x == 0) a.status[2] = 1;
+    };
     if (bad) {
         if (threadIdx.x == 0) atomicOr(&a.status[0], kStatusWidth);
+        close_pages();
         return;
     }
     // the lowest `need` free pages, the first in LDS
@@ -185,6 +198,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
             atomicOr(&a.status[0], kStatusPages);
             atomicMax(&a.status[1], (int)min(max(need - found, (int64_t)1), (int64_t)INT32_MAX));
         }
+        close_pages();
         return;
     }
     __syncthreads();
@@ -206,11 +220,16 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
             a.refs[to] = 1;
             *entry = to;
         }
+        if (marked && n > 0) {
+            const int p = row[(n - 1) >> a.page_shift];
+            if ((unsigned)p < (unsigned)a.npages) a.closed[p] = 0;
+        }
         const int64_t end = ((int64_t)n + c + P - 1) >> a.page_shift;
         for (int64_t e = ((int64_t)n + P - 1) >> a.page_shift; e < end; ++e) {
             const int to = take(at++);
             a.refs[to] = 1;
             row[e] = to;
+            if (marked) a.closed[to] = 0;
         }
         a.lens[b] = n + c;
     }
@@ -388,6 +407,8 @@ struct CompactArgs {
     int32_t *map;      // [npages] where a page goes
     int32_t *from, *to;
     int32_t *moves;    // how many
+    const int32_t *status;
+    uint8_t *closed;   // follows its pages
 };
 
 // Live pages past the front and free pages in it, paired in order.  Bound by one
@@ -395,6 +416,7 @@ struct CompactArgs {
 __global__ __launch_bounds__(kPlan) void compact_plan_kernel(CompactArgs a) {
     __shared__ int lds[kPlan / 64];
     const int64_t step = 4 * kPlan;
+    const bool marked = a.status[2] != 0;
     int64_t live = 0;
     for (int64_t p0 = 0; p0 < a.npages; p0 += step) {
         int cnt = 0;
@@ -441,6 +463,10 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(CompactArgs a) {
         const int f = a.from[i], t = a.to[i];
         a.map[f] = t;
         a.refs2[t] = a.refs[f];
+        if (marked) {
+            a.closed[t] = a.closed[f];
+            a.closed[f] = 0;
+        }
     }
     __syncthreads();
     for (int64_t p = live + threadIdx.x; p < a.npages; p += kPlan) a.refs2[p] = 0;
@@ -454,6 +480,7 @@ __global__ __launch_bounds__(kPlan) void compact_plan_small_kernel(CompactArgs a
     __shared__ int lds[kPlan / 64];
     __shared__ uint16_t to[kSmallPages / 2];
     const int chunks = (a.npages + 4 * kPlan - 1) / (4 * kPlan);
+    const bool marked = a.status[2] != 0;
     int ref[N][4], cnt = 0;
 #pragma unroll
     for (int c = 0; c < N; ++c)
@@ -501,6 +528,10 @@ __global__ __launch_bounds__(kPlan) void compact_plan_small_kernel(CompactArgs a
             a.refs2[dst] = ref[c][i];
             a.from[f] = p;
             a.to[f] = dst;
+            if (marked) {
+                a.closed[dst] = a.closed[p];
+                a.closed[p] = 0;
+            }
             ++f;
         }
     }
@@ -561,6 +592,7 @@ int vs_kv_extend(vs_kv *kv, const vs_kv_seqs *s, int64_t count, const int32_t *c
     a.count = (int)count;
     a.count_dev = count_dev;
     a.status = kv->status;
+    a.closed = kv->closed;
     a.holders = (int32_t *)ws;
     a.lowest = a.holders + np;
     a.fresh = a.lowest + np;
@@ -675,6 +707,8 @@ int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out, void *
     a.from = a.map + np;
     a.to = a.from + np;
     a.moves = a.to + np;
+    a.status = kv->status;
+    a.closed = kv->closed;
     if (np <= vs::kSmallPages)
         hipLaunchKernelGGL(vs::compact_plan_small_kernel, dim3(1), dim3(vs::kPlan), 0, st, a);
     else
@@ -707,9 +741,14 @@ int vs_kv_check(vs_kv *kv, void *stream) {
     int32_t got[vs::kStatusWords] = {0};
     hipError_t e = hipStreamSynchronize(st);
     if (e == hipSuccess) e = hipMemcpy(got, kv->status, sizeof got, hipMemcpyDeviceToHost);
-    const int32_t zero[vs::kStatusWords] = {0};
-    if (e == hipSuccess && got[0])
-        e = hipMemcpy(kv->status, zero, sizeof zero, hipMemcpyHostToDevice);
+    if (e == hipSuccess && got[2]) {
+        // what other streams still run behind a refused extend must find its pages closed
+        e = hipDeviceSynchronize();
+        if (e == hipSuccess) e = hipMemcpy(got, kv->status, sizeof got, hipMemcpyDeviceToHost);
+        if (e == hipSuccess) e = hipMemset(kv->closed, 0, (size_t)kv->npages);
+    }
+    if (e == hipSuccess && got[0]) e = hipMemset(kv->status, 0, sizeof got);
+    if (e == hipSuccess && got[0]) e = hipStreamSynchronize(nullptr);
     if (e != hipSuccess) return report_hip(e, "check");
     if (got[0] & vs::kStatusPages)
         return report(VS_ERR_OOM, "the cache was %d pages short", (int)got[1]);

@@ -267,7 +267,9 @@ class PagedKVCache:
 
     def extend(self, seqs: KVSequences, count=1, *, stream: int = 0) -> None:
         """`count` more positions for every sequence (an int, or an i32 buffer
-        [n]), with copies of shared, partly filled last pages (vs_kv_extend)."""
+        [n]), with copies of shared, partly filled last pages (vs_kv_extend).
+        Where it does not fit nothing changes, check() raises, and attend() and
+        append() store nothing for these sequences until then."""
         if isinstance(count, int):
             rc = self._lib.vs_kv_extend(self._h, self._seqs(seqs), count, None, stream)
         else:

@@ -296,7 +296,10 @@ VS_API int vs_kv_read(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t 
  * that others hold too is copied to a page of the sequence's own first (all
  * layers); where everyone who holds it is being extended here, the lowest of
  * them keeps it.  If pages or table columns do not suffice nothing changes,
- * and vs_kv_check says so. */
+ * and vs_kv_check says so.  Until it has, or until an extend of theirs fits,
+ * nothing is stored for the sequences that were to grow, nor for forks of
+ * theirs: vs_kv_attend's new tokens and vs_kv_append's rows, which have no
+ * position then, are dropped, and the cache stays as it was. */
 VS_API int vs_kv_extend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t count, const int32_t *count_dev,
                         void *stream);
 /* out's sequence i becomes a copy of in's sequence parents[i] (nseq of out
