@@ -282,6 +282,16 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(char *pool, int64_t pag
     }
 }
 
+// Another table whose pages compaction moved: two loads and a store per entry.
+__global__ __launch_bounds__(256) void remap_kernel(int32_t *table, int64_t entries, int npages,
+                                                    const int32_t *map) {
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < entries;
+         x += (int64_t)gridDim.x * 256) {
+        const int p = table[x];
+        if ((unsigned)p < (unsigned)npages) table[x] = map[p];
+    }
+}
+
 struct ForkArgs {
     const int32_t *table, *lens, *parents;
     int32_t *table2, *lens2, *refs;
@@ -686,12 +696,33 @@ int vs_kv_evict(vs_kv *kv, const vs_kv_seqs *s, int64_t window, int64_t sinks, v
 }
 
 int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out, void *stream) {
+    return vs_kv_compact_with(kv, in, out, nullptr, 0, nullptr, stream);
+}
+
+int vs_kv_compact_with(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out,
+                       const vs_kv_seqs *const *others, int64_t nothers, int32_t *map,
+                       void *stream) {
     if (!kv) return report(VS_ERR_INVALID, "null handle");
     int rc = vs::check_seqs(kv, in);
     if (!rc) rc = vs::check_seqs(kv, out);
     if (rc) return rc;
     if (in->width != out->width || in->nseq != out->nseq)
         return report(VS_ERR_INVALID, "compact: in and out differ in shape");
+    if (nothers < 0 || (nothers && !others) || (uintptr_t)map % 4)
+        return report(VS_ERR_INVALID, "null others, or an unaligned map");
+    if (nothers && in->refs != out->refs)
+        return report(VS_ERR_INVALID, "others stay on their counts: in and out have to share them");
+    for (int64_t i = 0; i < nothers; ++i) {
+        rc = vs::check_seqs(kv, others[i]);
+        if (rc) return rc;
+        if (others[i]->refs != in->refs)
+            return report(VS_ERR_INVALID, "other %lld is on other counts", (long long)i);
+        // (a table that is rewritten twice would follow its pages twice)
+        const int32_t *t = others[i]->table;
+        bool again = t && (t == in->table || t == out->table);
+        for (int64_t j = 0; j < i; ++j) again |= t && t == others[j]->table;
+        if (again) return report(VS_ERR_INVALID, "other %lld is named twice", (long long)i);
+    }
     vs::DeviceGuard g(kv->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
@@ -703,8 +734,8 @@ int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out, void *
     a.refs = in->refs;
     a.refs2 = out->refs;
     a.npages = (int)np;
-    a.map = (int32_t *)ws;
-    a.from = a.map + np;
+    a.map = map ? map : (int32_t *)ws;
+    a.from = (int32_t *)ws + np;
     a.to = a.from + np;
     a.moves = a.to + np;
     a.status = kv->status;
@@ -718,7 +749,15 @@ int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out, void *
                                out->table, out->lens, in->nseq * in->width,
                                (int)in->nseq};
     hipError_t e = vs::launch_copy(kv, a.moves, np / 2 + 1, a.from, a.to, 1, st, tables);
-    return e == hipSuccess ? VS_OK : report_hip(e, "page copies");
+    if (e != hipSuccess) return report_hip(e, "page copies");
+    for (int64_t i = 0; i < nothers; ++i) {
+        const int64_t entries = others[i]->nseq * others[i]->width;
+        if (!entries) continue;
+        hipLaunchKernelGGL(vs::remap_kernel, dim3(vs::grid_of((entries + 255) / 256, 2048)), dim3(256),
+                           0, st, others[i]->table, entries, (int)np, a.map);
+        VS_LAUNCHED("compact");
+    }
+    return VS_OK;
 }
 
 int vs_kv_copy(vs_kv *kv, const int32_t *from, const int32_t *to, int64_t n, void *stream) {

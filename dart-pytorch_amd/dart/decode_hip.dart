@@ -81,8 +81,9 @@ class _Lib {
       int Function(_P, _S, _P, int, _P)>('vs_kv_free');
   late final evict = lib.lookupFunction<ffi.Int32 Function(_P, _S, ffi.Int64, ffi.Int64, _P),
       int Function(_P, _S, int, int, _P)>('vs_kv_evict');
-  late final compact =
-      lib.lookupFunction<ffi.Int32 Function(_P, _S, _S, _P), int Function(_P, _S, _S, _P)>('vs_kv_compact');
+  late final compactWith = lib.lookupFunction<
+      ffi.Int32 Function(_P, _S, _S, ffi.Pointer<_S>, ffi.Int64, _P, _P),
+      int Function(_P, _S, _S, ffi.Pointer<_S>, int, _P, _P)>('vs_kv_compact_with');
   late final check = lib.lookupFunction<ffi.Int32 Function(_P, _P), int Function(_P, _P)>('vs_kv_check');
 
   late final beamCreate = lib.lookupFunction<ffi.Int32 Function(ffi.Int32, ffi.Pointer<_P>),
@@ -278,9 +279,24 @@ class PagedKvCache {
   void evict(KvSequences s, int window, {int sinks = 0, int stream = 0}) =>
       _vs.ok(_vs.evict(_handle, _seqs(s), window, sinks, _at(stream)));
 
-  /// Moves the pages in use to the cache's front.
-  void compact(KvSequences s, {KvSequences? out, int stream = 0}) =>
-      _vs.ok(_vs.compact(_handle, _seqs(s), _seqs(out ?? s), _at(stream)));
+  /// Moves the pages in use to the cache's front, whoever holds them: every
+  /// other set of sequences on the same counts has to be in [others], whose
+  /// tables follow in place; [moved] (i32 `[pages]`) receives where each page's
+  /// contents are now, for holds that are in no table.
+  void compact(KvSequences s,
+      {KvSequences? out, List<KvSequences> others = const [], GpuArray? moved, int stream = 0}) {
+    if (moved != null) _expect(moved, 'moved', [pages], GpuType.i32);
+    final more = calloc<_S>(math.max(1, others.length));
+    try {
+      for (var i = 0; i < others.length; i++) {
+        more[i] = _seqs(others[i]);
+      }
+      _vs.ok(_vs.compactWith(_handle, _seqs(s), _seqs(out ?? s), more, others.length,
+          moved?.pointer ?? ffi.nullptr, _at(stream)));
+    } finally {
+      calloc.free(more);
+    }
+  }
 
   /// Waits; throws what earlier calls met on the device (too few pages, ...).
   void check({int stream = 0}) => _vs.ok(_vs.check(_handle, _at(stream)));

@@ -44,7 +44,7 @@ EXPORTED = [
     "vs_index_sync", "vs_index_set_option",
     "vs_kv_create", "vs_kv_destroy", "vs_kv_page_bytes", "vs_kv_memory", "vs_kv_attend",
     "vs_kv_append", "vs_kv_read", "vs_kv_extend", "vs_kv_fork", "vs_kv_free", "vs_kv_evict",
-    "vs_kv_compact", "vs_kv_copy", "vs_kv_check",
+    "vs_kv_compact", "vs_kv_compact_with", "vs_kv_copy", "vs_kv_check",
     "vs_beam_create", "vs_beam_destroy", "vs_beam_select", "vs_beam_reorder",
 ]
 
@@ -158,6 +158,7 @@ def load() -> ctypes.CDLL:
         "vs_kv_free": ([p, p, p, i64, p], i32),
         "vs_kv_evict": ([p, p, i64, i64, p], i32),
         "vs_kv_compact": ([p, p, p, p], i32),
+        "vs_kv_compact_with": ([p, p, p, p, i64, p, p], i32),
         "vs_kv_copy": ([p, p, p, i64, p], i32),
         "vs_kv_check": ([p, p], i32),
         "vs_beam_create": ([i32, pp], i32),

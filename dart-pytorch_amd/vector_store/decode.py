@@ -280,7 +280,8 @@ class PagedKVCache:
 
     def fork(self, seqs: KVSequences, parents, out: KVSequences, *, stream: int = 0) -> None:
         """out[i] = a copy of seqs[parents[i]] that shares its pages; what is
-        no one's parent gives its pages back (vs_kv_fork)."""
+        no one's parent gives its pages back.  seqs' references go over to
+        out: it is not used again but as a later fork's `out` (vs_kv_fork)."""
         rc = self._lib.vs_kv_fork(self._h, self._seqs(seqs), _list(parents, "parents", out.n, _I32),
                                   self._seqs(out), stream)
         if rc:
@@ -298,9 +299,23 @@ class PagedKVCache:
         """Gives back whole pages behind the window (vs_kv_evict)."""
         N.check(self._lib.vs_kv_evict(self._h, self._seqs(seqs), window, sinks, stream))
 
-    def compact(self, seqs: KVSequences, out: KVSequences | None = None, *, stream: int = 0) -> None:
-        """Moves the pages in use to the cache's front (vs_kv_compact)."""
-        rc = self._lib.vs_kv_compact(self._h, self._seqs(seqs), self._seqs(seqs if out is None else out), stream)
+    def compact(self, seqs: KVSequences, out: KVSequences | None = None, *, others=(), moved=None, stream: int = 0) -> None:
+        """Moves the pages in use to the cache's front (vs_kv_compact).
+
+        All of them, whoever holds them: every other KVSequences on the same
+        counts has to be in `others`, whose tables follow in place.  moved
+        (i32 [pages]): receives where each page's contents are now, for holds
+        that are in no table (vs_kv_compact_with)."""
+        src, dst = self._seqs(seqs), self._seqs(seqs if out is None else out)
+        if moved is None and not others:
+            rc = self._lib.vs_kv_compact(self._h, src, dst, stream)
+        else:
+            for s in others:
+                self._seqs(s)
+            more = (ctypes.c_void_p * max(1, len(others)))(*(ctypes.addressof(s.c) for s in others))
+            rc = self._lib.vs_kv_compact_with(self._h, src, dst, more, len(others),
+                                              None if moved is None else _flat(moved, "moved", (self.npages,), _I32),
+                                              stream)
         if rc:
             N.check(rc)
 

@@ -307,7 +307,9 @@ VS_API int vs_kv_extend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t count, const 
  * are copied and refs follow; sequences of `in` that are no one's parent lose
  * their references, which frees pages that no one else holds.  in and out
  * have different table and lens buffers and equal width; refs may be one
- * buffer.  A parent outside [-1, nseq of in) counts as -1 and is reported. */
+ * buffer.  `in` is spent afterwards: its references have gone over to `out`, so
+ * its sequences are neither attended to, extended, freed nor forked again (one
+ * that is to stay is made the parent of one of out's).  A parent outside [-1, nseq of in) counts as -1 and is reported. */
 VS_API int vs_kv_fork(vs_kv *kv, const vs_kv_seqs *in, const int32_t *parents,
                       const vs_kv_seqs *out, void *stream);
 /* Drops the n listed sequences (device ids; null: all): their references are
@@ -320,9 +322,18 @@ VS_API int vs_kv_free(vs_kv *kv, const vs_kv_seqs *seqs, const int32_t *ids, int
 VS_API int vs_kv_evict(vs_kv *kv, const vs_kv_seqs *seqs, int64_t window, int64_t sinks,
                        void *stream);
 /* Moves the pages in use to the front: with L pages in use, the j-th of those
- * at or past L moves to the j-th free page below L; tables and refs follow.
- * Afterwards pages L and up are free.  out may be in. */
+ * at or past L moves to the j-th free page below L; in's table and refs follow,
+ * as out's.  Afterwards pages L and up are free.  out may be in.  Every page with
+ * a count is moved, whoever holds it: where sequences other than in's, or holds
+ * of the caller's own, are on these counts, vs_kv_compact_with is the call. */
 VS_API int vs_kv_compact(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out, void *stream);
+/* The same with everything else that names pages: the tables of `others`
+ * (nothers host pointers; in, out and they are on one refs buffer, no table is
+ * named twice) follow in place, and map, if not null (npages device words), tells
+ * where each page's contents are now: map[p], p itself if they were not moved. */
+VS_API int vs_kv_compact_with(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out,
+                              const vs_kv_seqs *const *others, int64_t nothers, int32_t *map,
+                              void *stream);
 /* Copies whole pages, to[i] = from[i] (n device ids each): pages outside
  * [0, npages) are skipped; no page may be both read and written, or written
  * twice. */
