@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <new>
 #include <vector>
 
@@ -31,20 +32,30 @@ struct DeviceGuard {
     }
 };
 
+// A number of the calling thread's own, never given to another.
+inline uint64_t thread_number() {
+    static std::atomic<uint64_t> last{0};
+    thread_local const uint64_t mine = ++last;
+    return mine;
+}
+
 // Scratch memory of a handle, one buffer per stream, so that calls on
-// different streams never share one.  A buffer that is outgrown is kept until
-// the handle ends: a recorded graph may still use it.
+// different streams never share one.  hipStreamPerThread is one name for a
+// stream of each thread's own, so there the thread counts too.  A buffer that
+// is outgrown is kept until the handle ends: a recorded graph may still use it.
 struct StreamScratch {
     struct Buf {
         hipStream_t st;
+        uint64_t thread;  // 0: the stream is the same for all
         void *p;
         size_t bytes;
     };
     std::vector<Buf> bufs;
 
     int get(hipStream_t st, size_t need, void **out) {
+        const uint64_t thread = st == hipStreamPerThread ? thread_number() : 0;
         for (auto it = bufs.rbegin(); it != bufs.rend(); ++it)
-            if (it->st == st) {
+            if (it->st == st && it->thread == thread) {
                 if (it->bytes < need) break;
                 *out = it->p;
                 return VS_OK;
@@ -63,7 +74,7 @@ struct StreamScratch {
         hipError_t e = device_alloc(&p, bytes);
         if (e != hipSuccess) return report_hip(e, "scratch memory");
         try {
-            bufs.push_back({st, p, bytes});
+            bufs.push_back({st, thread, p, bytes});
         } catch (const std::bad_alloc &) {
             (void)hipFree(p);
             return report(VS_ERR_OOM, "host allocation");

@@ -219,7 +219,8 @@ VS_API int vs_kmeans_step(vs_index *points, const float *centroids_in, int64_t K
  * default stream) and return without waiting for it.  Arguments that the
  * host can see are checked before anything is launched; what only the device
  * sees (table entries, lengths, parents) is checked by the kernels and told
- * by vs_kv_check.  Scratch memory is kept per handle and stream and grows at
+ * by vs_kv_check.  Scratch memory is kept per handle and stream (with
+ * hipStreamPerThread per thread, too) until the handle ends, and grows at
  * a first call of a size: a call that is recorded into a graph and would
  * have to allocate is refused (VS_ERR_UNSUPPORTED; run it once before).  A
  * recorded call keeps the scratch of the stream it was recorded on: replays
