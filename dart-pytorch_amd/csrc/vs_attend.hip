@@ -405,8 +405,9 @@ __global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 
             new_page = trow[(n - 1) >> a.page_shift];
             if (a.lens[it.b] > n) {  // past the table: n - 1 is not the new token's place
                 if (lane == 0) atomicOr(&a.status[0], kStatusWidth);
-            } else if ((unsigned)new_page < (unsigned)a.npages &&
-                       !(marked && a.closed[new_page])) {
+            } else if ((unsigned)new_page >= (unsigned)a.npages) {
+                if (lane == 0) atomicOr(&a.status[0], kStatusNoPage);
+            } else if (!(marked && a.closed[new_page])) {
                 u_new = u;
             }
         }
@@ -679,7 +680,7 @@ struct RowsArgs {
     const int32_t *table, *lens, *starts;
     int64_t width, nrows;
     int nseq, npages, page_shift, heads, dim;
-    const int32_t *status;
+    int32_t *status;
     const uint8_t *closed;
     const char *k, *v;
     int64_t k_row, k_head, v_row, v_head;
@@ -736,7 +737,11 @@ __global__ __launch_bounds__(256) void append_kernel(RowsArgs a, int64_t items) 
         const int64_t p0 = ((first >> 5) + blk) * kKvBlock;
         if (blk < 0 || count <= 0 || p0 < 0 || p0 >= end) continue;
         char *const at = block_of(a, (int)b, p0, sizeof(T));
-        if (!at) continue;
+        if (!at) {
+            if (p0 >> a.page_shift >= a.width && threadIdx.x == 0)
+                atomicOr(&a.status[0], kStatusWidth);
+            continue;
+        }
         if (end <= a.width << a.page_shift) {
             const int last = a.table[b * a.width + ((end - 1) >> a.page_shift)];
             if ((unsigned)last < (unsigned)a.npages && marked && a.closed[last]) continue;

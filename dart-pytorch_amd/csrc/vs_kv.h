@@ -33,7 +33,7 @@ namespace vs {
 // extend that fits opens the pages that it gives or leaves to a sequence,
 // vs_kv_check opens all.
 constexpr int kStatusWords = 4;
-constexpr int kStatusPages = 1, kStatusWidth = 2, kStatusParent = 4;
+constexpr int kStatusPages = 1, kStatusWidth = 2, kStatusParent = 4, kStatusNoPage = 8;
 
 // Positions per block, the unit of the cache's layout: what one bf16 matrix
 // instruction sums over.

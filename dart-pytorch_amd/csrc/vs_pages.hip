@@ -793,6 +793,7 @@ int vs_kv_check(vs_kv *kv, void *stream) {
         return report(VS_ERR_OOM, "the cache was %d pages short", (int)got[1]);
     if (got[0] & vs::kStatusWidth)
         return report(VS_ERR_INVALID, "a sequence outgrew its %s", "table row");
+    if (got[0] & vs::kStatusNoPage) return report(VS_ERR_INVALID, "a new token has no page");
     if (got[0] & vs::kStatusParent) return report(VS_ERR_INVALID, "a parent is out of range");
     return VS_OK;
 }

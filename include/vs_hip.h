@@ -272,7 +272,8 @@ VS_API void *vs_kv_memory(const vs_kv *kv);
  * head_dim values at [b * *_seq + h * *_head] elements; lse is [nseq][heads]
  * fp32.  With k and v (both or neither; [nseq][kv_heads] rows like q) the new
  * token's keys and values are stored at position n - 1 in the same pass, so
- * that page must be this sequence's alone (vs_kv_extend sees to it).
+ * that page must be this sequence's alone (vs_kv_extend sees to it).  Where that
+ * position is on no page it is not stored, and vs_kv_check says so.
  * Products of bf16 values, sums and the softmax are held in fp32. */
 VS_API int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t heads,
                         const void *q, int64_t q_seq, int64_t q_head, const void *k, int64_t k_seq,
@@ -282,7 +283,9 @@ VS_API int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_
 /* Stores keys and values of a layer: rows [starts[b], starts[b + 1]) of k and
  * v go to the last starts[b + 1] - starts[b] positions of sequence b (starts:
  * nseq + 1 ascending device values, starts[0] >= 0; null: one row each, row b
- * of sequence b).  nrows: how many rows k and v have. */
+ * of sequence b).  nrows: how many rows k and v have.  Rows of positions that are
+ * on no page are dropped (a prompt's positions behind a window need none); rows
+ * past the table's columns too, and vs_kv_check says so. */
 VS_API int vs_kv_append(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, const void *k,
                         int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
                         const int32_t *starts, int64_t nrows, void *stream);
@@ -341,8 +344,8 @@ VS_API int vs_kv_compact_with(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs 
 VS_API int vs_kv_copy(vs_kv *kv, const int32_t *from, const int32_t *to, int64_t n, void *stream);
 /* Waits for the stream and tells what earlier calls met on the device since
  * the last check: VS_ERR_OOM (an extend found too few free pages),
- * VS_ERR_INVALID (too few table columns for an extend or for an attend's new
- * token; a parent out of range). */
+ * VS_ERR_INVALID (too few table columns for an extend, an attend's new token or
+ * an append's rows; a new token without a page; a parent out of range). */
 VS_API int vs_kv_check(vs_kv *kv, void *stream);
 
 /* Beam search over device buffers.  A handle owns scratch memory only. */
