@@ -19,7 +19,8 @@ values, and the choice of the next tokens.
 Buffers are anything in device memory with data_ptr(), shape, stride() and
 dtype: DeviceArray of this module or a tensor of a framework that works on the
 same GPU (imported before this package loads its library, so that both use the
-HIP runtime that the framework brings).  Calls run on `stream` (an integer hipStream_t, 0 the default
+HIP runtime that the framework brings).  Where a buffer says where it lies
+(get_device(), -1 for host memory) it has to be the handle's device.  Calls run on `stream` (an integer hipStream_t, 0 the default
 stream) and return without waiting for it.
 """
 from __future__ import annotations
@@ -60,6 +61,7 @@ class DeviceArray:
         if any(s < 0 for s in self.shape):
             raise ValueError(f"negative size in {self.shape}")
         self.dtype = dtype
+        self.device = int(device)
         self._code = _code(dtype)
         out, s = [], 1
         for n in reversed(self.shape):
@@ -79,6 +81,12 @@ class DeviceArray:
 
     def stride(self):
         return self._stride
+
+    def is_contiguous(self) -> bool:
+        return True
+
+    def get_device(self) -> int:
+        return self.device
 
     def upload(self, a) -> "DeviceArray":
         a = np.ascontiguousarray(a, self._NUMPY[self._code])
@@ -100,8 +108,27 @@ class DeviceArray:
 # checks below take the straight way where all is well.
 
 
-def _rows(t, what, shape, code):
-    """Pointer and strides of a buffer of `shape` whose last dimension is contiguous."""
+def _device_of(t):
+    """The device that a buffer says it lies on; None if it does not say."""
+    try:
+        return t.get_device()
+    except AttributeError:
+        return None
+
+
+def _on(t, what, device) -> None:
+    try:
+        on = t.get_device()
+    except AttributeError:
+        return
+    if on != device:
+        raise ValueError(f"{what}: in {'host memory' if on < 0 else f'memory of device {on}'}, expected device {device}")
+
+
+def _rows(t, what, shape, code, device=None):
+    """Pointer and strides of a buffer of `shape` whose last dimension is contiguous (on `device`, if given)."""
+    if device is not None:
+        _on(t, what, device)
     st = t.stride()
     if t.shape != shape or _SEEN.get(t.dtype) != code or st[-1] != 1:
         if _code(t.dtype) != code:
@@ -113,10 +140,15 @@ def _rows(t, what, shape, code):
     return t.data_ptr(), st
 
 
-def _flat(t, what, shape, code) -> int:
-    """Pointer of a contiguous buffer of `shape`."""
-    if (t.shape != shape or _SEEN.get(t.dtype) != code
-            or t.stride() != ((shape[1], 1) if len(shape) == 2 else (1,))):
+def _flat(t, what, shape, code, device=None) -> int:
+    """Pointer of a contiguous buffer of `shape` (on `device`, if given)."""
+    if device is not None:
+        _on(t, what, device)
+    try:
+        fine = t.is_contiguous() and t.shape == shape and _SEEN.get(t.dtype) == code
+    except AttributeError:
+        fine = False
+    if not fine:
         _look_closely(t, what, shape, code)
     return t.data_ptr()
 
@@ -133,11 +165,17 @@ def _look_closely(t, what, shape, code) -> None:
         n *= size
 
 
-def _list(t, what, n, code) -> int:
-    """Pointer of a contiguous buffer of n elements, whatever its shape."""
+def _list(t, what, n, code, device=None) -> int:
+    """Pointer of a contiguous buffer of n elements, whatever its shape (on `device`, if given)."""
+    if device is not None:
+        _on(t, what, device)
     shape = t.shape
     if len(shape) == 2 and shape[0] * shape[1] == n:  # (beams' outputs, [requests, k])
-        if _SEEN.get(t.dtype) != code or t.stride() != (shape[1], 1):
+        try:
+            fine = t.is_contiguous() and _SEEN.get(t.dtype) == code
+        except AttributeError:
+            fine = False
+        if not fine:
             _look_closely(t, what, tuple(shape), code)
         return t.data_ptr()
     if math.prod(shape) != n:
@@ -161,6 +199,10 @@ class KVSequences:
         n, width = (int(s) for s in table.shape)
         self.table, self.lens, self.refs = table, lens, refs
         self.n, self.width, self.npages = n, width, int(refs.shape[0])
+        known = {d for d in map(_device_of, (table, lens, refs)) if d is not None}
+        if len(known) > 1 or min(known, default=0) < 0:
+            raise ValueError(f"table, lens and refs: devices {sorted(known)} (-1: host memory), expected one device")
+        self.device = known.pop() if known else None
         self.c = _SeqsC(_flat(table, "table", (n, width), _I32), _flat(lens, "lens", (n,), _I32),
                         _flat(refs, "refs", (int(refs.shape[0]),), _I32), n, width)
         self._ref = ctypes.byref(self.c)
@@ -173,7 +215,7 @@ class PagedKVCache:
                  dtype: str = "bf16", device: int = 0, memory=None):
         self._h = None
         self._lib = N.load()
-        self.device = device
+        self.device = int(device)
         self.npages, self.page_size, self.layers = int(npages), int(page_size), int(layers)
         self.kv_heads, self.head_dim = int(kv_heads), int(head_dim)
         self.code = _code(dtype)
@@ -184,7 +226,7 @@ class PagedKVCache:
         p = None
         if memory is not None:
             total = (self.npages * self.layers * 2 * self.kv_heads * self.page_size * self.head_dim)
-            p = _flat(memory, "memory", tuple(int(s) for s in memory.shape), self.code)
+            p = _flat(memory, "memory", tuple(int(s) for s in memory.shape), self.code, self.device)
             if math.prod(memory.shape) < total:
                 raise ValueError(f"memory holds {math.prod(memory.shape)} values of {total}")
         h = ctypes.c_void_p()
@@ -219,6 +261,8 @@ class PagedKVCache:
     def _seqs(self, s: KVSequences):
         if s.npages != self.npages:
             raise ValueError(f"refs of {s.npages} pages on a cache of {self.npages}")
+        if s.device != self.device and s.device is not None:
+            raise ValueError(f"sequences on device {s.device}, a cache on device {self.device}")
         return s._ref
 
     def attend(self, seqs: KVSequences, q, out, *, k=None, v=None, lse=None, layer: int = 0, scale=None,
@@ -228,19 +272,19 @@ class PagedKVCache:
         q, out [n, heads, head_dim]; k, v [n, kv_heads, head_dim]: the new
         token's, stored in the same pass; lse [n, heads] f32.  window > 0: the
         last `window` positions and the first `sinks` are visible."""
-        n, code, dim = seqs.n, self.code, self.head_dim
+        n, code, dim, dev = seqs.n, self.code, self.head_dim, self.device
         heads = int(q.shape[1])
-        qp, qs = _rows(q, "q", (n, heads, dim), code)
-        op, os_ = _rows(out, "out", (n, heads, dim), code)
+        qp, qs = _rows(q, "q", (n, heads, dim), code, dev)
+        op, os_ = _rows(out, "out", (n, heads, dim), code, dev)
         kp = vp = lp = None
         ks = vs = (0, 0)
         if k is not None or v is not None:
             if k is None or v is None:
                 raise ValueError("k and v are given together or not at all")
-            kp, ks = _rows(k, "k", (n, self.kv_heads, dim), code)
-            vp, vs = _rows(v, "v", (n, self.kv_heads, dim), code)
+            kp, ks = _rows(k, "k", (n, self.kv_heads, dim), code, dev)
+            vp, vs = _rows(v, "v", (n, self.kv_heads, dim), code, dev)
         if lse is not None:
-            lp = _flat(lse, "lse", (n, heads), N.VS_DTYPE_F32)
+            lp = _flat(lse, "lse", (n, heads), N.VS_DTYPE_F32, dev)
         rc = self._lib.vs_kv_attend(
             self._h, self._seqs(seqs), layer, heads, qp, qs[0], qs[1], kp, ks[0], ks[1], vp, vs[0], vs[1],
             op, os_[0], os_[1], lp, self._scale if scale is None else scale, window, sinks, stream)
@@ -252,9 +296,9 @@ class PagedKVCache:
         (vs_kv_append): k, v [rows, kv_heads, head_dim]; starts [n + 1] i32:
         rows starts[b] .. starts[b + 1] are sequence b's (none: one each)."""
         rows = int(k.shape[0])
-        kp, ks = _rows(k, "k", (rows, self.kv_heads, self.head_dim), self.code)
-        vp, vs = _rows(v, "v", (rows, self.kv_heads, self.head_dim), self.code)
-        sp = None if starts is None else _flat(starts, "starts", (seqs.n + 1,), _I32)
+        kp, ks = _rows(k, "k", (rows, self.kv_heads, self.head_dim), self.code, self.device)
+        vp, vs = _rows(v, "v", (rows, self.kv_heads, self.head_dim), self.code, self.device)
+        sp = None if starts is None else _flat(starts, "starts", (seqs.n + 1,), _I32, self.device)
         N.check(self._lib.vs_kv_append(self._h, self._seqs(seqs), layer, kp, ks[0], ks[1], vp, vs[0], vs[1],
                                        sp, rows, stream))
 
@@ -262,8 +306,8 @@ class PagedKVCache:
         """Positions first .. of sequence b as rows [positions, kv_heads, head_dim] (vs_kv_read)."""
         shape = (int(k_out.shape[0]), self.kv_heads, self.head_dim)
         N.check(self._lib.vs_kv_read(self._h, self._seqs(seqs), layer, b, first, shape[0],
-                                     _flat(k_out, "k_out", shape, self.code),
-                                     _flat(v_out, "v_out", shape, self.code), stream))
+                                     _flat(k_out, "k_out", shape, self.code, self.device),
+                                     _flat(v_out, "v_out", shape, self.code, self.device), stream))
 
     def extend(self, seqs: KVSequences, count=1, *, stream: int = 0) -> None:
         """`count` more positions for every sequence (an int, or an i32 buffer
@@ -274,7 +318,7 @@ class PagedKVCache:
             rc = self._lib.vs_kv_extend(self._h, self._seqs(seqs), count, None, stream)
         else:
             rc = self._lib.vs_kv_extend(self._h, self._seqs(seqs), 0,
-                                        _flat(count, "count", (seqs.n,), _I32), stream)
+                                        _flat(count, "count", (seqs.n,), _I32, self.device), stream)
         if rc:
             N.check(rc)
 
@@ -282,7 +326,7 @@ class PagedKVCache:
         """out[i] = a copy of seqs[parents[i]] that shares its pages; what is
         no one's parent gives its pages back.  seqs' references go over to
         out: it is not used again but as a later fork's `out` (vs_kv_fork)."""
-        rc = self._lib.vs_kv_fork(self._h, self._seqs(seqs), _list(parents, "parents", out.n, _I32),
+        rc = self._lib.vs_kv_fork(self._h, self._seqs(seqs), _list(parents, "parents", out.n, _I32, self.device),
                                   self._seqs(out), stream)
         if rc:
             N.check(rc)
@@ -292,7 +336,7 @@ class PagedKVCache:
         n = 0 if ids is None else int(ids.shape[0])
         if ids is not None and n == 0:
             return
-        p = None if ids is None else _flat(ids, "ids", (n,), _I32)
+        p = None if ids is None else _flat(ids, "ids", (n,), _I32, self.device)
         N.check(self._lib.vs_kv_free(self._h, self._seqs(seqs), p, n, stream))
 
     def evict(self, seqs: KVSequences, window: int, sinks: int = 0, *, stream: int = 0) -> None:
@@ -314,7 +358,7 @@ class PagedKVCache:
                 self._seqs(s)
             more = (ctypes.c_void_p * max(1, len(others)))(*(ctypes.addressof(s.c) for s in others))
             rc = self._lib.vs_kv_compact_with(self._h, src, dst, more, len(others),
-                                              None if moved is None else _flat(moved, "moved", (self.npages,), _I32),
+                                              None if moved is None else _flat(moved, "moved", (self.npages,), _I32, self.device),
                                               stream)
         if rc:
             N.check(rc)
@@ -322,7 +366,7 @@ class PagedKVCache:
     def copy(self, src, dst, *, stream: int = 0) -> None:
         """Page dst[i] = page src[i] (i32 buffers) (vs_kv_copy)."""
         n = int(src.shape[0])
-        N.check(self._lib.vs_kv_copy(self._h, _flat(src, "src", (n,), _I32), _flat(dst, "dst", (n,), _I32), n, stream))
+        N.check(self._lib.vs_kv_copy(self._h, _flat(src, "src", (n,), _I32, self.device), _flat(dst, "dst", (n,), _I32, self.device), n, stream))
 
     def check(self, *, stream: int = 0) -> None:
         """Waits for the stream; raises what earlier calls met on the device (vs_kv_check)."""
@@ -335,6 +379,7 @@ class BeamSearch:
     def __init__(self, device: int = 0):
         self._h = None
         self._lib = N.load()
+        self.device = int(device)
         h = ctypes.c_void_p()
         N.check(self._lib.vs_beam_create(device, ctypes.byref(h)))
         self._h = h
@@ -357,6 +402,16 @@ class BeamSearch:
         logits [requests * beams, vocab] f32 or bf16; scores [requests, beams]
         f32; finished [requests, beams] u8.  Outputs [requests, k]: scores f32,
         tokens and parents (rows of logits) i32, finished u8."""
+        dev = self.device
+        try:  # (all in one: a step of one request takes as long as its Python calls)
+            here = (logits.get_device() == scores.get_device() == scores_out.get_device() == tokens_out.get_device()
+                    == parents_out.get_device() == dev)
+        except AttributeError:
+            here = False
+        if not here:
+            for t, what in ((logits, "logits"), (scores, "scores"), (scores_out, "scores_out"),
+                            (tokens_out, "tokens_out"), (parents_out, "parents_out")):
+                _on(t, what, dev)
         requests, beams = shape = scores.shape
         rows, vocab = logits.shape
         code = _SEEN.get(logits.dtype)
@@ -373,10 +428,10 @@ class BeamSearch:
         rc = self._lib.vs_beam_select(
             self._h, logits.data_ptr(), code, ls[0] if rows > 1 else vocab, requests, beams, vocab,
             _flat(scores, "scores", shape, N.VS_DTYPE_F32),
-            None if finished is None else _flat(finished, "finished", shape, _U8), eos, k,
+            None if finished is None else _flat(finished, "finished", shape, _U8, dev), eos, k,
             _flat(scores_out, "scores_out", out, N.VS_DTYPE_F32), _flat(tokens_out, "tokens_out", out, _I32),
             _flat(parents_out, "parents_out", out, _I32),
-            None if finished_out is None else _flat(finished_out, "finished_out", out, _U8), stream)
+            None if finished_out is None else _flat(finished_out, "finished_out", out, _U8, dev), stream)
         if rc:
             N.check(rc)
 
@@ -387,6 +442,14 @@ class BeamSearch:
         code = _SEEN.get(out.dtype)
         if code is None:
             code = _code(out.dtype)
+        dev = self.device
+        try:
+            here = state.get_device() == out.get_device() == parents.get_device() == dev
+        except AttributeError:
+            here = False
+        if not here:
+            for t, what in ((state, "state"), (out, "out"), (parents, "parents")):
+                _on(t, what, dev)
         rows, cols = out.shape
         nin, wide = state.shape
         is_, os_ = state.stride(), out.stride()
@@ -398,7 +461,7 @@ class BeamSearch:
         if tail is not None:
             if code != _I32 or cols < 1:
                 raise ValueError("tail needs an i32 state of at least one column")
-            tp, keep = _list(tail, "tail", rows, _I32), cols - 1
+            tp, keep = _list(tail, "tail", rows, _I32, dev), cols - 1
         pp = _list(parents, "parents", rows, _I32)
         wide = cols * size
         rc = self._lib.vs_beam_reorder(
