@@ -14,6 +14,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kWaves = 4;      // per workgroup
 constexpr int kMinBlocks = 4;  // blocks per work item, at least: one per wave
 constexpr int kGoodBlocks = 8; // and before a CU takes a second workgroup
+constexpr int kFindSeqs = 384; // sequences that each workgroup divides for itself
 // dimensions joined over the waves at once, by what LDS holds
 constexpr int join_dims(int waves) { return waves == 8 ? 64 : 128; }
 constexpr int kWideDim = 128;  // heads up to this size have an eight-wave kernel
@@ -39,6 +40,8 @@ struct AttendArgs {
     int32_t *status;
     const uint8_t *closed;
     int2 *first;     // [nseq] first whole item; whole ones * 2 + whether there is a rest
+    int32_t *plan;   // blocks per piece, then [item] its sequence, or -1; null: find_item
+    int items;
 };
 
 // The blocks that a sequence of n positions attends to: nsb from its start,
@@ -66,8 +69,36 @@ __device__ __forceinline__ int length_of(const AttendArgs &a, int b) {
     return n < most ? n : (int)most;
 }
 
+// Blocks of sequence b.
+__device__ __forceinline__ int blocks_of(const AttendArgs &a, int b) {
+    return span_of(length_of(a, b), a.window, a.sinks).total;
+}
+
+// How many blocks a piece has: `total` of all sequences, `widest` of one.
+// Lengths far apart: pieces a third as long, which spread better (64
+// sequences of 65 to 8,190 positions 98 against 107 us, 256 of 100 to 4,000
+// 128 against 139); about equal ones: as few joins as can be (64 of 4,096
+// 191 against 196 us).
+__device__ __forceinline__ int blocks_per_piece(const AttendArgs &a, uint64_t total, int widest) {
+    auto over = [&](int items) {
+        return total >> 31 ? (int)((total + items - 1) / (uint64_t)items)
+                           : (int)(((uint32_t)total + items - 1) / (uint32_t)items);
+    };
+    const bool ragged = (uint64_t)widest * a.nseq > 2 * total;
+    const int items = max(ragged ? a.most_items : a.most_items / 3, 1);
+    int per = max(max(over(items), min(over(a.few_items), kGoodBlocks)), kMinBlocks);
+    // (and equal ones: a small rest of every sequence would be a workgroup more each)
+    if (!ragged && widest > per) {
+        int pieces = (widest + per - 1) / per;
+        if ((uint64_t)pieces * a.nseq > (uint64_t)items) pieces = widest / per;
+        per = (widest + pieces - 1) / pieces;
+    }
+    return per;
+}
+
 // Work item `item`: blocks [split * per, ...) of sequence b.  Every wave works
-// the division out by itself from the lengths.  `per` is all blocks of the
+// the division out by itself from the lengths (of up to kFindSeqs sequences: the
+// work is that of all lengths per workgroup).  `per` is all blocks of the
 // call over the workgroups that the card holds at once, so that long sequences
 // of a ragged batch are split and short ones are not.  First come all whole
 // pieces of `per` blocks, then what is left of the sequences: the smaller ones
@@ -80,48 +111,29 @@ struct Item {
 };
 
 __device__ __forceinline__ bool find_item(const AttendArgs &a, int item, int lane, Item &it) {
-    auto blocks_of = [&](int b) {
-        return b < a.nseq ? span_of(length_of(a, b), a.window, a.sinks).total : -1;
-    };
-    const int t0 = blocks_of(lane);  // (all there is to read for up to 64 sequences)
+    auto blocks = [&](int b) { return b < a.nseq ? blocks_of(a, b) : -1; };
+    const int t0 = blocks(lane);  // (all there is to read for up to 64 sequences)
     uint64_t mine = max(t0, 0);
     int widest = max(t0, 0);
     for (int b = lane + 64; b < a.nseq; b += 64) {
-        const int t = blocks_of(b);
+        const int t = blocks(b);
         mine += (uint64_t)t;
         widest = max(widest, t);
     }
     // (2^20 sequences of 2^26 blocks at most)
     const uint64_t total = ((uint64_t)wave_sum((uint32_t)(mine >> 20)) << 20) +
                            wave_sum((uint32_t)mine & 0xFFFFF);
-    auto over = [&](int items) {
-        return total >> 31 ? (int)((total + items - 1) / (uint64_t)items)
-                           : (int)(((uint32_t)total + items - 1) / (uint32_t)items);
-    };
-    // Lengths far apart: pieces a third as long, which spread better (64
-    // sequences of 65 to 8,190 positions 98 against 107 us, 256 of 100 to 4,000
-    // 128 against 139); about equal ones: as few joins as can be (64 of 4,096
-    // 191 against 196 us).
     // (past 2^24 blocks a float is off by two of them at most, less than a piece)
-    const int longest = (int)wave_max((float)widest);
-    const bool ragged = (uint64_t)longest * a.nseq > 2 * total;
-    const int items = max(ragged ? a.most_items : a.most_items / 3, 1);
-    int per = max(max(over(items), min(over(a.few_items), kGoodBlocks)), kMinBlocks);
-    // (and equal ones: a small rest of every sequence would be a workgroup more each)
-    if (!ragged && longest > per) {
-        int pieces = (longest + per - 1) / per;
-        if ((uint64_t)pieces * a.nseq > (uint64_t)items) pieces = longest / per;
-        per = (longest + pieces - 1) / pieces;
-    }
+    const int per = blocks_per_piece(a, total, (int)wave_max((float)widest));
     it.per = per;
     int wholes = 0;
     for (int b0 = 0; b0 < a.nseq; b0 += 64)
-        wholes += (int)wave_sum((uint32_t)max(b0 ? blocks_of(b0 + lane) : t0, 0) / (uint32_t)per);
+        wholes += (int)wave_sum((uint32_t)max(b0 ? blocks(b0 + lane) : t0, 0) / (uint32_t)per);
     // the sequence whose whole pieces, or whose rest, the item's number falls into
     const bool rest_item = item >= wholes;
     int base = 0, rank = wholes;
     for (int b0 = 0; b0 < a.nseq; b0 += 64) {
-        const int t = b0 ? blocks_of(b0 + lane) : t0;
+        const int t = b0 ? blocks(b0 + lane) : t0;
         const int whole = (int)((uint32_t)max(t, 0) / (uint32_t)per);
         // (a sequence without blocks has its empty answer to write)
         const int rest = t >= 0 && (t == 0 || t != whole * per);
@@ -140,6 +152,55 @@ __device__ __forceinline__ bool find_item(const AttendArgs &a, int item, int lan
         rank = __builtin_amdgcn_readlane(rsum, 63);
     }
     return false;
+}
+
+// The same division as find_item's, once for all workgroups of the call: a launch
+// and 9 us, but each workgroup then has three loads instead of all lengths to
+// read.  find_item against this, 8 key-value heads of 128 in bf16, lengths of 64 to
+// 3,000 (and of 64 but for one of 16,384): 256 sequences 127 and 133 us (45 and 45),
+// 384 184 and 187 (63 and 51), 512 242 and 241 (85 and 58), 1,024 491 and 460, 4,096
+// 2,975 and 1,802, 16,384 32,600 and 7,020.  With 1 head 256 30 and 36, 512 52 and
+// 51, 4,096 483 and 270.
+__global__ __launch_bounds__(kPlan) void attend_plan_kernel(AttendArgs a) {
+    __shared__ int lds[kPlan / 64];
+    __shared__ unsigned long long sum;
+    __shared__ int most;
+    if (threadIdx.x == 0) {
+        sum = 0;
+        most = 0;
+    }
+    uint64_t mine = 0;
+    int widest = 0;
+    for (int b = threadIdx.x; b < a.nseq; b += kPlan) {
+        const int t = blocks_of(a, b);
+        mine += (uint64_t)t;
+        widest = max(widest, t);
+    }
+    __syncthreads();
+    atomicAdd(&sum, (unsigned long long)mine);
+    atomicMax(&most, widest);
+    __syncthreads();
+    const int per = blocks_per_piece(a, sum, most);
+    int32_t *seq_of = a.plan + 1;
+    int base = 0, total;
+    for (int b0 = 0; b0 < a.nseq; b0 += kPlan) {
+        const int b = b0 + threadIdx.x, t = b < a.nseq ? blocks_of(a, b) : 0;
+        const int whole = (int)((uint32_t)t / (uint32_t)per);
+        const int at = base + block_scan(whole, &total, lds);
+        base += total;
+        if (b >= a.nseq) continue;
+        a.first[b] = make_int2(at, whole * 2 + (t == 0 || t != whole * per));
+        for (int i = 0; i < whole; ++i) seq_of[at + i] = b;
+    }
+    for (int b0 = 0; b0 < a.nseq; b0 += kPlan) {
+        const int b = b0 + threadIdx.x;
+        const int rest = b < a.nseq ? a.first[b].y & 1 : 0;  // (its own store)
+        const int at = base + block_scan(rest, &total, lds);
+        base += total;
+        if (rest) seq_of[at] = b;
+    }
+    for (int i = base + threadIdx.x; i < a.items; i += kPlan) seq_of[i] = -1;
+    if (threadIdx.x == 0) a.plan[0] = per;
 }
 
 // The larger of the four lanes that share a column (lanes apart by 16).
@@ -231,6 +292,16 @@ __global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 
         it.b = item;
         it.per = INT32_MAX / kKvBlock;
         it.rest = 1;
+    } else if (a.plan) {
+        it.b = __builtin_amdgcn_readfirstlane(a.plan[1 + item]);
+        if (it.b < 0) return;
+        it.per = __builtin_amdgcn_readfirstlane(a.plan[0]);
+        it.first = __builtin_amdgcn_readfirstlane(a.first[it.b].x);
+        const int pieces = __builtin_amdgcn_readfirstlane(a.first[it.b].y);
+        it.whole = pieces >> 1;
+        it.rest = pieces & 1;
+        // (the rests' numbers come behind all whole ones)
+        it.split = min(item - it.first, it.whole);
     } else if (!find_item(a, item, lane, it)) {
         return;
     }
@@ -580,7 +651,7 @@ __global__ __launch_bounds__(64 * NW, D <= 96 ? 3 : NW == 8 || D <= (ST ? 192 : 
             }
         }
     }
-    if (a.first && hh == 0 && it.split == 0 && threadIdx.x == 0)
+    if (a.first && !a.plan && hh == 0 && it.split == 0 && threadIdx.x == 0)
         a.first[it.b] = make_int2(it.first, it.whole * 2 + it.rest);
 }
 
@@ -1045,12 +1116,23 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
         const size_t slots = (size_t)(items * heads);
         const size_t o_bytes = slots * kv->head_dim * sizeof(float);
         const size_t ml_bytes = slots * sizeof(float2);
+        const bool planned = s->nseq > vs::kFindSeqs;
+        const size_t f_bytes = (size_t)s->nseq * sizeof(int2);
         void *ws = nullptr;
-        rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)s->nseq * sizeof(int2), &ws);
+        rc = kv->scratch.get(
+            st, o_bytes + ml_bytes + f_bytes + (planned ? (size_t)(items + 1) * sizeof(int32_t) : 0),
+            &ws);
         if (rc) return rc;
         a.part_o = (float *)ws;
         a.part_ml = (float2 *)((char *)ws + o_bytes);
         a.first = (int2 *)((char *)ws + o_bytes + ml_bytes);
+        if (planned) {
+            a.plan = (int32_t *)(a.first + s->nseq);
+            a.items = (int)items;
+            hipLaunchKernelGGL(vs::attend_plan_kernel, dim3(1), dim3(vs::kPlan), 0, st, a);
+            const hipError_t e_ = hipGetLastError();
+            if (e_ != hipSuccess) return report_hip(e_, "attend");
+        }
     }
     hipError_t err = kv->dtype == VS_DTYPE_BF16
                          ? vs::launch_attend_dim<1>(a, items, join ? vs::kWaves : waves, join,

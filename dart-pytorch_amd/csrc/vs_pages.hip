@@ -8,25 +8,11 @@
 namespace vs {
 namespace {
 
-constexpr int kPlan = 1024;         // threads of the one-workgroup plans
 constexpr int kMostFresh = 1 << 20;  // pages that one extend gives a sequence
 constexpr int kSmallPages = 16384;    // of a cache whose compaction is planned in registers
 constexpr int kForkSeqs = 1024;      // sequences and words of a fork that one workgroup does
 constexpr int kForkWords = 1 << 12;
 constexpr int kPieceBytes = 8192;   // of a page, per workgroup pass of the copy
-
-// Exclusive prefix sum of x over the workgroup's kPlan threads; *total its sum.
-__device__ __forceinline__ int block_scan(int x, int *total, int *lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int incl = prefix_sum(x);
-    __syncthreads();
-    if (lane == 63) lds[wave] = incl;
-    __syncthreads();
-    // every wave sums the waves' totals for itself
-    const int w = prefix_sum(lane < kPlan / 64 ? lds[lane] : 0);
-    *total = __builtin_amdgcn_readlane(w, 63);
-    return incl - x + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
-}
 
 struct ExtendArgs {
     int32_t *table, *lens, *refs;

@@ -43,4 +43,19 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_readlane(prefix_sum((int)x), 63);
 }
 
+constexpr int kPlan = 1024;  // threads of plans that are made by one workgroup
+
+// Exclusive prefix sum of x over the workgroup's kPlan threads; *total its sum.
+__device__ __forceinline__ int block_scan(int x, int *total, int *lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int incl = prefix_sum(x);
+    __syncthreads();
+    if (lane == 63) lds[wave] = incl;
+    __syncthreads();
+    // every wave sums the waves' totals for itself
+    const int w = prefix_sum(lane < kPlan / 64 ? lds[lane] : 0);
+    *total = __builtin_amdgcn_readlane(w, 63);
+    return incl - x + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
+}
+
 }  // namespace vs
