@@ -50,6 +50,8 @@ inline int check_seqs(const vs_kv *kv, const vs_kv_seqs *s) {
         return report(VS_ERR_UNSUPPORTED, "table columns past 2^31 positions");
     if (!s->refs || (s->nseq > 0 && (!s->lens || (!s->table && s->width > 0))))
         return report(VS_ERR_INVALID, "null table, lens or refs");
+    if (((uintptr_t)s->table | (uintptr_t)s->lens | (uintptr_t)s->refs) % 4)
+        return report(VS_ERR_INVALID, "table, lens or refs are not aligned to their elements");
     return VS_OK;
 }
 
