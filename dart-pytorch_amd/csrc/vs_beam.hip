@@ -716,6 +716,20 @@ int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_strid
         ((uintptr_t)scores | (uintptr_t)scores_out | (uintptr_t)tokens_out |
          (uintptr_t)parents_out) % 4)
         return report(VS_ERR_INVALID, "a buffer is not aligned to its elements");
+    // Requests are merged at once, each from its own scores and flags: another
+    // one's outputs must not lie there.
+    const struct {
+        const void *p;
+        int64_t size;
+    } ins[] = {{scores, 4}, {finished, 1}},
+      outs[] = {{scores_out, 4}, {tokens_out, 4}, {parents_out, 4}, {finished_out, 1}};
+    for (const auto &i : ins)
+        for (const auto &o : outs) {
+            if (!i.p || !o.p || (i.p == o.p && k == nbeam && i.size == o.size)) continue;
+            if ((const char *)i.p < (const char *)o.p + nreq * k * o.size &&
+                (const char *)o.p < (const char *)i.p + nreq * nbeam * i.size)
+                return report(VS_ERR_INVALID, "an output overlaps scores or finished");
+        }
     vs::DeviceGuard g(bs->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;

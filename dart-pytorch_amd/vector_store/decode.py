@@ -401,7 +401,8 @@ class BeamSearch:
 
         logits [requests * beams, vocab] f32 or bf16; scores [requests, beams]
         f32; finished [requests, beams] u8.  Outputs [requests, k]: scores f32,
-        tokens and parents (rows of logits) i32, finished u8."""
+        tokens and parents (rows of logits) i32, finished u8; in place of scores
+        and finished only where k is beams."""
         dev = self.device
         try:  # (all in one: a step of one request takes as long as its Python calls)
             here = (logits.get_device() == scores.get_device() == scores_out.get_device() == tokens_out.get_device()

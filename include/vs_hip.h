@@ -365,7 +365,9 @@ VS_API void vs_beam_destroy(vs_beam *bs);
  * NaN or whose logits hold a NaN or +inf.  Outputs [nreq][k]: scores_out
  * (the 64-bit total rounded to fp32), tokens, parents (the row
  * r * nbeam + w) and, if finished_out is not null, whether the token is eos.
- * Missing candidates: -inf, -1, -1, 0.  k <= 64, nbeam <= 128. */
+ * Missing candidates: -inf, -1, -1, 0.  k <= 64, nbeam <= 128.  No output
+ * overlaps scores or finished, but with k == nbeam scores_out may be scores and
+ * finished_out finished. */
 VS_API int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_stride,
                           int64_t nreq, int64_t nbeam, int64_t vocab, const float *scores,
                           const uint8_t *finished, int64_t eos, int64_t k, float *scores_out,

@@ -39,3 +39,41 @@ def test_sequences_off_their_alignment(vs, which, by):
     assert parts["lens"].numpy().tolist() == [33, 5] and parts["refs"].numpy().tolist() == [1, 1, 1, 0]
     assert np.array_equal(parts["table"].numpy(), [[0, 1], [2, -1]])
     cache.close()
+
+
+def test_a_selection_over_its_own_inputs(vs):
+    """In place with as many candidates as beams; refused where one request's outputs would lie on another's scores."""
+    A, rng = vs.DeviceArray, np.random.default_rng(1)
+    R, W, V = 40, 4, 3001
+    x, sc = rng.standard_normal((R * W, V)), -5 * rng.random((R, W)).astype(np.float32)
+    fin = (rng.random((R, W)) < 0.2).astype(np.uint8)
+    lg, bs = A.of(x, "f32"), vs.BeamSearch()
+    so, fo, to, po = A((R, W), "f32"), A((R, W), "u8"), A((R, W), "i32"), A((R, W), "i32")
+    bs.select(lg, A.of(sc, "f32"), so, to, po, finished=A.of(fin, "u8"), finished_out=fo, eos=2)
+    s, f = A.of(sc, "f32"), A.of(fin, "u8")
+    t2, p2 = A((R, W), "i32"), A((R, W), "i32")
+    bs.select(lg, s, s, t2, p2, finished=f, finished_out=f, eos=2)
+    for a, b in ((s, so), (f, fo), (t2, to), (p2, po)):
+        assert np.array_equal(a.numpy(), b.numpy())
+
+    class Part(Shifted):
+        def __init__(self, base, shape, by=0):
+            super().__init__(base, by)
+            self.shape = shape
+
+        def stride(self):
+            return (self.shape[1], 1)
+
+    out = lambda k: (A((R, k), "f32"), A((R, k), "i32"), A((R, k), "i32"))  # noqa: E731
+    s, f = A.of(sc, "f32"), A.of(fin, "u8")
+    so, to, po = out(2)
+    for args, kw in (((s, Part(s, (R, 2)), to, po), {}), ((s, so, to, po), dict(finished=f, finished_out=Part(f, (R, 2)))),
+                     ((s, Part(s, (R, 2), 8), to, po), {})):
+        with pytest.raises(ValueError, match="overlaps"):
+            bs.select(lg, *args, **kw)
+    half = Part(s, (R // 2, W)), Part(s, (R // 2, W), R // 2 * W * 4)
+    one = A((R // 2, W), "i32"), A((R // 2, W), "i32")
+    bs.select(Part(lg, (R // 2 * W, V)), half[0], half[1], *one)  # (side by side in one buffer)
+    with pytest.raises(ValueError, match="overlaps"):
+        bs.select(Part(lg, (R // 2 * W, V)), half[0], Part(s, (R // 2, W), R // 2 * W * 4 - 4), *one)
+    bs.close()
