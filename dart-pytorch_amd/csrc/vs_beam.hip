@@ -725,9 +725,8 @@ int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_strid
       outs[] = {{scores_out, 4}, {tokens_out, 4}, {parents_out, 4}, {finished_out, 1}};
     for (const auto &i : ins)
         for (const auto &o : outs) {
-            if (!i.p || !o.p || (i.p == o.p && k == nbeam && i.size == o.size)) continue;
-            if ((const char *)i.p < (const char *)o.p + nreq * k * o.size &&
-                (const char *)o.p < (const char *)i.p + nreq * nbeam * i.size)
+            if (i.p == o.p && k == nbeam && i.size == o.size) continue;
+            if (vs::overlap(i.p, nreq * nbeam * i.size, o.p, nreq * k * o.size))
                 return report(VS_ERR_INVALID, "an output overlaps scores or finished");
         }
     vs::DeviceGuard g(bs->device);
@@ -800,12 +799,14 @@ int vs_beam_reorder(vs_beam *bs, const int32_t *parents, int64_t nrows, const vo
         return report(VS_ERR_UNSUPPORTED, "more than 2^31 rows");
     if (tail && (((uintptr_t)tail | (uintptr_t)out | (uintptr_t)out_stride | (uintptr_t)bytes) % 4))
         return report(VS_ERR_INVALID, "with tail, out, out_stride and bytes are multiples of 4");
-    const char *i0 = (const char *)in, *o0 = (const char *)out;
-    if (in && i0 < o0 + nrows * out_stride && o0 < i0 + nrows_in * in_stride)
+    const int64_t written = (nrows - 1) * out_stride + wide;
+    if (vs::overlap(in, nrows_in * in_stride, out, nrows * out_stride))
         return report(VS_ERR_INVALID, "in and out overlap");
+    if (vs::overlap(parents, nrows * 4, out, written) || vs::overlap(tail, nrows * 4, out, written))
+        return report(VS_ERR_INVALID, "out overlaps parents or tail");
     vs::DeviceGuard g(bs->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
-    vs::GatherArgs a = {parents,   tail,       i0, (char *)out, nrows, nrows_in,
+    vs::GatherArgs a = {parents,   tail,       (const char *)in, (char *)out, nrows, nrows_in,
                         in_stride, out_stride, bytes};
     hipStream_t st = (hipStream_t)stream;
     const uintptr_t al = (uintptr_t)in | (uintptr_t)out | (uintptr_t)in_stride |

@@ -88,6 +88,11 @@ struct StreamScratch {
     }
 };
 
+// Whether [a, a + na) and [b, b + nb) share a byte.
+inline bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+    return a && b && (const char *)a < (const char *)b + nb && (const char *)b < (const char *)a + na;
+}
+
 // The device exists; VS_OK or the error.
 inline int check_device(int device) {
     int count = 0;

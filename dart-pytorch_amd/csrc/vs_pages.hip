@@ -612,10 +612,19 @@ int vs_kv_fork(vs_kv *kv, const vs_kv_seqs *in, const int32_t *parents, const vs
     if (in->width != out->width)
         return report(VS_ERR_INVALID, "tables of %lld and %lld columns", (long long)in->width,
                       (long long)out->width);
-    if (in->lens == out->lens || (in->table == out->table && in->width))
+    const int64_t in_table = in->nseq * in->width * 4, out_table = out->nseq * out->width * 4;
+    if ((in->nseq && in->lens == out->lens) || (in->table == out->table && in->width) ||
+        vs::overlap(in->lens, in->nseq * 4, out->lens, out->nseq * 4) ||
+        vs::overlap(in->table, in_table, out->table, out_table))
         return report(VS_ERR_INVALID, "fork needs another table and other lens to write to");
     if ((out->nseq && !parents) || (uintptr_t)parents % 4)
         return report(VS_ERR_INVALID, "null or unaligned parents");
+    if (vs::overlap(parents, out->nseq * 4, out->table, out_table) ||
+        vs::overlap(parents, out->nseq * 4, out->lens, out->nseq * 4))
+        return report(VS_ERR_INVALID, "fork: parents lie in out");
+    if (in->refs != out->refs &&
+        vs::overlap(in->refs, kv->npages * 4, out->refs, kv->npages * 4))
+        return report(VS_ERR_INVALID, "fork: counts that overlap in part");
     vs::DeviceGuard g(kv->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
@@ -694,6 +703,11 @@ int vs_kv_compact_with(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out,
     if (rc) return rc;
     if (in->width != out->width || in->nseq != out->nseq)
         return report(VS_ERR_INVALID, "compact: in and out differ in shape");
+    const int64_t table_bytes = in->nseq * in->width * 4;
+    if ((in->table != out->table && vs::overlap(in->table, table_bytes, out->table, table_bytes)) ||
+        (in->lens != out->lens && vs::overlap(in->lens, in->nseq * 4, out->lens, in->nseq * 4)) ||
+        (in->refs != out->refs && vs::overlap(in->refs, kv->npages * 4, out->refs, kv->npages * 4)))
+        return report(VS_ERR_INVALID, "compact: in and out overlap in part");
     if (nothers < 0 || (nothers && !others) || (uintptr_t)map % 4)
         return report(VS_ERR_INVALID, "null others, or an unaligned map");
     if (nothers && in->refs != out->refs)
@@ -704,9 +718,12 @@ int vs_kv_compact_with(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs *out,
         if (others[i]->refs != in->refs)
             return report(VS_ERR_INVALID, "other %lld is on other counts", (long long)i);
         // (a table that is rewritten twice would follow its pages twice)
-        const int32_t *t = others[i]->table;
-        bool again = t && (t == in->table || t == out->table);
-        for (int64_t j = 0; j < i; ++j) again |= t && t == others[j]->table;
+        auto same = [&](const vs_kv_seqs *s) {
+            return vs::overlap(others[i]->table, others[i]->nseq * others[i]->width * 4, s->table,
+                               s->nseq * s->width * 4);
+        };
+        bool again = same(in) || same(out);
+        for (int64_t j = 0; j < i; ++j) again |= same(others[j]);
         if (again) return report(VS_ERR_INVALID, "other %lld is named twice", (long long)i);
     }
     vs::DeviceGuard g(kv->device);

@@ -77,3 +77,46 @@ def test_a_selection_over_its_own_inputs(vs):
     with pytest.raises(ValueError, match="overlaps"):
         bs.select(Part(lg, (R // 2 * W, V)), half[0], Part(s, (R // 2, W), R // 2 * W * 4 - 4), *one)
     bs.close()
+
+
+class Cut(Shifted):
+    """Some rows of a buffer, at an offset in bytes."""
+
+    def __init__(self, base, shape, by=0):
+        super().__init__(base, by)
+        self.shape = shape
+
+    def stride(self):
+        return (self.shape[1], 1) if len(self.shape) == 2 else (1,)
+
+
+def test_sequences_that_overlap_in_part(vs):
+    """Rows that one workgroup writes while another reads them."""
+    A = vs.DeviceArray
+    cache = vs.PagedKVCache(4, 32, 1, 16)
+    table, lens, refs = A.of(np.full((4, 2), -1), "i32"), A.of(np.zeros(4), "i32"), A.of(np.zeros(8), "i32")
+    seqs = lambda t=0, ln=0, r=0: vs.KVSequences(Cut(table, (2, 2), t), Cut(lens, (2,), ln), Cut(refs, (4,), r))  # noqa: E731
+    parents = A.of([0, 1], "i32")
+    for out in (seqs(8, 8), seqs(16, 4), seqs(16, 8, 4)):
+        with pytest.raises(ValueError, match="fork"):
+            cache.fork(seqs(), parents, out)
+    for bad in (Cut(table, (2,), 24), Cut(lens, (2,), 8)):
+        with pytest.raises(ValueError, match="parents lie"):
+            cache.fork(seqs(), bad, seqs(16, 8))
+    for out in (seqs(8), seqs(0, 4), seqs(0, 0, 8)):
+        with pytest.raises(ValueError, match="in part"):
+            cache.compact(seqs(), out)
+    with pytest.raises(ValueError, match="twice"):
+        cache.compact(seqs(), others=[seqs(8)])
+    cache.fork(seqs(), parents, seqs(16, 8))  # side by side
+    cache.compact(seqs(), seqs(16, 8))
+    cache.compact(seqs(), others=[seqs(16)])
+    cache.check()
+    bs, h, t = vs.BeamSearch(), A.of(np.arange(24).reshape(6, 4), "i32"), A.of([7, 8], "i32")
+    state, low = Cut(h, (2, 4)), Cut(h, (2, 4), 64)
+    for args, kw in (((Cut(h, (2,), 80), state, low), {}), ((parents, state, low), dict(tail=Cut(h, (2,), 64)))):
+        with pytest.raises(ValueError, match="parents or tail"):
+            bs.reorder(*args, **kw)
+    bs.reorder(Cut(h, (2,)), A((2, 4), "i32"), low, tail=t)
+    bs.close()
+    cache.close()
