@@ -1106,10 +1106,13 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
     const int64_t units = most * (e == 2 ? 1 : 2), wgs = s->nseq * per_item;
     const int waves = wgs >= 2 * kv->num_cu || kv->head_dim > vs::kWideDim ? vs::kWaves : 8;
     const int each = wgs < kv->num_cu / 2 ? 2 : wgs < 2 * kv->num_cu ? 4 : 8;
-    a.unsplit = most <= vs::kMinBlocks || units <= each * waves;
+    // (nor are so many sequences that a launch of their parts, or of the join, is none)
+    a.unsplit = most <= vs::kMinBlocks || units <= each * waves ||
+                !vs::grid_ok((a.most_items + s->nseq) * per_item, 64 * vs::kWaves) ||
+                !vs::grid_ok(s->nseq * heads, 64 * vs::kWaves);
     const bool join = !a.unsplit;
     const int64_t items = a.unsplit ? s->nseq : a.most_items + s->nseq;
-    if (items * per_item > INT32_MAX || s->nseq * heads > INT32_MAX)
+    if (!vs::grid_ok(items * per_item, 64 * (join ? vs::kWaves : waves)))
         return report(VS_ERR_UNSUPPORTED, "%lld sequences of %lld heads", (long long)s->nseq,
                       (long long)heads);
     if (join) {

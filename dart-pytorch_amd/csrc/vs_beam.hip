@@ -760,7 +760,8 @@ int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t row_strid
     a.parents_out = parents_out;
     a.finished_out = finished_out;
     const int64_t slots = nreq * nbeam * a.npieces;
-    if (slots > INT32_MAX) return report(VS_ERR_UNSUPPORTED, "too many logits");
+    if (!vs::grid_ok((slots + 3) / 4, 256) || !vs::grid_ok(nreq, vs::kMergeThreads))
+        return report(VS_ERR_UNSUPPORTED, "too many logits or requests");
     void *ws = nullptr;
     int rc = bs->scratch.get(st, (size_t)slots * (sizeof(float2) + (size_t)k * 8), &ws);
     if (rc) return rc;

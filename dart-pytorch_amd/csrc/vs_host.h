@@ -93,6 +93,9 @@ inline bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
     return a && b && (const char *)a < (const char *)b + nb && (const char *)b < (const char *)a + na;
 }
 
+// A launch of so many workgroups: the runtime counts a grid's threads in 32 bits.
+inline bool grid_ok(int64_t workgroups, int threads) { return workgroups <= UINT32_MAX / threads; }
+
 // The device exists; VS_OK or the error.
 inline int check_device(int device) {
     int count = 0;

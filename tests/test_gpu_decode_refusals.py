@@ -120,3 +120,51 @@ def test_sequences_that_overlap_in_part(vs):
     bs.reorder(Cut(h, (2,)), A((2, 4), "i32"), low, tail=t)
     bs.close()
     cache.close()
+
+
+def test_more_workgroups_than_a_launch_has(vs):
+    """Refused on the host, before the first of a call's kernels (buffers named larger than they are: nothing reads them)."""
+    A = vs.DeviceArray
+    bs, n = vs.BeamSearch(), 1 << 23
+    some = {t: A((16,), t) for t in ("f32", "i32", "bf16")}
+    with pytest.raises(NotImplementedError, match="requests"):
+        bs.select(Cut(some["f32"], (n, 5)), Cut(some["f32"], (n, 1)), Cut(A((16,), "f32"), (n, 1), 1 << 40),
+                  Cut(some["i32"], (n, 1), 1 << 41), Cut(some["i32"], (n, 1), 1 << 42))
+    bs.close()
+    cache, n = vs.PagedKVCache(2, 32, 64, 16), 1 << 20
+    seqs = vs.KVSequences(Cut(some["i32"], (n, 40)), Cut(some["i32"], (n,)), A.of([0, 0], "i32"))
+
+    class Rows(Cut):
+        def stride(self):
+            return (64 * 16, 16, 1)
+
+    q = Rows(some["bf16"], (n, 64, 16))
+    with pytest.raises(NotImplementedError, match="sequences"):
+        cache.attend(seqs, q, q)
+    cache.check()
+    cache.close()
+
+
+def test_sequences_whose_join_would_be_no_launch(vs):
+    """2^18 sequences of 64 heads in tables that would be split: answered by a workgroup each."""
+    A, n, heads, dim, width = vs.DeviceArray, 1 << 18, 64, 16, 40
+    cache = vs.PagedKVCache(2, 32, 1, dim)
+    one = vs.KVSequences(A.of([[0, 1]], "i32"), A.of([64], "i32"), A.of([1, 1], "i32"))
+    ones = A.of(np.full((64, 1, dim), 0x3F80), "bf16")
+    cache.append(one, ones, ones, starts=A.of([0, 64], "i32"))
+    lens = np.arange(n) % 65
+    table = np.full((n, width), -1, np.int32)
+    table[:, :2] = [1, 0]
+    seqs = vs.KVSequences(A.of(table, "i32"), A.of(lens, "i32"), A.of([1, 1], "i32"))
+    q, out = A.of(np.zeros((n, heads, dim), np.uint16), "bf16"), A((n, heads, dim), "bf16")
+    lse = A((n, heads), "f32")
+    cache.attend(seqs, q, out, lse=lse)
+    cache.check()
+    assert np.array_equal(out.numpy(), np.broadcast_to(np.where(lens, 0x3F80, 0)[:, None, None], (n, heads, dim)))
+    with np.errstate(divide="ignore"):
+        want = np.log(lens)[:, None]
+    got = lse.numpy()
+    assert (got[lens == 0] == -np.inf).all()
+    np.testing.assert_allclose(got[lens > 0], np.broadcast_to(want[lens > 0], (int((lens > 0).sum()), heads)), rtol=0,
+                               atol=68 * 2.0 ** -23 + 2.0 ** -21 * 25)
+    cache.close()
