@@ -8,7 +8,6 @@
 namespace vs {
 namespace {
 
-constexpr int kMostFresh = 1 << 20;  // pages that one extend gives a sequence
 constexpr int kSmallPages = 16384;    // of a cache whose compaction is planned in registers
 constexpr int kForkSeqs = 1024;      // sequences and words of a fork that one workgroup does
 constexpr int kForkWords = 1 << 12;
@@ -37,7 +36,7 @@ template <bool SMALL>
 __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
     constexpr int kHash = 2 * kPlan;
     __shared__ int lds[kPlan / 64];
-    __shared__ int bad, huge;
+    __shared__ int bad;
     __shared__ int h_page[SMALL ? kHash : 1], h_holders[SMALL ? kHash : 1], h_lowest[SMALL ? kHash : 1];
     __shared__ int fresh[4 * kPlan];  // the first free pages that are needed
     const int P = 1 << a.page_shift;
@@ -67,7 +66,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
     };
     const bool marked = a.status[2] != 0;  // some page may be closed
     if (threadIdx.x == 0) {
-        bad = huge = 0;
+        bad = 0;
         a.copies[0] = 0;
     }
     if constexpr (SMALL) {
@@ -128,11 +127,10 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
             }
             want = copy + (int)(((int64_t)s.n + s.count + P - 1) >> a.page_shift) -
                    (int)(((int64_t)s.n + P - 1) >> a.page_shift);
-            if (want > min(a.npages, kMostFresh)) huge = 1;  // refused: no sum below passes 32 bits
-            want = min(want, kMostFresh);
         }
-        int total;
-        const int at = (int)min(need + block_scan(want, &total, lds), (int64_t)INT32_MAX);
+        // (a total that 32 bits cannot hold is more than there are pages: refused)
+        uint32_t total;
+        const int at = (int)min(need + block_scan_sat((uint32_t)want, &total, lds), (int64_t)INT32_MAX);
         if (b0 == 0) {
             at0 = at;
             copy0 = copy;
@@ -179,7 +177,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
             }
         found += total;
     }
-    if (found < need || huge) {
+    if (found < need) {
         if (threadIdx.x == 0) {
             atomicOr(&a.status[0], kStatusPages);
             atomicMax(&a.status[1], (int)min(max(need - found, (int64_t)1), (int64_t)INT32_MAX));

@@ -43,6 +43,17 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_readlane(prefix_sum((int)x), 63);
 }
 
+// The same, where a sum may pass 32 bits: it stays at the largest number then.
+__device__ __forceinline__ uint32_t prefix_sum_sat(uint32_t x) {
+    x = __builtin_elementwise_add_sat(x, dpp<0x111>(0, x));
+    x = __builtin_elementwise_add_sat(x, dpp<0x112>(0, x));
+    x = __builtin_elementwise_add_sat(x, dpp<0x114>(0, x));
+    x = __builtin_elementwise_add_sat(x, dpp<0x118>(0, x));
+    x = __builtin_elementwise_add_sat(x, dpp<kBcast15, 0xa>(0, x));
+    x = __builtin_elementwise_add_sat(x, dpp<kBcast31, 0xc>(0, x));
+    return x;
+}
+
 constexpr int kPlan = 1024;  // threads of plans that are made by one workgroup
 
 // Exclusive prefix sum of x over the workgroup's kPlan threads; *total its sum.
@@ -56,6 +67,19 @@ __device__ __forceinline__ int block_scan(int x, int *total, int *lds) {
     const int w = prefix_sum(lane < kPlan / 64 ? lds[lane] : 0);
     *total = __builtin_amdgcn_readlane(w, 63);
     return incl - x + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
+}
+
+// The same with sums that stay at the largest number; the prefixes hold where
+// the total is below it.
+__device__ __forceinline__ uint32_t block_scan_sat(uint32_t x, uint32_t *total, int *lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t incl = prefix_sum_sat(x);
+    __syncthreads();
+    if (lane == 63) lds[wave] = (int)incl;
+    __syncthreads();
+    const uint32_t w = prefix_sum_sat(lane < kPlan / 64 ? (uint32_t)lds[lane] : 0);
+    *total = (uint32_t)__builtin_amdgcn_readlane((int)w, 63);
+    return incl - x + (wave ? (uint32_t)__builtin_amdgcn_readlane((int)w, wave - 1) : 0);
 }
 
 }  // namespace vs

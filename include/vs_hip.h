@@ -299,7 +299,8 @@ VS_API int vs_kv_read(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t 
  * lowest free ones in the order of the sequences.  A partly filled last page
  * that others hold too is copied to a page of the sequence's own first (all
  * layers); where everyone who holds it is being extended here, the lowest of
- * them keeps it.  If pages or table columns do not suffice nothing changes,
+ * them keeps it.  Table entries past a sequence's positions are written over
+ * as they are: who shortens a sequence gives their pages back.  If pages or table columns do not suffice nothing changes,
  * and vs_kv_check says so.  Until it has, or until an extend of theirs fits,
  * nothing is stored for the sequences that were to grow, nor for forks of
  * theirs: vs_kv_attend's new tokens and vs_kv_append's rows, which have no
