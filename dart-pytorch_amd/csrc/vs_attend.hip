@@ -1038,7 +1038,8 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
     if (heads > (1 << 16)) return report(VS_ERR_UNSUPPORTED, "more than 65,536 heads");
     if (!k != !v) return report(VS_ERR_INVALID, "k and v are given together or not at all");
     if (window < 0 || sinks < 0) return report(VS_ERR_INVALID, "negative window or sinks");
-    if (!std::isfinite(scale)) return report(VS_ERR_INVALID, "scale is not finite");
+    if (!std::isfinite(scale * vs::kLog2e))
+        return report(VS_ERR_INVALID, "scale is not finite, or too large for its exponentials' base");
     const int64_t e = vs::kv_elem(kv->dtype);
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % e || (uintptr_t)lse % 4)
         return report(VS_ERR_INVALID, "a buffer is not aligned to its elements");

@@ -168,3 +168,17 @@ def test_sequences_whose_join_would_be_no_launch(vs):
     np.testing.assert_allclose(got[lens > 0], np.broadcast_to(want[lens > 0], (int((lens > 0).sum()), heads)), rtol=0,
                                atol=68 * 2.0 ** -23 + 2.0 ** -21 * 25)
     cache.close()
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), 3e38, -2.5e38])
+def test_a_scale_that_is_infinite_in_base_two(vs, scale):
+    """Scores of 0 times it would be NaN."""
+    A, cache = vs.DeviceArray, vs.PagedKVCache(1, 32, 1, 16)
+    seqs, q = vs.KVSequences(A.of([[0]], "i32"), A.of([2], "i32"), A.of([1], "i32")), A.of(np.zeros((1, 1, 16)), "bf16")
+    out, ones = A((1, 1, 16), "bf16"), A.of(np.full((2, 1, 16), 0x3F80), "bf16")
+    cache.append(seqs, ones, ones, starts=A.of([0, 2], "i32"))
+    with pytest.raises(ValueError, match="scale"):
+        cache.attend(seqs, q, out, scale=scale)
+    cache.attend(seqs, q, out, scale=2.3e38)
+    assert (out.numpy() == 0x3F80).all()
+    cache.close()
