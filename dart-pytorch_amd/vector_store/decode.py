@@ -314,8 +314,8 @@ class PagedKVCache:
         [n]), with copies of shared, partly filled last pages (vs_kv_extend).
         Where it does not fit nothing changes, check() raises, and attend() and
         append() store nothing for these sequences until then."""
-        if isinstance(count, int):
-            rc = self._lib.vs_kv_extend(self._h, self._seqs(seqs), count, None, stream)
+        if isinstance(count, (int, np.integer)):
+            rc = self._lib.vs_kv_extend(self._h, self._seqs(seqs), int(count), None, stream)
         else:
             rc = self._lib.vs_kv_extend(self._h, self._seqs(seqs), 0,
                                         _flat(count, "count", (seqs.n,), _I32, self.device), stream)

@@ -115,3 +115,12 @@ def test_buffers_that_do_not_say_are_trusted(there):
     s = there.seqs(1)
     there.cache.attend(s, Fake((3, 4, 16), "bf16"), Fake((3, 4, 16), "bf16"))
     assert there.lib.calls == 1
+
+
+@pytest.mark.parametrize("count", [3, "int32", "int64", "uint8"])
+def test_counts_of_any_whole_type(there, count):
+    """numpy's whole numbers are numbers, not buffers."""
+    import numpy as np
+
+    there.cache.extend(there.seqs(1), count if isinstance(count, int) else getattr(np, count)(3))
+    assert there.lib.calls == 1
