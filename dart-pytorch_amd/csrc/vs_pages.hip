@@ -10,7 +10,7 @@ namespace {
 
 constexpr int kSmallPages = 16384;    // of a cache whose compaction is planned in registers
 constexpr int kForkSeqs = 1024;      // sequences and words of a fork that one workgroup does
-constexpr int kForkWords = 1 << 12;
+constexpr int kForkWords = 6 << 10;
 constexpr int kPieceBytes = 8192;   // of a page, per workgroup pass of the copy
 
 struct ExtendArgs {
@@ -323,8 +323,13 @@ __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a) {
 }
 
 // The same as one workgroup, where that takes less than a second launch: the
-// counts are copied, then changed.  (4 sequences of 14 entries, 96 pages: 2.2
-// against 4.0 us; 256 of 36, 3,500 pages: 13.7 against 8.8, hence kForkWords.)
+// counts are copied, then changed.  By the words that it goes through (pages,
+// and table entries and lengths of both sides), one workgroup against two launches:
+// 216 (96 pages, 4 sequences of 14 entries) 2.4 and 3.5 us, 1,672 (1,000, 16 of
+// 20) 2.4 and 3.8, 2,920 (1,000, 64 of 14) 2.8 and 3.9, 4,968 (1,000, 64 of 30) 3.6
+// and 3.8, 5,840 (2,000, 128 of 14) 3.5 and 3.9, 6,248 (6,000, 4 of 30) 3.1 and 3.6;
+// 8,936 (1,000, 128 of 30) 4.7 and 3.8, 10,624 (8,000, 32 of 40) 4.1 and 3.9, 22,444
+// (3,500, 256 of 36) 8.8 and 4.0.  Hence kForkWords.
 __global__ __launch_bounds__(kPlan) void fork_small_kernel(ForkArgs a, const int32_t *refs_in) {
     __shared__ int children[kForkSeqs], parent_of[kForkSeqs];
     for (int i = threadIdx.x; i < a.nin; i += kPlan) children[i] = 0;
@@ -468,7 +473,7 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(CompactArgs a) {
 }
 
 // The same for up to kSmallPages pages: the counts are read once, into
-// registers, and the pairs meet in LDS (150 pages 2.9 us, 4,100 pages 6.6).
+// registers, and the pairs meet in LDS (150 pages 3.2 us, 4,100 pages 7.0).
 __global__ __launch_bounds__(kPlan) void compact_plan_small_kernel(CompactArgs a) {
     constexpr int N = kSmallPages / (4 * kPlan);  // rounds of four consecutive pages per thread
     __shared__ int lds[kPlan / 64];
