@@ -158,6 +158,9 @@ __device__ __forceinline__ void cut_list(uint64_t *cand, int n, int k, int lane)
 // Large batches in fp32 are bound by HBM: 64 x 8 x 128,000, k = 8, some beams
 // ended, 46 us (232 MB read: 5.0 TB/s).  bf16 has half the bytes for the same
 // work and is bound by that, 32 us.  1 x 4 x 50,001 takes 4.9 us, latency.
+// Long steps are held to six waves a SIMD, for which bf16 spills two
+// registers; with five and none spilled 38.2 against 37.4 us with the merge at 64 x
+// 8 x 128,000, k = 8, 56.8 against 55.8 at 128 x 16 x 30,000, k = 32.
 template <int ST, int PER>
 __global__ __launch_bounds__(256, PER == kLongStep ? 6 : 1) void beam_piece_kernel(BeamArgs a) {
     using S = Step<ST, PER>;

@@ -343,7 +343,7 @@ VS_API int vs_kv_compact_with(vs_kv *kv, const vs_kv_seqs *in, const vs_kv_seqs 
  * [0, npages) are skipped; no page may be both read and written, or written
  * twice. */
 VS_API int vs_kv_copy(vs_kv *kv, const int32_t *from, const int32_t *to, int64_t n, void *stream);
-/* Waits for the stream and tells what earlier calls met on the device since
+/* Waits for the stream (for the device, where an extend was refused) and tells what earlier calls met on the device since
  * the last check: VS_ERR_OOM (an extend found too few free pages),
  * VS_ERR_INVALID (too few table columns for an extend, an attend's new token or
  * an append's rows; a new token without a page; a parent out of range). */
