@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(ExtendArgs a) {
             a.refs[to] = 1;
             *entry = to;
         }
-        if (marked && n > 0) {
+        if (marked && (n & (P - 1))) {  // (a full one may be others' last page too)
             const int p = row[(n - 1) >> a.page_shift];
             if ((unsigned)p < (unsigned)a.npages) a.closed[p] = 0;
         }

@@ -175,3 +175,21 @@ def test_more_sequences_than_one_plan_keeps_in_registers(vs):
     for b in (0, 1023, 1024, n - 1):
         k, v = held(c, c.seqs, 1, b, 31)
         assert np.array_equal(k, kb[2 * b + 1]) and np.array_equal(v, vb[2 * b + 1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_full_page_that_others_end_in_too(vs, dtype):
+    """Two sets go on from one full page of a prompt; one is refused, the other's extend does not open that page."""
+    c = Cache(vs, 4, [[0, -1]], [32], dtype)
+    narrow = c.on(np.array([[0]]), [32])
+    c.cache.extend(narrow, 1)  # no column for it
+    c.cache.extend(c.seqs, 1)
+    before = c.mem.numpy()[0].copy()
+    c.step(narrow)
+    c.append(narrow, 1)
+    for layer, (_, _, kb, vb) in enumerate(c.step(c.seqs)):
+        k, v = held(c, c.seqs, layer, 0, 32)
+        assert np.array_equal(k, kb[0]) and np.array_equal(v, vb[0])
+    assert np.array_equal(c.mem.numpy()[0].view(np.uint16), before.view(np.uint16))
+    with pytest.raises(ValueError, match="table row"):
+        c.cache.check()
