@@ -774,9 +774,9 @@ __device__ __forceinline__ char *block_of(const RowsArgs &a, int b, int64_t pos,
 // their places, lanes in the order of those; values are turned in LDS.
 // Sequence b's rows touch at most rows / 32 + 2 blocks, so its items start at
 // starts[b] / 32 + 2 b, which needs no sum over the sequences before it.
-// 8 heads of 128 in bf16: 4,096 rows 7.8 us (33.6 MB read and written, 4.3
-// TB/s; a row at a time, with scattered stores, 27.8), 16 x 1,000 rows 23.7 (131
-// MB, 5.5 TB/s; 91).
+// 8 heads of 128 in bf16: 4,096 rows 8.1 us (33.6 MB read and written, 4.1
+// TB/s; a row at a time, with scattered stores, 27.8), 16 x 1,000 rows 24.4 (131
+// MB, 5.4 TB/s; 91).
 template <int ST>
 __global__ __launch_bounds__(256) void append_kernel(RowsArgs a, int64_t items) {
     using T = typename std::conditional<ST, uint16_t, uint32_t>::type;
@@ -813,9 +813,9 @@ __global__ __launch_bounds__(256) void append_kernel(RowsArgs a, int64_t items) 
                 atomicOr(&a.status[0], kStatusWidth);
             continue;
         }
-        if (end <= a.width << a.page_shift) {
+        if (marked && end <= a.width << a.page_shift) {
             const int last = a.table[b * a.width + ((end - 1) >> a.page_shift)];
-            if ((unsigned)last < (unsigned)a.npages && marked && a.closed[last]) continue;
+            if ((unsigned)last < (unsigned)a.npages && a.closed[last]) continue;
         }
         // positions t of the block that have a row
         const int64_t from = max(row0 < 0 ? first - row0 : first, p0);
