@@ -15,6 +15,8 @@ values, and the choice of the next tokens.
     beams.select(logits, scores, next_scores, tokens, parents)
     beams.reorder(parents, history, next_history, tail=tokens)
     cache.fork(seqs, parents, spare); seqs, spare = spare, seqs
+  now and then, and before the tokens are used:
+    cache.check()                                # raises what did not fit; the cache is whole then
 
 Buffers are anything in device memory with data_ptr(), shape, stride() and
 dtype: DeviceArray of this module or a tensor of a framework that works on the
