@@ -22,8 +22,9 @@ Buffers are anything in device memory with data_ptr(), shape, stride() and
 dtype: DeviceArray of this module or a tensor of a framework that works on the
 same GPU (imported before this package loads its library, so that both use the
 HIP runtime that the framework brings).  Where a buffer says where it lies
-(get_device(), -1 for host memory) it has to be the handle's device.  Calls run on `stream` (an integer hipStream_t, 0 the default
-stream) and return without waiting for it.
+(get_device(), -1 for host memory) it has to be the handle's device.  Calls run
+on `stream` (an integer hipStream_t, 0 the default stream) and return without
+waiting for it.
 """
 from __future__ import annotations
 
