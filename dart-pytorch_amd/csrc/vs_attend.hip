@@ -3,7 +3,7 @@
 #include <cmath>
 
 #include "vs_device.h"
-#include "vs_kv.h"
+#include "vs_rows.h"
 #include "vs_wave.h"
 
 namespace vs {
@@ -210,24 +210,6 @@ __device__ __forceinline__ float column_max(float x) {
     x = fmaxf(float_of(p.x), float_of(p.y));
     p = __builtin_amdgcn_permlane32_swap(bits_of(x), bits_of(x), false, false);
     return fmaxf(float_of(p.x), float_of(p.y));
-}
-
-// 16 bytes of a row from element x on, whatever the row's alignment.
-template <int ST>
-__device__ __forceinline__ u32x4_t load_piece(const char *row, int x, bool vec) {
-    constexpr int E = ST ? 8 : 4;
-    if (vec) return *(const u32x4_t *)(row + (int64_t)x * (16 / E));
-    u32x4_t w;
-    if constexpr (ST) {
-        const uint16_t *p = (const uint16_t *)row + x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-    } else {
-        const uint32_t *p = (const uint32_t *)row + x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = p[i];
-    }
-    return w;
 }
 
 // One pass over a work item's keys and values with the running maximum and
@@ -733,42 +715,6 @@ __global__ __launch_bounds__(64 * kWaves) void attend_join_kernel(AttendArgs a) 
         a.lse[blockIdx.x] = sum == 0.f ? kNone : (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// The place of position t of a block, dimension x, in elements.
-template <int ST>
-__host__ __device__ inline int key_place(int t, int x, int dim) {
-    constexpr int E = ST ? 8 : 4;
-    return ((t / 16 * (dim / E) + x / E) * 16 + t % 16) * E + x % E;
-}
-template <int ST>
-__host__ __device__ inline int value_place(int t, int x, int dim) {
-    const int h = t / 16, g = t % 16 / 4, i = t % 4;
-    return ST ? ((x * 4 + g) * 2 + h) * 4 + i : ((h * dim + x) * 4 + g) * 4 + i;
-}
-
-struct RowsArgs {
-    char *pool;
-    int64_t page_bytes, layer_off, kv_off, head_off;
-    const int32_t *table, *lens, *starts;
-    int64_t width, nrows;
-    int nseq, npages, page_shift, heads, dim;
-    int32_t *status;
-    const uint8_t *closed;
-    const char *k, *v;
-    int64_t k_row, k_head, v_row, v_head;
-    int k_vec, v_vec;  // rows readable in 16-byte pieces
-    char *k_out, *v_out;
-    int b, first;
-};
-
-// Where position pos of sequence b lies; null if nowhere.
-__device__ __forceinline__ char *block_of(const RowsArgs &a, int b, int64_t pos, int es) {
-    if (pos < 0 || pos >> a.page_shift >= a.width) return nullptr;
-    const int page = a.table[(int64_t)b * a.width + (pos >> a.page_shift)];
-    if ((unsigned)page >= (unsigned)a.npages) return nullptr;
-    const int64_t blk = (pos & ((1 << a.page_shift) - 1)) / kKvBlock;
-    return a.pool + (int64_t)page * a.page_bytes + a.layer_off + blk * kKvBlock * a.dim * es;
-}
-
 // Rows into the cache: a copy, bound by HBM.  One workgroup per block of 32
 // positions and head, so that both sides move whole lines: keys go straight to
 // their places, lanes in the order of those; values are turned in LDS.
@@ -839,31 +785,7 @@ __global__ __launch_bounds__(256) void append_kernel(RowsArgs a, int64_t items) 
                     load_piece<ST>((const char *)(ks + row_of(t) * a.k_row), c * E, a.k_vec);
         }
         __syncthreads();
-        for (int x = threadIdx.x; x < kKvBlock * pieces; x += 256) {
-            // bf16: [dimension][g][half][i], fp32: [half][dimension][g][i]
-            const int g = x % 4, d = ST ? x / 4 : x / 4 % dim, half = ST ? 0 : x / 4 / dim;
-            T out[E];
-            int have = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int t = 16 * (ST ? e / 4 : half) + 4 * g + e % 4;
-                const bool in = t >= t0 && t < t1;
-                out[e] = in ? rows[t * ld + d] : (T)0;
-                have += in;
-            }
-            T *dst = (T *)(vd + x * 16);
-            if (have == E) {
-                u32x4_t v;
-                __builtin_memcpy(&v, out, 16);
-                *(u32x4_t *)dst = v;
-            } else if (have) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int t = 16 * (ST ? e / 4 : half) + 4 * g + e % 4;
-                    if (t >= t0 && t < t1) dst[e] = out[e];
-                }
-            }
-        }
+        store_values<ST>(rows, ld, (T *)vd, dim, t0, t1);
     }
 }
 
@@ -923,22 +845,6 @@ hipError_t launch_attend_dim(const AttendArgs &a, int64_t items, int waves, bool
 #undef VS_DIM
     }
     return hipErrorInvalidValue;
-}
-
-void fill_geometry(const vs_kv *kv, int64_t layer, AttendArgs &a) {
-    const int64_t e = kv_elem(kv->dtype);
-    a.pool = kv->mem;
-    a.page_bytes = kv->page_bytes;
-    a.head_off = kv->page_size * kv->head_dim * e;
-    a.kv_off = kv->kv_heads * a.head_off;
-    a.layer_off = layer * 2 * a.kv_off;
-}
-
-// |stride| elements of rows and heads stay inside 2^62 bytes
-bool stride_ok(int64_t s) { return s >= -((int64_t)1 << 40) && s <= ((int64_t)1 << 40); }
-
-bool pieces_ok(const void *p, int64_t s0, int64_t s1, int64_t e) {
-    return (((uintptr_t)p | (uintptr_t)(s0 * e) | (uintptr_t)(s1 * e)) & 15) == 0;
 }
 
 }  // namespace
@@ -1147,30 +1053,6 @@ int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, c
     return VS_OK;
 }
 
-static int fill_rows(const vs_kv *kv, const vs_kv_seqs *s, int64_t layer, vs::RowsArgs &a) {
-    if (layer < 0 || layer >= kv->layers)
-        return report(VS_ERR_INVALID, "layer %lld out of range [0, %lld)", (long long)layer,
-                      (long long)kv->layers);
-    vs::AttendArgs geo = {};
-    vs::fill_geometry(kv, layer, geo);
-    a.pool = geo.pool;
-    a.page_bytes = geo.page_bytes;
-    a.layer_off = geo.layer_off;
-    a.kv_off = geo.kv_off;
-    a.head_off = geo.head_off;
-    a.table = s->table;
-    a.lens = s->lens;
-    a.width = s->width;
-    a.nseq = (int)s->nseq;
-    a.npages = (int)kv->npages;
-    a.status = kv->status;
-    a.closed = kv->closed;
-    a.page_shift = __builtin_ctzll((uint64_t)kv->page_size);
-    a.heads = (int)kv->kv_heads;
-    a.dim = (int)kv->head_dim;
-    return VS_OK;
-}
-
 int vs_kv_append(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, const void *k, int64_t k_row,
                  int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
                  const int32_t *starts, int64_t nrows, void *stream) {
@@ -1178,7 +1060,7 @@ int vs_kv_append(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, const void *k, i
     int rc = vs::check_seqs(kv, s);
     if (rc) return rc;
     vs::RowsArgs a = {};
-    rc = fill_rows(kv, s, layer, a);
+    rc = vs::fill_rows(kv, s, layer, a);
     if (rc) return rc;
     if (nrows < 0 || (!starts && nrows != s->nseq))
         return report(VS_ERR_INVALID, "nrows %lld: without starts, one row per sequence",
@@ -1219,7 +1101,7 @@ int vs_kv_read(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t b, int64_t
     int rc = vs::check_seqs(kv, s);
     if (rc) return rc;
     vs::RowsArgs a = {};
-    rc = fill_rows(kv, s, layer, a);
+    rc = vs::fill_rows(kv, s, layer, a);
     if (rc) return rc;
     if (b < 0 || b >= s->nseq)
         return report(VS_ERR_INVALID, "sequence %lld out of range [0, %lld)", (long long)b,

@@ -1,0 +1,760 @@
+// vs_chunk.hip -- attention of many new tokens over the paged key-value cache:
+// prompts in chunks, drafted tokens, rows that attend to other sequences' states:
+// kernels and entry point.
+#include <cmath>
+
+#include "vs_device.h"
+#include "vs_rows.h"
+#include "vs_wave.h"
+
+namespace vs {
+namespace {
+
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kWaves = 4;
+constexpr int kCols = 2;                      // columns of 16 rows per wave
+constexpr int kTile = kWaves * kCols * 16;    // rows of queries per workgroup
+constexpr int kMinBlocks = 4;                 // per piece of a tile's blocks, at least
+constexpr int kSplitSeqs = 384;               // sequences whose pieces each workgroup finds for itself
+constexpr int kJoinRows = 8;                  // rows per workgroup of the join
+
+struct ChunkArgs {
+    char *pool;
+    int64_t page_bytes, layer_off, kv_off, head_off;  // bytes; kv_off from keys to values
+    const int32_t *table, *lens, *starts;
+    int64_t width;
+    int nseq, npages, page_shift;
+    int64_t nrows;
+    const char *q;
+    char *out;
+    int64_t q_row, q_head, o_row, o_head;  // elements
+    float *lse;
+    int heads, kv_heads, group;  // group: query heads per key-value head
+    float scale2;                // |scale| * log2(e)
+    uint32_t flip;               // sign bits of an element's word, where scale is below 0
+    int causal, window, sinks;
+    int q_vec;                   // rows readable in 16-byte pieces
+    int64_t tiles;               // numbers of tiles, with gaps
+    int split;                   // tiles are divided along the length
+    int target;                  // pieces of all tiles, about
+    int2 *info;                  // [tile] its first piece, how many
+    float *part_o;               // [piece][kv head][row of the tile][dim]
+    float2 *part_ml;             // [piece][kv head][row of the tile] running maximum and sum
+};
+
+// The rows of a sequence: [row0, row0 + count) of the batch's, row i at position
+// i + shift; `cap` the last position that there is, at most.
+struct Seq {
+    int64_t row0, shift;
+    int count, cap;
+};
+
+__device__ __forceinline__ Seq seq_of(const ChunkArgs &a, int b) {
+    Seq s;
+    const int64_t n = max(a.lens[b], 0), most = a.width << a.page_shift;
+    int64_t from = b, to = (int64_t)b + 1;
+    if (a.starts) {
+        from = a.starts[b];
+        to = a.starts[b + 1];
+    }
+    s.shift = n - to;
+    s.cap = (int)min(n, most) - 1;
+    s.row0 = min(max(from, (int64_t)0), a.nrows);
+    s.count = (int)max(min(to, a.nrows) - s.row0, (int64_t)0);
+    return s;
+}
+
+// Query rows are (row, query head of the group) pairs, the head counting faster, so
+// that a tile's rows share their keys and values whatever the group.
+__device__ __forceinline__ int tiles_of(const ChunkArgs &a, const Seq &s) {
+    return (int)(((int64_t)s.count * a.group + kTile - 1) / kTile);
+}
+
+// The last position that row x of sequence s sees.
+__device__ __forceinline__ int last_of(const ChunkArgs &a, const Seq &s, int64_t x) {
+    return a.causal ? (int)min(s.row0 + x + s.shift, (int64_t)s.cap) : s.cap;
+}
+
+// A tile's number: those of sequence b start at base(b), which needs no sum over
+// the sequences before it and leaves a gap of one at most.
+__device__ __forceinline__ int64_t tile_base(const ChunkArgs &a, int64_t b) {
+    const int64_t from = a.starts ? min(max((int64_t)a.starts[b], (int64_t)0), a.nrows) : b;
+    return from * a.group / kTile + b;
+}
+
+// The sequence whose tiles the number falls among: 64 of them are looked at at once.
+__device__ __forceinline__ int find_tile(const ChunkArgs &a, int64_t tile, int lane) {
+    int64_t lo = 0, n = a.nseq;  // it is one of lo .. lo + n - 1
+    while (n > 1) {
+        const int64_t step = (n + 63) / 64, b = lo + lane * step;
+        const uint64_t in = __ballot(lane * step < n && tile_base(a, b) <= tile);
+        const int l = in ? 63 - __builtin_clzll(in) : 0;
+        lo += l * step;
+        n = min(step, n - l * step);
+    }
+    return (int)lo;
+}
+
+// The blocks that a tile attends to: nsb from the start, then from wb0 on.
+struct Span {
+    int nsb, wb0, total;
+};
+
+__device__ __forceinline__ Span span_of(const ChunkArgs &a, int low, int high) {
+    Span s = {0, 0, 0};
+    if (high < 0) return s;
+    const int nb = high / kKvBlock + 1;
+    if (a.window > 0 && low >= a.window) {
+        s.wb0 = (low - a.window + 1) / kKvBlock;
+        s.nsb = min(a.sinks / kKvBlock + (a.sinks % kKvBlock != 0), s.wb0);
+    }
+    s.total = s.nsb + nb - s.wb0;
+    return s;
+}
+
+// How many blocks any tile of a sequence has, at most.
+__device__ __forceinline__ int most_blocks(const ChunkArgs &a, const Seq &s) {
+    const int high = s.count ? last_of(a, s, s.count - 1) : -1;
+    if (high < 0) return 0;
+    const int nb = high / kKvBlock + 1;
+    if (a.window <= 0) return nb;
+    const int64_t w = ((int64_t)a.window + kTile / a.group) / kKvBlock + 3 + a.sinks / kKvBlock;
+    return (int)min((int64_t)nb, w);
+}
+
+__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// Piece `piece` of a divided call: piece split of tile `tile` (within its sequence).
+struct Piece {
+    int b, tile, split, per, first;  // first: the tile's first piece
+};
+
+__device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int lane, Piece &p) {
+    int64_t all = 0;
+    for (int b0 = 0; b0 < a.nseq; b0 += 64)
+        if (b0 + lane < a.nseq) {
+            const Seq s = seq_of(a, b0 + lane);
+            all += (int64_t)tiles_of(a, s) * most_blocks(a, s);
+        }
+    all = wave_sum64(all);
+    p.per = (int)max((all + a.target - 1) / a.target, (int64_t)kMinBlocks);
+    int base = 0;
+    for (int b0 = 0; b0 < a.nseq; b0 += 64) {
+        int tiles = 0, splits = 1;
+        if (b0 + lane < a.nseq) {
+            const Seq s = seq_of(a, b0 + lane);
+            tiles = tiles_of(a, s);
+            splits = max((most_blocks(a, s) + p.per - 1) / p.per, 1);
+        }
+        const int sum = base + prefix_sum(tiles * splits);
+        const uint64_t past = __ballot(sum > piece);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            tiles = __builtin_amdgcn_readlane(tiles, l);
+            splits = __builtin_amdgcn_readlane(splits, l);
+            const int local = piece - (__builtin_amdgcn_readlane(sum, l) - tiles * splits);
+            p.b = b0 + l;
+            p.tile = local / splits;
+            p.split = local % splits;
+            p.first = piece - p.split;
+            return true;
+        }
+        base = __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+// The larger of the four lanes that share a column (lanes apart by 16).
+__device__ __forceinline__ float column_max(float x) {
+    typedef unsigned u32pair __attribute__((ext_vector_type(2)));
+    u32pair p = __builtin_amdgcn_permlane16_swap(bits_of(x), bits_of(x), false, false);
+    x = fmaxf(float_of(p.x), float_of(p.y));
+    p = __builtin_amdgcn_permlane32_swap(bits_of(x), bits_of(x), false, false);
+    return fmaxf(float_of(p.x), float_of(p.y));
+}
+
+// blocks of 32 positions that are staged together
+constexpr int blocks_at_once(int st, int dim) { return st && dim <= 128 ? 2 : 1; }
+constexpr int buffer_bytes(int st, int dim) {
+    return blocks_at_once(st, dim) * 2 * kKvBlock * dim * (st ? 2 : 4);
+}
+
+template <int ST, int D>
+__global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_kernel(ChunkArgs a) {
+    constexpr int E = ST ? 8 : 4;
+    constexpr int ES = 16 / E;           // element size
+    constexpr int NC = (D / E + 3) / 4;  // 16-byte pieces per lane of a key row
+    constexpr int ND = D / 16;
+    constexpr int SB = blocks_at_once(ST, D);
+    constexpr int BLOCK = kKvBlock * D * ES;         // bytes of a block's keys
+    constexpr int LOADS = SB * 2 * BLOCK / 1024;     // of 16 bytes per lane, all waves
+    constexpr int MINE = (LOADS + kWaves - 1) / kWaves;
+    constexpr float kNone = -__builtin_huge_valf();
+    extern __shared__ __align__(16) char lds[];  // two buffers: [block][keys, values]
+    __shared__ int flagged[2];                   // the step whose values hold NaNs or infinities
+    __shared__ float lds_p[kWaves][kKvBlock][16];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % a.kv_heads;
+    const int64_t at = blockIdx.x / a.kv_heads;
+
+    // which rows, which blocks
+    Piece pc = {};
+    int64_t number;  // of the tile
+    if (a.split) {
+        if (!find_piece(a, (int)at, lane, pc)) return;
+        number = tile_base(a, pc.b) + pc.tile;
+    } else {
+        number = a.tiles - 1 - at;
+        pc.b = find_tile(a, number, lane);
+        pc.tile = (int)(number - tile_base(a, pc.b));
+        pc.per = INT32_MAX;
+    }
+    const Seq sq = seq_of(a, pc.b);
+    if (pc.tile < 0 || pc.tile >= tiles_of(a, sq)) return;
+    const int64_t x0 = (int64_t)pc.tile * kTile, rows = (int64_t)sq.count * a.group;
+    const int64_t x1 = min(x0 + kTile, rows);
+    const int high = __builtin_amdgcn_readfirstlane(last_of(a, sq, (x1 - 1) / a.group));
+    const int low = __builtin_amdgcn_readfirstlane(last_of(a, sq, x0 / a.group));
+    const Span sp = span_of(a, low, high);
+    int pieces = 1, j0 = 0, j1 = sp.total;
+    if (a.split) {
+        pieces = max((sp.total + pc.per - 1) / pc.per, 1);
+        if (pc.split >= pieces) return;
+        j0 = pc.split * pc.per;
+        j1 = min(j0 + pc.per, sp.total);
+        if (pc.split == 0 && kvh == 0 && threadIdx.x == 0) a.info[number] = make_int2(pc.first, pieces);
+    }
+
+    // the wave's rows: column c * 16 + r is query row `row[c]` of the sequence
+    const int64_t w0 = x0 + wave * (16 * kCols), w1 = min(w0 + 16 * kCols, x1);
+    const bool busy = w0 < w1;
+    const int wave_high = busy ? __builtin_amdgcn_readfirstlane(last_of(a, sq, (w1 - 1) / a.group)) : -1;
+    const int wave_low = busy ? __builtin_amdgcn_readfirstlane(last_of(a, sq, w0 / a.group)) : -1;
+    int last[kCols];
+    u32x4_t qf[kCols][NC];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+        const int64_t x = w0 + c * 16 + r;
+        const bool in = x < w1;
+        last[c] = in ? last_of(a, sq, x / a.group) : -1;
+        const char *row = a.q + ((sq.row0 + x / a.group) * a.q_row +
+                                 (kvh * a.group + x % a.group) * a.q_head) * ES;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            qf[c][i] = u32x4_t{0, 0, 0, 0};
+            if (in && i * 4 + g < D / E) {
+                qf[c][i] = load_piece<ST>(row, (i * 4 + g) * E, a.q_vec);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) qf[c][i][w] ^= a.flip;
+            }
+        }
+    }
+
+    float m[kCols], ms[kCols], l[kCols];  // running maximum, times scale2, and the lane's sum
+    f32x4_t o[kCols][ND];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+        m[c] = kNone;
+        ms[c] = l[c] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[c][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // The blocks in order: 64 at a time, lane i looks the page of the i-th up, and
+    // those that have one are a bit mask.
+    const int32_t *trow = a.table + (int64_t)pc.b * a.width;
+    char *const head_base = a.pool + a.layer_off + (int64_t)kvh * a.head_off;
+    const int bpp1 = (1 << (a.page_shift - 5)) - 1;
+    auto block_pos = [&](int j) { return (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock; };
+    int chunk = j0 - 64, pages = -1;
+    uint64_t ready = 0;
+    auto next_block = [&](const char *&kb, int &pos) {
+        while (!ready) {
+            chunk += 64;
+            if (chunk >= j1) return false;
+            pages = -1;
+            if (chunk + lane < j1) pages = trow[block_pos(chunk + lane) >> a.page_shift];
+            ready = __ballot((unsigned)pages < (unsigned)a.npages);
+        }
+        const int i = __builtin_ctzll(ready);
+        ready &= ready - 1;
+        pos = block_pos(chunk + i);
+        kb = head_base + (int64_t)__builtin_amdgcn_readlane(pages, i) * a.page_bytes +
+             ((pos >> 5) & bpp1) * BLOCK;
+        return true;
+    };
+    struct Step {
+        const char *kb[SB];
+        int pos[SB];  // first positions; past all rows' where there is no block
+    };
+    auto next_step = [&](Step &s) {
+        if (!next_block(s.kb[0], s.pos[0])) return false;
+#pragma unroll
+        for (int b = 1; b < SB; ++b)
+            if (!next_block(s.kb[b], s.pos[b])) {
+                s.kb[b] = s.kb[0];
+                s.pos[b] = INT32_MAX - kKvBlock;
+            }
+        return true;
+    };
+    // whether rows with last positions from lo to hi see all of a block
+    auto whole = [&](int pos, int lo, int hi) {
+        return pos + kKvBlock - 1 <= lo &&
+               (a.window == 0 || pos > hi - a.window || pos + kKvBlock <= a.sinks);
+    };
+    u32x4_t stage[MINE];
+    auto load_step = [&](const Step &s) {
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int x = wave + i * kWaves;
+            if (LOADS % kWaves == 0 || x < LOADS) {
+                const int b = x / (2 * BLOCK / 1024), y = x % (2 * BLOCK / 1024);
+                const int kv = y / (BLOCK / 1024), z = y % (BLOCK / 1024);
+                const char *p = s.kb[0];
+#pragma unroll
+                for (int k = 1; k < SB; ++k) p = b == k ? s.kb[k] : p;
+                stage[i] = *(const u32x4_t *)(p + (kv ? a.kv_off : 0) + z * 1024 + lane * 16);
+            }
+        }
+    };
+    // Positions that no row of the tile sees may hold anything, and 0 times a NaN
+    // is one: their values become 0.  Those that some rows see and others do not
+    // are looked through for what is not finite.
+    auto store_step = [&](const Step &s, char *buf, int step, int which) {
+        bool all = true;
+#pragma unroll
+        for (int b = 0; b < SB; ++b) all = all && whole(s.pos[b], low, high);
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int x = wave + i * kWaves;
+            if (LOADS % kWaves == 0 || x < LOADS) {
+                const int b = x / (2 * BLOCK / 1024), y = x % (2 * BLOCK / 1024);
+                if (!all && y >= BLOCK / 1024) {
+                    int pos = s.pos[0];
+#pragma unroll
+                    for (int k = 1; k < SB; ++k) pos = b == k ? s.pos[k] : pos;
+                    const int z = (y - BLOCK / 1024) * 64 + lane;  // 16-byte piece of the values
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const int h = ST ? e / 4 : z / (4 * D);
+                        const int p = pos + 16 * h + 4 * (z & 3) + (e & 3);
+                        const bool hidden =
+                            p > high || (a.window > 0 && p <= low - a.window && p >= a.sinks);
+                        if constexpr (ST) {
+                            const uint32_t mask = e % 2 ? 0xFFFF0000u : 0xFFFFu;
+                            const uint32_t inf = e % 2 ? 0x7F800000u : 0x7F80u;
+                            if (hidden) stage[i][e / 2] &= ~mask;
+                            odd = odd || (stage[i][e / 2] & inf) == inf;
+                        } else {
+                            if (hidden) stage[i][e] = 0;
+                            odd = odd || (stage[i][e] & 0x7F800000u) == 0x7F800000u;
+                        }
+                    }
+                }
+                *(u32x4_t *)(buf + x * 1024 + lane * 16) = stage[i];
+            }
+        }
+        if (odd) flagged[which] = step;
+    };
+
+    if (threadIdx.x < 2) flagged[threadIdx.x] = -1;
+    __syncthreads();
+    Step cur;
+    bool more = next_step(cur);
+    if (more) {
+        load_step(cur);
+        store_step(cur, lds, 0, 0);
+    }
+    __syncthreads();
+    for (int step = 0; more; ++step) {
+        Step nxt;
+        more = next_step(nxt);
+        if (more) load_step(nxt);
+        const char *buf = lds + (step & 1) * (SB * 2 * BLOCK);
+        bool clear = true, none = true;
+#pragma unroll
+        for (int b = 0; b < SB; ++b) {
+            clear = clear && whole(cur.pos[b], wave_low, wave_high);
+            none = none && cur.pos[b] > wave_high;
+        }
+        if (busy && !none) {
+            // S^T = K Q^T
+            f32x4_t s[SB][2][kCols];
+#pragma unroll
+            for (int b = 0; b < SB; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) s[b][h][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < NC; ++i) {
+                        // (a piece past the row's end is read again and zeroed)
+                        const int piece = D % (4 * E) ? min(i * 4 + g, D / E - 1) : i * 4 + g;
+                        u32x4_t kf = *(const u32x4_t *)(buf + b * 2 * BLOCK +
+                                                        ((h * (D / E) + piece) * 16 + r) * 16);
+                        if (D % (4 * E) && i == NC - 1 && i * 4 + g >= D / E) kf = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) {
+                            if constexpr (ST) {
+                                s[b][h][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    __builtin_bit_cast(bf16x8_t, kf),
+                                    __builtin_bit_cast(bf16x8_t, qf[c][i]), s[b][h][c], 0, 0, 0);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    s[b][h][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                        float_of(kf[e]), float_of(qf[c][i][e]), s[b][h][c], 0, 0, 0);
+                            }
+                        }
+                    }
+                }
+            if (!clear) {
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int p = cur.pos[b] + 16 * h + 4 * g + i;
+#pragma unroll
+                            for (int c = 0; c < kCols; ++c)
+                                if (p > last[c] ||
+                                    (a.window > 0 && p <= last[c] - a.window && p >= a.sinks))
+                                    s[b][h][c][i] = kNone;
+                        }
+            }
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                float top = s[0][0][c][0];
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][h][c][i]);
+                top = column_max(top);
+                if (__ballot(top > m[c])) {
+                    const float mn = fmaxf(m[c], top);
+                    const float msn = mn == kNone ? 0.f : mn * a.scale2;
+                    const float f = mn == m[c] ? 1.f : m[c] == kNone ? 0.f : __builtin_amdgcn_exp2f(ms[c] - msn);
+                    m[c] = mn;
+                    ms[c] = msn;
+                    l[c] *= f;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[c][d][i] *= f;
+                }
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float p = __builtin_amdgcn_exp2f(
+                                __builtin_fmaf(s[b][h][c][i], a.scale2, -ms[c]));
+                            s[b][h][c][i] = p;
+                            l[c] += p;
+                        }
+            }
+            // O^T += V^T P^T
+            if (clear || flagged[step & 1] != step) {
+#pragma unroll
+                for (int b = 0; b < SB; ++b) {
+                    const char *vb = buf + b * 2 * BLOCK + BLOCK;
+                    if constexpr (ST) {
+                        bf16x8_t p[kCols];
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) p[c][4 * h + i] = (__bf16)s[b][h][c][i];
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) {
+                            const bf16x8_t vf = __builtin_bit_cast(
+                                bf16x8_t, *(const u32x4_t *)(vb + ((d * 16 + r) * 4 + g) * 16));
+#pragma unroll
+                            for (int c = 0; c < kCols; ++c)
+                                o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, p[c], o[c][d], 0, 0, 0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int d = 0; d < ND; ++d) {
+                                const u32x4_t vf =
+                                    *(const u32x4_t *)(vb + h * (BLOCK / 2) + ((d * 16 + r) * 4 + g) * 16);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                    for (int c = 0; c < kCols; ++c)
+                                        o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                            float_of(vf[i]), s[b][h][c][i], o[c][d], 0, 0, 0);
+                            }
+                    }
+                }
+            } else {
+                // Values that are not finite, seen by some rows and not by others: a
+                // position at a time, only where it is seen.
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        lds_wave_sync();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) lds_p[wave][16 * h + 4 * g + i][r] = s[b][h][c][i];
+                        lds_wave_sync();
+                        const char *vb = buf + b * 2 * BLOCK + BLOCK;
+#pragma unroll 1
+                        for (int t = 0; t < kKvBlock; ++t) {
+                            const int p = cur.pos[b] + t;
+                            if (p > last[c] || (a.window > 0 && p <= last[c] - a.window && p >= a.sinks))
+                                continue;
+                            const float w = lds_p[wave][t][r];
+#pragma unroll
+                            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int place = value_place<ST>(t, d * 16 + g * 4 + i, D);
+                                    float v;
+                                    if constexpr (ST)
+                                        v = float_of((uint32_t)((const uint16_t *)vb)[place] << 16);
+                                    else
+                                        v = ((const float *)vb)[place];
+                                    o[c][d][i] = __builtin_fmaf(w, v, o[c][d][i]);
+                                }
+                        }
+                    }
+            }
+        }
+        if (more) store_step(nxt, lds + ((step + 1) & 1) * (SB * 2 * BLOCK), step + 1, (step + 1) & 1);
+        cur = nxt;
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+        l[c] += __shfl_xor(l[c], 16);
+        l[c] += __shfl_xor(l[c], 32);
+        const int64_t x = w0 + c * 16 + r;
+        if (x >= w1) continue;
+        if (pieces == 1) {
+            const int64_t row = sq.row0 + x / a.group;
+            const int head = kvh * a.group + (int)(x % a.group);
+            const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];
+            char *to = a.out + (row * a.o_row + head * a.o_head + g * 4) * ES;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (ST)
+                        ((__bf16 *)to)[d * 16 + i] = (__bf16)(o[c][d][i] * inv);
+                    else
+                        ((float *)to)[d * 16 + i] = o[c][d][i] * inv;
+                }
+            if (a.lse && g == 0)
+                a.lse[row * a.heads + head] =
+                    l[c] == 0.f ? kNone : (ms[c] + __builtin_amdgcn_logf(l[c])) * kLn2;
+        } else {
+            const int64_t slot = ((int64_t)(pc.first + pc.split) * a.kv_heads + kvh) * kTile + (x - x0);
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                *(f32x4_t *)(a.part_o + slot * D + d * 16 + g * 4) = o[c][d];
+            if (g == 0) a.part_ml[slot] = make_float2(m[c] == kNone ? kNone : ms[c], l[c]);
+        }
+    }
+}
+
+// Joins the pieces of a tile, in their order: a workgroup per kJoinRows rows.
+template <int ST, int D>
+__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
+    constexpr int NR = (D + 63) / 64;
+    constexpr float kNone = -__builtin_huge_valf();
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int kParts = kTile / kJoinRows;
+    const int part = blockIdx.x % kParts;
+    const int kvh = blockIdx.x / kParts % a.kv_heads;
+    const int64_t number = blockIdx.x / kParts / a.kv_heads;
+    const int b = find_tile(a, number, lane);
+    const int tile = (int)(number - tile_base(a, b));
+    const Seq sq = seq_of(a, b);
+    if (tile < 0 || tile >= tiles_of(a, sq)) return;
+    const int2 f = a.info[number];
+    if (f.y <= 1) return;
+    for (int j = wave; j < kJoinRows; j += kWaves) {
+        const int local = part * kJoinRows + j;
+        const int64_t x = (int64_t)tile * kTile + local;
+        if (x >= (int64_t)sq.count * a.group) return;
+        auto slot_of = [&](int s) { return ((int64_t)(f.x + s) * a.kv_heads + kvh) * kTile + local; };
+        float top = kNone, sum = 0.f, acc[NR];
+        for (int s = lane; s < f.y; s += 64) top = fmaxf(top, a.part_ml[slot_of(s)].x);
+        top = wave_max(top);
+        const float ms = top == kNone ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) acc[i] = 0.f;
+        for (int s = 0; s < f.y; ++s) {
+            const int64_t slot = slot_of(s);
+            const float2 ml = a.part_ml[slot];
+            const float w = __builtin_amdgcn_exp2f(ml.x - ms);
+            sum += w * ml.y;
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                acc[i] += w * a.part_o[slot * D + min(lane + 64 * i, D - 1)];
+        }
+        const int64_t row = sq.row0 + x / a.group;
+        const int head = kvh * a.group + (int)(x % a.group);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (lane + 64 * i < D) {
+                const int64_t to = row * a.o_row + head * a.o_head + lane + 64 * i;
+                if constexpr (ST)
+                    ((__bf16 *)a.out)[to] = (__bf16)(acc[i] * inv);
+                else
+                    ((float *)a.out)[to] = acc[i] * inv;
+            }
+        if (a.lse && lane == 0)
+            a.lse[row * a.heads + head] = sum == 0.f ? kNone : (ms + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+}
+
+template <int ST, int D>
+hipError_t launch_chunk(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
+    constexpr int lds = 2 * buffer_bytes(ST, D);
+    if constexpr (lds + sizeof(float) * kWaves * kKvBlock * 16 + 64 > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)chunk_kernel<ST, D>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((chunk_kernel<ST, D>), dim3((uint32_t)wgs), dim3(64 * kWaves), lds, st, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !a.split) return e;
+    hipLaunchKernelGGL((chunk_join_kernel<ST, D>),
+                       dim3((uint32_t)(a.tiles * a.kv_heads * (kTile / kJoinRows))), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+template <int ST>
+hipError_t launch_chunk_dim(const ChunkArgs &a, int64_t wgs, int dim, hipStream_t st) {
+    switch (dim) {
+#define VS_DIM(D) \
+    case D:       \
+        return launch_chunk<ST, D>(a, wgs, st);
+        VS_DIM(16) VS_DIM(32) VS_DIM(48) VS_DIM(64) VS_DIM(80) VS_DIM(96) VS_DIM(112) VS_DIM(128)
+        VS_DIM(144) VS_DIM(160) VS_DIM(176) VS_DIM(192) VS_DIM(208) VS_DIM(224) VS_DIM(240)
+        VS_DIM(256)
+#undef VS_DIM
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+}  // namespace vs
+
+using vs::report;
+using vs::report_hip;
+
+extern "C" {
+
+int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t heads, const void *q,
+                      int64_t q_row, int64_t q_head, void *out, int64_t out_row, int64_t out_head,
+                      float *lse, const int32_t *starts, int64_t nrows, float scale, int causal,
+                      int64_t window, int64_t sinks, void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, s);
+    if (rc) return rc;
+    if (layer < 0 || layer >= kv->layers)
+        return report(VS_ERR_INVALID, "layer %lld out of range [0, %lld)", (long long)layer,
+                      (long long)kv->layers);
+    if (heads <= 0 || heads % kv->kv_heads)
+        return report(VS_ERR_INVALID, "heads (%lld) must be a multiple of kv_heads (%lld)",
+                      (long long)heads, (long long)kv->kv_heads);
+    if (heads > (1 << 16)) return report(VS_ERR_UNSUPPORTED, "more than 65,536 heads");
+    if (nrows < 0 || (!starts && nrows != s->nseq))
+        return report(VS_ERR_INVALID, "nrows %lld: without starts, one row per sequence",
+                      (long long)nrows);
+    if (window < 0 || sinks < 0) return report(VS_ERR_INVALID, "negative window or sinks");
+    if (window > 0 && !causal)
+        return report(VS_ERR_INVALID, "a window is of causal rows");
+    if (!std::isfinite(scale * vs::kLog2e))
+        return report(VS_ERR_INVALID, "scale is not finite, or too large for its exponentials' base");
+    const int64_t e = vs::kv_elem(kv->dtype), group = heads / kv->kv_heads;
+    if (((uintptr_t)q | (uintptr_t)out) % e || ((uintptr_t)lse | (uintptr_t)starts) % 4)
+        return report(VS_ERR_INVALID, "a buffer is not aligned to its elements");
+    for (int64_t x : {q_row, q_head, out_row, out_head})
+        if (!vs::stride_ok(x)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
+    if (s->nseq == 0 || nrows == 0) return VS_OK;
+    if (!q || !out) return report(VS_ERR_INVALID, "null q or out");
+    if (nrows > INT32_MAX / group)
+        return report(VS_ERR_UNSUPPORTED, "%lld rows of %lld heads", (long long)nrows, (long long)heads);
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipStream_t st = (hipStream_t)stream;
+
+    vs::ChunkArgs a = {};
+    vs::fill_geometry(kv, layer, a);
+    a.table = s->table;
+    a.lens = s->lens;
+    a.starts = starts;
+    a.width = s->width;
+    a.nseq = (int)s->nseq;
+    a.npages = (int)kv->npages;
+    a.page_shift = __builtin_ctzll((uint64_t)kv->page_size);
+    a.nrows = nrows;
+    a.q = (const char *)q;
+    a.out = (char *)out;
+    a.q_row = q_row;
+    a.q_head = q_head;
+    a.o_row = out_row;
+    a.o_head = out_head;
+    a.lse = lse;
+    a.heads = (int)heads;
+    a.kv_heads = (int)kv->kv_heads;
+    a.group = (int)group;
+    // The running maximum is of products before the scale, so that is above 0 (0
+    // itself as so little that nothing of it is left).
+    a.scale2 = std::max(std::fabs(scale * vs::kLog2e), 0x1p-126f);
+    a.flip = scale < 0 ? (e == 2 ? 0x80008000u : 0x80000000u) : 0;
+    a.causal = causal != 0;
+    a.window = (int)std::min<int64_t>(window, INT32_MAX);
+    a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX - 64);
+    a.q_vec = vs::pieces_ok(q, q_row, q_head, e);
+    a.tiles = nrows * group / vs::kTile + s->nseq;
+    const int64_t most = s->width * (kv->page_size / vs::kKvBlock);
+    a.split = a.tiles * a.kv_heads < 4 * kv->num_cu && s->nseq <= vs::kSplitSeqs && most > vs::kMinBlocks;
+    int64_t wgs = a.tiles * a.kv_heads;
+    if (a.split) {
+        a.target = (int)std::max<int64_t>(1, 4 * kv->num_cu / a.kv_heads);
+        const int64_t pieces = a.target + a.tiles, slots = pieces * a.kv_heads * vs::kTile;
+        const size_t o_bytes = (size_t)slots * kv->head_dim * sizeof(float);
+        const size_t ml_bytes = (size_t)slots * sizeof(float2);
+        void *ws = nullptr;
+        rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)a.tiles * sizeof(int2), &ws);
+        if (rc) return rc;
+        a.part_o = (float *)ws;
+        a.part_ml = (float2 *)((char *)ws + o_bytes);
+        a.info = (int2 *)((char *)ws + o_bytes + ml_bytes);
+        wgs = pieces * a.kv_heads;
+    }
+    if (!vs::grid_ok(wgs, 64 * vs::kWaves))
+        return report(VS_ERR_UNSUPPORTED, "%lld rows of %lld heads", (long long)nrows, (long long)heads);
+    const hipError_t err = kv->dtype == VS_DTYPE_BF16
+                               ? vs::launch_chunk_dim<1>(a, wgs, (int)kv->head_dim, st)
+                               : vs::launch_chunk_dim<0>(a, wgs, (int)kv->head_dim, st);
+    return err == hipSuccess ? VS_OK : report_hip(err, "attend");
+}
+
+}  // extern "C"

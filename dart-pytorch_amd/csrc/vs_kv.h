@@ -34,6 +34,7 @@ namespace vs {
 // vs_kv_check opens all.
 constexpr int kStatusWords = 4;
 constexpr int kStatusPages = 1, kStatusWidth = 2, kStatusParent = 4, kStatusNoPage = 8;
+constexpr int kStatusRows = 16;
 
 // Positions per block, the unit of the cache's layout: what one bf16 matrix
 // instruction sums over.

@@ -11,6 +11,7 @@ namespace {
 constexpr int kSmallPages = 16384;    // of a cache whose compaction is planned in registers
 constexpr int kForkSeqs = 1024;      // sequences and words of a fork that one workgroup does
 constexpr int kForkWords = 6 << 10;
+constexpr int kPlaceSeqs = 8192;    // whose starts a workgroup holds in LDS
 constexpr int kPieceBytes = 8192;   // of a page, per workgroup pass of the copy
 
 struct ExtendArgs {
@@ -550,6 +551,95 @@ hipError_t launch_copy(const vs_kv *kv, const int32_t *n_dev, int64_t n_max, con
 
 uint32_t grid_of(int64_t n, int64_t most) { return (uint32_t)std::max<int64_t>(1, std::min(n, most)); }
 
+// Where the rows of a batch go: sequence b has the next count[b] of them, for its
+// last positions.
+struct PlaceArgs {
+    const int32_t *table, *lens, *counts;
+    int64_t width;
+    int nseq, npages, page_shift, count;  // count: of every sequence, without counts
+    int nrows;
+    int32_t *starts, *sequence, *position, *slot;
+    int32_t *status;
+    int whole;  // starts are there: only the rows are left
+};
+
+// Inclusive prefix sum over a wave, and over the workgroup's kPlan threads.
+__device__ __forceinline__ int64_t prefix_sum64(int64_t x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int64_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// Starts are summed by every workgroup for itself, in LDS, and searched there for
+// its rows: one launch.  Past kPlaceSeqs sequences the first workgroup alone sums
+// them, and a second launch searches them in memory.
+template <bool SMALL>
+__global__ __launch_bounds__(kPlan) void rows_kernel(PlaceArgs a) {
+    __shared__ int32_t lds_starts[SMALL ? kPlaceSeqs + 1 : 1];
+    __shared__ int64_t totals[kPlan / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (!a.whole) {
+        int64_t base = 0;
+        for (int b0 = 0; b0 < a.nseq; b0 += kPlan) {
+            const int b = b0 + threadIdx.x;
+            const int64_t mine = b < a.nseq ? max(a.counts ? a.counts[b] : a.count, 0) : 0;
+            int64_t incl = prefix_sum64(mine, lane);
+            __syncthreads();
+            if (lane == 63) totals[wave] = incl;
+            __syncthreads();
+            const int64_t w = prefix_sum64(lane < kPlan / 64 ? totals[lane] : 0, lane);
+            incl += base + (wave ? __shfl(w, wave - 1) : 0);
+            base += __shfl(w, kPlan / 64 - 1);
+            // (sums past 2^31 - 1 stay there: no row has such a number)
+            const int32_t s = (int32_t)min(incl, (int64_t)INT32_MAX);
+            if (b < a.nseq) {
+                if (SMALL) lds_starts[b + 1] = s;
+                if (blockIdx.x == 0) a.starts[b + 1] = s;
+            }
+        }
+        if (threadIdx.x == 0) {
+            if (SMALL) lds_starts[0] = 0;
+            if (blockIdx.x == 0) {
+                a.starts[0] = 0;
+                if (base > a.nrows) atomicOr(&a.status[0], kStatusRows);
+            }
+        }
+        if (!SMALL) return;
+        __syncthreads();
+    }
+    const int32_t *starts = SMALL ? lds_starts : a.starts;
+    const int64_t stride = (int64_t)gridDim.x * kPlan;
+    for (int64_t row = (int64_t)blockIdx.x * kPlan + threadIdx.x; row < a.nrows; row += stride) {
+        int lo = 0, hi = a.nseq;  // the last sequence that starts at or before the row
+        while (hi - lo > 1) {
+            const int mid = (int)(((unsigned)lo + (unsigned)hi) / 2);
+            if (starts[mid] <= row)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        int b = -1, slot = -1;
+        int64_t pos = -1;
+        if (a.nseq > 0 && row < starts[lo + 1]) {
+            b = lo;
+            pos = (int64_t)a.lens[b] - (starts[lo + 1] - row);
+            if (pos < 0) pos = -1;
+            if (pos >= 0 && pos >> a.page_shift < a.width) {
+                const int page = a.table[b * a.width + (pos >> a.page_shift)];
+                const int64_t at =
+                    ((int64_t)page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+                if ((unsigned)page < (unsigned)a.npages) slot = (int)at;
+            }
+        }
+        if (a.sequence) a.sequence[row] = b;
+        if (a.position) a.position[row] = (int32_t)pos;
+        if (a.slot) a.slot[row] = slot;
+    }
+}
+
 }  // namespace
 }  // namespace vs
 
@@ -778,6 +868,70 @@ int vs_kv_copy(vs_kv *kv, const int32_t *from, const int32_t *to, int64_t n, voi
     return e == hipSuccess ? VS_OK : report_hip(e, "page copies");
 }
 
+int vs_kv_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t count, const int32_t *count_dev,
+               int64_t nrows, int32_t *starts, int32_t *sequence, int32_t *position, int32_t *slot,
+               void *stream) {
+    if (!kv) return report(VS_ERR_INVALID, "null handle");
+    int rc = vs::check_seqs(kv, s);
+    if (rc) return rc;
+    if (!count_dev && (count < 0 || count > INT32_MAX))
+        return report(VS_ERR_INVALID, "count %lld", (long long)count);
+    if (nrows < 0 || nrows > INT32_MAX)
+        return report(VS_ERR_INVALID, "nrows %lld out of range [0, 2^31)", (long long)nrows);
+    if (!starts) return report(VS_ERR_INVALID, "null starts");
+    if (((uintptr_t)count_dev | (uintptr_t)starts | (uintptr_t)sequence | (uintptr_t)position |
+         (uintptr_t)slot) % 4)
+        return report(VS_ERR_INVALID, "a buffer is not aligned to its elements");
+    if (slot && kv->npages > INT32_MAX / kv->page_size)
+        return report(VS_ERR_UNSUPPORTED, "slots past 2^31: %lld pages of %lld positions",
+                      (long long)kv->npages, (long long)kv->page_size);
+    // Each row is looked up while others are written, and so are the starts.
+    const struct {
+        const void *p;
+        int64_t n;
+    } ins[] = {{count_dev, s->nseq}, {s->lens, s->nseq}, {s->table, s->nseq * s->width}},
+      outs[] = {{starts, s->nseq + 1}, {sequence, nrows}, {position, nrows}, {slot, nrows}};
+    for (int i = 0; i < 4; ++i) {
+        for (const auto &in : ins)
+            if (vs::overlap(in.p, in.n * 4, outs[i].p, outs[i].n * 4))
+                return report(VS_ERR_INVALID, "rows: an output overlaps an input");
+        for (int j = 0; j < i; ++j)
+            if (vs::overlap(outs[j].p, outs[j].n * 4, outs[i].p, outs[i].n * 4))
+                return report(VS_ERR_INVALID, "rows: two outputs overlap");
+    }
+    vs::DeviceGuard g(kv->device);
+    if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
+    hipStream_t st = (hipStream_t)stream;
+    vs::PlaceArgs a = {};
+    a.table = s->table;
+    a.lens = s->lens;
+    a.counts = count_dev;
+    a.count = (int)count;
+    a.width = s->width;
+    a.nseq = (int)s->nseq;
+    a.npages = (int)kv->npages;
+    a.page_shift = __builtin_ctzll((uint64_t)kv->page_size);
+    a.nrows = (int)nrows;
+    a.starts = starts;
+    a.sequence = sequence;
+    a.position = position;
+    a.slot = slot;
+    a.status = kv->status;
+    const bool any = sequence || position || slot;
+    const int64_t groups = any ? (nrows + vs::kPlan - 1) / vs::kPlan : 0;
+    const dim3 grid((uint32_t)std::max<int64_t>(1, std::min<int64_t>(groups, 2 * kv->num_cu)));
+    if (s->nseq <= vs::kPlaceSeqs) {
+        hipLaunchKernelGGL(vs::rows_kernel<true>, grid, dim3(vs::kPlan), 0, st, a);
+    } else {
+        hipLaunchKernelGGL(vs::rows_kernel<false>, dim3(1), dim3(vs::kPlan), 0, st, a);
+        VS_LAUNCHED("rows");
+        a.whole = 1;
+        if (groups) hipLaunchKernelGGL(vs::rows_kernel<false>, grid, dim3(vs::kPlan), 0, st, a);
+    }
+    VS_LAUNCHED("rows");
+    return VS_OK;
+}
+
 int vs_kv_check(vs_kv *kv, void *stream) {
     if (!kv) return report(VS_ERR_INVALID, "null handle");
     vs::DeviceGuard g(kv->device);
@@ -800,6 +954,8 @@ int vs_kv_check(vs_kv *kv, void *stream) {
     if (got[0] & vs::kStatusWidth)
         return report(VS_ERR_INVALID, "a sequence outgrew its %s", "table row");
     if (got[0] & vs::kStatusNoPage) return report(VS_ERR_INVALID, "a new token has no page");
+    if (got[0] & vs::kStatusRows)
+        return report(VS_ERR_INVALID, "the counts are of more rows than there are");
     if (got[0] & vs::kStatusParent) return report(VS_ERR_INVALID, "a parent is out of range");
     return VS_OK;
 }

@@ -45,7 +45,9 @@ EXPORTED = [
     "vs_kv_create", "vs_kv_destroy", "vs_kv_page_bytes", "vs_kv_memory", "vs_kv_attend",
     "vs_kv_append", "vs_kv_read", "vs_kv_extend", "vs_kv_fork", "vs_kv_free", "vs_kv_evict",
     "vs_kv_compact", "vs_kv_compact_with", "vs_kv_copy", "vs_kv_check",
-    "vs_beam_create", "vs_beam_destroy", "vs_beam_select", "vs_beam_reorder",
+    "vs_kv_attend_rows", "vs_kv_rows", "vs_kv_append_rotary",
+    "vs_rotary_create", "vs_rotary_destroy", "vs_rotary_apply",
+    "vs_beam_create", "vs_beam_destroy", "vs_beam_select", "vs_beam_reorder", "vs_beam_logprobs",
 ]
 
 
@@ -161,10 +163,18 @@ def load() -> ctypes.CDLL:
         "vs_kv_compact_with": ([p, p, p, p, i64, p, p], i32),
         "vs_kv_copy": ([p, p, p, i64, p], i32),
         "vs_kv_check": ([p, p], i32),
+        "vs_kv_attend_rows": ([p, p, i64, i64] + [p, i64, i64] * 2
+                              + [p, p, i64, ctypes.c_float, i32, i64, i64, p], i32),
+        "vs_kv_rows": ([p, p, i64, p, i64, p, p, p, p, p], i32),
+        "vs_kv_append_rotary": ([p, p, i64, p] + [p, i64, i64] * 3 + [i64] + [p, i64, i64, p, i64, p], i32),
+        "vs_rotary_create": ([i32, i64, p, ctypes.c_float, i32, pp], i32),
+        "vs_rotary_destroy": ([p], None),
+        "vs_rotary_apply": ([p, i32, p, i64, i64, p, i64, i64, i64, p, i64, i64, i32, p], i32),
         "vs_beam_create": ([i32, pp], i32),
         "vs_beam_destroy": ([p], None),
         "vs_beam_select": ([p, p, i32, i64, i64, i64, i64, p, p, i64, i64, p, p, p, p, p], i32),
         "vs_beam_reorder": ([p, p, i64, p, i64, i64, p, i64, i64, p, p], i32),
+        "vs_beam_logprobs": ([p, p, i32, i64, i64, i64, p, p, p, i64, p, p, p], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

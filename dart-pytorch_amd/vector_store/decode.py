@@ -211,6 +211,100 @@ class KVSequences:
         self._ref = ctypes.byref(self.c)
 
 
+class Rotary:
+    """Rotary positions of a head's first `dims` dimensions (vs_rotary_*).
+
+    Pair i turns by base ** (-2 i / dims) radians per position; its dimensions are
+    (i, i + dims / 2) in the "half" layout, (2 i, 2 i + 1) in the "interleaved"
+    one.  scaling, for contexts longer than the model's own:
+      "linear"  all angles divided by factor
+      "base"    base times factor ** (dims / (dims - 2))
+      "ramp"    by a pair's turns within the `original` positions: up to `low` of
+                them its angle is divided by factor, from `high` on it stays, in between
+                a share of both; ramp_by "turns" takes the share linear in the turns,
+                "index" linear in the pair's number (its ends rounded outwards)
+    gain multiplies cosines and sines (None: 0.1 ln(factor) + 1 for "ramp", else 1).
+    frequencies (radians per position, dims / 2 of them) stands for all that."""
+
+    def __init__(self, head_dim: int, *, dims: int | None = None, base: float = 10000.0, layout: str = "half",
+                 scaling: str = "none", factor: float = 1.0, original: int = 0, low: float = 1.0, high: float = 4.0,
+                 ramp_by: str = "turns", gain: float | None = None, frequencies=None, device: int = 0):
+        self._h = None
+        self.head_dim, self.dims = int(head_dim), int(head_dim if dims is None else dims)
+        self.device = int(device)
+        if self.dims <= 0 or self.dims % 2 or self.dims > self.head_dim:
+            raise ValueError(f"dims must be even and 2 to {head_dim}, got {self.dims}")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"layout must be half or interleaved, got {layout}")
+        if frequencies is None:
+            w = self._frequencies(base, scaling, factor, original, low, high, ramp_by)
+            if gain is None and scaling == "ramp":
+                gain = 0.1 * math.log(factor) + 1.0
+        else:
+            w = np.ascontiguousarray(frequencies, np.float64)
+            if w.shape != (self.dims // 2,):
+                raise ValueError(f"frequencies: shape {w.shape}, expected {(self.dims // 2,)}")
+        self.frequencies, self.layout, self.gain = w, layout, 1.0 if gain is None else float(gain)
+        self._lib = N.load()
+        h = ctypes.c_void_p()
+        N.check(self._lib.vs_rotary_create(device, self.dims, w.ctypes.data_as(ctypes.c_void_p), self.gain,
+                                           layout == "interleaved", ctypes.byref(h)))
+        self._h = h
+
+    def _frequencies(self, base, scaling, factor, original, low, high, ramp_by):
+        dims = self.dims
+        if not base > 1 or not factor > 0:
+            raise ValueError(f"base must be above 1 and factor above 0, got {base} and {factor}")
+        if scaling not in ("none", "linear", "base", "ramp"):
+            raise ValueError(f"scaling must be none, linear, base or ramp, got {scaling}")
+        if scaling == "base" and dims > 2:
+            base = base * factor ** (dims / (dims - 2))
+        w = base ** (-np.arange(0, dims, 2, dtype=np.float64) / dims)
+        if scaling == "linear":
+            return w / factor
+        if scaling != "ramp":
+            return w
+        if not original > 0 or not 0 < low < high:
+            raise ValueError(f"ramp needs original > 0 and 0 < low < high, got {original}, {low} and {high}")
+        if ramp_by == "turns":
+            keep = np.clip((original * w / (2 * math.pi) - low) / (high - low), 0.0, 1.0)
+        elif ramp_by == "index":
+            # the pair (a real number) whose turns are `n`
+            at = [dims * math.log(original / (n * 2 * math.pi)) / (2 * math.log(base)) for n in (high, low)]
+            first, last = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dims - 1)
+            keep = 1.0 - np.clip((np.arange(dims // 2) - first) / max(last - first, 1e-3), 0.0, 1.0)
+        else:
+            raise ValueError(f"ramp_by must be turns or index, got {ramp_by}")
+        return w * keep + w / factor * (1.0 - keep)
+
+    def close(self) -> None:
+        if self._h:
+            self._lib.vs_rotary_destroy(self._h)
+            self._h = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def rotate(self, x, out, positions, *, backward: bool = False, stream: int = 0) -> None:
+        """out = x [rows, heads, head_dim] (f32 or bf16) turned, row i by
+        positions[i] (i32) (vs_rotary_apply); out may be x.  backward: the other
+        way round, a gradient of out into one of x."""
+        rows, heads = int(x.shape[0]), int(x.shape[1])
+        code = _code(x.dtype)
+        if code < 0:
+            raise ValueError(f"x: element type {x.dtype}")
+        xp, xs = _rows(x, "x", (rows, heads, self.head_dim), code, self.device)
+        op, os_ = _rows(out, "out", (rows, heads, self.head_dim), code, self.device)
+        rc = self._lib.vs_rotary_apply(self._h, code, xp, xs[0], xs[1],
+                                       _flat(positions, "positions", (rows,), _I32, self.device), rows, heads,
+                                       self.head_dim, op, os_[0], os_[1], bool(backward), stream)
+        if rc:
+            N.check(rc)
+
+
 class PagedKVCache:
     """Keys and values of every layer, in pages that stay in HBM (vs_kv_* of the C ABI)."""
 
@@ -294,16 +388,92 @@ class PagedKVCache:
         if rc:
             N.check(rc)
 
-    def append(self, seqs: KVSequences, k, v, *, starts=None, layer: int = 0, stream: int = 0) -> None:
+    def attend_rows(self, seqs: KVSequences, q, out, *, starts=None, lse=None, layer: int = 0, scale=None,
+                    causal: bool = True, window: int = 0, sinks: int = 0, stream: int = 0) -> None:
+        """Attention of many rows at once (vs_kv_attend_rows): chunks of prompts,
+        drafted tokens, or rows over other sequences' states.
+
+        q, out [rows, heads, head_dim]; starts [n + 1] i32: rows starts[b] ..
+        starts[b + 1] are the last positions of sequence b (none: one each), whose
+        keys and values are in the cache already; lse [rows, heads] f32.  Rows
+        see the positions up to their own (of them, with window > 0, the last
+        `window` and the first `sinks`), or all of the sequence's if not causal."""
+        rows, heads = int(q.shape[0]), int(q.shape[1])
+        code, dim, dev = self.code, self.head_dim, self.device
+        qp, qs = _rows(q, "q", (rows, heads, dim), code, dev)
+        op, os_ = _rows(out, "out", (rows, heads, dim), code, dev)
+        sp = None if starts is None else _flat(starts, "starts", (seqs.n + 1,), _I32, dev)
+        lp = None if lse is None else _flat(lse, "lse", (rows, heads), N.VS_DTYPE_F32, dev)
+        rc = self._lib.vs_kv_attend_rows(
+            self._h, self._seqs(seqs), layer, heads, qp, qs[0], qs[1], op, os_[0], os_[1], lp, sp, rows,
+            self._scale if scale is None else scale, bool(causal), window, sinks, stream)
+        if rc:
+            N.check(rc)
+
+    def rows(self, seqs: KVSequences, count, starts, *, sequence=None, position=None, slot=None,
+             stream: int = 0) -> None:
+        """Where the rows of a batch go (vs_kv_rows): sequence b has the next
+        count[b] rows (an int, or an i32 buffer [n]), for its last positions.
+
+        starts [n + 1] i32 receives the sums of the counts; sequence, position and
+        slot ([rows] i32 each, all of one length) each row's sequence, position
+        and page * page_size + place on the page; -1 where there is none."""
+        dev = self.device
+        nrows = None
+        ptrs = []
+        for t, what in ((sequence, "sequence"), (position, "position"), (slot, "slot")):
+            if t is None:
+                ptrs.append(None)
+                continue
+            if nrows is None:
+                nrows = int(t.shape[0])
+            ptrs.append(_flat(t, what, (nrows,), _I32, dev))
+        each, cp = (int(count), None) if isinstance(count, (int, np.integer)) else \
+            (0, _flat(count, "count", (seqs.n,), _I32, dev))
+        rc = self._lib.vs_kv_rows(self._h, self._seqs(seqs), each, cp, 2**31 - 1 if nrows is None else nrows,
+                                  _flat(starts, "starts", (seqs.n + 1,), _I32, dev), *ptrs, stream)
+        if rc:
+            N.check(rc)
+
+    def append(self, seqs: KVSequences, k, v, *, starts=None, layer: int = 0, rotary: Rotary | None = None, q=None,
+               q_out=None, stream: int = 0) -> None:
         """Stores rows of keys and values at the sequences' last positions
         (vs_kv_append): k, v [rows, kv_heads, head_dim]; starts [n + 1] i32:
-        rows starts[b] .. starts[b + 1] are sequence b's (none: one each)."""
+        rows starts[b] .. starts[b + 1] are sequence b's (none: one each).
+
+        With rotary the keys are turned to their positions on the way, and the
+        queries q [rows, heads, head_dim] into q_out (q itself, or another buffer)
+        (vs_kv_append_rotary)."""
         rows = int(k.shape[0])
+        if rotary is not None:
+            return self._append_rotary(seqs, k, v, rows, starts, layer, rotary, q, q_out, stream)
+        if q is not None or q_out is not None:
+            raise ValueError("q and q_out go with rotary")
         kp, ks = _rows(k, "k", (rows, self.kv_heads, self.head_dim), self.code, self.device)
         vp, vs = _rows(v, "v", (rows, self.kv_heads, self.head_dim), self.code, self.device)
         sp = None if starts is None else _flat(starts, "starts", (seqs.n + 1,), _I32, self.device)
         N.check(self._lib.vs_kv_append(self._h, self._seqs(seqs), layer, kp, ks[0], ks[1], vp, vs[0], vs[1],
                                        sp, rows, stream))
+
+    def _append_rotary(self, seqs, k, v, rows, starts, layer, rotary, q, q_out, stream) -> None:
+        code, dim, dev = self.code, self.head_dim, self.device
+        kp, ks = _rows(k, "k", (rows, self.kv_heads, dim), code, dev)
+        vp, vs = _rows(v, "v", (rows, self.kv_heads, dim), code, dev)
+        qp = op = None
+        qs = os_ = (0, 0)
+        heads = 0
+        if q is not None or q_out is not None:
+            if q is None or q_out is None:
+                raise ValueError("q and q_out are given together or not at all")
+            heads = int(q.shape[1])
+            qp, qs = _rows(q, "q", (rows, heads, dim), code, dev)
+            op, os_ = _rows(q_out, "q_out", (rows, heads, dim), code, dev)
+        sp = None if starts is None else _flat(starts, "starts", (seqs.n + 1,), _I32, dev)
+        rc = self._lib.vs_kv_append_rotary(
+            self._h, self._seqs(seqs), layer, rotary._h, kp, ks[0], ks[1], vp, vs[0], vs[1], qp, qs[0], qs[1], heads,
+            op, os_[0], os_[1], sp, rows, stream)
+        if rc:
+            N.check(rc)
 
     def read(self, seqs: KVSequences, b: int, first: int, k_out, v_out, *, layer: int = 0, stream: int = 0) -> None:
         """Positions first .. of sequence b as rows [positions, kv_heads, head_dim] (vs_kv_read)."""
@@ -436,6 +606,35 @@ class BeamSearch:
             _flat(scores_out, "scores_out", out, N.VS_DTYPE_F32), _flat(tokens_out, "tokens_out", out, _I32),
             _flat(parents_out, "parents_out", out, _I32),
             None if finished_out is None else _flat(finished_out, "finished_out", out, _U8, dev), stream)
+        if rc:
+            N.check(rc)
+
+    def logprobs(self, logits, tokens, out, *, entropy=None, top_tokens=None, top_logprobs=None,
+                 stream: int = 0) -> None:
+        """Log probabilities of given tokens (vs_beam_logprobs).
+
+        logits [rows, vocab] f32 or bf16; tokens [rows] i32 (-1: none, 0 comes
+        out) and out [rows] f32, both or neither (None); entropy [rows] f32;
+        top_tokens i32 and top_logprobs f32 [rows, k]: the k likeliest."""
+        dev = self.device
+        rows, vocab = logits.shape
+        code = _code(logits.dtype)
+        if code < 0:
+            raise ValueError(f"logits: element type {logits.dtype}")
+        lp, ls = _rows(logits, "logits", (rows, vocab), code, dev)
+        if (tokens is None) != (out is None):
+            raise ValueError("tokens and out are given together or not at all")
+        if (top_tokens is None) != (top_logprobs is None):
+            raise ValueError("top_tokens and top_logprobs are given together or not at all")
+        f32 = N.VS_DTYPE_F32
+        k = 0 if top_tokens is None else int(top_tokens.shape[1])
+        rc = self._lib.vs_beam_logprobs(
+            self._h, lp, code, ls[0] if rows > 1 else vocab, rows, vocab,
+            None if tokens is None else _flat(tokens, "tokens", (rows,), _I32, dev),
+            None if out is None else _flat(out, "out", (rows,), f32, dev),
+            None if entropy is None else _flat(entropy, "entropy", (rows,), f32, dev), k,
+            _flat(top_tokens, "top_tokens", (rows, k), _I32, dev) if k else None,
+            _flat(top_logprobs, "top_logprobs", (rows, k), f32, dev) if k else None, stream)
         if rc:
             N.check(rc)
 

@@ -280,6 +280,22 @@ VS_API int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_
                         int64_t k_head, const void *v, int64_t v_seq, int64_t v_head, void *out,
                         int64_t out_seq, int64_t out_head, float *lse, float scale, int64_t window,
                         int64_t sinks, void *stream);
+/* Attention of many new tokens at once: rows [starts[b], starts[b + 1]) of q
+ * (nseq + 1 ascending device values, starts[0] >= 0; null: one row each) are the
+ * last positions of sequence b, whose keys and values are in the cache already
+ * (vs_kv_append).  nrows: how many rows q and out have; rows of no sequence are
+ * left as they were.  The row at position t sees
+ *   causal != 0  p <= t on a page, and window == 0 or p > t - window or p < sinks
+ *   causal == 0  every p < n on a page (window is 0): rows over other sequences' states
+ * and out, lse ([nrows][heads]) and the rest are vs_kv_attend's; nothing visible
+ * (positions below 0 too): out 0, lse -inf.  What lies at positions that a row does not see may be anything.
+ * Scores, the softmax and sums are held in fp32; with BF16 a weight is rounded to
+ * bf16 before it multiplies its value, by 2^-8 of the weight at most. */
+VS_API int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t heads,
+                             const void *q, int64_t q_row, int64_t q_head, void *out,
+                             int64_t out_row, int64_t out_head, float *lse, const int32_t *starts,
+                             int64_t nrows, float scale, int causal, int64_t window, int64_t sinks,
+                             void *stream);
 /* Stores keys and values of a layer: rows [starts[b], starts[b + 1]) of k and
  * v go to the last starts[b + 1] - starts[b] positions of sequence b (starts:
  * nseq + 1 ascending device values, starts[0] >= 0; null: one row each, row b
@@ -294,6 +310,38 @@ VS_API int vs_kv_append(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, const 
 VS_API int vs_kv_read(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t b, int64_t first,
                       int64_t n, void *k_out, void *v_out, void *stream);
 
+/* Rotary positions.  Pairs of a head's first `dims` dimensions turn by the row's
+ * position times the pair's angle, radians[i] per position (dims / 2 host values):
+ *   y0 = gain (x0 cos - x1 sin)      y1 = gain (x1 cos + x0 sin)
+ * The pairs are (i, i + dims / 2), or (2 i, 2 i + 1) if interleaved is not 0;
+ * dimensions from `dims` on stay as they are.  Angles are exact to 2^-33 of a
+ * turn at positions below 2^31, cosines and sines to fp32.  A handle is not
+ * changed by its calls. */
+typedef struct vs_rotary vs_rotary;
+VS_API int vs_rotary_create(int device, int64_t dims, const double *radians, float gain,
+                            int interleaved, vs_rotary **out);
+/* Waits for the device's work. */
+VS_API void vs_rotary_destroy(vs_rotary *r);
+/* Rows of `heads` heads of head_dim values of `dtype`, at [i * *_row + h * *_head]
+ * elements, row i at positions[i] (device, any sign).  out is x with its strides
+ * (in place) or does not overlap it.  backward != 0: the turn the other way, by
+ * which a gradient of `out` is one of `x`. */
+VS_API int vs_rotary_apply(const vs_rotary *r, int dtype, const void *x, int64_t x_row,
+                           int64_t x_head, const int32_t *positions, int64_t nrows, int64_t heads,
+                           int64_t head_dim, void *out, int64_t out_row, int64_t out_head,
+                           int backward, void *stream);
+/* vs_kv_append with keys turned to their positions on the way, and queries with
+ * them: row i of q (`heads` heads; null: none) goes to row i of q_out.  Rows of
+ * q that are not a sequence's are left out; those whose keys have no place are
+ * turned all the same.  q_out is q with its strides or does not overlap it; it does not overlap k
+ * or v. */
+VS_API int vs_kv_append_rotary(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer,
+                               const vs_rotary *r, const void *k, int64_t k_row, int64_t k_head,
+                               const void *v, int64_t v_row, int64_t v_head, const void *q,
+                               int64_t q_row, int64_t q_head, int64_t heads, void *q_out,
+                               int64_t out_row, int64_t out_head, const int32_t *starts,
+                               int64_t nrows, void *stream);
+
 /* Gives every sequence `count` more positions (or count_dev[b], if not null;
  * negative counts are 0): lens grow, and the pages for them are taken, the
  * lowest free ones in the order of the sequences.  A partly filled last page
@@ -307,6 +355,19 @@ VS_API int vs_kv_read(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t 
  * position then, are dropped, and the cache stays as it was. */
 VS_API int vs_kv_extend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t count, const int32_t *count_dev,
                         void *stream);
+/* Where the rows of a batch go: sequence b has the next count_dev[b] of them
+ * (count, if that is null; negative counts are 0), for its last positions.
+ * starts[b] (nseq + 1 of them, for vs_kv_append and the other calls) is the sum
+ * of the counts before b.  Of row i < nrows of sequence b
+ *   sequence[i]  b
+ *   position[i]  lens[b] - (starts[b + 1] - i); -1 if that is below 0
+ *   slot[i]      page * page_size + the position's place on it; -1: on no page
+ * (each may be null; -1 in rows past the last sequence's).  Counts of more than
+ * nrows rows: those past nrows are left out of the three, and vs_kv_check says
+ * so.  No output overlaps an input or another output. */
+VS_API int vs_kv_rows(vs_kv *kv, const vs_kv_seqs *seqs, int64_t count, const int32_t *count_dev,
+                      int64_t nrows, int32_t *starts, int32_t *sequence, int32_t *position,
+                      int32_t *slot, void *stream);
 /* out's sequence i becomes a copy of in's sequence parents[i] (nseq of out
  * entries; -1: an empty sequence) that shares its pages: the table and length
  * are copied and refs follow; sequences of `in` that are no one's parent lose
@@ -346,7 +407,8 @@ VS_API int vs_kv_copy(vs_kv *kv, const int32_t *from, const int32_t *to, int64_t
 /* Waits for the stream (for the device, where an extend was refused) and tells what earlier calls met on the device since
  * the last check: VS_ERR_OOM (an extend found too few free pages),
  * VS_ERR_INVALID (too few table columns for an extend, an attend's new token or
- * an append's rows; a new token without a page; a parent out of range). */
+ * an append's rows; a new token without a page; counts of more rows than
+ * vs_kv_rows was given; a parent out of range). */
 VS_API int vs_kv_check(vs_kv *kv, void *stream);
 
 /* Beam search over device buffers.  A handle owns scratch memory only. */
@@ -382,6 +444,23 @@ VS_API int vs_beam_select(vs_beam *bs, const void *logits, int dtype, int64_t ro
 VS_API int vs_beam_reorder(vs_beam *bs, const int32_t *parents, int64_t nrows, const void *in,
                            int64_t nrows_in, int64_t in_stride, void *out, int64_t out_stride,
                            int64_t bytes, const int32_t *tail, void *stream);
+
+/* Log probabilities of given tokens.  Row i of `logits` (vocab values of
+ * `dtype`, rows row_stride apart) is the distribution that tokens[i] was taken
+ * from:
+ *   logprobs[i]  x_t - log sum exp x, t = tokens[i]; 0 where t is -1 (no token),
+ *                NaN where it is any other outside [0, vocab)
+ *   entropy[i]   -sum of p log p over the row
+ *   top_tokens, top_logprobs [nrows][k]: the k largest, larger logit first, then
+ *                the lower token; -1 and -inf where there are fewer above -inf
+ * tokens and logprobs may both be null, entropy too; k is 0 to 64.  A token at
+ * -inf has -inf.  A row that holds a NaN or +inf, or nothing but -inf, is no
+ * distribution: NaN, NaN, and -1 and -inf.  Sums are held in fp32, what comes of
+ * them in 64 bits and rounded once.  No output overlaps another or an input. */
+VS_API int vs_beam_logprobs(vs_beam *bs, const void *logits, int dtype, int64_t row_stride,
+                            int64_t nrows, int64_t vocab, const int32_t *tokens, float *logprobs,
+                            float *entropy, int64_t k, int32_t *top_tokens, float *top_logprobs,
+                            void *stream);
 
 /* ---- errors ---- */
 VS_API const char *vs_last_error(void);
