@@ -15,9 +15,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kWaves = 4;
 constexpr int kCols = 2;                      // columns of 16 rows per wave
 constexpr int kTile = kWaves * kCols * 16;    // rows of queries per workgroup
-constexpr int kMinBlocks = 4;                 // per piece of a tile's blocks, at least
+constexpr int kMinBlocks = 8;                 // per piece of a tile's blocks, at least
 constexpr int kSplitSeqs = 384;               // sequences whose pieces each workgroup finds for itself
-constexpr int kJoinRows = 8;                  // rows per workgroup of the join
+constexpr float kSlack = 8.f;                 // of a running maximum, in powers of two
+constexpr int kJoinRows = 4;                  // rows per workgroup of the join
 
 struct ChunkArgs {
     char *pool;
@@ -37,11 +38,17 @@ struct ChunkArgs {
     int q_vec;                   // rows readable in 16-byte pieces
     int64_t tiles;               // numbers of tiles, with gaps
     int split;                   // tiles are divided along the length
-    int target;                  // pieces of all tiles, about
-    int2 *info;                  // [tile] its first piece, how many
+    int slots;                   // pieces at work at once, per key-value head
+    int4 *info;                  // [tile] its first whole piece, how many, its rest; how many in use
     float *part_o;               // [piece][kv head][row of the tile][dim]
     float2 *part_ml;             // [piece][kv head][row of the tile] running maximum and sum
 };
+
+// A value that all lanes have, for the scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
+}
 
 // The rows of a sequence: [row0, row0 + count) of the batch's, row i at position
 // i + shift; `cap` the last position that there is, at most.
@@ -129,42 +136,69 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
     return x;
 }
 
-// Piece `piece` of a divided call: piece split of tile `tile` (within its sequence).
+// Piece `piece` of a divided call: the split-th `per` blocks of tile `tile` of
+// sequence b.  All whole pieces come first, then what is left of each tile, so
+// that the smaller ones fill the places that come free.
 struct Piece {
-    int b, tile, split, per, first;  // first: the tile's first piece
+    int b, tile, split, per;
+    int first, whole, rest;  // the tile's pieces: first .. first + whole - 1, and rest (-1: none)
 };
 
 __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int lane, Piece &p) {
-    int64_t all = 0;
-    for (int b0 = 0; b0 < a.nseq; b0 += 64)
-        if (b0 + lane < a.nseq) {
-            const Seq s = seq_of(a, b0 + lane);
-            all += (int64_t)tiles_of(a, s) * most_blocks(a, s);
-        }
-    all = wave_sum64(all);
-    p.per = (int)max((all + a.target - 1) / a.target, (int64_t)kMinBlocks);
-    int base = 0;
-    for (int b0 = 0; b0 < a.nseq; b0 += 64) {
-        int tiles = 0, splits = 1;
-        if (b0 + lane < a.nseq) {
-            const Seq s = seq_of(a, b0 + lane);
+    auto look = [&](int b, int &tiles, int &blocks) {
+        tiles = blocks = 0;
+        if (b < a.nseq) {
+            const Seq s = seq_of(a, b);
             tiles = tiles_of(a, s);
-            splits = max((most_blocks(a, s) + p.per - 1) / p.per, 1);
+            blocks = most_blocks(a, s);
         }
-        const int sum = base + prefix_sum(tiles * splits);
-        const uint64_t past = __ballot(sum > piece);
+    };
+    int t0, n0;  // (all there is to read for up to 64 sequences)
+    look(lane, t0, n0);
+    int64_t all = (int64_t)t0 * n0;
+    int count = t0;
+    for (int b = lane + 64; b < a.nseq; b += 64) {
+        int t, n;
+        look(b, t, n);
+        all += (int64_t)t * n;
+        count += t;
+    }
+    all = uniform(wave_sum64(all));
+    count = (int)wave_sum((uint32_t)count);
+    // pieces of such a length that all are at work at once, or that there are
+    // enough to spread
+    const int target = 2 * count <= a.slots ? a.slots - count : 2 * a.slots;
+    p.per = (int)max((all + target - 1) / target, (int64_t)kMinBlocks);
+    int wholes = 0;
+    for (int b0 = 0; b0 < a.nseq; b0 += 64) {
+        int t = t0, n = n0;
+        if (b0) look(b0 + lane, t, n);
+        wholes += (int)wave_sum((uint32_t)(t * (n / p.per)));
+    }
+    const bool is_rest = piece >= wholes;
+    int base = 0, rank = wholes;
+    for (int b0 = 0; b0 < a.nseq; b0 += 64) {
+        int t = t0, n = n0;
+        if (b0) look(b0 + lane, t, n);
+        const int whole = n / p.per, rest = n == 0 || n % p.per != 0;
+        const int wsum = base + prefix_sum(t * whole), rsum = rank + prefix_sum(t * rest);
+        const uint64_t past = __ballot((is_rest ? rsum : wsum) > piece);
         if (past) {
             const int l = __builtin_ctzll(past);
-            tiles = __builtin_amdgcn_readlane(tiles, l);
-            splits = __builtin_amdgcn_readlane(splits, l);
-            const int local = piece - (__builtin_amdgcn_readlane(sum, l) - tiles * splits);
+            const int tiles = __builtin_amdgcn_readlane(t, l);
+            const int w = __builtin_amdgcn_readlane(whole, l), r = __builtin_amdgcn_readlane(rest, l);
+            const int first = __builtin_amdgcn_readlane(wsum, l) - tiles * w;
+            const int left = __builtin_amdgcn_readlane(rsum, l) - tiles * r;
             p.b = b0 + l;
-            p.tile = local / splits;
-            p.split = local % splits;
-            p.first = piece - p.split;
+            p.tile = is_rest ? piece - left : (piece - first) / w;
+            p.split = is_rest ? w : (piece - first) % w;
+            p.whole = w;
+            p.first = first + p.tile * w;
+            p.rest = r ? left + p.tile : -1;
             return true;
         }
-        base = __builtin_amdgcn_readlane(sum, 63);
+        base = __builtin_amdgcn_readlane(wsum, 63);
+        rank = __builtin_amdgcn_readlane(rsum, 63);
     }
     return false;
 }
@@ -217,12 +251,19 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
         pc.tile = (int)(number - tile_base(a, pc.b));
         pc.per = INT32_MAX;
     }
-    const Seq sq = seq_of(a, pc.b);
+    pc.b = uniform(pc.b);
+    pc.tile = uniform(pc.tile);
+    pc.split = uniform(pc.split);
+    Seq sq = seq_of(a, pc.b);
+    sq.row0 = uniform(sq.row0);
+    sq.shift = uniform(sq.shift);
+    sq.count = uniform(sq.count);
+    sq.cap = uniform(sq.cap);
     if (pc.tile < 0 || pc.tile >= tiles_of(a, sq)) return;
     const int64_t x0 = (int64_t)pc.tile * kTile, rows = (int64_t)sq.count * a.group;
     const int64_t x1 = min(x0 + kTile, rows);
-    const int high = __builtin_amdgcn_readfirstlane(last_of(a, sq, (x1 - 1) / a.group));
-    const int low = __builtin_amdgcn_readfirstlane(last_of(a, sq, x0 / a.group));
+    const int high = uniform(last_of(a, sq, (x1 - 1) / a.group));
+    const int low = uniform(last_of(a, sq, x0 / a.group));
     const Span sp = span_of(a, low, high);
     int pieces = 1, j0 = 0, j1 = sp.total;
     if (a.split) {
@@ -230,21 +271,23 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
         if (pc.split >= pieces) return;
         j0 = pc.split * pc.per;
         j1 = min(j0 + pc.per, sp.total);
-        if (pc.split == 0 && kvh == 0 && threadIdx.x == 0) a.info[number] = make_int2(pc.first, pieces);
+        if (pc.split == 0 && kvh == 0 && threadIdx.x == 0)
+            a.info[number] = make_int4(pc.first, pc.whole, pc.rest, pieces);
     }
 
     // the wave's rows: column c * 16 + r is query row `row[c]` of the sequence
     const int64_t w0 = x0 + wave * (16 * kCols), w1 = min(w0 + 16 * kCols, x1);
     const bool busy = w0 < w1;
-    const int wave_high = busy ? __builtin_amdgcn_readfirstlane(last_of(a, sq, (w1 - 1) / a.group)) : -1;
-    const int wave_low = busy ? __builtin_amdgcn_readfirstlane(last_of(a, sq, w0 / a.group)) : -1;
-    int last[kCols];
+    const int wave_high = busy ? uniform(last_of(a, sq, (w1 - 1) / a.group)) : -1;
+    const int wave_low = busy ? uniform(last_of(a, sq, w0 / a.group)) : -1;
+    int last[kCols], below[kCols];  // sees positions above `below` up to `last`, and the sinks
     u32x4_t qf[kCols][NC];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
         const int64_t x = w0 + c * 16 + r;
         const bool in = x < w1;
         last[c] = in ? last_of(a, sq, x / a.group) : -1;
+        below[c] = a.window > 0 ? last[c] - a.window : -1;
         const char *row = a.q + ((sq.row0 + x / a.group) * a.q_row +
                                  (kvh * a.group + x % a.group) * a.q_head) * ES;
 #pragma unroll
@@ -307,9 +350,11 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     };
     // whether rows with last positions from lo to hi see all of a block
     auto whole = [&](int pos, int lo, int hi) {
-        return pos + kKvBlock - 1 <= lo &&
-               (a.window == 0 || pos > hi - a.window || pos + kKvBlock <= a.sinks);
+        return (pos + kKvBlock - 1 <= lo) &
+               ((a.window == 0) | (pos > hi - a.window) | (pos + kKvBlock <= a.sinks));
     };
+    const int tile_below = a.window > 0 ? low - a.window : -1;
+    auto hides = [&](int p, int lst, int blw) { return (p > lst) | ((p <= blw) & (p >= a.sinks)); };
     u32x4_t stage[MINE];
     auto load_step = [&](const Step &s) {
 #pragma unroll
@@ -347,8 +392,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
                     for (int e = 0; e < E; ++e) {
                         const int h = ST ? e / 4 : z / (4 * D);
                         const int p = pos + 16 * h + 4 * (z & 3) + (e & 3);
-                        const bool hidden =
-                            p > high || (a.window > 0 && p <= low - a.window && p >= a.sinks);
+                        const bool hidden = hides(p, high, tile_below);
                         if constexpr (ST) {
                             const uint32_t mask = e % 2 ? 0xFFFF0000u : 0xFFFFu;
                             const uint32_t inf = e % 2 ? 0x7F800000u : 0x7F80u;
@@ -427,9 +471,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
                             const int p = cur.pos[b] + 16 * h + 4 * g + i;
 #pragma unroll
                             for (int c = 0; c < kCols; ++c)
-                                if (p > last[c] ||
-                                    (a.window > 0 && p <= last[c] - a.window && p >= a.sinks))
-                                    s[b][h][c][i] = kNone;
+                                s[b][h][c][i] = hides(p, last[c], below[c]) ? kNone : s[b][h][c][i];
                         }
             }
 #pragma unroll
@@ -442,7 +484,9 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
 #pragma unroll
                         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][h][c][i]);
                 top = column_max(top);
-                if (__ballot(top > m[c])) {
+                // (a maximum is let stand until one is kSlack above it in powers of two: the
+                // weights may be that much larger than 1, and the sums are seldom rescaled)
+                if (__ballot(__builtin_fmaf(top, a.scale2, -ms[c]) > (m[c] == kNone ? kNone : kSlack))) {
                     const float mn = fmaxf(m[c], top);
                     const float msn = mn == kNone ? 0.f : mn * a.scale2;
                     const float f = mn == m[c] ? 1.f : m[c] == kNone ? 0.f : __builtin_amdgcn_exp2f(ms[c] - msn);
@@ -520,8 +564,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
 #pragma unroll 1
                         for (int t = 0; t < kKvBlock; ++t) {
                             const int p = cur.pos[b] + t;
-                            if (p > last[c] || (a.window > 0 && p <= last[c] - a.window && p >= a.sinks))
-                                continue;
+                            if (hides(p, last[c], below[c])) continue;
                             const float w = lds_p[wave][t][r];
 #pragma unroll
                             for (int d = 0; d < ND; ++d)
@@ -568,7 +611,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
                 a.lse[row * a.heads + head] =
                     l[c] == 0.f ? kNone : (ms[c] + __builtin_amdgcn_logf(l[c])) * kLn2;
         } else {
-            const int64_t slot = ((int64_t)(pc.first + pc.split) * a.kv_heads + kvh) * kTile + (x - x0);
+            const int64_t slot = (at * a.kv_heads + kvh) * kTile + (x - x0);
 #pragma unroll
             for (int d = 0; d < ND; ++d)
                 *(f32x4_t *)(a.part_o + slot * D + d * 16 + g * 4) = o[c][d];
@@ -577,11 +620,16 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     }
 }
 
-// Joins the pieces of a tile, in their order: a workgroup per kJoinRows rows.
+// Joins the pieces of a tile: a workgroup per kJoinRows rows, whose waves take the
+// pieces in turn, several at once.
 template <int ST, int D>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
-    constexpr int NR = (D + 63) / 64;
+    constexpr int L = D <= 16 ? 4 : D <= 32 ? 8 : D <= 64 ? 16 : D <= 128 ? 32 : 64;  // lanes per row
+    constexpr int P = 64 / L;          // pieces per wave at once
+    constexpr int LD = L * 4 + 4;
     constexpr float kNone = -__builtin_huge_valf();
+    __shared__ __align__(16) float lds_o[kWaves][kJoinRows][LD];
+    __shared__ float lds_l[kWaves][kJoinRows];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr int kParts = kTile / kJoinRows;
@@ -592,43 +640,82 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     const int tile = (int)(number - tile_base(a, b));
     const Seq sq = seq_of(a, b);
     if (tile < 0 || tile >= tiles_of(a, sq)) return;
-    const int2 f = a.info[number];
-    if (f.y <= 1) return;
-    for (int j = wave; j < kJoinRows; j += kWaves) {
-        const int local = part * kJoinRows + j;
-        const int64_t x = (int64_t)tile * kTile + local;
-        if (x >= (int64_t)sq.count * a.group) return;
-        auto slot_of = [&](int s) { return ((int64_t)(f.x + s) * a.kv_heads + kvh) * kTile + local; };
-        float top = kNone, sum = 0.f, acc[NR];
-        for (int s = lane; s < f.y; s += 64) top = fmaxf(top, a.part_ml[slot_of(s)].x);
-        top = wave_max(top);
-        const float ms = top == kNone ? 0.f : top;
+    const int64_t x0 = (int64_t)tile * kTile + part * kJoinRows;
+    const int rows = (int)min((int64_t)sq.count * a.group - x0, (int64_t)kJoinRows);
+    if (rows <= 0) return;
+    const int4 f = a.info[number];
+    const int cnt = f.w;
+    if (cnt <= 1) return;
+    auto slot_of = [&](int s, int j) {
+        const int piece = s < f.y ? f.x + s : f.z;
+        return ((int64_t)piece * a.kv_heads + kvh) * kTile + part * kJoinRows + j;
+    };
+    float ms[kJoinRows], sum[kJoinRows];
+    f32x4_t acc[kJoinRows];
 #pragma unroll
-        for (int i = 0; i < NR; ++i) acc[i] = 0.f;
-        for (int s = 0; s < f.y; ++s) {
-            const int64_t slot = slot_of(s);
-            const float2 ml = a.part_ml[slot];
-            const float w = __builtin_amdgcn_exp2f(ml.x - ms);
-            sum += w * ml.y;
-#pragma unroll
-            for (int i = 0; i < NR; ++i)
-                acc[i] += w * a.part_o[slot * D + min(lane + 64 * i, D - 1)];
-        }
-        const int64_t row = sq.row0 + x / a.group;
-        const int head = kvh * a.group + (int)(x % a.group);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-            if (lane + 64 * i < D) {
-                const int64_t to = row * a.o_row + head * a.o_head + lane + 64 * i;
-                if constexpr (ST)
-                    ((__bf16 *)a.out)[to] = (__bf16)(acc[i] * inv);
-                else
-                    ((float *)a.out)[to] = acc[i] * inv;
-            }
-        if (a.lse && lane == 0)
-            a.lse[row * a.heads + head] = sum == 0.f ? kNone : (ms + __builtin_amdgcn_logf(sum)) * kLn2;
+    for (int j = 0; j < kJoinRows; ++j) {
+        ms[j] = kNone;
+        sum[j] = 0.f;
+        acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
+    for (int s = lane; s < cnt; s += 64)
+#pragma unroll
+        for (int j = 0; j < kJoinRows; ++j)
+            ms[j] = fmaxf(ms[j], a.part_ml[slot_of(s, min(j, rows - 1))].x);
+#pragma unroll
+    for (int j = 0; j < kJoinRows; ++j) {
+        ms[j] = wave_max(ms[j]);
+        ms[j] = ms[j] == kNone ? 0.f : ms[j];
+    }
+    const int at = min(lane % L * 4, D - 4);
+#pragma unroll 2
+    for (int s = wave * P + lane / L; s < cnt; s += kWaves * P) {
+#pragma unroll
+        for (int j = 0; j < kJoinRows; ++j) {
+            const int64_t slot = slot_of(s, min(j, rows - 1));
+            const float2 ml = a.part_ml[slot];
+            const f32x4_t o = *(const f32x4_t *)(a.part_o + slot * D + at);
+            const float w = __builtin_amdgcn_exp2f(ml.x - ms[j]);
+            sum[j] = __builtin_fmaf(w, ml.y, sum[j]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_fmaf(w, o[i], acc[j][i]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kJoinRows; ++j) {
+#pragma unroll
+        for (int d = L; d < 64; d *= 2) {
+            sum[j] += __shfl_xor(sum[j], d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], d);
+        }
+        if (lane < L) *(f32x4_t *)&lds_o[wave][j][lane * 4] = acc[j];
+        if (lane == 0) lds_l[wave][j] = sum[j];
+    }
+    __syncthreads();
+    // a wave per row
+    static_assert(kJoinRows == kWaves, "");
+    if (wave >= rows) return;
+    float l = 0.f, top = ms[0];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) l += lds_l[w][wave];
+#pragma unroll
+    for (int j = 1; j < kJoinRows; ++j) top = wave == j ? ms[j] : top;
+    const int64_t x = x0 + wave, row = sq.row0 + x / a.group;
+    const int head = kvh * a.group + (int)(x % a.group);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int d = lane; d < D; d += 64) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) y += lds_o[w][wave][d];
+        const int64_t to = row * a.o_row + head * a.o_head + d;
+        if constexpr (ST)
+            ((__bf16 *)a.out)[to] = (__bf16)(y * inv);
+        else
+            ((float *)a.out)[to] = y * inv;
+    }
+    if (a.lse && lane == 0)
+        a.lse[row * a.heads + head] = l == 0.f ? kNone : (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 template <int ST, int D>
@@ -737,16 +824,17 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     a.split = a.tiles * a.kv_heads < 4 * kv->num_cu && s->nseq <= vs::kSplitSeqs && most > vs::kMinBlocks;
     int64_t wgs = a.tiles * a.kv_heads;
     if (a.split) {
-        a.target = (int)std::max<int64_t>(1, 4 * kv->num_cu / a.kv_heads);
-        const int64_t pieces = a.target + a.tiles, slots = pieces * a.kv_heads * vs::kTile;
+        const int at_once = kv->head_dim <= (e == 2 ? 192 : 128) ? 2 : 1;
+        a.slots = (int)std::max<int64_t>(1, at_once * kv->num_cu / a.kv_heads);
+        const int64_t pieces = 2 * a.slots + a.tiles, slots = pieces * a.kv_heads * vs::kTile;
         const size_t o_bytes = (size_t)slots * kv->head_dim * sizeof(float);
         const size_t ml_bytes = (size_t)slots * sizeof(float2);
         void *ws = nullptr;
-        rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)a.tiles * sizeof(int2), &ws);
+        rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)a.tiles * sizeof(int4), &ws);
         if (rc) return rc;
         a.part_o = (float *)ws;
+        a.info = (int4 *)((char *)ws + o_bytes + ml_bytes);
         a.part_ml = (float2 *)((char *)ws + o_bytes);
-        a.info = (int2 *)((char *)ws + o_bytes + ml_bytes);
         wgs = pieces * a.kv_heads;
     }
     if (!vs::grid_ok(wgs, 64 * vs::kWaves))
