@@ -224,6 +224,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     constexpr int ES = 16 / E;           // element size
     constexpr int NC = (D / E + 3) / 4;  // 16-byte pieces per lane of a key row
     constexpr int ND = D / 16;
+    constexpr int VF = ND;               // 16-byte pieces per lane of a block's (fp32: a half's) values
     constexpr int SB = blocks_at_once(ST, D);
     constexpr int BLOCK = kKvBlock * D * ES;         // bytes of a block's keys
     constexpr int LOADS = SB * 2 * BLOCK / 1024;     // of 16 bytes per lane, all waves
@@ -311,32 +312,42 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
         for (int d = 0; d < ND; ++d) o[c][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // The blocks in order: 64 at a time, lane i looks the page of the i-th up, and
-    // those that have one are a bit mask.
+    // The blocks in order: 64 at a time, lane i looks the i-th up (where it lies, its
+    // first position), and those that are on a page are a bit mask.
     const int32_t *trow = a.table + (int64_t)pc.b * a.width;
     char *const head_base = a.pool + a.layer_off + (int64_t)kvh * a.head_off;
-    const int bpp1 = (1 << (a.page_shift - 5)) - 1;
-    auto block_pos = [&](int j) { return (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock; };
-    int chunk = j0 - 64, pages = -1;
+    int chunk = j0 - 64, at_pos = 0;
+    uint32_t at_low = 0, at_high = 0;
     uint64_t ready = 0;
     auto next_block = [&](const char *&kb, int &pos) {
         while (!ready) {
             chunk += 64;
             if (chunk >= j1) return false;
-            pages = -1;
-            if (chunk + lane < j1) pages = trow[block_pos(chunk + lane) >> a.page_shift];
-            ready = __ballot((unsigned)pages < (unsigned)a.npages);
+            const int j = min(chunk + lane, j1 - 1);
+            at_pos = (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock;
+            const int page = trow[at_pos >> a.page_shift];
+            const int64_t off = (int64_t)page * a.page_bytes +
+                                (int64_t)(at_pos & ((1 << a.page_shift) - 1)) * (D * ES);
+            at_low = (uint32_t)off;
+            at_high = (uint32_t)(off >> 32);
+            ready = __ballot(chunk + lane < j1 && (unsigned)page < (unsigned)a.npages);
         }
         const int i = __builtin_ctzll(ready);
         ready &= ready - 1;
-        pos = block_pos(chunk + i);
-        kb = head_base + (int64_t)__builtin_amdgcn_readlane(pages, i) * a.page_bytes +
-             ((pos >> 5) & bpp1) * BLOCK;
+        pos = __builtin_amdgcn_readlane(at_pos, i);
+        kb = head_base + ((int64_t)__builtin_amdgcn_readlane((int)at_high, i) << 32 |
+                          (uint32_t)__builtin_amdgcn_readlane((int)at_low, i));
         return true;
     };
     struct Step {
         const char *kb[SB];
         int pos[SB];  // first positions; past all rows' where there is no block
+        bool all;     // every row of the tile sees all of it
+    };
+    // whether rows with last positions from lo to hi see all of a block
+    auto whole = [&](int pos, int lo, int hi) {
+        return (pos + kKvBlock - 1 <= lo) &
+               ((a.window == 0) | (pos > hi - a.window) | (pos + kKvBlock <= a.sinks));
     };
     auto next_step = [&](Step &s) {
         if (!next_block(s.kb[0], s.pos[0])) return false;
@@ -346,68 +357,78 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
                 s.kb[b] = s.kb[0];
                 s.pos[b] = INT32_MAX - kKvBlock;
             }
+        s.all = true;
+#pragma unroll
+        for (int b = 0; b < SB; ++b) s.all &= whole(s.pos[b], low, high);
         return true;
-    };
-    // whether rows with last positions from lo to hi see all of a block
-    auto whole = [&](int pos, int lo, int hi) {
-        return (pos + kKvBlock - 1 <= lo) &
-               ((a.window == 0) | (pos > hi - a.window) | (pos + kKvBlock <= a.sinks));
     };
     const int tile_below = a.window > 0 ? low - a.window : -1;
     auto hides = [&](int p, int lst, int blw) { return (p > lst) | ((p <= blw) & (p >= a.sinks)); };
+    // Kilobyte x of a step's: of which block, keys or values, where in them.  (What
+    // does not go by the wave is known here.)
+    constexpr int KB = BLOCK / 1024;
+    auto kilobyte = [&](int i, int &b, int &kv, int &z) {
+        const int x = i * kWaves + wave;
+        b = 2 * KB % kWaves == 0 ? i * kWaves / (2 * KB) : x / (2 * KB);
+        kv = KB % kWaves == 0 ? i * kWaves / KB % 2 : x / KB % 2;
+        z = KB % kWaves == 0 ? i * kWaves % KB + wave : x % KB;
+        return LOADS % kWaves == 0 || x < LOADS;
+    };
     u32x4_t stage[MINE];
     auto load_step = [&](const Step &s) {
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
-            const int x = wave + i * kWaves;
-            if (LOADS % kWaves == 0 || x < LOADS) {
-                const int b = x / (2 * BLOCK / 1024), y = x % (2 * BLOCK / 1024);
-                const int kv = y / (BLOCK / 1024), z = y % (BLOCK / 1024);
-                const char *p = s.kb[0];
+            int b, kv, z;
+            if (!kilobyte(i, b, kv, z)) continue;
+            const char *p = s.kb[0];
 #pragma unroll
-                for (int k = 1; k < SB; ++k) p = b == k ? s.kb[k] : p;
-                stage[i] = *(const u32x4_t *)(p + (kv ? a.kv_off : 0) + z * 1024 + lane * 16);
-            }
+            for (int k = 1; k < SB; ++k) p = b == k ? s.kb[k] : p;
+            stage[i] = *(const u32x4_t *)(p + (kv ? a.kv_off : 0) + z * 1024 + lane * 16);
         }
     };
     // Positions that no row of the tile sees may hold anything, and 0 times a NaN
-    // is one: their values become 0.  Those that some rows see and others do not
-    // are looked through for what is not finite.
-    auto store_step = [&](const Step &s, char *buf, int step, int which) {
-        bool all = true;
-#pragma unroll
-        for (int b = 0; b < SB; ++b) all = all && whole(s.pos[b], low, high);
+    // is one: their values become 0.  So do those that are not finite where some
+    // rows see them and others do not; they are added by themselves.
+    auto clean_step = [&](const Step &s, int step) {
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
-            const int x = wave + i * kWaves;
-            if (LOADS % kWaves == 0 || x < LOADS) {
-                const int b = x / (2 * BLOCK / 1024), y = x % (2 * BLOCK / 1024);
-                if (!all && y >= BLOCK / 1024) {
-                    int pos = s.pos[0];
+            int b, kv, z;
+            if (!kilobyte(i, b, kv, z) || !kv) continue;
+            int pos = s.pos[0];
 #pragma unroll
-                    for (int k = 1; k < SB; ++k) pos = b == k ? s.pos[k] : pos;
-                    const int z = (y - BLOCK / 1024) * 64 + lane;  // 16-byte piece of the values
+            for (int k = 1; k < SB; ++k) pos = b == k ? s.pos[k] : pos;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const int h = ST ? e / 4 : z / (4 * D);
-                        const int p = pos + 16 * h + 4 * (z & 3) + (e & 3);
-                        const bool hidden = hides(p, high, tile_below);
-                        if constexpr (ST) {
-                            const uint32_t mask = e % 2 ? 0xFFFF0000u : 0xFFFFu;
-                            const uint32_t inf = e % 2 ? 0x7F800000u : 0x7F80u;
-                            if (hidden) stage[i][e / 2] &= ~mask;
-                            odd = odd || (stage[i][e / 2] & inf) == inf;
-                        } else {
-                            if (hidden) stage[i][e] = 0;
-                            odd = odd || (stage[i][e] & 0x7F800000u) == 0x7F800000u;
-                        }
-                    }
+            for (int e = 0; e < E; ++e) {
+                const int h = ST ? e / 4 : z / (KB / 2);
+                const bool hidden = hides(pos + 16 * h + 4 * (lane & 3) + (e & 3), high, tile_below);
+                if constexpr (ST) {
+                    const uint32_t mask = e % 2 ? 0xFFFF0000u : 0xFFFFu;
+                    const uint32_t inf = e % 2 ? 0x7F800000u : 0x7F80u;
+                    const bool bad = (stage[i][e / 2] & inf) == inf;
+                    odd |= bad & !hidden;
+                    stage[i][e / 2] &= hidden | bad ? ~mask : ~0u;
+                } else {
+                    const bool bad = (stage[i][e] & 0x7F800000u) == 0x7F800000u;
+                    odd |= bad & !hidden;
+                    stage[i][e] = hidden | bad ? 0 : stage[i][e];
                 }
-                *(u32x4_t *)(buf + x * 1024 + lane * 16) = stage[i];
             }
         }
-        if (odd) flagged[which] = step;
+        if (odd) flagged[step & 1] = step;
+    };
+    // Values go to LDS with a piece's lane group turned by its dimension, so that
+    // the 16 lanes of a group, which read pieces 64 bytes apart, meet all banks.
+    const int k_at = lane * 16, v_at = (lane ^ (lane >> 4)) * 16;
+    auto store_step = [&](const Step &s, int step) {
+        if (!s.all) clean_step(s, step);
+        char *buf = lds + (step & 1) * (SB * 2 * BLOCK);
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            int b, kv, z;
+            if (!kilobyte(i, b, kv, z)) continue;
+            *(u32x4_t *)(buf + (b * 2 + kv) * BLOCK + z * 1024 + (kv ? v_at : k_at)) = stage[i];
+        }
     };
 
     if (threadIdx.x < 2) flagged[threadIdx.x] = -1;
@@ -416,7 +437,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     bool more = next_step(cur);
     if (more) {
         load_step(cur);
-        store_step(cur, lds, 0, 0);
+        store_step(cur, 0);
     }
     __syncthreads();
     for (int step = 0; more; ++step) {
@@ -431,36 +452,58 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
             none = none && cur.pos[b] > wave_high;
         }
         if (busy && !none) {
-            // S^T = K Q^T
+            // S^T = K Q^T, a half of a block at a time; the keys of the next two halves
+            // are on their way meanwhile
             f32x4_t s[SB][2][kCols];
+            u32x4_t kf[2][NC], vf[VF];
+            auto load_keys = [&](int x) {
 #pragma unroll
-            for (int b = 0; b < SB; ++b)
+                for (int i = 0; i < NC; ++i) {
+                    // (a piece past the row's end is read again and zeroed)
+                    const int piece = D % (4 * E) ? min(i * 4 + g, D / E - 1) : i * 4 + g;
+                    kf[x & 1][i] = *(const u32x4_t *)(buf + (x >> 1) * 2 * BLOCK +
+                                                      (((x & 1) * (D / E) + piece) * 16 + r) * 16);
+                }
+            };
+            const int v_lane = (r * 4 + (g ^ (r >> 2))) * 16;
+            auto load_value = [&](int x, int i) {
+                const int b = x / (ST ? 1 : 2), h = ST ? 0 : x % 2;
+                vf[i] = *(const u32x4_t *)(buf + b * 2 * BLOCK + BLOCK + h * (BLOCK / 2) +
+                                           i * 1024 + v_lane);
+            };
+            load_keys(0);
+            load_keys(1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+            for (int x = 0; x < 2 * SB; ++x) {
 #pragma unroll
-                    for (int c = 0; c < kCols; ++c) s[b][h][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                for (int c = 0; c < kCols; ++c) s[x >> 1][x & 1][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < NC; ++i) {
-                        // (a piece past the row's end is read again and zeroed)
-                        const int piece = D % (4 * E) ? min(i * 4 + g, D / E - 1) : i * 4 + g;
-                        u32x4_t kf = *(const u32x4_t *)(buf + b * 2 * BLOCK +
-                                                        ((h * (D / E) + piece) * 16 + r) * 16);
-                        if (D % (4 * E) && i == NC - 1 && i * 4 + g >= D / E) kf = u32x4_t{0, 0, 0, 0};
+                for (int i = 0; i < NC; ++i) {
+                    u32x4_t k = kf[x & 1][i];
+                    if (D % (4 * E) && i == NC - 1 && i * 4 + g >= D / E) k = u32x4_t{0, 0, 0, 0};
 #pragma unroll
-                        for (int c = 0; c < kCols; ++c) {
-                            if constexpr (ST) {
-                                s[b][h][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                    __builtin_bit_cast(bf16x8_t, kf),
-                                    __builtin_bit_cast(bf16x8_t, qf[c][i]), s[b][h][c], 0, 0, 0);
-                            } else {
+                    for (int c = 0; c < kCols; ++c) {
+                        f32x4_t &t = s[x >> 1][x & 1][c];
+                        if constexpr (ST) {
+                            t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                __builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, qf[c][i]),
+                                t, 0, 0, 0);
+                        } else {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    s[b][h][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                        float_of(kf[e]), float_of(qf[c][i][e]), s[b][h][c], 0, 0, 0);
-                            }
+                            for (int e = 0; e < 4; ++e)
+                                t = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    float_of(k[e]), float_of(qf[c][i][e]), t, 0, 0, 0);
                         }
                     }
                 }
+                if (x + 2 < 2 * SB) load_keys(x + 2);
+                if (x == 2 * SB - 2) {  // (the values' latency passes behind the softmax)
+#pragma unroll
+                    for (int i = 0; i < VF; ++i) load_value(0, i);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (!clear) {
 #pragma unroll
                 for (int b = 0; b < SB; ++b)
@@ -510,44 +553,49 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
                             l[c] += p;
                         }
             }
-            // O^T += V^T P^T
-            if (clear || flagged[step & 1] != step) {
+            // O^T += V^T P^T; a piece of values is replaced by the next block's as soon
+            // as it is multiplied
+            if constexpr (ST) {
+                bf16x8_t p[SB][kCols];
 #pragma unroll
-                for (int b = 0; b < SB; ++b) {
-                    const char *vb = buf + b * 2 * BLOCK + BLOCK;
-                    if constexpr (ST) {
-                        bf16x8_t p[kCols];
+                for (int b = 0; b < SB; ++b)
 #pragma unroll
-                        for (int c = 0; c < kCols; ++c)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) p[c][4 * h + i] = (__bf16)s[b][h][c][i];
-#pragma unroll
-                        for (int d = 0; d < ND; ++d) {
-                            const bf16x8_t vf = __builtin_bit_cast(
-                                bf16x8_t, *(const u32x4_t *)(vb + ((d * 16 + r) * 4 + g) * 16));
-#pragma unroll
-                            for (int c = 0; c < kCols; ++c)
-                                o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, p[c], o[c][d], 0, 0, 0);
-                        }
-                    } else {
+                    for (int c = 0; c < kCols; ++c)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int d = 0; d < ND; ++d) {
-                                const u32x4_t vf =
-                                    *(const u32x4_t *)(vb + h * (BLOCK / 2) + ((d * 16 + r) * 4 + g) * 16);
+                            for (int i = 0; i < 4; ++i) p[b][c][4 * h + i] = (__bf16)s[b][h][c][i];
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
+                for (int b = 0; b < SB; ++b)
 #pragma unroll
-                                    for (int c = 0; c < kCols; ++c)
-                                        o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                            float_of(vf[i]), s[b][h][c][i], o[c][d], 0, 0, 0);
-                            }
+                    for (int d = 0; d < ND; ++d) {
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c)
+                            o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                __builtin_bit_cast(bf16x8_t, vf[d]), p[b][c], o[c][d], 0, 0, 0);
+                        if (b + 1 < SB) {
+                            load_value(b + 1, d);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
-                }
             } else {
+#pragma unroll
+                for (int x = 0; x < 2 * SB; ++x)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int c = 0; c < kCols; ++c)
+                                o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    float_of(vf[d][i]), s[x >> 1][x & 1][c][i], o[c][d], 0, 0, 0);
+                        if (x + 1 < 2 * SB) {
+                            load_value(x + 1, d);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+            }
+            if (!cur.all && flagged[step & 1] == step) {
                 // Values that are not finite, seen by some rows and not by others: a
                 // position at a time, only where it is seen.
 #pragma unroll
@@ -560,29 +608,29 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
 #pragma unroll
                             for (int i = 0; i < 4; ++i) lds_p[wave][16 * h + 4 * g + i][r] = s[b][h][c][i];
                         lds_wave_sync();
-                        const char *vb = buf + b * 2 * BLOCK + BLOCK;
+                        const char *vb = cur.kb[b] + a.kv_off;
 #pragma unroll 1
                         for (int t = 0; t < kKvBlock; ++t) {
-                            const int p = cur.pos[b] + t;
-                            if (hides(p, last[c], below[c])) continue;
+                            if (hides(cur.pos[b] + t, last[c], below[c])) continue;
                             const float w = lds_p[wave][t][r];
 #pragma unroll
                             for (int d = 0; d < ND; ++d)
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
                                     const int place = value_place<ST>(t, d * 16 + g * 4 + i, D);
-                                    float v;
+                                    uint32_t v;
                                     if constexpr (ST)
-                                        v = float_of((uint32_t)((const uint16_t *)vb)[place] << 16);
+                                        v = (uint32_t)((const uint16_t *)vb)[place] << 16;
                                     else
-                                        v = ((const float *)vb)[place];
-                                    o[c][d][i] = __builtin_fmaf(w, v, o[c][d][i]);
+                                        v = ((const uint32_t *)vb)[place];
+                                    if ((v & 0x7F800000u) == 0x7F800000u)
+                                        o[c][d][i] = __builtin_fmaf(w, float_of(v), o[c][d][i]);
                                 }
                         }
                     }
             }
         }
-        if (more) store_step(nxt, lds + ((step + 1) & 1) * (SB * 2 * BLOCK), step + 1, (step + 1) & 1);
+        if (more) store_step(nxt, step + 1);
         cur = nxt;
         __syncthreads();
     }
