@@ -12,11 +12,12 @@ namespace {
 
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kWaves = 4;
 constexpr int kCols = 2;                      // columns of 16 rows per wave
-constexpr int kTile = kWaves * kCols * 16;    // rows of queries per workgroup
+constexpr int kFew = 4, kMany = 8;            // waves per workgroup
+constexpr int rows_of(int waves) { return waves * kCols * 16; }  // of queries, in a tile
 constexpr int kMinBlocks = 8;                 // per piece of a tile's blocks, at least
 constexpr int kSplitSeqs = 384;               // sequences whose pieces each workgroup finds for itself
+constexpr int kWideDim = 128;                 // heads up to this size have an eight-wave kernel
 constexpr float kSlack = 8.f;                 // of a running maximum, in powers of two
 constexpr int kJoinRows = 4;                  // rows per workgroup of the join
 
@@ -36,6 +37,7 @@ struct ChunkArgs {
     uint32_t flip;               // sign bits of an element's word, where scale is below 0
     int causal, window, sinks;
     int q_vec;                   // rows readable in 16-byte pieces
+    int tile;                    // rows of queries per workgroup
     int64_t tiles;               // numbers of tiles, with gaps
     int split;                   // tiles are divided along the length
     int slots;                   // pieces at work at once, per key-value head
@@ -75,7 +77,7 @@ __device__ __forceinline__ Seq seq_of(const ChunkArgs &a, int b) {
 // Query rows are (row, query head of the group) pairs, the head counting faster, so
 // that a tile's rows share their keys and values whatever the group.
 __device__ __forceinline__ int tiles_of(const ChunkArgs &a, const Seq &s) {
-    return (int)(((int64_t)s.count * a.group + kTile - 1) / kTile);
+    return (int)(((int64_t)s.count * a.group + a.tile - 1) / a.tile);
 }
 
 // The last position that row x of sequence s sees.
@@ -87,7 +89,7 @@ __device__ __forceinline__ int last_of(const ChunkArgs &a, const Seq &s, int64_t
 // the sequences before it and leaves a gap of one at most.
 __device__ __forceinline__ int64_t tile_base(const ChunkArgs &a, int64_t b) {
     const int64_t from = a.starts ? min(max((int64_t)a.starts[b], (int64_t)0), a.nrows) : b;
-    return from * a.group / kTile + b;
+    return from * a.group / a.tile + b;
 }
 
 // The sequence whose tiles the number falls among: 64 of them are looked at at once.
@@ -126,7 +128,7 @@ __device__ __forceinline__ int most_blocks(const ChunkArgs &a, const Seq &s) {
     if (high < 0) return 0;
     const int nb = high / kKvBlock + 1;
     if (a.window <= 0) return nb;
-    const int64_t w = ((int64_t)a.window + kTile / a.group) / kKvBlock + 3 + a.sinks / kKvBlock;
+    const int64_t w = ((int64_t)a.window + a.tile / a.group) / kKvBlock + 3 + a.sinks / kKvBlock;
     return (int)min((int64_t)nb, w);
 }
 
@@ -156,19 +158,23 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
     int t0, n0;  // (all there is to read for up to 64 sequences)
     look(lane, t0, n0);
     int64_t all = (int64_t)t0 * n0;
-    int count = t0;
+    int count = t0, widest = n0;
     for (int b = lane + 64; b < a.nseq; b += 64) {
         int t, n;
         look(b, t, n);
         all += (int64_t)t * n;
         count += t;
+        widest = max(widest, n);
     }
     all = uniform(wave_sum64(all));
     count = (int)wave_sum((uint32_t)count);
-    // pieces of such a length that all are at work at once, or that there are
-    // enough to spread
+    widest = uniform((int)wave_max((float)widest));  // (past 2^24 off by two at most: a piece more)
+    // Pieces of such a length that all are at work at once where tiles are few;
+    // none at all where the longest is not what the call waits for; else enough of
+    // them to spread.
     const int target = 2 * count <= a.slots ? a.slots - count : 2 * a.slots;
     p.per = (int)max((all + target - 1) / target, (int64_t)kMinBlocks);
+    if (count >= a.slots && 4 * (int64_t)widest * a.slots <= 5 * all) p.per = max(p.per, widest + 2);
     int wholes = 0;
     for (int b0 = 0; b0 < a.nseq; b0 += 64) {
         int t = t0, n = n0;
@@ -218,8 +224,16 @@ constexpr int buffer_bytes(int st, int dim) {
     return blocks_at_once(st, dim) * 2 * kKvBlock * dim * (st ? 2 : 4);
 }
 
-template <int ST, int D>
-__global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_kernel(ChunkArgs a) {
+template <int ST, int D, int NW>
+__global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_kernel(ChunkArgs args) {
+    // (what only the loop's edges need is read from the arguments again: held in the
+    // scalar registers it would be moved out of them and back in every step)
+    const ChunkArgs &a = args;
+    const auto again = [] {
+        auto *p = (const __attribute__((address_space(4))) ChunkArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(p));
+        return p;
+    };
     constexpr int E = ST ? 8 : 4;
     constexpr int ES = 16 / E;           // element size
     constexpr int NC = (D / E + 3) / 4;  // 16-byte pieces per lane of a key row
@@ -228,11 +242,12 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     constexpr int SB = blocks_at_once(ST, D);
     constexpr int BLOCK = kKvBlock * D * ES;         // bytes of a block's keys
     constexpr int LOADS = SB * 2 * BLOCK / 1024;     // of 16 bytes per lane, all waves
-    constexpr int MINE = (LOADS + kWaves - 1) / kWaves;
+    constexpr int MINE = (LOADS + NW - 1) / NW;
+    constexpr int kTile = rows_of(NW);
     constexpr float kNone = -__builtin_huge_valf();
     extern __shared__ __align__(16) char lds[];  // two buffers: [block][keys, values]
     __shared__ int flagged[2];                   // the step whose values hold NaNs or infinities
-    __shared__ float lds_p[kWaves][kKvBlock][16];
+    __shared__ float lds_p[NW][kKvBlock][16];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -261,8 +276,8 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     sq.count = uniform(sq.count);
     sq.cap = uniform(sq.cap);
     if (pc.tile < 0 || pc.tile >= tiles_of(a, sq)) return;
-    const int64_t x0 = (int64_t)pc.tile * kTile, rows = (int64_t)sq.count * a.group;
-    const int64_t x1 = min(x0 + kTile, rows);
+    // (rows times heads fit 31 bits with a tile to spare)
+    const int x0 = pc.tile * kTile, x1 = min(x0 + kTile, sq.count * a.group);
     const int high = uniform(last_of(a, sq, (x1 - 1) / a.group));
     const int low = uniform(last_of(a, sq, x0 / a.group));
     const Span sp = span_of(a, low, high);
@@ -277,7 +292,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     }
 
     // the wave's rows: column c * 16 + r is query row `row[c]` of the sequence
-    const int64_t w0 = x0 + wave * (16 * kCols), w1 = min(w0 + 16 * kCols, x1);
+    const int w0 = x0 + wave * (16 * kCols), w1 = min(w0 + 16 * kCols, x1);
     const bool busy = w0 < w1;
     const int wave_high = busy ? uniform(last_of(a, sq, (w1 - 1) / a.group)) : -1;
     const int wave_low = busy ? uniform(last_of(a, sq, w0 / a.group)) : -1;
@@ -285,7 +300,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     u32x4_t qf[kCols][NC];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
-        const int64_t x = w0 + c * 16 + r;
+        const int x = w0 + c * 16 + r;
         const bool in = x < w1;
         last[c] = in ? last_of(a, sq, x / a.group) : -1;
         below[c] = a.window > 0 ? last[c] - a.window : -1;
@@ -314,7 +329,6 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
 
     // The blocks in order: 64 at a time, lane i looks the i-th up (where it lies, its
     // first position), and those that are on a page are a bit mask.
-    const int32_t *trow = a.table + (int64_t)pc.b * a.width;
     char *const head_base = a.pool + a.layer_off + (int64_t)kvh * a.head_off;
     int chunk = j0 - 64, at_pos = 0;
     uint32_t at_low = 0, at_high = 0;
@@ -325,12 +339,13 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
             if (chunk >= j1) return false;
             const int j = min(chunk + lane, j1 - 1);
             at_pos = (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock;
-            const int page = trow[at_pos >> a.page_shift];
-            const int64_t off = (int64_t)page * a.page_bytes +
-                                (int64_t)(at_pos & ((1 << a.page_shift) - 1)) * (D * ES);
+            const auto *a = again();
+            const int page = a->table[(int64_t)pc.b * a->width + (at_pos >> a->page_shift)];
+            const int64_t off = (int64_t)page * a->page_bytes +
+                                (int64_t)(at_pos & ((1 << a->page_shift) - 1)) * (D * ES);
             at_low = (uint32_t)off;
             at_high = (uint32_t)(off >> 32);
-            ready = __ballot(chunk + lane < j1 && (unsigned)page < (unsigned)a.npages);
+            ready = __ballot(chunk + lane < j1 && (unsigned)page < (unsigned)a->npages);
         }
         const int i = __builtin_ctzll(ready);
         ready &= ready - 1;
@@ -340,21 +355,21 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
         return true;
     };
     struct Step {
-        const char *kb[SB];
-        int pos[SB];  // first positions; past all rows' where there is no block
+        int pos[SB];  // blocks' first positions; past all rows' where there is none
         bool all;     // every row of the tile sees all of it
     };
+    const char *kb[SB];  // the next step's blocks
     // whether rows with last positions from lo to hi see all of a block
     auto whole = [&](int pos, int lo, int hi) {
         return (pos + kKvBlock - 1 <= lo) &
                ((a.window == 0) | (pos > hi - a.window) | (pos + kKvBlock <= a.sinks));
     };
     auto next_step = [&](Step &s) {
-        if (!next_block(s.kb[0], s.pos[0])) return false;
+        if (!next_block(kb[0], s.pos[0])) return false;
 #pragma unroll
         for (int b = 1; b < SB; ++b)
-            if (!next_block(s.kb[b], s.pos[b])) {
-                s.kb[b] = s.kb[0];
+            if (!next_block(kb[b], s.pos[b])) {
+                kb[b] = kb[0];
                 s.pos[b] = INT32_MAX - kKvBlock;
             }
         s.all = true;
@@ -368,21 +383,21 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     // does not go by the wave is known here.)
     constexpr int KB = BLOCK / 1024;
     auto kilobyte = [&](int i, int &b, int &kv, int &z) {
-        const int x = i * kWaves + wave;
-        b = 2 * KB % kWaves == 0 ? i * kWaves / (2 * KB) : x / (2 * KB);
-        kv = KB % kWaves == 0 ? i * kWaves / KB % 2 : x / KB % 2;
-        z = KB % kWaves == 0 ? i * kWaves % KB + wave : x % KB;
-        return LOADS % kWaves == 0 || x < LOADS;
+        const int x = i * NW + wave;
+        b = 2 * KB % NW == 0 ? i * NW / (2 * KB) : x / (2 * KB);
+        kv = KB % NW == 0 ? i * NW / KB % 2 : x / KB % 2;
+        z = KB % NW == 0 ? i * NW % KB + wave : x % KB;
+        return LOADS % NW == 0 || x < LOADS;
     };
     u32x4_t stage[MINE];
-    auto load_step = [&](const Step &s) {
+    auto load_step = [&]() {
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
             int b, kv, z;
             if (!kilobyte(i, b, kv, z)) continue;
-            const char *p = s.kb[0];
+            const char *p = kb[0];
 #pragma unroll
-            for (int k = 1; k < SB; ++k) p = b == k ? s.kb[k] : p;
+            for (int k = 1; k < SB; ++k) p = b == k ? kb[k] : p;
             stage[i] = *(const u32x4_t *)(p + (kv ? a.kv_off : 0) + z * 1024 + lane * 16);
         }
     };
@@ -418,8 +433,9 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
         if (odd) flagged[step & 1] = step;
     };
     // Values go to LDS with a piece's lane group turned by its dimension, so that
-    // the 16 lanes of a group, which read pieces 64 bytes apart, meet all banks.
-    const int k_at = lane * 16, v_at = (lane ^ (lane >> 4)) * 16;
+    // lanes that are served together, which read pieces 64 bytes apart, meet all
+    // banks (lanes 0 to 3, 12 to 15 and 20 to 27 are, and so on).
+    const int k_at = lane * 16, v_at = (lane ^ (-(lane >> 4) & 3)) * 16;
     auto store_step = [&](const Step &s, int step) {
         if (!s.all) clean_step(s, step);
         char *buf = lds + (step & 1) * (SB * 2 * BLOCK);
@@ -436,14 +452,14 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     Step cur;
     bool more = next_step(cur);
     if (more) {
-        load_step(cur);
+        load_step();
         store_step(cur, 0);
     }
     __syncthreads();
     for (int step = 0; more; ++step) {
         Step nxt;
         more = next_step(nxt);
-        if (more) load_step(nxt);
+        if (more) load_step();
         const char *buf = lds + (step & 1) * (SB * 2 * BLOCK);
         bool clear = true, none = true;
 #pragma unroll
@@ -465,7 +481,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
                                                       (((x & 1) * (D / E) + piece) * 16 + r) * 16);
                 }
             };
-            const int v_lane = (r * 4 + (g ^ (r >> 2))) * 16;
+            const int v_lane = (r * 4 + (g ^ (-(r >> 2) & 3))) * 16;
             auto load_value = [&](int x, int i) {
                 const int b = x / (ST ? 1 : 2), h = ST ? 0 : x % 2;
                 vf[i] = *(const u32x4_t *)(buf + b * 2 * BLOCK + BLOCK + h * (BLOCK / 2) +
@@ -608,7 +624,11 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
 #pragma unroll
                             for (int i = 0; i < 4; ++i) lds_p[wave][16 * h + 4 * g + i][r] = s[b][h][c][i];
                         lds_wave_sync();
-                        const char *vb = cur.kb[b] + a.kv_off;
+                        const auto *a = again();
+                        const int pos = min(cur.pos[b], high);  // (none is seen where there is no block)
+                        const char *vb = head_base + a->kv_off +
+                            (int64_t)a->table[(int64_t)pc.b * a->width + (pos >> a->page_shift)] * a->page_bytes +
+                            (int64_t)(pos & ((1 << a->page_shift) - 1) & ~(kKvBlock - 1)) * (D * ES);
 #pragma unroll 1
                         for (int t = 0; t < kKvBlock; ++t) {
                             if (hides(cur.pos[b] + t, last[c], below[c])) continue;
@@ -639,13 +659,14 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
     for (int c = 0; c < kCols; ++c) {
         l[c] += __shfl_xor(l[c], 16);
         l[c] += __shfl_xor(l[c], 32);
-        const int64_t x = w0 + c * 16 + r;
+        const int x = w0 + c * 16 + r;
         if (x >= w1) continue;
+        const auto *a = again();
         if (pieces == 1) {
-            const int64_t row = sq.row0 + x / a.group;
-            const int head = kvh * a.group + (int)(x % a.group);
+            const int64_t row = sq.row0 + x / a->group;
+            const int head = kvh * a->group + (int)(x % a->group);
             const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];
-            char *to = a.out + (row * a.o_row + head * a.o_head + g * 4) * ES;
+            char *to = a->out + (row * a->o_row + head * a->o_head + g * 4) * ES;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -655,15 +676,15 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
                     else
                         ((float *)to)[d * 16 + i] = o[c][d][i] * inv;
                 }
-            if (a.lse && g == 0)
-                a.lse[row * a.heads + head] =
+            if (a->lse && g == 0)
+                a->lse[row * a->heads + head] =
                     l[c] == 0.f ? kNone : (ms[c] + __builtin_amdgcn_logf(l[c])) * kLn2;
         } else {
-            const int64_t slot = (at * a.kv_heads + kvh) * kTile + (x - x0);
+            const int64_t slot = (at * a->kv_heads + kvh) * kTile + (x - x0);
 #pragma unroll
             for (int d = 0; d < ND; ++d)
-                *(f32x4_t *)(a.part_o + slot * D + d * 16 + g * 4) = o[c][d];
-            if (g == 0) a.part_ml[slot] = make_float2(m[c] == kNone ? kNone : ms[c], l[c]);
+                *(f32x4_t *)(a->part_o + slot * D + d * 16 + g * 4) = o[c][d];
+            if (g == 0) a->part_ml[slot] = make_float2(m[c] == kNone ? kNone : ms[c], l[c]);
         }
     }
 }
@@ -672,6 +693,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= (ST ? 192 : 128) ? 2 : 1) void ch
 // pieces in turn, several at once.
 template <int ST, int D>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
+    constexpr int kWaves = 4;
     constexpr int L = D <= 16 ? 4 : D <= 32 ? 8 : D <= 64 ? 16 : D <= 128 ? 32 : 64;  // lanes per row
     constexpr int P = 64 / L;          // pieces per wave at once
     constexpr int LD = L * 4 + 4;
@@ -680,7 +702,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     __shared__ float lds_l[kWaves][kJoinRows];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    constexpr int kParts = kTile / kJoinRows;
+    const int kTile = a.tile, kParts = kTile / kJoinRows;
     const int part = blockIdx.x % kParts;
     const int kvh = blockIdx.x / kParts % a.kv_heads;
     const int64_t number = blockIdx.x / kParts / a.kv_heads;
@@ -766,19 +788,27 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
         a.lse[row * a.heads + head] = l == 0.f ? kNone : (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <int ST, int D>
-hipError_t launch_chunk(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
+template <int ST, int D, int NW>
+hipError_t launch_tiles(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
     constexpr int lds = 2 * buffer_bytes(ST, D);
-    if constexpr (lds + sizeof(float) * kWaves * kKvBlock * 16 + 64 > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)chunk_kernel<ST, D>,
+    if constexpr (lds + sizeof(float) * NW * kKvBlock * 16 + 64 > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)chunk_kernel<ST, D, NW>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((chunk_kernel<ST, D>), dim3((uint32_t)wgs), dim3(64 * kWaves), lds, st, a);
-    hipError_t e = hipGetLastError();
+    hipLaunchKernelGGL((chunk_kernel<ST, D, NW>), dim3((uint32_t)wgs), dim3(64 * NW), lds, st, a);
+    return hipGetLastError();
+}
+
+template <int ST, int D>
+hipError_t launch_chunk(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
+    if constexpr (D <= kWideDim) {
+        if (a.tile == rows_of(kMany)) return launch_tiles<ST, D, kMany>(a, wgs, st);
+    }
+    const hipError_t e = launch_tiles<ST, D, kFew>(a, wgs, st);
     if (e != hipSuccess || !a.split) return e;
     hipLaunchKernelGGL((chunk_join_kernel<ST, D>),
-                       dim3((uint32_t)(a.tiles * a.kv_heads * (kTile / kJoinRows))), dim3(256), 0, st, a);
+                       dim3((uint32_t)(a.tiles * a.kv_heads * (a.tile / kJoinRows))), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -833,7 +863,7 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
         if (!vs::stride_ok(x)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
     if (s->nseq == 0 || nrows == 0) return VS_OK;
     if (!q || !out) return report(VS_ERR_INVALID, "null q or out");
-    if (nrows > INT32_MAX / group)
+    if (nrows > (INT32_MAX - 1024) / group)
         return report(VS_ERR_UNSUPPORTED, "%lld rows of %lld heads", (long long)nrows, (long long)heads);
     vs::DeviceGuard g(kv->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
@@ -867,14 +897,18 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     a.window = (int)std::min<int64_t>(window, INT32_MAX);
     a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX - 64);
     a.q_vec = vs::pieces_ok(q, q_row, q_head, e);
-    a.tiles = nrows * group / vs::kTile + s->nseq;
+    auto tiles_of = [&](int waves) { return nrows * group / vs::rows_of(waves) + s->nseq; };
     const int64_t most = s->width * (kv->page_size / vs::kKvBlock);
-    a.split = a.tiles * a.kv_heads < 4 * kv->num_cu && s->nseq <= vs::kSplitSeqs && most > vs::kMinBlocks;
+    const bool many = kv->head_dim <= vs::kWideDim && tiles_of(vs::kMany) * a.kv_heads >= 2 * kv->num_cu;
+    a.tile = vs::rows_of(many ? vs::kMany : vs::kFew);
+    a.tiles = tiles_of(many ? vs::kMany : vs::kFew);
+    a.split = !many && a.tiles * a.kv_heads < 4 * kv->num_cu && s->nseq <= vs::kSplitSeqs &&
+              most > vs::kMinBlocks;
     int64_t wgs = a.tiles * a.kv_heads;
     if (a.split) {
         const int at_once = kv->head_dim <= (e == 2 ? 192 : 128) ? 2 : 1;
         a.slots = (int)std::max<int64_t>(1, at_once * kv->num_cu / a.kv_heads);
-        const int64_t pieces = 2 * a.slots + a.tiles, slots = pieces * a.kv_heads * vs::kTile;
+        const int64_t pieces = 2 * a.slots + a.tiles, slots = pieces * a.kv_heads * a.tile;
         const size_t o_bytes = (size_t)slots * kv->head_dim * sizeof(float);
         const size_t ml_bytes = (size_t)slots * sizeof(float2);
         void *ws = nullptr;
@@ -885,7 +919,7 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
         a.part_ml = (float2 *)((char *)ws + o_bytes);
         wgs = pieces * a.kv_heads;
     }
-    if (!vs::grid_ok(wgs, 64 * vs::kWaves))
+    if (!vs::grid_ok(wgs, 2 * a.tile))
         return report(VS_ERR_UNSUPPORTED, "%lld rows of %lld heads", (long long)nrows, (long long)heads);
     const hipError_t err = kv->dtype == VS_DTYPE_BF16
                                ? vs::launch_chunk_dim<1>(a, wgs, (int)kv->head_dim, st)
