@@ -18,7 +18,7 @@ constexpr int rows_of(int waves) { return waves * kCols * 16; }  // of queries, 
 constexpr int kMinBlocks = 8;                 // per piece of a tile's blocks, at least
 constexpr int kSplitSeqs = 384;               // sequences whose pieces each workgroup finds for itself
 constexpr int kWideDim = 128;                 // heads up to this size have an eight-wave kernel
-constexpr float kSlack = 8.f;                 // of a running maximum, in powers of two
+constexpr float kSlack = 256.f;               // the largest weight that is let stand
 constexpr int kJoinRows = 4;                  // rows per workgroup of the join
 
 struct ChunkArgs {
@@ -238,7 +238,6 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
     constexpr int ES = 16 / E;           // element size
     constexpr int NC = (D / E + 3) / 4;  // 16-byte pieces per lane of a key row
     constexpr int ND = D / 16;
-    constexpr int VF = ND;               // 16-byte pieces per lane of a block's (fp32: a half's) values
     constexpr int SB = blocks_at_once(ST, D);
     constexpr int BLOCK = kKvBlock * D * ES;         // bytes of a block's keys
     constexpr int LOADS = SB * 2 * BLOCK / 1024;     // of 16 bytes per lane, all waves
@@ -317,64 +316,82 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
         }
     }
 
-    float m[kCols], ms[kCols], l[kCols];  // running maximum, times scale2, and the lane's sum
+    // a column's reference (a score times scale2), whether it has none yet (then past
+    // kSlack), and the lane's sum
+    float ref[kCols], unset[kCols], l[kCols];
     f32x4_t o[kCols][ND];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
-        m[c] = kNone;
-        ms[c] = l[c] = 0.f;
+        ref[c] = l[c] = 0.f;
+        unset[c] = w0 + c * 16 + r < w1 ? 2.f * kSlack : 0.f;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[c][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // The blocks in order: 64 at a time, lane i looks the i-th up (where it lies, its
-    // first position), and those that are on a page are a bit mask.
+    // The blocks in order: 64 at a time, lane i looks the i-th up (where it lies; its
+    // first position, a multiple of 32, and below that what masks it needs), and
+    // those that are on a page are a bit mask.
+    constexpr int kTileWhole = 1;  // every row of the tile sees all of the block
+    constexpr int kWaveWhole = 2;  // every row of the wave does
+    constexpr int kWaveNone = 4;   // no row of the wave sees any of it
+    // no block: past all rows' positions
+    constexpr int kNoBlock = (INT32_MAX & ~(kKvBlock - 1)) - kKvBlock + kWaveNone;
     char *const head_base = a.pool + a.layer_off + (int64_t)kvh * a.head_off;
     int chunk = j0 - 64, at_pos = 0;
     uint32_t at_low = 0, at_high = 0;
     uint64_t ready = 0;
-    auto next_block = [&](const char *&kb, int &pos) {
-        while (!ready) {
-            chunk += 64;
-            if (chunk >= j1) return false;
-            const int j = min(chunk + lane, j1 - 1);
-            at_pos = (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock;
-            const auto *a = again();
-            const int page = a->table[(int64_t)pc.b * a->width + (at_pos >> a->page_shift)];
-            const int64_t off = (int64_t)page * a->page_bytes +
-                                (int64_t)(at_pos & ((1 << a->page_shift) - 1)) * (D * ES);
-            at_low = (uint32_t)off;
-            at_high = (uint32_t)(off >> 32);
-            ready = __ballot(chunk + lane < j1 && (unsigned)page < (unsigned)a->npages);
-        }
-        const int i = __builtin_ctzll(ready);
-        ready &= ready - 1;
-        pos = __builtin_amdgcn_readlane(at_pos, i);
-        kb = head_base + ((int64_t)__builtin_amdgcn_readlane((int)at_high, i) << 32 |
-                          (uint32_t)__builtin_amdgcn_readlane((int)at_low, i));
-        return true;
-    };
-    struct Step {
-        int pos[SB];  // blocks' first positions; past all rows' where there is none
-        bool all;     // every row of the tile sees all of it
-    };
-    const char *kb[SB];  // the next step's blocks
-    // whether rows with last positions from lo to hi see all of a block
     auto whole = [&](int pos, int lo, int hi) {
         return (pos + kKvBlock - 1 <= lo) &
                ((a.window == 0) | (pos > hi - a.window) | (pos + kKvBlock <= a.sinks));
     };
+    auto refill = [&]() {  // whether there are any left
+        do {
+            chunk += 64;
+            if (chunk >= j1) return false;
+            const auto *a = again();
+            const int j = min(chunk + lane, j1 - 1);
+            const int pos = (j < sp.nsb ? j : j - sp.nsb + sp.wb0) * kKvBlock;
+            const int page = a->table[(int64_t)pc.b * a->width + (pos >> a->page_shift)];
+            const uint64_t to = (uint64_t)(a->pool + a->layer_off + (int64_t)kvh * a->head_off +
+                                           (int64_t)page * a->page_bytes +
+                                           (int64_t)(pos & ((1 << a->page_shift) - 1)) * (D * ES));
+            at_low = (uint32_t)to;
+            at_high = (uint32_t)(to >> 32);
+            at_pos = pos | (whole(pos, low, high) ? kTileWhole : 0) |
+                     (whole(pos, wave_low, wave_high) ? kWaveWhole : 0) |
+                     (pos > wave_high ? kWaveNone : 0);
+            ready = __ballot((chunk + lane < j1) & ((unsigned)page < (unsigned)a->npages));
+        } while (!ready);
+        return true;
+    };
+    auto next_block = [&](const char *&kb, int &block) {
+        if (!ready && !refill()) return false;
+        const int i = __builtin_ctzll(ready);
+        ready &= ready - 1;
+        block = __builtin_amdgcn_readlane(at_pos, i);
+        kb = (const char *)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_high, i) << 32 |
+                            (uint32_t)__builtin_amdgcn_readlane((int)at_low, i));
+        return true;
+    };
+    struct Step {
+        int block[SB];
+    };
+    auto all_of = [](const Step &s, int flag) {
+        int x = s.block[0];
+#pragma unroll
+        for (int b = 1; b < SB; ++b) x &= s.block[b];
+        return (x & flag) != 0;
+    };
+    auto pos_of = [](const Step &s, int b) { return s.block[b] & ~(kKvBlock - 1); };
+    const char *kb[SB];  // the next step's blocks
     auto next_step = [&](Step &s) {
-        if (!next_block(kb[0], s.pos[0])) return false;
+        if (!next_block(kb[0], s.block[0])) return false;
 #pragma unroll
         for (int b = 1; b < SB; ++b)
-            if (!next_block(kb[b], s.pos[b])) {
+            if (!next_block(kb[b], s.block[b])) {
                 kb[b] = kb[0];
-                s.pos[b] = INT32_MAX - kKvBlock;
+                s.block[b] = kNoBlock;
             }
-        s.all = true;
-#pragma unroll
-        for (int b = 0; b < SB; ++b) s.all &= whole(s.pos[b], low, high);
         return true;
     };
     const int tile_below = a.window > 0 ? low - a.window : -1;
@@ -389,6 +406,8 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
         z = KB % NW == 0 ? i * NW % KB + wave : x % KB;
         return LOADS % NW == 0 || x < LOADS;
     };
+    const int64_t kv_off = a.kv_off;
+    const uint32_t lane_at = lane * 16;
     u32x4_t stage[MINE];
     auto load_step = [&]() {
 #pragma unroll
@@ -398,7 +417,8 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
             const char *p = kb[0];
 #pragma unroll
             for (int k = 1; k < SB; ++k) p = b == k ? kb[k] : p;
-            stage[i] = *(const u32x4_t *)(p + (kv ? a.kv_off : 0) + z * 1024 + lane * 16);
+            p += (kv ? kv_off : 0) + z * 1024;
+            stage[i] = *(const u32x4_t *)(p + lane_at);
         }
     };
     // Positions that no row of the tile sees may hold anything, and 0 times a NaN
@@ -410,9 +430,9 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
         for (int i = 0; i < MINE; ++i) {
             int b, kv, z;
             if (!kilobyte(i, b, kv, z) || !kv) continue;
-            int pos = s.pos[0];
+            int pos = pos_of(s, 0);
 #pragma unroll
-            for (int k = 1; k < SB; ++k) pos = b == k ? s.pos[k] : pos;
+            for (int k = 1; k < SB; ++k) pos = b == k ? pos_of(s, k) : pos;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int h = ST ? e / 4 : z / (KB / 2);
@@ -437,7 +457,7 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
     // banks (lanes 0 to 3, 12 to 15 and 20 to 27 are, and so on).
     const int k_at = lane * 16, v_at = (lane ^ (-(lane >> 4) & 3)) * 16;
     auto store_step = [&](const Step &s, int step) {
-        if (!s.all) clean_step(s, step);
+        if (!all_of(s, kTileWhole)) clean_step(s, step);
         char *buf = lds + (step & 1) * (SB * 2 * BLOCK);
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
@@ -461,157 +481,188 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
         more = next_step(nxt);
         if (more) load_step();
         const char *buf = lds + (step & 1) * (SB * 2 * BLOCK);
-        bool clear = true, none = true;
-#pragma unroll
-        for (int b = 0; b < SB; ++b) {
-            clear = clear && whole(cur.pos[b], wave_low, wave_high);
-            none = none && cur.pos[b] > wave_high;
-        }
-        if (busy && !none) {
-            // S^T = K Q^T, a half of a block at a time; the keys of the next two halves
-            // are on their way meanwhile
-            f32x4_t s[SB][2][kCols];
-            u32x4_t kf[2][NC], vf[VF];
-            auto load_keys = [&](int x) {
-#pragma unroll
-                for (int i = 0; i < NC; ++i) {
-                    // (a piece past the row's end is read again and zeroed)
-                    const int piece = D % (4 * E) ? min(i * 4 + g, D / E - 1) : i * 4 + g;
-                    kf[x & 1][i] = *(const u32x4_t *)(buf + (x >> 1) * 2 * BLOCK +
-                                                      (((x & 1) * (D / E) + piece) * 16 + r) * 16);
-                }
+        const bool clear = all_of(cur, kWaveWhole), none = all_of(cur, kWaveNone);
+        if (!none) {  // (nor does a wave without rows)
+            // One block's products beside another's softmax: S^T = K Q^T of the second
+            // while the first's exponentials are taken, O^T += V^T P^T of the first
+            // beside the second's.  Pieces of keys and values are replaced by the next
+            // block's as soon as they are multiplied.
+            f32x4_t s[SB][2][kCols], w[SB][2][kCols];
+            bf16x8_t pb[ST ? SB : 1][kCols];
+            u32x4_t kf[2][NC], vf[ND];
+            auto load_key = [&](int b, int h, int i) {
+                // (a piece past the row's end is read again and zeroed)
+                const int piece = D % (4 * E) ? min(i * 4 + g, D / E - 1) : i * 4 + g;
+                kf[h][i] = *(const u32x4_t *)(buf + b * 2 * BLOCK + ((h * (D / E) + piece) * 16 + r) * 16);
+                if (D % (4 * E) && i == NC - 1 && i * 4 + g >= D / E) kf[h][i] = u32x4_t{0, 0, 0, 0};
             };
             const int v_lane = (r * 4 + (g ^ (-(r >> 2) & 3))) * 16;
-            auto load_value = [&](int x, int i) {
-                const int b = x / (ST ? 1 : 2), h = ST ? 0 : x % 2;
-                vf[i] = *(const u32x4_t *)(buf + b * 2 * BLOCK + BLOCK + h * (BLOCK / 2) +
-                                           i * 1024 + v_lane);
+            auto load_value = [&](int x, int d) {  // of block x, or of half x of fp32's one
+                vf[d] = *(const u32x4_t *)(buf + (ST ? x * 2 : 0) * BLOCK + BLOCK +
+                                           (ST ? 0 : x * (BLOCK / 2)) + d * 1024 + v_lane);
             };
-            load_keys(0);
-            load_keys(1);
-            __builtin_amdgcn_sched_barrier(0);
+            auto keys_queries = [&](int b) {
 #pragma unroll
-            for (int x = 0; x < 2 * SB; ++x) {
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int c = 0; c < kCols; ++c) s[x >> 1][x & 1][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    for (int c = 0; c < kCols; ++c) s[b][h][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < NC; ++i) {
-                    u32x4_t k = kf[x & 1][i];
-                    if (D % (4 * E) && i == NC - 1 && i * 4 + g >= D / E) k = u32x4_t{0, 0, 0, 0};
 #pragma unroll
-                    for (int c = 0; c < kCols; ++c) {
-                        f32x4_t &t = s[x >> 1][x & 1][c];
-                        if constexpr (ST) {
-                            t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, qf[c][i]),
-                                t, 0, 0, 0);
-                        } else {
+                    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                t = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    float_of(k[e]), float_of(qf[c][i][e]), t, 0, 0, 0);
+                        for (int c = 0; c < kCols; ++c) {
+                            f32x4_t &t = s[b][h][c];
+                            if constexpr (ST) {
+                                t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    __builtin_bit_cast(bf16x8_t, kf[h][i]),
+                                    __builtin_bit_cast(bf16x8_t, qf[c][i]), t, 0, 0, 0);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    t = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                        float_of(kf[h][i][e]), float_of(qf[c][i][e]), t, 0, 0, 0);
+                            }
                         }
+                        if (b + 1 < SB) load_key(b + 1, h, i);
                     }
                 }
-                if (x + 2 < 2 * SB) load_keys(x + 2);
-                if (x == 2 * SB - 2) {  // (the values' latency passes behind the softmax)
+            };
+            auto mask = [&](int b) {
+                if (clear) return;
 #pragma unroll
-                    for (int i = 0; i < VF; ++i) load_value(0, i);
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int p = pos_of(cur, b) + 16 * h + 4 * g + i;
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c)
+                            s[b][h][c][i] = hides(p, last[c], below[c]) ? kNone : s[b][h][c][i];
+                    }
+            };
+            // Weights are exp2 of a score less the column's reference.  That stands
+            // until a weight is past kSlack: they may be that much larger than 1, so
+            // no maximum is taken and nothing is rescaled in most steps.
+            auto weights = [&](int b) {
+#pragma unroll
+                for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[b][h][c][i] = __builtin_amdgcn_exp2f(
+                                __builtin_fmaf(s[b][h][c][i], a.scale2, -ref[c]));
+            };
+            auto check = [&](int b) {
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    float top = unset[c];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, w[b][h][c][i]);
+                    if (__ballot(top > kSlack)) {
+                        top = kNone;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][h][c][i]);
+                        top = column_max(top) * a.scale2;
+                        // (a column that has seen nothing yet has no reference: 0)
+                        const bool none = unset[c] > 0.f;
+                        const float to = top == kNone ? ref[c] : none ? top : fmaxf(ref[c], top);
+                        const float f = to == ref[c] || none ? 1.f : __builtin_amdgcn_exp2f(ref[c] - to);
+                        if (top != kNone) unset[c] = 0.f;
+                        ref[c] = to;
+                        l[c] *= f;
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[c][d][i] *= f;
+                        if (b > 0)  // (not among the sums yet)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) w[b - 1][h][c][i] *= f;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[b][h][c][i] = __builtin_amdgcn_exp2f(
+                                    __builtin_fmaf(s[b][h][c][i], a.scale2, -to));
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) l[c] += w[b][h][c][i];
                 }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (!clear) {
-#pragma unroll
-                for (int b = 0; b < SB; ++b)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int p = cur.pos[b] + 16 * h + 4 * g + i;
-#pragma unroll
-                            for (int c = 0; c < kCols; ++c)
-                                s[b][h][c][i] = hides(p, last[c], below[c]) ? kNone : s[b][h][c][i];
-                        }
-            }
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-                float top = s[0][0][c][0];
-#pragma unroll
-                for (int b = 0; b < SB; ++b)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][h][c][i]);
-                top = column_max(top);
-                // (a maximum is let stand until one is kSlack above it in powers of two: the
-                // weights may be that much larger than 1, and the sums are seldom rescaled)
-                if (__ballot(__builtin_fmaf(top, a.scale2, -ms[c]) > (m[c] == kNone ? kNone : kSlack))) {
-                    const float mn = fmaxf(m[c], top);
-                    const float msn = mn == kNone ? 0.f : mn * a.scale2;
-                    const float f = mn == m[c] ? 1.f : m[c] == kNone ? 0.f : __builtin_amdgcn_exp2f(ms[c] - msn);
-                    m[c] = mn;
-                    ms[c] = msn;
-                    l[c] *= f;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[c][d][i] *= f;
-                }
-#pragma unroll
-                for (int b = 0; b < SB; ++b)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float p = __builtin_amdgcn_exp2f(
-                                __builtin_fmaf(s[b][h][c][i], a.scale2, -ms[c]));
-                            s[b][h][c][i] = p;
-                            l[c] += p;
-                        }
-            }
-            // O^T += V^T P^T; a piece of values is replaced by the next block's as soon
-            // as it is multiplied
-            if constexpr (ST) {
-                bf16x8_t p[SB][kCols];
-#pragma unroll
-                for (int b = 0; b < SB; ++b)
+            };
+            auto round_weights = [&](int b) {
+                if constexpr (ST)
 #pragma unroll
                     for (int c = 0; c < kCols; ++c)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) p[b][c][4 * h + i] = (__bf16)s[b][h][c][i];
-#pragma unroll
-                for (int b = 0; b < SB; ++b)
+                            for (int i = 0; i < 4; ++i) pb[b][c][4 * h + i] = (__bf16)w[b][h][c][i];
+            };
+            auto weigh_values = [&](int b) {
+                if constexpr (ST) {
 #pragma unroll
                     for (int d = 0; d < ND; ++d) {
 #pragma unroll
                         for (int c = 0; c < kCols; ++c)
                             o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(bf16x8_t, vf[d]), p[b][c], o[c][d], 0, 0, 0);
+                                __builtin_bit_cast(bf16x8_t, vf[d]), pb[b][c], o[c][d], 0, 0, 0);
                         if (b + 1 < SB) {
                             load_value(b + 1, d);
                             __builtin_amdgcn_sched_barrier(0);
                         }
                     }
-            } else {
+                } else {
 #pragma unroll
-                for (int x = 0; x < 2 * SB; ++x)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) {
+                        for (int d = 0; d < ND; ++d) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int c = 0; c < kCols; ++c)
-                                o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    float_of(vf[d][i]), s[x >> 1][x & 1][c][i], o[c][d], 0, 0, 0);
-                        if (x + 1 < 2 * SB) {
-                            load_value(x + 1, d);
-                            __builtin_amdgcn_sched_barrier(0);
+                                for (int c = 0; c < kCols; ++c)
+                                    o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                        float_of(vf[d][i]), w[b][h][c][i], o[c][d], 0, 0, 0);
+                            if (h == 0) load_value(1, d);
                         }
-                    }
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                load_key(0, 0, i);
+                load_key(0, 1, i);
             }
-            if (!cur.all && flagged[step & 1] == step) {
+            __builtin_amdgcn_sched_barrier(0);
+            keys_queries(0);
+            mask(0);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(0);
+            if constexpr (SB == 2) keys_queries(1);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) load_value(0, d);
+            __builtin_amdgcn_sched_barrier(0);
+            check(0);
+            if constexpr (SB == 2) {
+                mask(1);
+                __builtin_amdgcn_sched_barrier(0);
+                weights(1);
+                check(1);
+            }
+#pragma unroll
+            for (int b = 0; b < SB; ++b) round_weights(b);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int b = 0; b < SB; ++b) weigh_values(b);
+            __builtin_amdgcn_s_setprio(0);
+            if (!all_of(cur, kTileWhole) && flagged[step & 1] == step) {
                 // Values that are not finite, seen by some rows and not by others: a
                 // position at a time, only where it is seen.
 #pragma unroll
@@ -622,16 +673,18 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) lds_p[wave][16 * h + 4 * g + i][r] = s[b][h][c][i];
+                            for (int i = 0; i < 4; ++i)
+                                lds_p[wave][16 * h + 4 * g + i][r] =
+                                    ST ? (float)pb[ST ? b : 0][c][4 * h + i] : w[b][h][c][i];
                         lds_wave_sync();
                         const auto *a = again();
-                        const int pos = min(cur.pos[b], high);  // (none is seen where there is no block)
+                        const int pos = min(pos_of(cur, b), high);  // (none is seen where there is no block)
                         const char *vb = head_base + a->kv_off +
                             (int64_t)a->table[(int64_t)pc.b * a->width + (pos >> a->page_shift)] * a->page_bytes +
                             (int64_t)(pos & ((1 << a->page_shift) - 1) & ~(kKvBlock - 1)) * (D * ES);
 #pragma unroll 1
                         for (int t = 0; t < kKvBlock; ++t) {
-                            if (hides(cur.pos[b] + t, last[c], below[c])) continue;
+                            if (hides(pos_of(cur, b) + t, last[c], below[c])) continue;
                             const float w = lds_p[wave][t][r];
 #pragma unroll
                             for (int d = 0; d < ND; ++d)
@@ -678,13 +731,13 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
                 }
             if (a->lse && g == 0)
                 a->lse[row * a->heads + head] =
-                    l[c] == 0.f ? kNone : (ms[c] + __builtin_amdgcn_logf(l[c])) * kLn2;
+                    l[c] == 0.f ? kNone : (ref[c] + __builtin_amdgcn_logf(l[c])) * kLn2;
         } else {
             const int64_t slot = (at * a->kv_heads + kvh) * kTile + (x - x0);
 #pragma unroll
             for (int d = 0; d < ND; ++d)
                 *(f32x4_t *)(a->part_o + slot * D + d * 16 + g * 4) = o[c][d];
-            if (g == 0) a->part_ml[slot] = make_float2(m[c] == kNone ? kNone : ms[c], l[c]);
+            if (g == 0) a->part_ml[slot] = make_float2(unset[c] > 0.f ? kNone : ref[c], l[c]);
         }
     }
 }
