@@ -15,7 +15,6 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kCols = 2;                      // columns of 16 rows per wave
 constexpr int kFew = 4, kMany = 8;            // waves per workgroup
 constexpr int rows_of(int waves) { return waves * kCols * 16; }  // of queries, in a tile
-constexpr int kMinBlocks = 8;                 // per piece of a tile's blocks, at least
 constexpr int kSplitSeqs = 384;               // sequences whose pieces each workgroup finds for itself
 constexpr int kWideDim = 128;                 // heads up to this size have an eight-wave kernel
 constexpr float kSlack = 256.f;               // the largest weight that is let stand
@@ -41,7 +40,10 @@ struct ChunkArgs {
     int64_t tiles;               // numbers of tiles, with gaps
     int split;                   // tiles are divided along the length
     int slots;                   // pieces at work at once, per key-value head
-    int4 *info;                  // [tile] its first whole piece, how many, its rest; how many in use
+    int least;                   // blocks of a piece
+    int parts;                   // workgroups of the join per tile and key-value head
+    int4 *info;                  // how many tiles; then each one's pieces: the first whole one, how
+                                 // many, the rest, how many in use; and its sequence and place there
     float *part_o;               // [piece][kv head][row of the tile][dim]
     float2 *part_ml;             // [piece][kv head][row of the tile] running maximum and sum
 };
@@ -144,50 +146,54 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
 struct Piece {
     int b, tile, split, per;
     int first, whole, rest;  // the tile's pieces: first .. first + whole - 1, and rest (-1: none)
+    int number, count;       // of the tile among all, and how many they are
 };
 
 __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int lane, Piece &p) {
-    auto look = [&](int b, int &tiles, int &blocks) {
+    int64_t all = 0;
+    int count = 0, widest = 0;
+    auto look = [&](int b, int &tiles, int &blocks, bool sum) {
         tiles = blocks = 0;
-        if (b < a.nseq) {
-            const Seq s = seq_of(a, b);
-            tiles = tiles_of(a, s);
-            blocks = most_blocks(a, s);
-        }
+        if (b >= a.nseq) return;
+        const Seq s = seq_of(a, b);
+        tiles = tiles_of(a, s);
+        blocks = most_blocks(a, s);
+        if (!sum) return;
+        // (causal tiles grow from the first to the last)
+        const int least = min(max(last_of(a, s, 0), 0) / kKvBlock + 1, blocks);
+        all += ((int64_t)tiles * (blocks + least) + 1) / 2;
+        count += tiles;
+        widest = max(widest, blocks);
     };
     int t0, n0;  // (all there is to read for up to 64 sequences)
-    look(lane, t0, n0);
-    int64_t all = (int64_t)t0 * n0;
-    int count = t0, widest = n0;
+    look(lane, t0, n0, true);
     for (int b = lane + 64; b < a.nseq; b += 64) {
         int t, n;
-        look(b, t, n);
-        all += (int64_t)t * n;
-        count += t;
-        widest = max(widest, n);
+        look(b, t, n, true);
     }
     all = uniform(wave_sum64(all));
-    count = (int)wave_sum((uint32_t)count);
+    p.count = count = (int)wave_sum((uint32_t)count);
     widest = uniform((int)wave_max((float)widest));  // (past 2^24 off by two at most: a piece more)
     // Pieces of such a length that all are at work at once where tiles are few;
     // none at all where the longest is not what the call waits for; else enough of
     // them to spread.
     const int target = 2 * count <= a.slots ? a.slots - count : 2 * a.slots;
-    p.per = (int)max((all + target - 1) / target, (int64_t)kMinBlocks);
+    p.per = (int)max((all + target - 1) / target, (int64_t)a.least);
     if (count >= a.slots && 4 * (int64_t)widest * a.slots <= 5 * all) p.per = max(p.per, widest + 2);
     int wholes = 0;
     for (int b0 = 0; b0 < a.nseq; b0 += 64) {
         int t = t0, n = n0;
-        if (b0) look(b0 + lane, t, n);
+        if (b0) look(b0 + lane, t, n, false);
         wholes += (int)wave_sum((uint32_t)(t * (n / p.per)));
     }
     const bool is_rest = piece >= wholes;
-    int base = 0, rank = wholes;
+    int base = 0, rank = wholes, tbase = 0;
     for (int b0 = 0; b0 < a.nseq; b0 += 64) {
         int t = t0, n = n0;
-        if (b0) look(b0 + lane, t, n);
+        if (b0) look(b0 + lane, t, n, false);
         const int whole = n / p.per, rest = n == 0 || n % p.per != 0;
         const int wsum = base + prefix_sum(t * whole), rsum = rank + prefix_sum(t * rest);
+        const int tsum = tbase + prefix_sum(t);
         const uint64_t past = __ballot((is_rest ? rsum : wsum) > piece);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -201,10 +207,12 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
             p.whole = w;
             p.first = first + p.tile * w;
             p.rest = r ? left + p.tile : -1;
+            p.number = __builtin_amdgcn_readlane(tsum, l) - tiles + p.tile;
             return true;
         }
         base = __builtin_amdgcn_readlane(wsum, 63);
         rank = __builtin_amdgcn_readlane(rsum, 63);
+        tbase = __builtin_amdgcn_readlane(tsum, 63);
     }
     return false;
 }
@@ -256,12 +264,12 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
 
     // which rows, which blocks
     Piece pc = {};
-    int64_t number;  // of the tile
     if (a.split) {
-        if (!find_piece(a, (int)at, lane, pc)) return;
-        number = tile_base(a, pc.b) + pc.tile;
+        const bool found = find_piece(a, (int)at, lane, pc);
+        if (at == 0 && kvh == 0 && threadIdx.x == 0) a.info[0].x = pc.count;
+        if (!found) return;
     } else {
-        number = a.tiles - 1 - at;
+        const int64_t number = a.tiles - 1 - at;
         pc.b = find_tile(a, number, lane);
         pc.tile = (int)(number - tile_base(a, pc.b));
         pc.per = INT32_MAX;
@@ -286,8 +294,10 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
         if (pc.split >= pieces) return;
         j0 = pc.split * pc.per;
         j1 = min(j0 + pc.per, sp.total);
-        if (pc.split == 0 && kvh == 0 && threadIdx.x == 0)
-            a.info[number] = make_int4(pc.first, pc.whole, pc.rest, pieces);
+        if (pc.split == 0 && kvh == 0 && threadIdx.x == 0) {
+            a.info[1 + 2 * pc.number] = make_int4(pc.first, pc.whole, pc.rest, pieces);
+            a.info[2 + 2 * pc.number] = make_int4(pc.b, pc.tile, 0, 0);
+        }
     }
 
     // the wave's rows: column c * 16 + r is query row `row[c]` of the sequence
@@ -755,20 +765,19 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     __shared__ float lds_l[kWaves][kJoinRows];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kTile = a.tile, kParts = kTile / kJoinRows;
-    const int part = blockIdx.x % kParts;
-    const int kvh = blockIdx.x / kParts % a.kv_heads;
-    const int64_t number = blockIdx.x / kParts / a.kv_heads;
-    const int b = find_tile(a, number, lane);
-    const int tile = (int)(number - tile_base(a, b));
-    const Seq sq = seq_of(a, b);
-    if (tile < 0 || tile >= tiles_of(a, sq)) return;
-    const int64_t x0 = (int64_t)tile * kTile + part * kJoinRows;
-    const int rows = (int)min((int64_t)sq.count * a.group - x0, (int64_t)kJoinRows);
-    if (rows <= 0) return;
-    const int4 f = a.info[number];
+    const int part0 = blockIdx.x % a.parts;
+    const int kvh = blockIdx.x / a.parts % a.kv_heads;
+    const int number = blockIdx.x / a.parts / a.kv_heads;
+    // (as many as there may be: what is not a tile is not looked at)
+    const int4 f = a.info[1 + 2 * number], place = a.info[2 + 2 * number];
     const int cnt = f.w;
-    if (cnt <= 1) return;
+    if (number >= a.info[0].x || cnt <= 1) return;
+    const int kTile = a.tile, tile = place.y;
+    const Seq sq = seq_of(a, place.x);
+    for (int part = part0; part < kTile / kJoinRows; part += a.parts) {
+    const int x0 = tile * kTile + part * kJoinRows;
+    const int rows = min(sq.count * a.group - x0, kJoinRows);
+    if (rows <= 0) return;
     auto slot_of = [&](int s, int j) {
         const int piece = s < f.y ? f.x + s : f.z;
         return ((int64_t)piece * a.kv_heads + kvh) * kTile + part * kJoinRows + j;
@@ -818,13 +827,14 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     __syncthreads();
     // a wave per row
     static_assert(kJoinRows == kWaves, "");
-    if (wave >= rows) return;
+    if (wave < rows) {
     float l = 0.f, top = ms[0];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) l += lds_l[w][wave];
 #pragma unroll
     for (int j = 1; j < kJoinRows; ++j) top = wave == j ? ms[j] : top;
-    const int64_t x = x0 + wave, row = sq.row0 + x / a.group;
+    const int x = x0 + wave;
+    const int64_t row = sq.row0 + x / a.group;
     const int head = kvh * a.group + (int)(x % a.group);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     for (int d = lane; d < D; d += 64) {
@@ -839,6 +849,9 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     }
     if (a.lse && lane == 0)
         a.lse[row * a.heads + head] = l == 0.f ? kNone : (top + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+    __syncthreads();
+    }
 }
 
 template <int ST, int D, int NW>
@@ -861,7 +874,7 @@ hipError_t launch_chunk(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
     const hipError_t e = launch_tiles<ST, D, kFew>(a, wgs, st);
     if (e != hipSuccess || !a.split) return e;
     hipLaunchKernelGGL((chunk_join_kernel<ST, D>),
-                       dim3((uint32_t)(a.tiles * a.kv_heads * (a.tile / kJoinRows))), dim3(256), 0, st, a);
+                       dim3((uint32_t)(a.tiles * a.kv_heads * a.parts)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -956,16 +969,19 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     a.tile = vs::rows_of(many ? vs::kMany : vs::kFew);
     a.tiles = tiles_of(many ? vs::kMany : vs::kFew);
     a.split = !many && a.tiles * a.kv_heads < 4 * kv->num_cu && s->nseq <= vs::kSplitSeqs &&
-              most > vs::kMinBlocks;
+              most > 4;
     int64_t wgs = a.tiles * a.kv_heads;
     if (a.split) {
         const int at_once = kv->head_dim <= (e == 2 ? 192 : 128) ? 2 : 1;
         a.slots = (int)std::max<int64_t>(1, at_once * kv->num_cu / a.kv_heads);
+        a.least = e == 2 ? 8 : 4;
+        // (so many workgroups that those without work are soon through)
+        a.parts = (int)std::clamp<int64_t>(4096 / (a.tiles * a.kv_heads), 1, a.tile / vs::kJoinRows);
         const int64_t pieces = 2 * a.slots + a.tiles, slots = pieces * a.kv_heads * a.tile;
         const size_t o_bytes = (size_t)slots * kv->head_dim * sizeof(float);
         const size_t ml_bytes = (size_t)slots * sizeof(float2);
         void *ws = nullptr;
-        rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)a.tiles * sizeof(int4), &ws);
+        rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)(2 * a.tiles + 1) * sizeof(int4), &ws);
         if (rc) return rc;
         a.part_o = (float *)ws;
         a.info = (int4 *)((char *)ws + o_bytes + ml_bytes);
