@@ -12,11 +12,11 @@ namespace {
 
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kCols = 2;                      // columns of 16 rows per wave
-constexpr int kFew = 4, kMany = 8;            // waves per workgroup
-constexpr int rows_of(int waves) { return waves * kCols * 16; }  // of queries, in a tile
+// Workgroups: tiles of 64, 128 or 256 rows of queries, by four waves of 16 or 32
+// rows or eight of 32.
+constexpr int kSmallTile = 64, kTile = 128, kLargeTile = 256;
 constexpr int kSplitSeqs = 384;               // sequences whose pieces each workgroup finds for itself
-constexpr int kWideDim = 128;                 // heads up to this size have an eight-wave kernel
+constexpr int kWideDim = 128;                 // bf16 heads up to this size have the larger ones
 constexpr float kSlack = 256.f;               // the largest weight that is let stand
 constexpr int kJoinRows = 4;                  // rows per workgroup of the join
 
@@ -40,7 +40,7 @@ struct ChunkArgs {
     int64_t tiles;               // numbers of tiles, with gaps
     int split;                   // tiles are divided along the length
     int slots;                   // pieces at work at once, per key-value head
-    int least;                   // blocks of a piece
+    int least, cost;             // blocks of a piece; what one costs, in blocks
     int parts;                   // workgroups of the join per tile and key-value head
     int4 *info;                  // how many tiles; then each one's pieces: the first whole one, how
                                  // many, the rest, how many in use; and its sequence and place there
@@ -150,7 +150,7 @@ struct Piece {
 };
 
 __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int lane, Piece &p) {
-    int64_t all = 0;
+    int64_t all = 0, filled = 0;
     int count = 0, widest = 0;
     auto look = [&](int b, int &tiles, int &blocks, bool sum) {
         tiles = blocks = 0;
@@ -163,6 +163,7 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
         const int least = min(max(last_of(a, s, 0), 0) / kKvBlock + 1, blocks);
         all += ((int64_t)tiles * (blocks + least) + 1) / 2;
         count += tiles;
+        filled += (int64_t)s.count * a.group;
         widest = max(widest, blocks);
     };
     int t0, n0;  // (all there is to read for up to 64 sequences)
@@ -174,12 +175,16 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
     all = uniform(wave_sum64(all));
     p.count = count = (int)wave_sum((uint32_t)count);
     widest = uniform((int)wave_max((float)widest));  // (past 2^24 off by two at most: a piece more)
-    // Pieces of such a length that all are at work at once where tiles are few;
-    // none at all where the longest is not what the call waits for; else enough of
-    // them to spread.
+    // Pieces of such a length that all are at work at once where tiles are few, or
+    // so many that they spread.  They cost their start and the join of their rows,
+    // kPieceCost blocks for a full tile: where whole tiles take no more than that
+    // longer, there are none.
     const int target = 2 * count <= a.slots ? a.slots - count : 2 * a.slots;
     p.per = (int)max((all + target - 1) / target, (int64_t)a.least);
-    if (count >= a.slots && 4 * (int64_t)widest * a.slots <= 5 * all) p.per = max(p.per, widest + 2);
+    const int64_t ideal = all / a.slots;
+    const int64_t undivided = count <= a.slots ? widest : max((int64_t)widest, ideal + widest / 2);
+    const int64_t full = uniform(wave_sum64(filled)) * 16 / ((int64_t)max(count, 1) * a.tile);  // 16ths
+    if (undivided <= ideal + a.cost / 8 + a.cost * full * a.tile / (16 * kTile)) p.per = max(p.per, widest + 2);
     int wholes = 0;
     for (int b0 = 0; b0 < a.nseq; b0 += 64) {
         int t = t0, n = n0;
@@ -232,8 +237,8 @@ constexpr int buffer_bytes(int st, int dim) {
     return blocks_at_once(st, dim) * 2 * kKvBlock * dim * (st ? 2 : 4);
 }
 
-template <int ST, int D, int NW>
-__global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_kernel(ChunkArgs args) {
+template <int ST, int D, int NW, int kCols>
+__global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(ChunkArgs args) {
     // (what only the loop's edges need is read from the arguments again: held in the
     // scalar registers it would be moved out of them and back in every step)
     const ChunkArgs &a = args;
@@ -250,7 +255,7 @@ __global__ __launch_bounds__(64 * NW, D <= (ST ? 192 : 128) ? 2 : 1) void chunk_
     constexpr int BLOCK = kKvBlock * D * ES;         // bytes of a block's keys
     constexpr int LOADS = SB * 2 * BLOCK / 1024;     // of 16 bytes per lane, all waves
     constexpr int MINE = (LOADS + NW - 1) / NW;
-    constexpr int kTile = rows_of(NW);
+    constexpr int kTile = NW * kCols * 16;  // rows of queries
     constexpr float kNone = -__builtin_huge_valf();
     extern __shared__ __align__(16) char lds[];  // two buffers: [block][keys, values]
     __shared__ int flagged[2];                   // the step whose values hold NaNs or infinities
@@ -854,24 +859,26 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     }
 }
 
-template <int ST, int D, int NW>
+template <int ST, int D, int NW, int C>
 hipError_t launch_tiles(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
     constexpr int lds = 2 * buffer_bytes(ST, D);
     if constexpr (lds + sizeof(float) * NW * kKvBlock * 16 + 64 > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)chunk_kernel<ST, D, NW>,
+        const hipError_t e = hipFuncSetAttribute((const void *)chunk_kernel<ST, D, NW, C>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((chunk_kernel<ST, D, NW>), dim3((uint32_t)wgs), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL((chunk_kernel<ST, D, NW, C>), dim3((uint32_t)wgs), dim3(64 * NW), lds, st, a);
     return hipGetLastError();
 }
 
 template <int ST, int D>
 hipError_t launch_chunk(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
-    if constexpr (D <= kWideDim) {
-        if (a.tile == rows_of(kMany)) return launch_tiles<ST, D, kMany>(a, wgs, st);
+    hipError_t e = hipSuccess;
+    if constexpr (ST && D <= kWideDim) {
+        if (a.tile == kLargeTile) return launch_tiles<ST, D, 8, 2>(a, wgs, st);
+        if (a.tile == kTile) e = launch_tiles<ST, D, 4, 2>(a, wgs, st);
     }
-    const hipError_t e = launch_tiles<ST, D, kFew>(a, wgs, st);
+    if (a.tile == kSmallTile) e = launch_tiles<ST, D, 4, 1>(a, wgs, st);
     if (e != hipSuccess || !a.split) return e;
     hipLaunchKernelGGL((chunk_join_kernel<ST, D>),
                        dim3((uint32_t)(a.tiles * a.kv_heads * a.parts)), dim3(256), 0, st, a);
@@ -963,18 +970,21 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     a.window = (int)std::min<int64_t>(window, INT32_MAX);
     a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX - 64);
     a.q_vec = vs::pieces_ok(q, q_row, q_head, e);
-    auto tiles_of = [&](int waves) { return nrows * group / vs::rows_of(waves) + s->nseq; };
     const int64_t most = s->width * (kv->page_size / vs::kKvBlock);
-    const bool many = kv->head_dim <= vs::kWideDim && tiles_of(vs::kMany) * a.kv_heads >= 2 * kv->num_cu;
-    a.tile = vs::rows_of(many ? vs::kMany : vs::kFew);
-    a.tiles = tiles_of(many ? vs::kMany : vs::kFew);
-    a.split = !many && a.tiles * a.kv_heads < 4 * kv->num_cu && s->nseq <= vs::kSplitSeqs &&
-              most > 4;
+    auto tiles_of = [&](int tile) { return nrows * group / tile + s->nseq; };
+    a.tile = vs::kSmallTile;
+    const bool few = nrows * group <= s->nseq * vs::kSmallTile;  // per sequence
+    const bool prompts = tiles_of(vs::kSmallTile) * a.kv_heads <= 4 * kv->num_cu &&
+                         most * vs::kKvBlock * s->nseq <= 4 * nrows;
+    if (e == 2 && kv->head_dim <= vs::kWideDim && !few && !prompts)
+        a.tile = tiles_of(vs::kLargeTile) * a.kv_heads >= 4 * kv->num_cu ? vs::kLargeTile : vs::kTile;
+    a.tiles = tiles_of(a.tile);
+    a.split = a.tiles * a.kv_heads < 4 * kv->num_cu && s->nseq <= vs::kSplitSeqs && most > 4;
     int64_t wgs = a.tiles * a.kv_heads;
     if (a.split) {
-        const int at_once = kv->head_dim <= (e == 2 ? 192 : 128) ? 2 : 1;
-        a.slots = (int)std::max<int64_t>(1, at_once * kv->num_cu / a.kv_heads);
+        a.slots = (int)std::max<int64_t>(1, 2 * kv->num_cu / a.kv_heads);
         a.least = e == 2 ? 8 : 4;
+        a.cost = e == 2 ? 48 : 16;
         // (so many workgroups that those without work are soon through)
         a.parts = (int)std::clamp<int64_t>(4096 / (a.tiles * a.kv_heads), 1, a.tile / vs::kJoinRows);
         const int64_t pieces = 2 * a.slots + a.tiles, slots = pieces * a.kv_heads * a.tile;
@@ -988,7 +998,7 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
         a.part_ml = (float2 *)((char *)ws + o_bytes);
         wgs = pieces * a.kv_heads;
     }
-    if (!vs::grid_ok(wgs, 2 * a.tile))
+    if (!vs::grid_ok(wgs, 512))
         return report(VS_ERR_UNSUPPORTED, "%lld rows of %lld heads", (long long)nrows, (long long)heads);
     const hipError_t err = kv->dtype == VS_DTYPE_BF16
                                ? vs::launch_chunk_dim<1>(a, wgs, (int)kv->head_dim, st)
