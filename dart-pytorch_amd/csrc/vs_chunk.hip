@@ -16,6 +16,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // rows or eight of 32.
 constexpr int kSmallTile = 64, kTile = 128, kLargeTile = 256;
 constexpr int kSplitSeqs = 384;               // sequences whose pieces each workgroup finds for itself
+constexpr int kMinBlocks = 4;                 // per piece of a tile's blocks, at least
+constexpr int kLong = 48;                     // blocks per place from which on there are three pieces to one
 constexpr int kWideDim = 128;                 // bf16 heads up to this size have the larger ones
 constexpr float kSlack = 256.f;               // the largest weight that is let stand
 constexpr int kJoinRows = 4;                  // rows per workgroup of the join
@@ -40,7 +42,8 @@ struct ChunkArgs {
     int64_t tiles;               // numbers of tiles, with gaps
     int split;                   // tiles are divided along the length
     int slots;                   // pieces at work at once, per key-value head
-    int least, cost;             // blocks of a piece; what one costs, in blocks
+    int cost;                    // of a full tile's piece, in blocks
+    int spread;                  // pieces per place, at most
     int parts;                   // workgroups of the join per tile and key-value head
     int4 *info;                  // how many tiles; then each one's pieces: the first whole one, how
                                  // many, the rest, how many in use; and its sequence and place there
@@ -179,9 +182,9 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
     // so many that they spread.  They cost their start and the join of their rows,
     // kPieceCost blocks for a full tile: where whole tiles take no more than that
     // longer, there are none.
-    const int target = 2 * count <= a.slots ? a.slots - count : 2 * a.slots;
-    p.per = (int)max((all + target - 1) / target, (int64_t)a.least);
     const int64_t ideal = all / a.slots;
+    const int target = 2 * count <= a.slots ? a.slots - count : (ideal < kLong ? 2 : a.spread) * a.slots;
+    p.per = (int)max((all + target - 1) / target, (int64_t)kMinBlocks);
     const int64_t undivided = count <= a.slots ? widest : max((int64_t)widest, ideal + widest / 2);
     const int64_t full = uniform(wave_sum64(filled)) * 16 / ((int64_t)max(count, 1) * a.tile);  // 16ths
     if (undivided <= ideal + a.cost / 8 + a.cost * full * a.tile / (16 * kTile)) p.per = max(p.per, widest + 2);
@@ -232,9 +235,9 @@ __device__ __forceinline__ float column_max(float x) {
 }
 
 // blocks of 32 positions that are staged together
-constexpr int blocks_at_once(int st, int dim) { return st && dim <= 128 ? 2 : 1; }
-constexpr int buffer_bytes(int st, int dim) {
-    return blocks_at_once(st, dim) * 2 * kKvBlock * dim * (st ? 2 : 4);
+constexpr int blocks_at_once(int st, int dim, int waves, int cols) { return st && dim <= 128 && waves == 8 ? 2 : 1; }
+constexpr int buffer_bytes(int st, int dim, int waves, int cols) {
+    return blocks_at_once(st, dim, waves, cols) * 2 * kKvBlock * dim * (st ? 2 : 4);
 }
 
 template <int ST, int D, int NW, int kCols>
@@ -251,7 +254,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
     constexpr int ES = 16 / E;           // element size
     constexpr int NC = (D / E + 3) / 4;  // 16-byte pieces per lane of a key row
     constexpr int ND = D / 16;
-    constexpr int SB = blocks_at_once(ST, D);
+    constexpr int SB = blocks_at_once(ST, D, NW, kCols);
     constexpr int BLOCK = kKvBlock * D * ES;         // bytes of a block's keys
     constexpr int LOADS = SB * 2 * BLOCK / 1024;     // of 16 bytes per lane, all waves
     constexpr int MINE = (LOADS + NW - 1) / NW;
@@ -861,7 +864,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
 
 template <int ST, int D, int NW, int C>
 hipError_t launch_tiles(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
-    constexpr int lds = 2 * buffer_bytes(ST, D);
+    constexpr int lds = 2 * buffer_bytes(ST, D, NW, C);
     if constexpr (lds + sizeof(float) * NW * kKvBlock * 16 + 64 > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void *)chunk_kernel<ST, D, NW, C>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -983,11 +986,11 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     int64_t wgs = a.tiles * a.kv_heads;
     if (a.split) {
         a.slots = (int)std::max<int64_t>(1, 2 * kv->num_cu / a.kv_heads);
-        a.least = e == 2 ? 8 : 4;
         a.cost = e == 2 ? 48 : 16;
         // (so many workgroups that those without work are soon through)
         a.parts = (int)std::clamp<int64_t>(4096 / (a.tiles * a.kv_heads), 1, a.tile / vs::kJoinRows);
-        const int64_t pieces = 2 * a.slots + a.tiles, slots = pieces * a.kv_heads * a.tile;
+        a.spread = a.tiles * most < vs::kLong * a.slots ? 2 : 3;
+        const int64_t pieces = a.spread * a.slots + a.tiles, slots = pieces * a.kv_heads * a.tile;
         const size_t o_bytes = (size_t)slots * kv->head_dim * sizeof(float);
         const size_t ml_bytes = (size_t)slots * sizeof(float2);
         void *ws = nullptr;
