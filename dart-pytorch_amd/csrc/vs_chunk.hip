@@ -48,7 +48,8 @@ struct ChunkArgs {
     int4 *info;                  // how many tiles; then each one's pieces: the first whole one, how
                                  // many, the rest, how many in use; and its sequence and place there
     float *part_o;               // [piece][kv head][row of the tile][dim]
-    float2 *part_ml;             // [piece][kv head][row of the tile] running maximum and sum
+    float4 *part_ml;             // [piece][kv head][row of the tile] reference, sums of weights as they
+                                 // are and as they are multiplied
 };
 
 // A value that all lanes have, for the scalar registers.
@@ -97,19 +98,6 @@ __device__ __forceinline__ int64_t tile_base(const ChunkArgs &a, int64_t b) {
     return from * a.group / a.tile + b;
 }
 
-// The sequence whose tiles the number falls among: 64 of them are looked at at once.
-__device__ __forceinline__ int find_tile(const ChunkArgs &a, int64_t tile, int lane) {
-    int64_t lo = 0, n = a.nseq;  // it is one of lo .. lo + n - 1
-    while (n > 1) {
-        const int64_t step = (n + 63) / 64, b = lo + lane * step;
-        const uint64_t in = __ballot(lane * step < n && tile_base(a, b) <= tile);
-        const int l = in ? 63 - __builtin_clzll(in) : 0;
-        lo += l * step;
-        n = min(step, n - l * step);
-    }
-    return (int)lo;
-}
-
 // The blocks that a tile attends to: nsb from the start, then from wb0 on.
 struct Span {
     int nsb, wb0, total;
@@ -153,7 +141,7 @@ struct Piece {
 };
 
 __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int lane, Piece &p) {
-    int64_t all = 0, filled = 0;
+    int64_t all = 0, bound = 0, filled = 0;
     int count = 0, widest = 0;
     auto look = [&](int b, int &tiles, int &blocks, bool sum) {
         tiles = blocks = 0;
@@ -165,6 +153,7 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
         // (causal tiles grow from the first to the last)
         const int least = min(max(last_of(a, s, 0), 0) / kKvBlock + 1, blocks);
         all += ((int64_t)tiles * (blocks + least) + 1) / 2;
+        bound += (int64_t)tiles * blocks;
         count += tiles;
         filled += (int64_t)s.count * a.group;
         widest = max(widest, blocks);
@@ -176,6 +165,7 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
         look(b, t, n, true);
     }
     all = uniform(wave_sum64(all));
+    bound = uniform(wave_sum64(bound));
     p.count = count = (int)wave_sum((uint32_t)count);
     widest = uniform((int)wave_max((float)widest));  // (past 2^24 off by two at most: a piece more)
     // Pieces of such a length that all are at work at once where tiles are few, or
@@ -184,7 +174,9 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
     // longer, there are none.
     const int64_t ideal = all / a.slots;
     const int target = 2 * count <= a.slots ? a.slots - count : (ideal < kLong ? 2 : a.spread) * a.slots;
-    p.per = (int)max((all + target - 1) / target, (int64_t)kMinBlocks);
+    // (by the bound, which the pieces' numbers go by: there are no more than
+    // target of them and one of each tile)
+    p.per = (int)max((bound + target - 1) / target, (int64_t)kMinBlocks);
     const int64_t undivided = count <= a.slots ? widest : max((int64_t)widest, ideal + widest / 2);
     const int64_t full = uniform(wave_sum64(filled)) * 16 / ((int64_t)max(count, 1) * a.tile);  // 16ths
     if (undivided <= ideal + a.cost / 8 + a.cost * full * a.tile / (16 * kTile)) p.per = max(p.per, widest + 2);
@@ -278,7 +270,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
         if (!found) return;
     } else {
         const int64_t number = a.tiles - 1 - at;
-        pc.b = find_tile(a, number, lane);
+        pc.b = (int)last_at_or_below(a.nseq, number, lane, [&](int64_t b) { return tile_base(a, b); });
         pc.tile = (int)(number - tile_base(a, pc.b));
         pc.per = INT32_MAX;
     }
@@ -335,12 +327,12 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
     }
 
     // a column's reference (a score times scale2), whether it has none yet (then past
-    // kSlack), and the lane's sum
-    float ref[kCols], unset[kCols], l[kCols];
+    // kSlack), and the lane's sums of weights, and of weights rounded to bf16
+    float ref[kCols], unset[kCols], l[kCols], lr[kCols];
     f32x4_t o[kCols][ND];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
-        ref[c] = l[c] = 0.f;
+        ref[c] = l[c] = lr[c] = 0.f;
         unset[c] = w0 + c * 16 + r < w1 ? 2.f * kSlack : 0.f;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[c][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -593,6 +585,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
                         if (top != kNone) unset[c] = 0.f;
                         ref[c] = to;
                         l[c] *= f;
+                        lr[c] *= f;
 #pragma unroll
                         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -623,6 +616,17 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) pb[b][c][4 * h + i] = (__bf16)w[b][h][c][i];
+                if constexpr (ST) {
+                    // what they are divided by in the end: weights that add up to 1
+                    typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+                    const pair_t one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            lr[c] = __builtin_amdgcn_fdot2_f32_bf16(
+                                pair_t{pb[b][c][2 * i], pb[b][c][2 * i + 1]}, one, lr[c], false);
+                }
             };
             auto weigh_values = [&](int b) {
                 if constexpr (ST) {
@@ -730,13 +734,19 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
     for (int c = 0; c < kCols; ++c) {
         l[c] += __shfl_xor(l[c], 16);
         l[c] += __shfl_xor(l[c], 32);
+        if constexpr (ST) {
+            lr[c] += __shfl_xor(lr[c], 16);
+            lr[c] += __shfl_xor(lr[c], 32);
+        } else {
+            lr[c] = l[c];
+        }
         const int x = w0 + c * 16 + r;
         if (x >= w1) continue;
         const auto *a = again();
         if (pieces == 1) {
             const int64_t row = sq.row0 + x / a->group;
             const int head = kvh * a->group + (int)(x % a->group);
-            const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];
+            const float inv = lr[c] == 0.f ? 0.f : 1.f / lr[c];
             char *to = a->out + (row * a->o_row + head * a->o_head + g * 4) * ES;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -755,7 +765,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
 #pragma unroll
             for (int d = 0; d < ND; ++d)
                 *(f32x4_t *)(a->part_o + slot * D + d * 16 + g * 4) = o[c][d];
-            if (g == 0) a->part_ml[slot] = make_float2(unset[c] > 0.f ? kNone : ref[c], l[c]);
+            if (g == 0) a->part_ml[slot] = make_float4(unset[c] > 0.f ? kNone : ref[c], l[c], lr[c], 0.f);
         }
     }
 }
@@ -770,7 +780,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     constexpr int LD = L * 4 + 4;
     constexpr float kNone = -__builtin_huge_valf();
     __shared__ __align__(16) float lds_o[kWaves][kJoinRows][LD];
-    __shared__ float lds_l[kWaves][kJoinRows];
+    __shared__ float2 lds_l[kWaves][kJoinRows];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part0 = blockIdx.x % a.parts;
@@ -790,12 +800,12 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
         const int piece = s < f.y ? f.x + s : f.z;
         return ((int64_t)piece * a.kv_heads + kvh) * kTile + part * kJoinRows + j;
     };
-    float ms[kJoinRows], sum[kJoinRows];
+    float ms[kJoinRows], sum[kJoinRows], sumr[kJoinRows];
     f32x4_t acc[kJoinRows];
 #pragma unroll
     for (int j = 0; j < kJoinRows; ++j) {
         ms[j] = kNone;
-        sum[j] = 0.f;
+        sum[j] = sumr[j] = 0.f;
         acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
     for (int s = lane; s < cnt; s += 64)
@@ -813,10 +823,11 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
 #pragma unroll
         for (int j = 0; j < kJoinRows; ++j) {
             const int64_t slot = slot_of(s, min(j, rows - 1));
-            const float2 ml = a.part_ml[slot];
+            const float4 ml = a.part_ml[slot];
             const f32x4_t o = *(const f32x4_t *)(a.part_o + slot * D + at);
             const float w = __builtin_amdgcn_exp2f(ml.x - ms[j]);
             sum[j] = __builtin_fmaf(w, ml.y, sum[j]);
+            sumr[j] = __builtin_fmaf(w, ml.z, sumr[j]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_fmaf(w, o[i], acc[j][i]);
         }
@@ -826,25 +837,29 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
 #pragma unroll
         for (int d = L; d < 64; d *= 2) {
             sum[j] += __shfl_xor(sum[j], d);
+            sumr[j] += __shfl_xor(sumr[j], d);
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], d);
         }
         if (lane < L) *(f32x4_t *)&lds_o[wave][j][lane * 4] = acc[j];
-        if (lane == 0) lds_l[wave][j] = sum[j];
+        if (lane == 0) lds_l[wave][j] = make_float2(sum[j], sumr[j]);
     }
     __syncthreads();
     // a wave per row
     static_assert(kJoinRows == kWaves, "");
     if (wave < rows) {
-    float l = 0.f, top = ms[0];
+    float l = 0.f, lr = 0.f, top = ms[0];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) l += lds_l[w][wave];
+    for (int w = 0; w < kWaves; ++w) {
+        l += lds_l[w][wave].x;
+        lr += lds_l[w][wave].y;
+    }
 #pragma unroll
     for (int j = 1; j < kJoinRows; ++j) top = wave == j ? ms[j] : top;
     const int x = x0 + wave;
     const int64_t row = sq.row0 + x / a.group;
     const int head = kvh * a.group + (int)(x % a.group);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = lr == 0.f ? 0.f : 1.f / lr;
     for (int d = lane; d < D; d += 64) {
         float y = 0.f;
 #pragma unroll
@@ -992,13 +1007,13 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
         a.spread = a.tiles * most < vs::kLong * a.slots ? 2 : 3;
         const int64_t pieces = a.spread * a.slots + a.tiles, slots = pieces * a.kv_heads * a.tile;
         const size_t o_bytes = (size_t)slots * kv->head_dim * sizeof(float);
-        const size_t ml_bytes = (size_t)slots * sizeof(float2);
+        const size_t ml_bytes = (size_t)slots * sizeof(float4);
         void *ws = nullptr;
         rc = kv->scratch.get(st, o_bytes + ml_bytes + (size_t)(2 * a.tiles + 1) * sizeof(int4), &ws);
         if (rc) return rc;
         a.part_o = (float *)ws;
         a.info = (int4 *)((char *)ws + o_bytes + ml_bytes);
-        a.part_ml = (float2 *)((char *)ws + o_bytes);
+        a.part_ml = (float4 *)((char *)ws + o_bytes);
         wgs = pieces * a.kv_heads;
     }
     if (!vs::grid_ok(wgs, 512))

@@ -75,7 +75,7 @@ __device__ __forceinline__ Row finish_row(const ScoreArgs &a, int row, const Sum
 // the k largest is beam search's: what is at or above a threshold that k logits
 // seen so far reach.
 template <int ST, int PER, bool TOP>
-__global__ __launch_bounds__(256, PER == kLongStep ? 6 : 1) void logprob_piece_kernel(ScoreArgs a) {
+__global__ __launch_bounds__(256, PER == kLongStep ? (ST ? 6 : 4) : 1) void logprob_piece_kernel(ScoreArgs a) {
     using S = Step<ST, PER>;
     constexpr int kStep = 64 * PER, kNext = 4 * kStep;
     __shared__ uint64_t lists[TOP ? 4 : 1][TOP ? kCap : 1];
@@ -353,12 +353,12 @@ int vs_beam_logprobs(vs_beam *bs, const void *logits, int dtype, int64_t row_str
     a.entropy = entropy;
     a.top_tokens = top_tokens;
     a.top_logprobs = top_logprobs;
-    // Rows are divided where there are fewer than 32 workgroups to a CU.
+    // Rows are divided where there are fewer than 16 workgroups to a CU.
     const bool is_long = nrows * vocab >= (int64_t)bs->num_cu * 32 * 64 * vs::kLongStep;
     const int64_t stretch = 4 * 64 * (is_long ? vs::kLongStep : vs::kShortStep);
     const int64_t row_steps = (vocab + stretch - 1) / stretch;
     int64_t pieces = std::min<int64_t>({row_steps, vs::kMostPieces,
-                                        std::max<int64_t>(1, (int64_t)bs->num_cu * 32 / nrows)});
+                                        std::max<int64_t>(1, (int64_t)bs->num_cu * 16 / nrows)});
     const int64_t steps = (row_steps + pieces - 1) / pieces;
     pieces = (row_steps + steps - 1) / steps;
     a.steps = (int)steps;

@@ -233,15 +233,7 @@ __global__ __launch_bounds__(256) void enter_kernel(EnterArgs a, int64_t items) 
         int64_t b = item, blk = 0, row0 = item, count = 1;  // the sequence's rows
         if (c.starts) {
             auto base = [&](int64_t x) { return ((int64_t)c.starts[x] >> 5) + 2 * x; };
-            int64_t lo = 0, hi = c.nseq;  // the last one that starts at or before the item
-            while (hi - lo > 1) {
-                const int64_t mid = (lo + hi) / 2;
-                if (base(mid) <= item)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            b = lo;
+            b = last_at_or_below(c.nseq, item, threadIdx.x & 63, base);
             blk = item - base(b);
             row0 = c.starts[b];
             count = c.starts[b + 1] - row0;

@@ -92,6 +92,21 @@ __device__ __forceinline__ void store_values(const T *rows, int ld, T *to, int d
     }
 }
 
+// The last of n ascending values (value(i), i < n) that is at or below x, or 0:
+// the wave's lanes look at 64 of them at once.
+template <typename F>
+__device__ __forceinline__ int64_t last_at_or_below(int64_t n, int64_t x, int lane, F value) {
+    int64_t lo = 0;  // it is one of lo .. lo + n - 1
+    while (n > 1) {
+        const int64_t step = (n + 63) / 64, i = lo + lane * step;
+        const uint64_t in = __ballot(lane * step < n && value(i) <= x);
+        const int l = in ? 63 - __builtin_clzll(in) : 0;
+        lo += l * step;
+        n = min(step, n - l * step);
+    }
+    return lo;
+}
+
 // Where a layer's heads lie in a page, in bytes.
 template <typename Args>
 inline void fill_geometry(const vs_kv *kv, int64_t layer, Args &a) {

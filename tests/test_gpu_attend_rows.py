@@ -316,3 +316,14 @@ def test_refusals(vs):
             call(**kw)
     # nothing to do
     c.cache.attend_rows(c.seqs, A((0, 4, 32), "bf16"), A((0, 4, 32), "bf16"), starts=A.of([0, 0], "i32"))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [700, 2000])
+def test_prompts_in_pieces(vs, dtype, rows):
+    """Causal tiles that grow from the first to the last, divided along the length: no piece is left out, whatever
+    their numbers go by."""
+    c = Rows(vs, [2000, 33], [rows, 33], 2, 1, 32, 64, dtype, tail=1)
+    c.compare(c.run())
+    c.compare(c.run(window=900, sinks=40), 900, 40)
+    c.compare(c.run(causal=False), causal=False)
