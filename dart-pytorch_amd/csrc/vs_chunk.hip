@@ -232,6 +232,37 @@ constexpr int buffer_bytes(int st, int dim, int waves, int cols) {
     return blocks_at_once(st, dim, waves, cols) * 2 * kKvBlock * dim * (st ? 2 : 4);
 }
 
+// One tile's pass over its blocks, with the running sums of the softmax.  Query
+// rows are (row, head of the group) pairs, so all heads of a key-value head share what
+// is staged: a step's blocks go through registers into one of two buffers in LDS, in
+// the cache's own layout, while the other one is multiplied.  A wave holds 16 kCols
+// query rows as columns; lane (r, g) = (lane & 15, lane >> 4).
+//   S^T = K Q^T    A operand: key rows (position r, 16 bytes of dimensions g);
+//                  B operand: the queries, column r
+//   O^T = V^T P^T  A operand: dimension r, the positions of lane group g;
+//                  B operand: P^T, S^T's accumulator as it stands
+// bf16: weights are rounded to bf16, half a step (2^-8 of a weight) at most, because
+// more of their bits would cost a second product with the values (a third of the
+// matrix work); they are divided by the sum of what they are rounded to, so that they
+// add up to 1 and one position alone is answered exactly.  lse goes by their sum
+// before that.  fp32 has fp32 products.
+//
+// What bounds it: the matrix pipe and, beside it, the vector unit (32 positions of 32
+// rows are 32 products of 16 cycles at head size 128, and 16 exponentials with four to
+// five other instructions each), which overlap only in part.  8,192 rows of 32/8
+// heads of 128 577 us (953 TFLOP/s; a library product of 8,192^3 1,394), 4,096 173 us
+// (795); of 64 105 us (653); fp32, 4,096 rows of 12 heads of 64 194 us (133 of 157).
+// What was gained on the way, 8,192 rows: positions, masks and pages in scalar
+// registers 952 -> 818 us; keys and values read ahead of their products 810 -> 695; values
+// with their lane groups turned, so that no bank is asked twice 695 -> 673; 256 rows per
+// staged block 673 -> 602; no maximum in most steps, block flags and addresses ready in
+// the lanes 602 -> 553; the sum of the rounded weights 553 -> 577.
+// Tiles: 256 rows by eight waves where they fill the card twice over (a workgroup to a
+// CU, two blocks a step; half the staging of 128 rows: 552 against 594 us), 64 rows where
+// even those do not fill it (2,048 rows 69 us against 115 by 128; 512 rows 23 and 28) and
+// for fp32 and heads past 128, whose accumulators fill the registers (head size 256, 4,096
+// rows of 16/8 221 us against 255), 128 between them.  Steps of two blocks leave four
+// waves too few registers (4,096 rows 158 us with one, 171 with two).
 template <int ST, int D, int NW, int kCols>
 __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(ChunkArgs args) {
     // (what only the loop's edges need is read from the arguments again: held in the
@@ -770,8 +801,10 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
     }
 }
 
-// Joins the pieces of a tile: a workgroup per kJoinRows rows, whose waves take the
-// pieces in turn, several at once.
+// Joins the pieces of a tile: a workgroup per kJoinRows rows at a time, whose waves
+// take the pieces in turn, several at once.  Bound by the partial sums' bytes: 4 x 5
+// rows of 32 heads in some 100 pieces 7 us, 1,052 rows in 2 to 3 each 30 us (which is
+// why tiles are divided only where that saves more).
 template <int ST, int D>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     constexpr int kWaves = 4;
@@ -793,87 +826,87 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     const int kTile = a.tile, tile = place.y;
     const Seq sq = seq_of(a, place.x);
     for (int part = part0; part < kTile / kJoinRows; part += a.parts) {
-    const int x0 = tile * kTile + part * kJoinRows;
-    const int rows = min(sq.count * a.group - x0, kJoinRows);
-    if (rows <= 0) return;
-    auto slot_of = [&](int s, int j) {
-        const int piece = s < f.y ? f.x + s : f.z;
-        return ((int64_t)piece * a.kv_heads + kvh) * kTile + part * kJoinRows + j;
-    };
-    float ms[kJoinRows], sum[kJoinRows], sumr[kJoinRows];
-    f32x4_t acc[kJoinRows];
-#pragma unroll
-    for (int j = 0; j < kJoinRows; ++j) {
-        ms[j] = kNone;
-        sum[j] = sumr[j] = 0.f;
-        acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int s = lane; s < cnt; s += 64)
-#pragma unroll
-        for (int j = 0; j < kJoinRows; ++j)
-            ms[j] = fmaxf(ms[j], a.part_ml[slot_of(s, min(j, rows - 1))].x);
-#pragma unroll
-    for (int j = 0; j < kJoinRows; ++j) {
-        ms[j] = wave_max(ms[j]);
-        ms[j] = ms[j] == kNone ? 0.f : ms[j];
-    }
-    const int at = min(lane % L * 4, D - 4);
-#pragma unroll 2
-    for (int s = wave * P + lane / L; s < cnt; s += kWaves * P) {
+        const int x0 = tile * kTile + part * kJoinRows;
+        const int rows = min(sq.count * a.group - x0, kJoinRows);
+        if (rows <= 0) return;
+        auto slot_of = [&](int s, int j) {
+            const int piece = s < f.y ? f.x + s : f.z;
+            return ((int64_t)piece * a.kv_heads + kvh) * kTile + part * kJoinRows + j;
+        };
+        float ms[kJoinRows], sum[kJoinRows], sumr[kJoinRows];
+        f32x4_t acc[kJoinRows];
 #pragma unroll
         for (int j = 0; j < kJoinRows; ++j) {
-            const int64_t slot = slot_of(s, min(j, rows - 1));
-            const float4 ml = a.part_ml[slot];
-            const f32x4_t o = *(const f32x4_t *)(a.part_o + slot * D + at);
-            const float w = __builtin_amdgcn_exp2f(ml.x - ms[j]);
-            sum[j] = __builtin_fmaf(w, ml.y, sum[j]);
-            sumr[j] = __builtin_fmaf(w, ml.z, sumr[j]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_fmaf(w, o[i], acc[j][i]);
+            ms[j] = kNone;
+            sum[j] = sumr[j] = 0.f;
+            acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
-    }
+        for (int s = lane; s < cnt; s += 64)
 #pragma unroll
-    for (int j = 0; j < kJoinRows; ++j) {
+            for (int j = 0; j < kJoinRows; ++j)
+                ms[j] = fmaxf(ms[j], a.part_ml[slot_of(s, min(j, rows - 1))].x);
 #pragma unroll
-        for (int d = L; d < 64; d *= 2) {
-            sum[j] += __shfl_xor(sum[j], d);
-            sumr[j] += __shfl_xor(sumr[j], d);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], d);
+        for (int j = 0; j < kJoinRows; ++j) {
+            ms[j] = wave_max(ms[j]);
+            ms[j] = ms[j] == kNone ? 0.f : ms[j];
         }
-        if (lane < L) *(f32x4_t *)&lds_o[wave][j][lane * 4] = acc[j];
-        if (lane == 0) lds_l[wave][j] = make_float2(sum[j], sumr[j]);
-    }
-    __syncthreads();
-    // a wave per row
-    static_assert(kJoinRows == kWaves, "");
-    if (wave < rows) {
-    float l = 0.f, lr = 0.f, top = ms[0];
+        const int at = min(lane % L * 4, D - 4);
+#pragma unroll 2
+        for (int s = wave * P + lane / L; s < cnt; s += kWaves * P) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        l += lds_l[w][wave].x;
-        lr += lds_l[w][wave].y;
-    }
+            for (int j = 0; j < kJoinRows; ++j) {
+                const int64_t slot = slot_of(s, min(j, rows - 1));
+                const float4 ml = a.part_ml[slot];
+                const f32x4_t o = *(const f32x4_t *)(a.part_o + slot * D + at);
+                const float w = __builtin_amdgcn_exp2f(ml.x - ms[j]);
+                sum[j] = __builtin_fmaf(w, ml.y, sum[j]);
+                sumr[j] = __builtin_fmaf(w, ml.z, sumr[j]);
 #pragma unroll
-    for (int j = 1; j < kJoinRows; ++j) top = wave == j ? ms[j] : top;
-    const int x = x0 + wave;
-    const int64_t row = sq.row0 + x / a.group;
-    const int head = kvh * a.group + (int)(x % a.group);
-    const float inv = lr == 0.f ? 0.f : 1.f / lr;
-    for (int d = lane; d < D; d += 64) {
-        float y = 0.f;
+                for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_fmaf(w, o[i], acc[j][i]);
+            }
+        }
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) y += lds_o[w][wave][d];
-        const int64_t to = row * a.o_row + head * a.o_head + d;
-        if constexpr (ST)
-            ((__bf16 *)a.out)[to] = (__bf16)(y * inv);
-        else
-            ((float *)a.out)[to] = y * inv;
-    }
-    if (a.lse && lane == 0)
-        a.lse[row * a.heads + head] = l == 0.f ? kNone : (top + __builtin_amdgcn_logf(l)) * kLn2;
-    }
-    __syncthreads();
+        for (int j = 0; j < kJoinRows; ++j) {
+#pragma unroll
+            for (int d = L; d < 64; d *= 2) {
+                sum[j] += __shfl_xor(sum[j], d);
+                sumr[j] += __shfl_xor(sumr[j], d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], d);
+            }
+            if (lane < L) *(f32x4_t *)&lds_o[wave][j][lane * 4] = acc[j];
+            if (lane == 0) lds_l[wave][j] = make_float2(sum[j], sumr[j]);
+        }
+        __syncthreads();
+        // a wave per row
+        static_assert(kJoinRows == kWaves, "");
+        if (wave < rows) {
+            float l = 0.f, lr = 0.f, top = ms[0];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                l += lds_l[w][wave].x;
+                lr += lds_l[w][wave].y;
+            }
+#pragma unroll
+            for (int j = 1; j < kJoinRows; ++j) top = wave == j ? ms[j] : top;
+            const int x = x0 + wave;
+            const int64_t row = sq.row0 + x / a.group;
+            const int head = kvh * a.group + (int)(x % a.group);
+            const float inv = lr == 0.f ? 0.f : 1.f / lr;
+            for (int d = lane; d < D; d += 64) {
+                float y = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) y += lds_o[w][wave][d];
+                const int64_t to = row * a.o_row + head * a.o_head + d;
+                if constexpr (ST)
+                    ((__bf16 *)a.out)[to] = (__bf16)(y * inv);
+                else
+                    ((float *)a.out)[to] = y * inv;
+            }
+            if (a.lse && lane == 0)
+                a.lse[row * a.heads + head] = l == 0.f ? kNone : (top + __builtin_amdgcn_logf(l)) * kLn2;
+        }
+        __syncthreads();
     }
 }
 
@@ -956,6 +989,15 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     if (!q || !out) return report(VS_ERR_INVALID, "null q or out");
     if (nrows > (INT32_MAX - 1024) / group)
         return report(VS_ERR_UNSUPPORTED, "%lld rows of %lld heads", (long long)nrows, (long long)heads);
+    // Rows are answered while others are read.
+    const vs::Extent from(q, q_row, q_head, nrows, heads, kv->head_dim, e),
+        to(out, out_row, out_head, nrows, heads, kv->head_dim, e);
+    const bool same = q == out && (q_row == out_row || nrows == 1) && (q_head == out_head || heads == 1);
+    if (!same && vs::meet(from, to))
+        return report(VS_ERR_INVALID, "out overlaps q (in place, it is q with its strides)");
+    if (vs::overlap(lse, nrows * heads * 4, to.low, to.bytes) ||
+        vs::overlap(lse, nrows * heads * 4, from.low, from.bytes))
+        return report(VS_ERR_INVALID, "lse overlaps q or out");
     vs::DeviceGuard g(kv->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
@@ -980,7 +1022,7 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     a.heads = (int)heads;
     a.kv_heads = (int)kv->kv_heads;
     a.group = (int)group;
-    // The running maximum is of products before the scale, so that is above 0 (0
+    // A reference is the largest product times the scale, so that is above 0 (0
     // itself as so little that nothing of it is left).
     a.scale2 = std::max(std::fabs(scale * vs::kLog2e), 0x1p-126f);
     a.flip = scale < 0 ? (e == 2 ? 0x80008000u : 0x80000000u) : 0;
@@ -989,6 +1031,10 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX - 64);
     a.q_vec = vs::pieces_ok(q, q_row, q_head, e);
     const int64_t most = s->width * (kv->page_size / vs::kKvBlock);
+    // Which tile: see the kernel.  Few rows per sequence never fill a larger one; and
+    // prompts (the table has no more than four times their rows) have tiles that grow
+    // from the first to the last, which small ones spread: 1,024 rows of 32/8 heads of
+    // 128 38 us against 42 by 128; 512 rows over 8,192 positions 178 and 120.
     auto tiles_of = [&](int tile) { return nrows * group / tile + s->nseq; };
     a.tile = vs::kSmallTile;
     const bool few = nrows * group <= s->nseq * vs::kSmallTile;  // per sequence

@@ -216,7 +216,9 @@ struct EnterArgs {
 // Rows into the cache, keys and queries turned on the way: a workgroup per block of
 // 32 positions and either one key-value head or a set of query heads, which share
 // their angles.  Keys are stored as they come, a piece of 16 bytes each; values
-// are turned into their layout through LDS.
+// are turned into their layout through LDS.  Bound by HBM: 12,700 rows of 32/8 heads of
+// 128 in bf16 47 us (253 MB read and written, 5.4 TB/s; a copy 5.2 to 6.0).  48 rows in
+// fp32 8 us, the latency of the lookups (start, length, page) before the rows.
 template <int ST, bool VEC>
 __global__ __launch_bounds__(256) void enter_kernel(EnterArgs a, int64_t items) {
     using U = Unit<ST, VEC>;
@@ -348,32 +350,6 @@ hipError_t launch_rotate(const TurnArgs &a, int num_cu, hipStream_t st) {
     const dim3 grid((uint32_t)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 1 << 20)));
     hipLaunchKernelGGL((rotate_kernel<ST, VEC>), grid, dim3(256), 0, st, a, spread);
     return hipGetLastError();
-}
-
-// Rows of `heads` heads of dim elements of e bytes: the bytes from their first to
-// their last, and those of one row.
-struct Extent {
-    const char *low, *row_low;
-    int64_t bytes, row_bytes, stride;
-    Extent(const void *p, int64_t row, int64_t head, int64_t nrows, int64_t heads, int64_t dim,
-           int64_t e) {
-        const int64_t dr = (nrows - 1) * row, dh = (heads - 1) * head;
-        row_low = (const char *)p + std::min<int64_t>(dh, 0) * e;
-        row_bytes = (std::abs(dh) + dim) * e;
-        low = row_low + std::min<int64_t>(dr, 0) * e;
-        bytes = std::abs(dr) * e + row_bytes;
-        stride = nrows > 1 ? row * e : 0;
-    }
-};
-
-// Whether they may share a byte.  Rows of one stride side by side (parts of one
-// projection's output) do not.
-bool meet(const Extent &a, const Extent &b) {
-    if (!overlap(a.low, a.bytes, b.low, b.bytes)) return false;
-    const int64_t s = std::abs(a.stride);
-    if (a.stride != b.stride || a.row_bytes > s || b.row_bytes > s) return true;
-    const int64_t apart = (((int64_t)((uintptr_t)b.row_low - (uintptr_t)a.row_low)) % s + s) % s;
-    return apart < a.row_bytes || s - apart < b.row_bytes;
 }
 
 }  // namespace

@@ -21,7 +21,9 @@ def attend_rows(q, k, v, seen, scale, dtype):
     the products' sizes; scale * log2(e) and its product with them 2^-22 of the score, exp2 2^-22.  A weight is off by
     that share, the sums over n positions and their parts by (n + 400) 2^-23 of the sum of the weights.  The output is
     a weighted mean of values: twice the weights' error of the largest value.  bf16: each weight is rounded to bf16
-    besides, half a step, 2^-8 of it, which moves the output by that share of the mean of the values' sizes."""
+    besides, half a step, 2^-8 of it, and divided by the sum of what they are rounded to: with p (1 + d) for p and out =
+    sum of p v, the output moves by sum of p d (v - out) over 1 + sum of p d, at most 2^-8 (1 + 2^-7) of the sum of
+    p (|v| + |out|)."""
     rows, heads, dim = q.shape
     kv, n = k.shape[1], k.shape[0]
     out, lse = np.zeros((rows, heads, dim)), np.full((rows, heads), -np.inf)
@@ -45,7 +47,7 @@ def attend_rows(q, k, v, seen, scale, dtype):
         dw = ds + (n + 400) * 2.0 ** -23
         off[:, h] = (np.abs(v[hit, g]).max() * 2 * dw)[:, None]
         if dtype == "bf16":
-            off[:, h] += 2.0 ** -8 * (1 + dw[:, None]) * (p @ np.abs(v[hit, g]))
+            off[:, h] += 2.0 ** -8 * (1 + 2.0 ** -7) * (1 + dw[:, None]) * (p @ np.abs(v[hit, g]) + np.abs(out[:, h]))
         loff[:, h] = dw + 2.0 ** -21 * (size + 20)
     return out, lse, off, loff
 

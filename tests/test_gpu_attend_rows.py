@@ -327,3 +327,45 @@ def test_prompts_in_pieces(vs, dtype, rows):
     c.compare(c.run())
     c.compare(c.run(window=900, sinks=40), 900, 40)
     c.compare(c.run(causal=False), causal=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_one_position_is_answered_by_its_value(vs, dtype):
+    """A single weight divided by itself: the value, whatever its score (a reciprocal's rounding, 2^-23, is below half
+    a step of bf16)."""
+    c = Rows(vs, [70, 200], [70, 150], 4, 2, 48, 32, dtype, spread=3.0)
+    out, _ = c.run(window=1)
+    for b, (n, r) in enumerate(zip(c.lens, c.counts)):
+        want = np.repeat(c.v[b][n - r:], 2, 1)
+        got = out[c.starts[b]:c.starts[b + 1]]
+        if dtype == "bf16":
+            assert np.array_equal(got, want)
+        else:
+            np.testing.assert_allclose(got, want, rtol=2.0 ** -22, atol=0)
+
+
+def test_in_place_and_overlaps(vs):
+    """Answers may take the queries' place; other overlaps are refused."""
+    A = vs.DeviceArray
+    for lens, counts in (([300, 70], [200, 70]), ([6000], [9])):  # whole tiles, and tiles in pieces
+        c = Rows(vs, lens, counts, 4, 2, 32, 32, "bf16")
+        q, starts, want = A.of(c.qb, "bf16"), A.of(c.starts, "i32"), c.run()[0]
+        c.cache.attend_rows(c.seqs, q, q, starts=starts)
+        assert np.array_equal(D.from_bf16(q.numpy()), want)
+    with pytest.raises(ValueError, match="overlaps"):
+        c.cache.attend_rows(c.seqs, q, View(q, (9, 4, 32), (128, 32, 1), 8), starts=starts)
+    with pytest.raises(ValueError, match="overlaps"):
+        c.cache.attend_rows(c.seqs, q, q, starts=starts, lse=LseOver(q, 9, 4))
+
+
+class LseOver:
+    """fp32 over another array's memory."""
+
+    def __init__(self, base, rows, heads):
+        self.base, self.shape, self.dtype = base, (rows, heads), "f32"
+
+    def data_ptr(self):
+        return self.base.data_ptr()
+
+    def stride(self):
+        return (self.shape[1], 1)
