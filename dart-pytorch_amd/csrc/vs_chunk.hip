@@ -86,9 +86,9 @@ __device__ __forceinline__ int tiles_of(const ChunkArgs &a, const Seq &s) {
     return (int)(((int64_t)s.count * a.group + a.tile - 1) / a.tile);
 }
 
-// The last position that row x of sequence s sees.
+// The last position that row x of sequence s sees; -1: none.
 __device__ __forceinline__ int last_of(const ChunkArgs &a, const Seq &s, int64_t x) {
-    return a.causal ? (int)min(s.row0 + x + s.shift, (int64_t)s.cap) : s.cap;
+    return a.causal ? (int)max(min(s.row0 + x + s.shift, (int64_t)s.cap), (int64_t)-1) : s.cap;
 }
 
 // A tile's number: those of sequence b start at base(b), which needs no sum over

@@ -1,6 +1,7 @@
 /// Decoding on the GPU that holds the index: a paged key-value cache with the
-/// attention of one new token, and beam search, over libvs_hip.so (C ABI:
-/// include/vs_hip.h, `vs_kv_*` and `vs_beam_*`) through `dart:ffi`.
+/// attention of one new token or of many, rotary positions, beam search and
+/// log probabilities, over libvs_hip.so (C ABI: include/vs_hip.h, `vs_kv_*`,
+/// `vs_rotary_*` and `vs_beam_*`) through `dart:ffi`.
 ///
 /// The calls work on device memory: `GpuArray` here, or addresses that another
 /// library on the same GPU hands over.  They run on `stream` (a hipStream_t's
@@ -73,6 +74,27 @@ class _Lib {
   late final append = lib.lookupFunction<
       ffi.Int32 Function(_P, _S, ffi.Int64, _P, ffi.Int64, ffi.Int64, _P, ffi.Int64, ffi.Int64, _P, ffi.Int64, _P),
       int Function(_P, _S, int, _P, int, int, _P, int, int, _P, int, _P)>('vs_kv_append');
+  late final attendRows = lib.lookupFunction<
+      ffi.Int32 Function(_P, _S, ffi.Int64, ffi.Int64, _P, ffi.Int64, ffi.Int64, _P, ffi.Int64, ffi.Int64, _P, _P,
+          ffi.Int64, ffi.Float, ffi.Int32, ffi.Int64, ffi.Int64, _P),
+      int Function(_P, _S, int, int, _P, int, int, _P, int, int, _P, _P, int, double, int, int, int,
+          _P)>('vs_kv_attend_rows');
+  late final rows = lib.lookupFunction<
+      ffi.Int32 Function(_P, _S, ffi.Int64, _P, ffi.Int64, _P, _P, _P, _P, _P),
+      int Function(_P, _S, int, _P, int, _P, _P, _P, _P, _P)>('vs_kv_rows');
+  late final appendRotary = lib.lookupFunction<
+      ffi.Int32 Function(_P, _S, ffi.Int64, _P, _P, ffi.Int64, ffi.Int64, _P, ffi.Int64, ffi.Int64, _P, ffi.Int64,
+          ffi.Int64, ffi.Int64, _P, ffi.Int64, ffi.Int64, _P, ffi.Int64, _P),
+      int Function(_P, _S, int, _P, _P, int, int, _P, int, int, _P, int, int, int, _P, int, int, _P, int,
+          _P)>('vs_kv_append_rotary');
+  late final rotaryCreate = lib.lookupFunction<
+      ffi.Int32 Function(ffi.Int32, ffi.Int64, ffi.Pointer<ffi.Double>, ffi.Float, ffi.Int32, ffi.Pointer<_P>),
+      int Function(int, int, ffi.Pointer<ffi.Double>, double, int, ffi.Pointer<_P>)>('vs_rotary_create');
+  late final rotaryDestroy = lib.lookupFunction<ffi.Void Function(_P), void Function(_P)>('vs_rotary_destroy');
+  late final rotaryApply = lib.lookupFunction<
+      ffi.Int32 Function(_P, ffi.Int32, _P, ffi.Int64, ffi.Int64, _P, ffi.Int64, ffi.Int64, ffi.Int64, _P, ffi.Int64,
+          ffi.Int64, ffi.Int32, _P),
+      int Function(_P, int, _P, int, int, _P, int, int, int, _P, int, int, int, _P)>('vs_rotary_apply');
   late final extend = lib.lookupFunction<ffi.Int32 Function(_P, _S, ffi.Int64, _P, _P),
       int Function(_P, _S, int, _P, _P)>('vs_kv_extend');
   late final fork = lib.lookupFunction<ffi.Int32 Function(_P, _S, _P, _S, _P),
@@ -93,6 +115,9 @@ class _Lib {
       ffi.Int32 Function(_P, _P, ffi.Int32, ffi.Int64, ffi.Int64, ffi.Int64, ffi.Int64, _P, _P, ffi.Int64, ffi.Int64,
           _P, _P, _P, _P, _P),
       int Function(_P, _P, int, int, int, int, int, _P, _P, int, int, _P, _P, _P, _P, _P)>('vs_beam_select');
+  late final beamLogprobs = lib.lookupFunction<
+      ffi.Int32 Function(_P, _P, ffi.Int32, ffi.Int64, ffi.Int64, ffi.Int64, _P, _P, _P, ffi.Int64, _P, _P, _P),
+      int Function(_P, _P, int, int, int, int, _P, _P, _P, int, _P, _P, _P)>('vs_beam_logprobs');
   late final beamReorder = lib.lookupFunction<
       ffi.Int32 Function(_P, _P, ffi.Int64, _P, ffi.Int64, ffi.Int64, _P, ffi.Int64, ffi.Int64, _P, _P),
       int Function(_P, _P, int, _P, int, int, _P, int, int, _P, _P)>('vs_beam_reorder');
@@ -193,6 +218,48 @@ class KvSequences {
   void dispose() => calloc.free(_c);
 }
 
+/// Rotary positions of a head's first `2 * radians.length` dimensions: pair i
+/// turns by radians[i] per position; its dimensions are `(i, i + n)`, or
+/// `(2 i, 2 i + 1)` where [interleaved].
+class Rotary {
+  Rotary(List<double> radians, {double gain = 1, bool interleaved = false, this.device = 0}) {
+    final host = calloc<ffi.Double>(math.max(1, radians.length));
+    final out = calloc<_P>();
+    try {
+      host.asTypedList(radians.length).setAll(0, radians);
+      _vs.ok(_vs.rotaryCreate(device, 2 * radians.length, host, gain, interleaved ? 1 : 0, out));
+      _h = out.value;
+    } finally {
+      calloc.free(host);
+      calloc.free(out);
+    }
+  }
+
+  /// base ^ (-2 i / dims) radians per position, the usual ones.
+  static List<double> frequencies(int dims, {double base = 10000}) =>
+      [for (var i = 0; i < dims ~/ 2; i++) math.pow(base, -2 * i / dims).toDouble()];
+
+  final int device;
+  late _P _h;
+
+  _P get _handle => _h.address == 0 ? throw StateError('Rotary used after dispose()') : _h;
+
+  /// out = x `[rows, heads, headDim]`, row i turned by positions[i]; out may be x.
+  void rotate(GpuArray x, GpuArray out, GpuArray positions, {bool backward = false, int stream = 0}) {
+    final rows = x.shape[0], heads = x.shape[1], dim = x.shape[2];
+    if (x.type.code < 0) throw ArgumentError('x is f32 or bf16');
+    _expect(out, 'out', [rows, heads, dim], x.type);
+    _expect(positions, 'positions', [rows], GpuType.i32);
+    _vs.ok(_vs.rotaryApply(_handle, x.type.code, x.pointer, heads * dim, dim, positions.pointer, rows, heads, dim,
+        out.pointer, heads * dim, dim, backward ? 1 : 0, _at(stream)));
+  }
+
+  void dispose() {
+    if (_h.address != 0) _vs.rotaryDestroy(_h);
+    _h = ffi.nullptr;
+  }
+}
+
 /// Keys and values of every layer, in pages that stay in HBM.
 class PagedKvCache {
   PagedKvCache(this.pages, this.pageSize, this.kvHeads, this.headDim,
@@ -249,12 +316,66 @@ class PagedKvCache {
         scale ?? 1 / math.sqrt(headDim), window, sinks, _at(stream)));
   }
 
+  /// Attention of many rows at once: q, out `[rows, heads, headDim]`; rows
+  /// starts[b] to starts[b + 1] are the last positions of sequence b, whose keys
+  /// and values are in the cache. Rows see what lies up to their own position,
+  /// or all of the sequence if not [causal].
+  void attendRows(KvSequences s, GpuArray q, GpuArray out,
+      {GpuArray? starts,
+      GpuArray? lse,
+      int layer = 0,
+      double? scale,
+      bool causal = true,
+      int window = 0,
+      int sinks = 0,
+      int stream = 0}) {
+    final rows = q.shape[0], heads = q.shape[1], row = heads * headDim;
+    _expect(q, 'q', [rows, heads, headDim], type);
+    _expect(out, 'out', [rows, heads, headDim], type);
+    if (starts != null) _expect(starts, 'starts', [s.n + 1], GpuType.i32);
+    if (lse != null) _expect(lse, 'lse', [rows, heads], GpuType.f32);
+    _vs.ok(_vs.attendRows(
+        _handle, _seqs(s), layer, heads, q.pointer, row, headDim, out.pointer, row, headDim,
+        lse?.pointer ?? ffi.nullptr, starts?.pointer ?? ffi.nullptr, rows, scale ?? 1 / math.sqrt(headDim),
+        causal ? 1 : 0, window, sinks, _at(stream)));
+  }
+
+  /// Where a batch's rows go: sequence b has the next counts[b] of them, for its
+  /// last positions. starts `[n + 1]`; sequence, position, slot `[rows]`, all i32.
+  void rows(KvSequences s, GpuArray counts, GpuArray starts,
+      {GpuArray? sequence, GpuArray? position, GpuArray? slot, int stream = 0}) {
+    _expect(counts, 'counts', [s.n], GpuType.i32);
+    _expect(starts, 'starts', [s.n + 1], GpuType.i32);
+    final n = (sequence ?? position ?? slot)?.shape[0] ?? 0x7fffffff;
+    for (final a in [sequence, position, slot]) {
+      if (a != null) _expect(a, 'sequence, position and slot', [n], GpuType.i32);
+    }
+    _vs.ok(_vs.rows(_handle, _seqs(s), 0, counts.pointer, n, starts.pointer, sequence?.pointer ?? ffi.nullptr,
+        position?.pointer ?? ffi.nullptr, slot?.pointer ?? ffi.nullptr, _at(stream)));
+  }
+
   /// Rows `[rows, kvHeads, headDim]` to the sequences' last positions; starts `[n + 1]`: whose rows they are.
-  void append(KvSequences s, GpuArray k, GpuArray v, {GpuArray? starts, int layer = 0, int stream = 0}) {
+  /// With [rotary] the keys are turned to their positions on the way, and queries q `[rows, heads, headDim]` into qOut.
+  void append(KvSequences s, GpuArray k, GpuArray v,
+      {GpuArray? starts, int layer = 0, Rotary? rotary, GpuArray? q, GpuArray? qOut, int stream = 0}) {
     final rows = k.shape[0], row = kvHeads * headDim;
     _expect(k, 'k', [rows, kvHeads, headDim], type);
     _expect(v, 'v', [rows, kvHeads, headDim], type);
     if (starts != null) _expect(starts, 'starts', [s.n + 1], GpuType.i32);
+    if ((q == null) != (qOut == null) || (q != null && rotary == null)) {
+      throw ArgumentError('q and qOut go together, and with rotary');
+    }
+    if (rotary != null) {
+      final heads = q?.shape[1] ?? 0, qRow = heads * headDim;
+      for (final a in [q, qOut]) {
+        if (a != null) _expect(a, 'q and qOut', [rows, heads, headDim], type);
+      }
+      _vs.ok(_vs.appendRotary(
+          _handle, _seqs(s), layer, rotary._handle, k.pointer, row, headDim, v.pointer, row, headDim,
+          q?.pointer ?? ffi.nullptr, qRow, headDim, heads, qOut?.pointer ?? ffi.nullptr, qRow, headDim,
+          starts?.pointer ?? ffi.nullptr, rows, _at(stream)));
+      return;
+    }
     _vs.ok(_vs.append(_handle, _seqs(s), layer, k.pointer, row, headDim, v.pointer, row, headDim,
         starts?.pointer ?? ffi.nullptr, rows, _at(stream)));
   }
@@ -340,6 +461,25 @@ class BeamSearch {
         _handle, logits.pointer, logits.type.code, vocab, requests, beams, vocab, scores.pointer,
         finished?.pointer ?? ffi.nullptr, eos, k, scoresOut.pointer, tokensOut.pointer, parentsOut.pointer,
         finishedOut?.pointer ?? ffi.nullptr, _at(stream)));
+  }
+
+  /// Log probabilities of given tokens: logits `[rows, vocab]`, tokens `[rows]` i32
+  /// (-1: none), out and entropy `[rows]` f32; topTokens i32 and topLogprobs f32
+  /// `[rows, k]`: the k likeliest.
+  void logprobs(GpuArray logits, GpuArray tokens, GpuArray out,
+      {GpuArray? entropy, GpuArray? topTokens, GpuArray? topLogprobs, int stream = 0}) {
+    final rows = logits.shape[0], vocab = logits.shape[1], k = topTokens?.shape[1] ?? 0;
+    if (logits.type.code < 0) throw ArgumentError('logits are f32 or bf16');
+    _expect(tokens, 'tokens', [rows], GpuType.i32);
+    _expect(out, 'out', [rows], GpuType.f32);
+    if (entropy != null) _expect(entropy, 'entropy', [rows], GpuType.f32);
+    if ((topTokens == null) != (topLogprobs == null)) throw ArgumentError('topTokens and topLogprobs go together');
+    if (topTokens != null) _expect(topTokens, 'topTokens', [rows, k], GpuType.i32);
+    if (topLogprobs != null) _expect(topLogprobs, 'topLogprobs', [rows, k], GpuType.f32);
+    _vs.ok(_vs.beamLogprobs(
+        _handle, logits.pointer, logits.type.code, vocab, rows, vocab, tokens.pointer, out.pointer,
+        entropy?.pointer ?? ffi.nullptr, k, topTokens?.pointer ?? ffi.nullptr, topLogprobs?.pointer ?? ffi.nullptr,
+        _at(stream)));
   }
 
   /// Row i of [out] = row parents[i] of [state]; with [tail], an i32 state's last column is tail's.
