@@ -1,5 +1,6 @@
 """Decoding on the GPU that holds the index: a paged key-value cache with the
-attention of one new token, and beam search.
+attention of one new token or of many, rotary positions, beam search and log
+probabilities.
 
 The reference's vector store has no counterpart.  A program retrieves passages
 with an index of this package and lets a model answer with them; these are the
@@ -17,6 +18,17 @@ values, and the choice of the next tokens.
     cache.fork(seqs, parents, spare); seqs, spare = spare, seqs
   now and then, and before the tokens are used:
     cache.check()                                # raises what did not fit; the cache is whole then
+
+A prompt enters in chunks of any size, beside requests that decode:
+
+  rotary = Rotary(head_dim)
+  per chunk:
+    cache.extend(seqs, counts)                   # how many rows each sequence brings
+    cache.rows(seqs, counts, starts, position=positions)
+    per layer:
+      cache.append(seqs, k, v, starts=starts, layer=i, rotary=rotary, q=q, q_out=q)
+      cache.attend_rows(seqs, q, out, starts=starts, layer=i)
+    beams.logprobs(logits, tokens, out)          # where given tokens are scored
 
 Buffers are anything in device memory with data_ptr(), shape, stride() and
 dtype: DeviceArray of this module or a tensor of a framework that works on the
