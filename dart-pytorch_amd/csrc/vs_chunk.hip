@@ -253,13 +253,14 @@ constexpr int buffer_bytes(int st, int dim, int waves, int cols) {
 // What bounds it: the matrix pipe and, beside it, the vector unit (32 positions of 32
 // rows are 32 products of 16 cycles at head size 128, and 16 exponentials with four to
 // five other instructions each), which overlap only in part.  8,192 rows of 32/8
-// heads of 128 577 us (953 TFLOP/s; a library product of 8,192^3 1,394), 4,096 173 us
-// (795); of 64 105 us (653); fp32, 4,096 rows of 12 heads of 64 194 us (133 of 157).
+// heads of 128 571 us (964 TFLOP/s; a library product of 8,192^3 1,394), 4,096 163 us
+// (843); of 64 104 us (663); fp32, 4,096 rows of 12 heads of 64 194 us (133 of 157).
 // What was gained on the way, 8,192 rows: positions, masks and pages in scalar
 // registers 952 -> 818 us; keys and values read ahead of their products 810 -> 695; values
 // with their lane groups turned, so that no bank is asked twice 695 -> 673; 256 rows per
 // staged block 673 -> 602; no maximum in most steps, block flags and addresses ready in
-// the lanes 602 -> 553; the sum of the rounded weights 553 -> 577.
+// the lanes 602 -> 553; the sum of the rounded weights, a product with ones, 553 -> 571
+// (by the vector unit 577).
 // Tiles: 256 rows by eight waves where they fill the card twice over (a workgroup to a
 // CU, two blocks a step; half the staging of 128 rows: 552 against 594 us), 64 rows where
 // even those do not fill it (2,048 rows 69 us against 115 by 128; 512 rows 23 and 28) and
@@ -361,12 +362,14 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
     }
 
     // a column's reference (a score times scale2), whether it has none yet (then past
-    // kSlack), and the lane's sums of weights, and of weights rounded to bf16
-    float ref[kCols], unset[kCols], l[kCols], lr[kCols];
+    // kSlack), the lane's sum of weights, and the column's of weights rounded to bf16
+    float ref[kCols], unset[kCols], l[kCols];
+    f32x4_t lr[kCols];
     f32x4_t o[kCols][ND];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
-        ref[c] = l[c] = lr[c] = 0.f;
+        ref[c] = l[c] = 0.f;
+        lr[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         unset[c] = w0 + c * 16 + r < w1 ? 2.f * kSlack : 0.f;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[c][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -619,7 +622,8 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
                         if (top != kNone) unset[c] = 0.f;
                         ref[c] = to;
                         l[c] *= f;
-                        lr[c] *= f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) lr[c][i] *= f;
 #pragma unroll
                         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -650,20 +654,16 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) pb[b][c][4 * h + i] = (__bf16)w[b][h][c][i];
-                if constexpr (ST) {
-                    // what they are divided by in the end: weights that add up to 1
-                    typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
-                    const pair_t one = {(__bf16)1.f, (__bf16)1.f};
-#pragma unroll
-                    for (int c = 0; c < kCols; ++c)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            lr[c] = __builtin_amdgcn_fdot2_f32_bf16(
-                                pair_t{pb[b][c][2 * i], pb[b][c][2 * i + 1]}, one, lr[c], false);
-                }
             };
             auto weigh_values = [&](int b) {
                 if constexpr (ST) {
+                    // what they are divided by in the end: weights that add up to 1 (a
+                    // product with ones, whose rows are all the sum)
+                    const __bf16 u = (__bf16)1.f;
+                    const bf16x8_t ones = {u, u, u, u, u, u, u, u};
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c)
+                        lr[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[b][c], lr[c], 0, 0, 0);
 #pragma unroll
                     for (int d = 0; d < ND; ++d) {
 #pragma unroll
@@ -768,19 +768,14 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
     for (int c = 0; c < kCols; ++c) {
         l[c] += __shfl_xor(l[c], 16);
         l[c] += __shfl_xor(l[c], 32);
-        if constexpr (ST) {
-            lr[c] += __shfl_xor(lr[c], 16);
-            lr[c] += __shfl_xor(lr[c], 32);
-        } else {
-            lr[c] = l[c];
-        }
+        const float divisor = ST ? lr[c][0] : l[c];
         const int x = w0 + c * 16 + r;
         if (x >= w1) continue;
         const auto *a = again();
         if (pieces == 1) {
             const int64_t row = sq.row0 + x / a->group;
             const int head = kvh * a->group + (int)(x % a->group);
-            const float inv = lr[c] == 0.f ? 0.f : 1.f / lr[c];
+            const float inv = divisor == 0.f ? 0.f : 1.f / divisor;
             char *to = a->out + (row * a->o_row + head * a->o_head + g * 4) * ES;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -799,7 +794,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
 #pragma unroll
             for (int d = 0; d < ND; ++d)
                 *(f32x4_t *)(a->part_o + slot * D + d * 16 + g * 4) = o[c][d];
-            if (g == 0) a->part_ml[slot] = make_float4(unset[c] > 0.f ? kNone : ref[c], l[c], lr[c], 0.f);
+            if (g == 0) a->part_ml[slot] = make_float4(unset[c] > 0.f ? kNone : ref[c], l[c], divisor, 0.f);
         }
     }
 }
