@@ -40,6 +40,7 @@ struct ChunkArgs {
     int causal, window, sinks;
     int q_vec;                   // rows readable in 16-byte pieces
     int tile;                    // rows of queries per workgroup
+    int exact;                   // bf16 weights are multiplied with all their bits
     int64_t tiles;               // numbers of tiles, with gaps
     int split;                   // tiles are divided along the length
     int slots;                   // pieces at work at once, per key-value head
@@ -244,11 +245,19 @@ constexpr int buffer_bytes(int st, int dim, int waves, int cols) {
 //                  B operand: the queries, column r
 //   O^T = V^T P^T  A operand: dimension r, the positions of lane group g;
 //                  B operand: P^T, S^T's accumulator as it stands
-// bf16: weights are rounded to bf16, half a step (2^-8 of a weight) at most, because
-// more of their bits would cost a second product with the values (a third of the
-// matrix work); they are divided by the sum of what they are rounded to, so that they
-// add up to 1 and one position alone is answered exactly.  lse goes by their sum
-// before that.  fp32 has fp32 products.
+// bf16, kParts = 1: weights are rounded to bf16, half a step (2^-8 of a weight) at
+// most; they are divided by the sum of what they are rounded to, so that they add up to
+// 1 and one position alone is answered exactly.  lse goes by their sum before that.
+// kParts = 3: a weight is multiplied as the sum of three bf16 values, its 24 bits eight
+// at a time, so that answers are those of 32-bit weights, rounded once.  That is for
+// calls with few rows per sequence (up to 64 rows times heads of the group on average:
+// decoding, drafts), as the attention of one new token has it, because it costs them
+// little: 64 x 8 rows over 4,000 positions 184 -> 185 us, 4 x 5 over 900 to 30,000 33.3 ->
+// 35.3, 1 x 4 over 1,000 15.6 -> 16.3.  Others are bound by the matrix pipe enough
+// to pay (32/8 heads of 128, by one, two and three parts): 8,192 rows 570, 859 and 965 us,
+// 4,096 164, - and 239, two chunks of 511 among 30 single rows 186, 204 and 224, window 2,048
+// 154, 177 and 207; 16 x 40 to 130 rows over 200 to 4,000, 16/16 of 64, 48, 53 and 61.
+// fp32 has fp32 products.
 //
 // What bounds it: the matrix pipe and, beside it, the vector unit (32 positions of 32
 // rows are 32 products of 16 cycles at head size 128, and 16 exponentials with four to
@@ -267,8 +276,8 @@ constexpr int buffer_bytes(int st, int dim, int waves, int cols) {
 // for fp32 and heads past 128, whose accumulators fill the registers (head size 256, 4,096
 // rows of 16/8 221 us against 255), 128 between them.  Steps of two blocks leave four
 // waves too few registers (4,096 rows 158 us with one, 171 with two).
-template <int ST, int D, int NW, int kCols>
-__global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(ChunkArgs args) {
+template <int ST, int D, int NW, int kCols, int kParts>
+__global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : kParts == 3 && D <= 128 ? 3 : 2) void chunk_kernel(ChunkArgs args) {
     // (what only the loop's edges need is read from the arguments again: held in the
     // scalar registers it would be moved out of them and back in every step)
     const ChunkArgs &a = args;
@@ -535,7 +544,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
             // beside the second's.  Pieces of keys and values are replaced by the next
             // block's as soon as they are multiplied.
             f32x4_t s[SB][2][kCols], w[SB][2][kCols];
-            bf16x8_t pb[ST ? SB : 1][kCols];
+            bf16x8_t pb[ST ? SB : 1][kCols], first[kCols];
             u32x4_t kf[2][NC], vf[ND];
             auto load_key = [&](int b, int h, int i) {
                 // (a piece past the row's end is read again and zeroed)
@@ -662,17 +671,33 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
                     const __bf16 u = (__bf16)1.f;
                     const bf16x8_t ones = {u, u, u, u, u, u, u, u};
 #pragma unroll
-                    for (int c = 0; c < kCols; ++c)
-                        lr[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[b][c], lr[c], 0, 0, 0);
+                    for (int part = 0; part < kParts; ++part) {
+                        if constexpr (kParts == 1)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) {
+                            for (int c = 0; c < kCols; ++c)
+                                lr[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[b][c], lr[c], 0, 0, 0);
 #pragma unroll
-                        for (int c = 0; c < kCols; ++c)
-                            o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(bf16x8_t, vf[d]), pb[b][c], o[c][d], 0, 0, 0);
-                        if (b + 1 < SB) {
-                            load_value(b + 1, d);
-                            __builtin_amdgcn_sched_barrier(0);
+                        for (int d = 0; d < ND; ++d) {
+#pragma unroll
+                            for (int c = 0; c < kCols; ++c)
+                                o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    __builtin_bit_cast(bf16x8_t, vf[d]), pb[b][c], o[c][d], 0, 0, 0);
+                            if (b + 1 < SB) {
+                                load_value(b + 1, d);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                        }
+                        if (part + 1 < kParts) {  // what is left of the weights
+#pragma unroll
+                            for (int c = 0; c < kCols; ++c) {
+                                if (part == 0) first[c] = pb[b][c];
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        w[b][h][c][i] -= (float)pb[b][c][4 * h + i];
+                            }
+                            round_weights(b);
                         }
                     }
                 } else {
@@ -731,7 +756,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 lds_p[wave][16 * h + 4 * g + i][r] =
-                                    ST ? (float)pb[ST ? b : 0][c][4 * h + i] : w[b][h][c][i];
+                                    ST ? (float)(kParts == 1 ? pb[ST ? b : 0] : first)[c][4 * h + i] : w[b][h][c][i];
                         lds_wave_sync();
                         const auto *a = again();
                         const int pos = min(pos_of(cur, b), high);  // (none is seen where there is no block)
@@ -768,7 +793,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : 2) void chunk_kernel(
     for (int c = 0; c < kCols; ++c) {
         l[c] += __shfl_xor(l[c], 16);
         l[c] += __shfl_xor(l[c], 32);
-        const float divisor = ST ? lr[c][0] : l[c];
+        const float divisor = ST && kParts == 1 ? lr[c][0] : l[c];
         const int x = w0 + c * 16 + r;
         if (x >= w1) continue;
         const auto *a = again();
@@ -908,15 +933,15 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
     }
 }
 
-template <int ST, int D, int NW, int C>
+template <int ST, int D, int NW, int C, int P = 1>
 hipError_t launch_tiles(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
     constexpr int lds = 2 * buffer_bytes(ST, D, NW, C);
     if constexpr (lds + sizeof(float) * NW * kKvBlock * 16 + 64 > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)chunk_kernel<ST, D, NW, C>,
+        const hipError_t e = hipFuncSetAttribute((const void *)chunk_kernel<ST, D, NW, C, P>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((chunk_kernel<ST, D, NW, C>), dim3((uint32_t)wgs), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL((chunk_kernel<ST, D, NW, C, P>), dim3((uint32_t)wgs), dim3(64 * NW), lds, st, a);
     return hipGetLastError();
 }
 
@@ -927,7 +952,8 @@ hipError_t launch_chunk(const ChunkArgs &a, int64_t wgs, hipStream_t st) {
         if (a.tile == kLargeTile) return launch_tiles<ST, D, 8, 2>(a, wgs, st);
         if (a.tile == kTile) e = launch_tiles<ST, D, 4, 2>(a, wgs, st);
     }
-    if (a.tile == kSmallTile) e = launch_tiles<ST, D, 4, 1>(a, wgs, st);
+    if (a.tile == kSmallTile)
+        e = ST && a.exact ? launch_tiles<ST, D, 4, 1, ST ? 3 : 1>(a, wgs, st) : launch_tiles<ST, D, 4, 1>(a, wgs, st);
     if (e != hipSuccess || !a.split) return e;
     hipLaunchKernelGGL((chunk_join_kernel<ST, D>),
                        dim3((uint32_t)(a.tiles * a.kv_heads * a.parts)), dim3(256), 0, st, a);
@@ -1040,6 +1066,7 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
                          most * vs::kKvBlock * s->nseq <= 4 * nrows;
     if (e == 2 && kv->head_dim <= vs::kWideDim && !few && !prompts)
         a.tile = tiles_of(vs::kLargeTile) * a.kv_heads >= 4 * kv->num_cu ? vs::kLargeTile : vs::kTile;
+    a.exact = few;  // (the weights' bits: see the kernel)
     a.tiles = tiles_of(a.tile);
     a.split = a.tiles * a.kv_heads < 4 * kv->num_cu && s->nseq <= vs::kSplitSeqs && most > 4;
     int64_t wgs = a.tiles * a.kv_heads;

@@ -289,8 +289,10 @@ VS_API int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_
  *   causal == 0  every p < n on a page (window is 0): rows over other sequences' states
  * and out, lse ([nrows][heads]) and the rest are vs_kv_attend's; nothing visible
  * (positions below 0 too): out 0, lse -inf.  What lies at positions that a row does not see may be anything.
- * Scores, the softmax and sums are held in fp32; with BF16 a weight is rounded to
- * bf16 before it multiplies its value, by 2^-8 of the weight at most. */
+ * Scores, the softmax and sums are held in fp32.  With BF16 a weight is rounded to
+ * bf16 before it multiplies its value, by 2^-8 of the weight at most, but in calls
+ * with few rows (nrows * heads / kv_heads <= 64 * nseq: decoding, drafts), whose
+ * weights have all their bits, as vs_kv_attend's. */
 VS_API int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t heads,
                              const void *q, int64_t q_row, int64_t q_head, void *out,
                              int64_t out_row, int64_t out_head, float *lse, const int32_t *starts,
