@@ -390,8 +390,9 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : kParts == 3 && D <= 1
     constexpr int kTileWhole = 1;  // every row of the tile sees all of the block
     constexpr int kWaveWhole = 2;  // every row of the wave does
     constexpr int kWaveNone = 4;   // no row of the wave sees any of it
-    // no block: past all rows' positions
-    constexpr int kNoBlock = (INT32_MAX & ~(kKvBlock - 1)) - kKvBlock + kWaveNone;
+    // no block: past all positions, whose last one is 2^31 - 33 at most (a table has
+    // fewer than 2^31 of them, in whole blocks)
+    constexpr int kNoBlock = (INT32_MAX & ~(kKvBlock - 1)) + kWaveNone;
     char *const head_base = a.pool + a.layer_off + (int64_t)kvh * a.head_off;
     int chunk = j0 - 64, at_pos = 0;
     uint32_t at_low = 0, at_high = 0;
