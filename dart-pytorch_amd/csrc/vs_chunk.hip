@@ -169,6 +169,10 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
     all = uniform(wave_sum64(all));
     bound = uniform(wave_sum64(bound));
     p.count = count = (int)wave_sum((uint32_t)count);
+    if (count > a.tiles) {  // starts that do not ascend: there is no room for so many
+        p.count = 0;
+        return false;
+    }
     widest = uniform((int)wave_max((float)widest));  // (past 2^24 off by two at most: a piece more)
     // Pieces of such a length that all are at work at once where tiles are few, or
     // so many that they spread.  They cost their start and the join of their rows,

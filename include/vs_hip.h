@@ -284,7 +284,8 @@ VS_API int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_
  * (nseq + 1 ascending device values, starts[0] >= 0; null: one row each) are the
  * last positions of sequence b, whose keys and values are in the cache already
  * (vs_kv_append).  nrows: how many rows q and out have; rows of no sequence are
- * left as they were.  The row at position t sees
+ * left as they were.  (Starts that do not ascend: so may any rows be, and what is
+ * answered belongs to one of the sequences that name it.)  The row at position t sees
  *   causal != 0  p <= t on a page, and window == 0 or p > t - window or p < sinks
  *   causal == 0  every p < n on a page (window is 0): rows over other sequences' states
  * and out, lse ([nrows][heads]) and the rest are vs_kv_attend's; nothing visible

@@ -186,6 +186,21 @@ def test_in_place_and_rows_before_the_first_position(vs, tile, kv, lens, counts)
     m.check()
 
 
+@pytest.mark.parametrize("n", [4, 40, 300])
+def test_starts_that_do_not_ascend(vs, n):
+    """Sequences that name the same rows again and again: more tiles than there is room for are not answered, and the
+    next call is as ever."""
+    c = Rows(vs, [400] + [150] * (n - 1), [200] + [0] * (n - 1), 4, 2, 32, 32, "bf16")
+    assert kernel(vs, 200, 4, 2, n, c.table.shape[1], 32, 32, "bf16")[1]
+    want, good = c.run(), c.starts
+    c.starts = np.arange(n + 1) % 2 * 200
+    out, lse = c.run()
+    assert np.isnan(out).all() and (lse == 77.0).all()
+    c.starts = good
+    for got, w in zip(c.run(), want):
+        assert np.array_equal(got, w)
+
+
 @pytest.mark.parametrize("dtype,dim,counts", [("f32", 64, [90, 33, 70]), ("f32", 192, [90, 33, 70]), ("bf16", 192, [90, 33, 90]),
                                               ("bf16", 64, [20, 1, 3]), ("bf16", 256, [1, 1, 1])])
 def test_small_tiles_that_are_not_divided(vs, dtype, dim, counts):
