@@ -558,6 +558,7 @@ struct PlaceArgs {
     int64_t width;
     int nseq, npages, page_shift, count;  // count: of every sequence, without counts
     int nrows;
+    int listed;  // of them, whose places are asked for
     int32_t *starts, *sequence, *position, *slot;
     int32_t *status;
     int whole;  // starts are there: only the rows are left
@@ -613,7 +614,7 @@ __global__ __launch_bounds__(kPlan) void rows_kernel(PlaceArgs a) {
     }
     const int32_t *starts = SMALL ? lds_starts : a.starts;
     const int64_t stride = (int64_t)gridDim.x * kPlan;
-    for (int64_t row = (int64_t)blockIdx.x * kPlan + threadIdx.x; row < a.nrows; row += stride) {
+    for (int64_t row = (int64_t)blockIdx.x * kPlan + threadIdx.x; row < a.listed; row += stride) {
         int lo = 0, hi = a.nseq;  // the last sequence that starts at or before the row
         while (hi - lo > 1) {
             const int mid = (int)(((unsigned)lo + (unsigned)hi) / 2);
@@ -918,8 +919,8 @@ int vs_kv_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t count, const int32_t *cou
     a.position = position;
     a.slot = slot;
     a.status = kv->status;
-    const bool any = sequence || position || slot;
-    const int64_t groups = any ? (nrows + vs::kPlan - 1) / vs::kPlan : 0;
+    a.listed = sequence || position || slot ? (int)nrows : 0;
+    const int64_t groups = ((int64_t)a.listed + vs::kPlan - 1) / vs::kPlan;
     const dim3 grid((uint32_t)std::max<int64_t>(1, std::min<int64_t>(groups, 2 * kv->num_cu)));
     if (s->nseq <= vs::kPlaceSeqs) {
         hipLaunchKernelGGL(vs::rows_kernel<true>, grid, dim3(vs::kPlan), 0, st, a);

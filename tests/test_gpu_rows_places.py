@@ -115,3 +115,22 @@ def test_refusals(vs):
                      ((out, out), {})):
         with pytest.raises(ValueError):
             cache.rows(seqs, *args, **kw)
+
+
+@pytest.mark.parametrize("n", [3, 9000])
+def test_starts_alone_take_no_time_for_rows(vs, n):
+    """nrows is 2^31 - 1 where no row's place is asked for: none of them is visited (doing so takes half a second)."""
+    import time
+
+    A = vs.DeviceArray
+    counts = np.arange(n) % 7
+    cache, seqs, _ = setup(vs, counts, np.full(n, 40))
+    starts, c = A((n + 1,), "i32"), A.of(counts, "i32")
+    cache.rows(seqs, c, starts)
+    cache.check()
+    t = time.perf_counter()
+    for _ in range(10):
+        cache.rows(seqs, c, starts)
+    cache.check()
+    assert time.perf_counter() - t < 0.5
+    assert np.array_equal(starts.numpy(), np.concatenate([[0], counts.cumsum()]))
