@@ -93,6 +93,62 @@ inline bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
     return a && b && (const char *)a < (const char *)b + nb && (const char *)b < (const char *)a + na;
 }
 
+// Rows of `heads` heads of dim elements of e bytes, wherever the strides (in
+// elements) put them: the bytes from the first to the last, and what is between.
+struct Extent {
+    const char *low;
+    int64_t bytes, width;  // width: of one head of one row
+    int64_t n[2], s[2];    // how many rows and heads, and how far apart, upwards
+    Extent(const void *p, int64_t row, int64_t head, int64_t nrows, int64_t heads, int64_t dim,
+           int64_t e)
+        : low((const char *)p), width(dim * e), n{nrows, heads}, s{row * e, head * e} {
+        bytes = width;
+        for (int i = 0; i < 2; ++i) {
+            if (s[i] < 0) low += (n[i] - 1) * s[i], s[i] = -s[i];
+            bytes += (n[i] - 1) * s[i];
+        }
+    }
+    // Its bytes lie in the first span(period) of every `period` from low on.
+    int64_t span(int64_t period) const {
+        int64_t x = width;
+        for (int i = 0; i < 2; ++i)
+            if (s[i] % period) x += (n[i] - 1) * s[i];
+        return x;
+    }
+};
+
+// Whether they may share a byte.  Parts of one projection's output do not: what comes
+// again after the same stretch, side by side within it, be it rows or heads, or the
+// heads of rows that do.
+inline bool meet(const Extent &a, const Extent &b) {
+    if (!overlap(a.low, a.bytes, b.low, b.bytes)) return false;
+    auto apart = [&](int64_t period) {
+        const int64_t d = (int64_t)((uintptr_t)b.low - (uintptr_t)a.low) % period;
+        return d < 0 ? d + period : d;
+    };
+    for (const Extent *x : {&a, &b})
+        for (int i = 0; i < 2; ++i) {
+            const int64_t period = x->s[i];
+            if (x->n[i] < 2 || period == 0) continue;
+            const int64_t d = apart(period);
+            if (d >= a.span(period) && period - d >= b.span(period)) return false;
+        }
+    for (int i = 0; i < 2; ++i) {
+        const int64_t period = a.s[i];
+        if (a.n[i] < 2 || b.n[i] < 2 || period == 0 || b.s[i] != period) continue;
+        Extent x = a, y = b;  // one of each, which no other repetition reaches into
+        x.n[i] = y.n[i] = 1;
+        x.bytes -= (a.n[i] - 1) * period;
+        y.bytes -= (b.n[i] - 1) * period;
+        if (x.bytes > period || y.bytes > period) continue;
+        y.low = x.low + apart(period);
+        if (meet(x, y)) return true;
+        y.low -= period;
+        return meet(x, y);
+    }
+    return true;
+}
+
 // A launch of so many workgroups: the runtime counts a grid's threads in 32 bits.
 inline bool grid_ok(int64_t workgroups, int threads) { return workgroups <= UINT32_MAX / threads; }
 

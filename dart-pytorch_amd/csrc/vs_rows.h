@@ -125,32 +125,6 @@ inline bool pieces_ok(const void *p, int64_t s0, int64_t s1, int64_t e) {
     return (((uintptr_t)p | (uintptr_t)(s0 * e) | (uintptr_t)(s1 * e)) & 15) == 0;
 }
 
-// Rows of `heads` heads of dim elements of e bytes: the bytes from their first to
-// their last, and those of one row.
-struct Extent {
-    const char *low, *row_low;
-    int64_t bytes, row_bytes, stride;
-    Extent(const void *p, int64_t row, int64_t head, int64_t nrows, int64_t heads, int64_t dim,
-           int64_t e) {
-        const int64_t dr = (nrows - 1) * row, dh = (heads - 1) * head;
-        row_low = (const char *)p + std::min<int64_t>(dh, 0) * e;
-        row_bytes = (std::abs(dh) + dim) * e;
-        low = row_low + std::min<int64_t>(dr, 0) * e;
-        bytes = std::abs(dr) * e + row_bytes;
-        stride = nrows > 1 ? row * e : 0;
-    }
-};
-
-// Whether they may share a byte.  Rows of one stride side by side (parts of one
-// projection's output) do not.
-inline bool meet(const Extent &a, const Extent &b) {
-    if (!overlap(a.low, a.bytes, b.low, b.bytes)) return false;
-    const int64_t s = std::abs(a.stride);
-    if (a.stride != b.stride || a.row_bytes > s || b.row_bytes > s) return true;
-    const int64_t apart = (((int64_t)((uintptr_t)b.row_low - (uintptr_t)a.row_low)) % s + s) % s;
-    return apart < a.row_bytes || s - apart < b.row_bytes;
-}
-
 inline int fill_rows(const vs_kv *kv, const vs_kv_seqs *s, int64_t layer, RowsArgs &a) {
     if (layer < 0 || layer >= kv->layers)
         return report(VS_ERR_INVALID, "layer %lld out of range [0, %lld)", (long long)layer,

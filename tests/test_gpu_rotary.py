@@ -299,3 +299,22 @@ def test_refusals(vs):
                dict(rotary=small, q=q, q_out=View(q, (40, 2, 32), (64, 32, 1), 2))):
         with pytest.raises(ValueError):
             e.cache.append(e.seqs, k, v, starts=starts, **kw)
+
+
+@pytest.mark.parametrize("pad", [0, 24])
+def test_parts_of_a_head_turned_in_place(vs, pad):
+    """Queries, keys and values side by side in each head, [rows, heads, 3, dim]: they share no byte, so the queries are
+    turned where they lie."""
+    A, heads, dim = vs.DeviceArray, 3, 32
+    e = Entered(vs, [40, 90], [30, 90], heads, heads, dim, 32, "bf16")
+    rows, rot, wide = len(e.pos), vs.Rotary(dim), heads * 3 * dim + pad
+    host = np.zeros((rows, wide), np.uint16)
+    host[:, :wide - pad] = np.stack([e.qb, e.kb, e.vb], 2).reshape(rows, -1)
+    base = A.of(host, "bf16")
+    part = lambda i: View(base, (rows, heads, dim), (wide, 3 * dim, 1), i * dim)  # noqa: E731
+    e.cache.append(e.seqs, part(1), part(2), starts=A.of(e.starts, "i32"), rotary=rot, q=part(0), q_out=part(0))
+    got = base.numpy()[:, :wide - pad].reshape(rows, heads, 3, dim)
+    assert np.array_equal(got[:, :, 1:], np.stack([e.kb, e.vb], 2))
+    e.compare(rot, A.of(np.ascontiguousarray(got[:, :, 0]), "bf16"))
+    with pytest.raises(ValueError, match="overlaps k or v"):
+        e.cache.append(e.seqs, part(1), part(2), starts=A.of(e.starts, "i32"), rotary=rot, q=A.of(e.qb, "bf16"), q_out=part(1))
