@@ -1013,7 +1013,7 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     if (((uintptr_t)q | (uintptr_t)out) % e || ((uintptr_t)lse | (uintptr_t)starts) % 4)
         return report(VS_ERR_INVALID, "a buffer is not aligned to its elements");
     for (int64_t x : {q_row, q_head, out_row, out_head})
-        if (!vs::stride_ok(x)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
+        if (!vs::stride_ok(x, nrows)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
     if (s->nseq == 0 || nrows == 0) return VS_OK;
     if (!q || !out) return report(VS_ERR_INVALID, "null q or out");
     if (nrows > (INT32_MAX - 1024) / group)

@@ -431,7 +431,7 @@ int vs_rotary_apply(const vs_rotary *r, int dtype, const void *x, int64_t x_row,
     int rc = vs::check_rotary(r, head_dim);
     if (rc) return rc;
     for (int64_t s : {x_row, x_head, out_row, out_head})
-        if (!vs::stride_ok(s)) return report(VS_ERR_INVALID, "stride %lld", (long long)s);
+        if (!vs::stride_ok(s, nrows)) return report(VS_ERR_INVALID, "stride %lld", (long long)s);
     if (nrows == 0) return VS_OK;
     const int64_t e = dtype == VS_DTYPE_BF16 ? 2 : 4;
     if (!x || !out || !positions) return report(VS_ERR_INVALID, "null buffer");
@@ -493,7 +493,7 @@ int vs_kv_append_rotary(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, const vs_
     if (q && (heads <= 0 || heads > (1 << 16)))
         return report(VS_ERR_INVALID, "heads %lld out of range [1, 65,536]", (long long)heads);
     for (int64_t x : {k_row, k_head, v_row, v_head, q_row, q_head, out_row, out_head})
-        if (!vs::stride_ok(x)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
+        if (!vs::stride_ok(x, nrows)) return report(VS_ERR_INVALID, "stride %lld", (long long)x);
     if (nrows == 0 || s->nseq == 0) return VS_OK;
     if (!k || !v) return report(VS_ERR_INVALID, "null k or v");
     const int64_t e = vs::kv_elem(kv->dtype), d = kv->head_dim, hk = kv->kv_heads;

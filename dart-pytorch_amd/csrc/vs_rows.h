@@ -118,8 +118,11 @@ inline void fill_geometry(const vs_kv *kv, int64_t layer, Args &a) {
     a.layer_off = layer * 2 * a.kv_off;
 }
 
-// |stride| elements of rows and heads stay inside 2^62 bytes
-inline bool stride_ok(int64_t s) { return s >= -((int64_t)1 << 40) && s <= ((int64_t)1 << 40); }
+// |stride| elements of n rows and of heads stay inside 2^62 bytes
+inline bool stride_ok(int64_t s, int64_t n = 1 << 20) {
+    const int64_t most = ((int64_t)1 << 60) / std::clamp<int64_t>(n, 1 << 20, INT32_MAX);
+    return s >= -most && s <= most;
+}
 
 inline bool pieces_ok(const void *p, int64_t s0, int64_t s1, int64_t e) {
     return (((uintptr_t)p | (uintptr_t)(s0 * e) | (uintptr_t)(s1 * e)) & 15) == 0;

@@ -318,3 +318,20 @@ def test_parts_of_a_head_turned_in_place(vs, pad):
     e.compare(rot, A.of(np.ascontiguousarray(got[:, :, 0]), "bf16"))
     with pytest.raises(ValueError, match="overlaps k or v"):
         e.cache.append(e.seqs, part(1), part(2), starts=A.of(e.starts, "i32"), rotary=rot, q=A.of(e.qb, "bf16"), q_out=part(1))
+
+
+def test_strides_past_all_memory(vs):
+    """Strides of so many rows that no address holds their sum are refused before it is taken."""
+    A = vs.DeviceArray
+    base, rot, n = A((4, 1, 64), "f32"), vs.Rotary(64), 2**31 - 2000
+    far = View(base, (n, 1, 64), (2**40, 64, 1))
+    near = View(base, (n, 1, 64), (64, 64, 1))
+    for x, out in ((far, near), (near, far), (far, far)):
+        with pytest.raises(ValueError, match="stride"):
+            rot.rotate(x, out, View(A((4,), "i32"), (n,), (1,)))
+    e = Entered(vs, [40], [40], 1, 1, 64, 32, "f32")
+    starts = A.of(e.starts, "i32")
+    with pytest.raises(ValueError, match="stride"):
+        e.cache.append(e.seqs, near, near, starts=starts, rotary=rot, q=near, q_out=far)
+    with pytest.raises(ValueError, match="stride"):
+        e.cache.attend_rows(e.seqs, near, far, starts=starts)
