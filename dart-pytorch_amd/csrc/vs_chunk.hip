@@ -1027,6 +1027,9 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     if (vs::overlap(lse, nrows * heads * 4, to.low, to.bytes) ||
         vs::overlap(lse, nrows * heads * 4, from.low, from.bytes))
         return report(VS_ERR_INVALID, "lse overlaps q or out");
+    if (vs::over_places(to, s, starts) ||
+        (lse && vs::over_places(vs::Extent(lse, 0, 0, 1, 1, nrows * heads, 4), s, starts)))
+        return report(VS_ERR_INVALID, "out or lse overlaps starts, lens or table");
     vs::DeviceGuard g(kv->device);
     if (g.err != hipSuccess) return report_hip(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;

@@ -508,6 +508,8 @@ int vs_kv_append_rotary(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, const vs_
         if (vs::meet(vs::Extent(k, k_row, k_head, nrows, hk, d, e), to) ||
             vs::meet(vs::Extent(v, v_row, v_head, nrows, hk, d, e), to))
             return report(VS_ERR_INVALID, "q_out overlaps k or v");
+        if (vs::over_places(to, s, starts))
+            return report(VS_ERR_INVALID, "q_out overlaps starts, lens or table");
         a.q_heads = (int)heads;
     }
     vs::DeviceGuard g(kv->device);

@@ -128,6 +128,12 @@ inline bool pieces_ok(const void *p, int64_t s0, int64_t s1, int64_t e) {
     return (((uintptr_t)p | (uintptr_t)(s0 * e) | (uintptr_t)(s1 * e)) & 15) == 0;
 }
 
+// Whether an output shares a byte with what tells the kernels where rows go.
+inline bool over_places(const Extent &out, const vs_kv_seqs *s, const int32_t *starts) {
+    auto shares = [&](const int32_t *p, int64_t n) { return p && n > 0 && meet(out, Extent(p, 0, 0, 1, 1, n, 4)); };
+    return shares(starts, s->nseq + 1) || shares(s->lens, s->nseq) || shares(s->table, s->nseq * s->width);
+}
+
 inline int fill_rows(const vs_kv *kv, const vs_kv_seqs *s, int64_t layer, RowsArgs &a) {
     if (layer < 0 || layer >= kv->layers)
         return report(VS_ERR_INVALID, "layer %lld out of range [0, %lld)", (long long)layer,

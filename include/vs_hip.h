@@ -289,7 +289,8 @@ VS_API int vs_kv_attend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_
  *   causal != 0  p <= t on a page, and window == 0 or p > t - window or p < sinks
  *   causal == 0  every p < n on a page (window is 0): rows over other sequences' states
  * and out, lse ([nrows][heads]) and the rest are vs_kv_attend's; nothing visible
- * (positions below 0 too): out 0, lse -inf.  What lies at positions that a row does not see may be anything.
+ * (positions below 0 too): out 0, lse -inf.  out is q with its strides or does not
+ * overlap it; neither out nor lse overlaps the other, starts, lens or table.  What lies at positions that a row does not see may be anything.
  * Scores, the softmax and sums are held in fp32.  With BF16 a weight is rounded to
  * bf16 before it multiplies its value, by 2^-8 of the weight at most, but in calls
  * with few rows (nrows * heads / kv_heads <= 64 * nseq: decoding, drafts), whose
@@ -336,8 +337,8 @@ VS_API int vs_rotary_apply(const vs_rotary *r, int dtype, const void *x, int64_t
 /* vs_kv_append with keys turned to their positions on the way, and queries with
  * them: row i of q (`heads` heads; null: none) goes to row i of q_out.  Rows of
  * q that are not a sequence's are left out; those whose keys have no place are
- * turned all the same.  q_out is q with its strides or does not overlap it; it does not overlap k
- * or v. */
+ * turned all the same.  q_out is q with its strides or does not overlap it; it does not overlap k,
+ * v, starts, lens or table. */
 VS_API int vs_kv_append_rotary(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer,
                                const vs_rotary *r, const void *k, int64_t k_row, int64_t k_head,
                                const void *v, int64_t v_row, int64_t v_head, const void *q,

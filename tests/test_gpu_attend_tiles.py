@@ -207,3 +207,33 @@ def test_small_tiles_that_are_not_divided(vs, dtype, dim, counts):
     m = Many(vs, 64, [300, 257, 120], counts, 384, dim=dim, dtype=dtype, distinct=2)
     m.check()
     m.check(window=50, sinks=3)
+
+
+class Over:
+    """A buffer of another shape and type over an array's memory."""
+
+    def __init__(self, base, shape, dtype):
+        self.base, self.shape, self.dtype = base, shape, dtype
+
+    def data_ptr(self):
+        return self.base.data_ptr()
+
+    def stride(self):
+        return tuple(int(np.prod(self.shape[i + 1:])) for i in range(len(self.shape)))
+
+
+def test_outputs_over_what_tells_the_places(vs):
+    """Starts, lengths and the table are read while rows are answered and stored."""
+    A = vs.DeviceArray
+    c = Rows(vs, [64, 30], [5, 2], 2, 1, 32, 32, "bf16", width=300)
+    rows, starts = c.nrows, A.of(c.starts, "i32")
+    q, k, rot = A.of(c.qb, "bf16"), A((rows, 1, 32), "bf16"), vs.Rotary(32)
+    for base in (starts, c.seqs.lens, c.seqs.table):
+        over = Over(base, (rows, 2, 32), "bf16")
+        with pytest.raises(ValueError, match="overlaps starts"):
+            c.cache.attend_rows(c.seqs, q, over, starts=starts)
+        with pytest.raises(ValueError, match="overlaps starts"):
+            c.cache.attend_rows(c.seqs, q, A((rows, 2, 32), "bf16"), lse=Over(base, (rows, 2), "f32"), starts=starts)
+        with pytest.raises(ValueError, match="overlaps starts"):
+            c.cache.append(c.seqs, k, k, starts=starts, rotary=rot, q=q, q_out=over)
+    c.compare(c.run())
