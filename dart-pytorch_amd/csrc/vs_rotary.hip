@@ -25,14 +25,17 @@ struct Turn {
 
 // Angles are whole numbers of 2^-64 turns, so their product with a position wraps
 // at whole turns by itself and is exact however far the position is; what is
-// rounded is the frequency, once, to 2^-65 turns per position.  Of the product the
-// nearest quarter turn is taken off; the rest, at most an eighth of a turn, goes
-// through the Taylor polynomials of sine and cosine, whose first terms left out
-// are (pi/4)^11 / 11! = 1.8e-9 and (pi/4)^12 / 12! = 1.2e-10.
+// rounded is the frequency, once, to 2^-64 turns per position.  Of the product the
+// nearest quarter turn is taken off; the rest, at most an eighth of a turn, becomes
+// an fp32 angle with both of its words (the upper one alone would cut off up to
+// 2^-32 of a turn, all of a small angle) and goes through the Taylor polynomials of
+// sine and cosine, whose first terms left out are (pi/4)^11 / 11! = 1.8e-9 and
+// (pi/4)^12 / 12! = 1.2e-10.
 __device__ __forceinline__ Turn turn_of(uint64_t phase, float gain) {
     const uint32_t u = (uint32_t)(phase >> 32);
     const uint32_t quarter = (u + 0x20000000u) >> 30;
-    const float x = (float)(int32_t)(u - (quarter << 30)) * (float)(6.283185307179586 * 0x1p-32);
+    const float x = __builtin_fmaf((float)(uint32_t)phase, (float)(6.283185307179586 * 0x1p-64),
+                                   (float)(int32_t)(u - (quarter << 30)) * (float)(6.283185307179586 * 0x1p-32));
     const float x2 = x * x;
     float s = 1.f / 362880.f, c = -1.f / 3628800.f;
     s = __builtin_fmaf(s, x2, -1.f / 5040.f);
@@ -383,8 +386,12 @@ int vs_rotary_create(int device, int64_t dims, const double *radians, float gain
         return report(VS_ERR_OOM, "host allocation");
     }
     for (int64_t i = 0; i < dims / 2; ++i) {
-        // (long double: 64 bits of the quotient; whole turns make no difference)
-        long double t = (long double)radians[i] / 6.283185307179586476925286766559006L;
+        // Whole turns make no difference, and are taken off in radians first: 2 pi in
+        // two parts, of 64 bits each, so that what is left is good to 2^-64 of itself
+        // however many they are.
+        const long double turn = 0xc90fdaa22168c235p-61L, more = -0xece675d1fc8f8cbbp-127L;
+        const long double whole = std::rint((long double)radians[i] / turn);
+        long double t = std::fma(-whole, more, std::fma(-whole, turn, (long double)radians[i])) / turn;
         t -= std::floor(t);
         const long double n = std::round(t * 0x1p64L);
         turns[i] = n >= 0x1p64L ? 0 : (uint64_t)n;

@@ -318,8 +318,9 @@ VS_API int vs_kv_read(vs_kv *kv, const vs_kv_seqs *seqs, int64_t layer, int64_t 
  * position times the pair's angle, radians[i] per position (dims / 2 host values):
  *   y0 = gain (x0 cos - x1 sin)      y1 = gain (x1 cos + x0 sin)
  * The pairs are (i, i + dims / 2), or (2 i, 2 i + 1) if interleaved is not 0;
- * dimensions from `dims` on stay as they are.  Angles are exact to 2^-33 of a
- * turn at positions below 2^31, cosines and sines to fp32.  A handle is not
+ * dimensions from `dims` on stay as they are.  An angle is radians[i] (up to 2^40)
+ * rounded to 2^-64 of a turn, times the position, exactly: within 2^-33 of a turn at
+ * positions below 2^31.  Cosines and sines are held in fp32.  A handle is not
  * changed by its calls. */
 typedef struct vs_rotary vs_rotary;
 VS_API int vs_rotary_create(int device, int64_t dims, const double *radians, float gain,
