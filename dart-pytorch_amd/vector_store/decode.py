@@ -269,7 +269,9 @@ class Rotary:
             raise ValueError(f"base must be above 1 and factor above 0, got {base} and {factor}")
         if scaling not in ("none", "linear", "base", "ramp"):
             raise ValueError(f"scaling must be none, linear, base or ramp, got {scaling}")
-        if scaling == "base" and dims > 2:
+        if scaling == "base":
+            if dims == 2:
+                raise ValueError("scaling base needs more than 2 dims: a single pair turns by one radian whatever the base")
             base = base * factor ** (dims / (dims - 2))
         w = base ** (-np.arange(0, dims, 2, dtype=np.float64) / dims)
         if scaling == "linear":

@@ -88,3 +88,11 @@ def test_plain_forms_agree_with_each_other():
     np.testing.assert_allclose(p.sum(1), 1, rtol=1e-12)
     np.testing.assert_allclose(ent, -(p * tl).sum(1), rtol=1e-12)
     assert lp[0] == pytest.approx(tl[0][tt[0] == 4][0]) and lp[1] == 0 and np.isnan(lp[2])
+
+
+def test_one_pair_has_no_base_to_scale():
+    """Its angle is base ** 0: the factor would be ignored."""
+    import vector_store
+
+    with pytest.raises(ValueError, match="more than 2 dims"):
+        vector_store.Rotary(64, dims=2, scaling="base", factor=8.0)
