@@ -236,6 +236,9 @@ class Rotary:
                 a share of both; ramp_by "turns" takes the share linear in the turns,
                 "index" linear in the pair's number (its ends rounded outwards)
     gain multiplies cosines and sines (None: 0.1 ln(factor) + 1 for "ramp", else 1).
+    A model's "ramp" is all of these together, and the defaults are no model's: name
+    low, high, ramp_by and gain as it was trained with (in use are low=1, high=4, gain=1
+    over "turns", and low=1, high=32 with gain=None over "index").
     frequencies (radians per position, dims / 2 of them) stands for all that."""
 
     def __init__(self, head_dim: int, *, dims: int | None = None, base: float = 10000.0, layout: str = "half",
