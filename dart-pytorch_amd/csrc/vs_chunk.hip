@@ -1095,7 +1095,7 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
         a.part_ml = (float4 *)((char *)ws + o_bytes);
         wgs = pieces * a.kv_heads;
     }
-    if (!vs::grid_ok(wgs, 512))
+    if (!vs::grid_ok(wgs, a.tile == vs::kLargeTile ? 512 : 256))
         return report(VS_ERR_UNSUPPORTED, "%lld rows of %lld heads", (long long)nrows, (long long)heads);
     const hipError_t err = kv->dtype == VS_DTYPE_BF16
                                ? vs::launch_chunk_dim<1>(a, wgs, (int)kv->head_dim, st)

@@ -41,3 +41,20 @@ def test_last_positions(vs, kv, tile, rows, missing):
     D.assert_rounded(got[:, :1], eo, to, "bf16")
     assert (np.abs(got_lse[:, :1] - el) <= tl).all()
     cache.close()
+
+
+def test_as_many_sequences_as_there_may_be(vs):
+    """2^20 of them, one row each, 8 key-value heads: 8.5 million workgroups of 256 threads are a launch that the runtime
+    takes (below 2^32 threads).  Each sees one position of a page that it has to itself or shares."""
+    A, rng, n, kv, dim, held = vs.DeviceArray, np.random.default_rng(3), 2**20, 8, 16, 64
+    table = rng.integers(0, held, (n, 1)).astype(np.int32)
+    seqs = vs.KVSequences(A.of(table, "i32"), A.of(np.ones(n), "i32"), A.of(np.zeros(held), "i32"))
+    cache = vs.PagedKVCache(held, 32, kv, dim)
+    own = vs.KVSequences(A.of(np.arange(held)[:, None], "i32"), A.of(np.ones(held), "i32"), seqs.refs)
+    kb, vb = (D.stored(rng.standard_normal((held, kv, dim)), "bf16")[0] for _ in range(2))
+    cache.append(own, A.of(kb, "bf16"), A.of(vb, "bf16"))
+    q, out = A.of(np.full((n, kv, dim), 0x3F80), "bf16"), A((n, kv, dim), "bf16")
+    cache.attend_rows(seqs, q, out)
+    cache.check()
+    assert np.array_equal(out.numpy(), vb[table[:, 0]])  # a single weight: the value itself
+    cache.close()
