@@ -561,6 +561,7 @@ struct PlaceArgs {
     int listed;  // of them, whose places are asked for
     int32_t *starts, *sequence, *position, *slot;
     int32_t *status;
+    const uint8_t *closed;
     int whole;  // starts are there: only the rows are left
 };
 
@@ -613,6 +614,7 @@ __global__ __launch_bounds__(kPlan) void rows_kernel(PlaceArgs a) {
         __syncthreads();
     }
     const int32_t *starts = SMALL ? lds_starts : a.starts;
+    const int marked = a.status[2];  // some page may take no new rows
     const int64_t stride = (int64_t)gridDim.x * kPlan;
     for (int64_t row = (int64_t)blockIdx.x * kPlan + threadIdx.x; row < a.listed; row += stride) {
         int lo = 0, hi = a.nseq;  // the last sequence that starts at or before the row
@@ -634,6 +636,11 @@ __global__ __launch_bounds__(kPlan) void rows_kernel(PlaceArgs a) {
                 const int64_t at =
                     ((int64_t)page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
                 if ((unsigned)page < (unsigned)a.npages) slot = (int)at;
+                const int64_t end = (int64_t)a.lens[b] - 1;
+                if (marked && slot >= 0 && end >> a.page_shift < a.width) {
+                    const int last = a.table[b * a.width + (end >> a.page_shift)];
+                    if ((unsigned)last < (unsigned)a.npages && a.closed[last]) slot = -1;
+                }
             }
         }
         if (a.sequence) a.sequence[row] = b;
@@ -919,6 +926,7 @@ int vs_kv_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t count, const int32_t *cou
     a.position = position;
     a.slot = slot;
     a.status = kv->status;
+    a.closed = kv->closed;
     a.listed = sequence || position || slot ? (int)nrows : 0;
     const int64_t groups = ((int64_t)a.listed + vs::kPlan - 1) / vs::kPlan;
     const dim3 grid((uint32_t)std::max<int64_t>(1, std::min<int64_t>(groups, 2 * kv->num_cu)));

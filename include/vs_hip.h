@@ -366,7 +366,8 @@ VS_API int vs_kv_extend(vs_kv *kv, const vs_kv_seqs *seqs, int64_t count, const 
  * of the counts before b.  Of row i < nrows of sequence b
  *   sequence[i]  b
  *   position[i]  lens[b] - (starts[b + 1] - i); -1 if that is below 0
- *   slot[i]      page * page_size + the position's place on it; -1: on no page
+ *   slot[i]      page * page_size + the position's place on it; -1: on no page, or
+ *                behind an extend that did not fit (where vs_kv_append stores nothing)
  * (each may be null; -1 in rows past the last sequence's).  Counts of more than
  * nrows rows: those past nrows are left out of the three, and vs_kv_check says
  * so.  No output overlaps an input or another output. */

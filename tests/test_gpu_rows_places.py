@@ -134,3 +134,27 @@ def test_starts_alone_take_no_time_for_rows(vs, n):
     cache.check()
     assert time.perf_counter() - t < 0.5
     assert np.array_equal(starts.numpy(), np.concatenate([[0], counts.cumsum()]))
+
+
+def test_no_slots_behind_an_extend_that_did_not_fit(vs):
+    """The sequences' last positions hold tokens in use then: who stores by the slots leaves them alone, as append does.
+    Other sequences' rows, and everyone's behind the check, have theirs."""
+    A = vs.DeviceArray
+    cache = vs.PagedKVCache(5, 32, 1, 16)
+    seqs = cache.new_sequences(2, 8)
+    cache.extend(seqs, A.of([90, 10], "i32"))
+    cache.check()
+    other = vs.KVSequences(A.of(np.full((1, 8), -1), "i32"), A.of([0], "i32"), seqs.refs)
+    cache.extend(other, 5)
+    cache.check()
+    table, lens = seqs.table.numpy(), [90, 10]
+    cache.extend(seqs, A.of([70, 0], "i32"))  # (not a page is left)
+    counts = [40, 3]
+    want = P.rows_of(counts, lens, table, 32, 5, 45)
+    closed = [w.copy() for w in want]
+    closed[3][:40] = -1
+    compare(run(vs, cache, seqs, counts, 45), closed)
+    compare(run(vs, cache, other, [5], 5), P.rows_of([5], [5], other.table.numpy(), 32, 5, 5))
+    with pytest.raises(vs.VsError, match="pages short"):
+        cache.check()
+    compare(run(vs, cache, seqs, counts, 45), want)
