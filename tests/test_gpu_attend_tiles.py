@@ -8,6 +8,7 @@ import pytest
 
 import _decode as D
 import _prompt as P
+from _hip import Stream
 from test_gpu_attend_rows import Rows
 
 pytestmark = pytest.mark.gpu
@@ -237,3 +238,45 @@ def test_outputs_over_what_tells_the_places(vs):
         with pytest.raises(ValueError, match="overlaps starts"):
             c.cache.append(c.seqs, k, k, starts=starts, rotary=rot, q=q, q_out=over)
     c.compare(c.run())
+
+
+@pytest.mark.parametrize("lens,counts", [([150, 90], [9, 20]), ([3000, 90], [9, 20])])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("window", [0, 6])
+def test_few_rows_and_values_that_are_not_finite(vs, lens, counts, bad, window):
+    """Weights in several parts: a value that is not finite counts once, with the whole weight, where it is seen."""
+    c = Rows(vs, lens, counts, 4, 2, 64, 32, "bf16", spread=0.5)
+    assert kernel(vs, c.nrows, 4, 2, 2, c.table.shape[1], 32, 64, "bf16")[0] == 64 and c.nrows * 2 <= 2 * 64
+    free, n, at = c.run(window=window), lens[0], lens[0] - 6
+    _, vp = D.places(64, "bf16")
+    c.pool[c.table[0, at // 32], 0, 1, 1, vp[at % 32, 5]] = D.stored(np.full(1, bad), "bf16")[0][0]
+    c.mem.upload(c.pool)
+    out, lse = c.run(window=window)
+    hit = np.zeros(out.shape, bool)
+    hit[:counts[0], 2:, 5] = P.seen_mask(np.arange(n - counts[0], n), n, window, 0)[:, at, None]
+    assert hit.any() and not hit[:counts[0], 2:, 5].all()
+    assert np.array_equal(lse, free[1]) and not np.isfinite(out[hit]).any()
+    if not np.isnan(bad):  # (no weight of these scores is too small for 32 bits)
+        assert (out[hit] == bad).all()
+    want = np.where(hit, 0, free[0])
+    np.testing.assert_allclose(np.where(hit, 0, out), want, rtol=0, atol=np.abs(want).max() * 2.0 ** -7)
+
+
+@pytest.mark.parametrize("dtype,dim,kv,counts", [("f32", 256, 2, [90, 40]), ("bf16", 256, 2, [90, 40]), ("bf16", 128, 256, [500, 600])])
+def test_recorded_calls(vs, dtype, dim, kv, counts):
+    """Kernels of more shared memory than a launch has by itself, recorded and replayed with other work between."""
+    A, st = vs.DeviceArray, Stream()
+    c = Rows(vs, [700, 650], counts, kv, kv, dim, 32, dtype)
+    want = c.run()
+    q, starts, (out, lse) = A.of(c.qb, dtype), A.of(c.starts, "i32"), c.poisoned()
+    c.cache.attend_rows(c.seqs, q, out, lse=lse, starts=starts, stream=st.ptr)  # (scratch of this stream)
+    st.sync()
+    st.begin()
+    c.cache.attend_rows(c.seqs, q, out, lse=lse, starts=starts, stream=st.ptr)
+    graph = st.end()
+    for _ in range(3):
+        out.upload(c.poisoned()[0].numpy())
+        other = c.run()
+        st.replay(graph)
+        for got in (c.values(out, lse), other):
+            assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
