@@ -176,10 +176,13 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int piece, int la
     widest = uniform((int)wave_max((float)widest));  // (past 2^24 off by two at most: a piece more)
     // Pieces of such a length that all are at work at once where tiles are few, or
     // so many that they spread.  They cost their start and the join of their rows,
-    // kPieceCost blocks for a full tile: where whole tiles take no more than that
-    // longer, there are none.
+    // a.cost blocks for a full tile of kTile rows: where whole tiles take no more than
+    // that longer, there are none.
     const int64_t ideal = all / a.slots;
-    // (twice as many of causal tiles that grow from nothing: half of theirs are empty)
+    // (twice as many of causal tiles that grow from nothing: half of theirs are empty.
+    // By 2, 3, 4 and 6 per place: fp32, 4,096 rows of 8/8 of 128 536, 466, 586 and 403 us,
+    // of 12/12 of 64 304, 339, 326 and 315; two chunks of 511 among 30 single rows
+    // 179, 185, 193 and 214; fp32, 6 prompts of 17 to 1,023 of 12/12 of 64 63, 66, 70 and 72)
     const int each = ideal < kLong || a.spread == 2 ? 2 : 2 * bound <= 3 * all ? a.spread / 2 : a.spread;
     const int target = 2 * count <= a.slots ? a.slots - count : each * a.slots;
     // (by the bound, which the pieces' numbers go by: there are no more than
@@ -266,8 +269,11 @@ constexpr int buffer_bytes(int st, int dim, int waves, int cols) {
 // What bounds it: the matrix pipe and, beside it, the vector unit (32 positions of 32
 // rows are 32 products of 16 cycles at head size 128, and 16 exponentials with four to
 // five other instructions each), which overlap only in part.  8,192 rows of 32/8
-// heads of 128 571 us (964 TFLOP/s; a library product of 8,192^3 1,394), 4,096 163 us
-// (843); of 64 104 us (663); fp32, 4,096 rows of 12 heads of 64 194 us (133 of 157).
+// heads of 128 571 us (964 TFLOP/s; a library product of 8,192^3 1,394), 4,096 164 us
+// (838); of 64 103 us (667); fp32, 4,096 rows of 12 heads of 64 315 us (82 of 154).  Head
+// sizes that are no multiple of 32 fill neither the last pieces of a key row nor the
+// waves' shares of a block: 4,096 rows of 16/8 of 144 200 us, of 160 150, of 176 246, of
+// 192 172, of 208 299, of 224 203, of 240 345, of 256 227.
 // What was gained on the way, 8,192 rows: positions, masks and pages in scalar
 // registers 952 -> 818 us; keys and values read ahead of their products 810 -> 695; values
 // with their lane groups turned, so that no bank is asked twice 695 -> 673; 256 rows per
@@ -275,11 +281,12 @@ constexpr int buffer_bytes(int st, int dim, int waves, int cols) {
 // the lanes 602 -> 553; the sum of the rounded weights, a product with ones, 553 -> 571
 // (by the vector unit 577).
 // Tiles: 256 rows by eight waves where they fill the card twice over (a workgroup to a
-// CU, two blocks a step; half the staging of 128 rows: 552 against 594 us), 64 rows where
-// even those do not fill it (2,048 rows 69 us against 115 by 128; 512 rows 23 and 28) and
-// for fp32 and heads past 128, whose accumulators fill the registers (head size 256, 4,096
-// rows of 16/8 221 us against 255), 128 between them.  Steps of two blocks leave four
-// waves too few registers (4,096 rows 158 us with one, 171 with two).
+// CU, two blocks a step; half the staging of 128 rows: 552 against 594 us, without the
+// rounded weights' sum), 64 rows where even 128 do not fill it (prompts of 256, 512, 1,024
+// and 1,500 rows 17, 23, 38 and 55 us against 20, 28, 41 and 60 by 128) and for fp32 and
+// heads past 128, whose accumulators fill the registers (head size 256, 4,096 rows of 16/8
+// 226 us; by 128 rows 255), 128 between them.  Steps of two blocks leave four waves too few
+// registers (4,096 rows 158 us with one, 171 with two, without that sum).
 template <int ST, int D, int NW, int kCols, int kParts>
 __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : kParts == 3 && D <= 128 ? 3 : 2) void chunk_kernel(ChunkArgs args) {
     // (what only the loop's edges need is read from the arguments again: held in the
@@ -831,7 +838,7 @@ __global__ __launch_bounds__(64 * NW, !ST && D > 192 ? 1 : kParts == 3 && D <= 1
 
 // Joins the pieces of a tile: a workgroup per kJoinRows rows at a time, whose waves
 // take the pieces in turn, several at once.  Bound by the partial sums' bytes: 4 x 5
-// rows of 32 heads in some 100 pieces 7 us, 1,052 rows in 2 to 3 each 30 us (which is
+// rows of 32 heads in some 100 pieces 8 us, 1,052 rows in 2 to 3 each 36 us (which is
 // why tiles are divided only where that saves more).
 template <int ST, int D>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
@@ -1065,8 +1072,9 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     const int64_t most = s->width * (kv->page_size / vs::kKvBlock);
     // Which tile: see the kernel.  Few rows per sequence never fill a larger one; and
     // prompts (the table has no more than four times their rows) have tiles that grow
-    // from the first to the last, which small ones spread: 1,024 rows of 32/8 heads of
-    // 128 38 us against 42 by 128; 512 rows over 8,192 positions 178 and 120.
+    // from the first to the last, which small ones spread: 32/8 heads of 128, 512 rows
+    // over 512, 1,500 and 8,192 positions 23, 43 and 171 us by 64, 28, 53 and 122 by 128
+    // (1,000 over 5,000 139 and 146: the limit is on the safe side there).
     auto tiles_of = [&](int tile) { return nrows * group / tile + s->nseq; };
     a.tile = vs::kSmallTile;
     const bool few = nrows * group <= s->nseq * vs::kSmallTile;  // per sequence
@@ -1080,6 +1088,11 @@ int vs_kv_attend_rows(vs_kv *kv, const vs_kv_seqs *s, int64_t layer, int64_t hea
     int64_t wgs = a.tiles * a.kv_heads;
     if (a.split) {
         a.slots = (int)std::max<int64_t>(1, 2 * kv->num_cu / a.kv_heads);
+        // What pieces cost, in blocks (a tile's start and join take about as long as so
+        // many; fp32's blocks take longer).  bf16, 32/8 heads of 128, by 16, 32, 48, 64 and
+        // 96: 1,500 rows 64, 64, 55, 55 and 55 us, 3,000 196, 196, 142, 142 and 142, 512 over
+        // 2,500 62, 62, 62, 79 and 80.  fp32, 12/12 of 64, by 0, 16, 32 and 48: 512 rows 28, 28,
+        // 33 and 33, 6 prompts of 17 to 1,023 63, 63, 63 and 58.
         a.cost = e == 2 ? 48 : 16;
         // (so many workgroups that those without work are soon through)
         a.parts = (int)std::clamp<int64_t>(4096 / (a.tiles * a.kv_heads), 1, a.tile / vs::kJoinRows);

@@ -74,8 +74,9 @@ __device__ __forceinline__ Row finish_row(const ScoreArgs &a, int row, const Sum
 // of 64 PER logits in turn.  Per logit one exponential and two sums.  The list of
 // the k largest is beam search's: what is at or above a threshold that k logits
 // seen so far reach.  Bound by HBM: 2,048 x 128,000 in bf16 92 us (5.7 TB/s of the 6.3
-// that a plain read reaches), 1,024 x 64,000 in fp32 43 us with its join (6.0); 20 x
-// 50,001 with k = 5 by latency, 7 us.  fp32's long steps are held to four waves a SIMD:
+// that a plain read reaches), 1,024 x 64,000 in fp32 44 us with its join (6.0); 20 x
+// 50,001 with k = 5 by latency, 7 us.  Lists add their thresholds' instructions: k = 5 and
+// 20 114 and 132 us, 51 and 67 (k = 0 97 and 44, joins included).  fp32's long steps are held to four waves a SIMD:
 // with six they spill 90 registers.
 template <int ST, int PER, bool TOP>
 __global__ __launch_bounds__(256, PER == kLongStep ? (ST ? 6 : 4) : 1) void logprob_piece_kernel(ScoreArgs a) {

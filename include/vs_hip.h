@@ -222,10 +222,11 @@ VS_API int vs_kmeans_step(vs_index *points, const float *centroids_in, int64_t K
  * by vs_kv_check.  Scratch memory is kept per handle and stream (with
  * hipStreamPerThread per thread, too) until the handle ends, and grows at
  * a first call of a size: a call that is recorded into a graph and would
- * have to allocate is refused (VS_ERR_UNSUPPORTED; run it once before).  A
- * recorded call keeps the scratch of the stream it was recorded on: replays
- * must not overlap that stream's other calls on the handle.  One thread at a
- * time uses a handle.
+ * have to allocate is refused (VS_ERR_UNSUPPORTED; run it once before).  It is
+ * taken as powers of two; the largest is vs_kv_attend_rows' of calls of a few
+ * thousand rows or a hundred sequences, up to 290 MB.  A recorded call keeps
+ * the scratch of the stream it was recorded on: replays must not overlap that
+ * stream's other calls on the handle.  One thread at a time uses a handle.
  *
  * The cache is npages pages of page_size positions; a page holds the keys and
  * values of consecutive positions of one sequence, of every layer and
@@ -241,7 +242,9 @@ typedef struct vs_kv vs_kv;
  * b lies in page table[b * width + p / page_size]; an entry outside
  * [0, npages) (use -1) is no page, its positions are never visible.  refs[p]
  * counts the table entries (and the caller's own holds) on page p; a page
- * with refs 0 is free. */
+ * with refs 0 is free.  A length past the table's columns (width * page_size
+ * positions) counts as their end where it is attended to, and a row past them as
+ * the last one there. */
 typedef struct vs_kv_seqs {
     int32_t *table; /* nseq x width */
     int32_t *lens;  /* nseq: positions in use */
