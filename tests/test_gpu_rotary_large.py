@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import _decode as D
+import _prompt as P
 from test_gpu_attend import View
 from test_gpu_rotary import Entered, check, host
 
@@ -75,4 +76,32 @@ def test_rows_enter_the_cache_turned(vs, layout, dtype, dim, dims, heads, kv):
     e.cache.append(e.seqs, k, v, starts=starts, rotary=rot, q=q, q_out=q)  # in place
     assert np.array_equal(q.numpy(), out.numpy())
     e.cache.close()
+    rot.close()
+
+
+def test_more_blocks_than_one_pass_of_the_grid(vs):
+    """Past 2^20 workgroups: 540,000 sequences of one row, a key-value head and a query head each."""
+    A, rng, n, dim = vs.DeviceArray, np.random.default_rng(8), 540_000, 16
+    lens = 1 + np.arange(n) % 32
+    mem = A((n, 2, 32 * dim), "bf16")
+    cache = vs.PagedKVCache(n, 32, 1, dim, memory=mem)
+    seqs = vs.KVSequences(A.of(rng.permutation(n)[:, None], "i32"), A.of(lens, "i32"), A.of(np.ones(n), "i32"))
+    rot = vs.Rotary(dim)
+    (kb, k), (vb, _), (qb, q) = (D.stored(rng.standard_normal((n, 1, dim)), "bf16") for _ in range(3))
+    out = A((n, 1, dim), "bf16")
+    cache.append(seqs, A.of(kb, "bf16"), A.of(vb, "bf16"), rotary=rot, q=A.of(qb, "bf16"), q_out=out)
+    cache.check()
+    kp, vp = D.places(dim, "bf16")
+    pages, pool = seqs.table.numpy()[:, 0], mem.numpy()
+    at = lens - 1
+    assert np.array_equal(pool[pages[:, None], 1, vp[at]], vb[:, 0])
+    got_k = D.from_bf16(pool[pages[:, None], 0, kp[at]])
+    angle = at[:, None] * rot.frequencies
+    c, s = np.cos(angle), np.sin(angle)
+    for got, x in ((got_k, k[:, 0]), (D.from_bf16(out.numpy())[:, 0], q[:, 0])):
+        a, b = x[:, :8].astype(np.float64), x[:, 8:].astype(np.float64)
+        want = np.concatenate([a * c - b * s, b * c + a * s], 1)
+        size = np.tile(np.abs(a) + np.abs(b), 2)
+        D.assert_rounded(got, want, P.turn_tolerance(size, at, rot.frequencies), "bf16")
+    cache.close()
     rot.close()

@@ -158,3 +158,20 @@ def test_no_slots_behind_an_extend_that_did_not_fit(vs):
     with pytest.raises(vs.VsError, match="pages short"):
         cache.check()
     compare(run(vs, cache, seqs, counts, 45), want)
+
+
+@pytest.mark.parametrize("n", [3, 9000])
+def test_more_rows_than_one_pass_of_the_grid(vs, n):
+    """Past 512 workgroups of 1,024 rows each."""
+    counts = np.full(n, 700_000 // n)
+    lens = counts + np.arange(n) % 50
+    cache, seqs, table = setup(vs, counts, lens, width=20, npages=400)
+    nrows = int(counts.sum()) + 9
+    starts = np.concatenate([[0], counts.cumsum()])
+    b = np.repeat(np.arange(n), counts)
+    pos = lens[b] - (starts[b + 1] - np.arange(len(b)))
+    page = np.where(pos < 20 * 32, table[b, np.minimum(pos // 32, 19)], -1)
+    slot = np.where((page >= 0) & (page < 400), page * 32 + pos % 32, -1)
+    pad = lambda x: np.concatenate([x, np.full(9, -1)])  # noqa: E731
+    compare(run(vs, cache, seqs, counts, nrows), [starts, pad(b), pad(pos), pad(slot)])
+    cache.check()
